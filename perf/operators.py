@@ -393,6 +393,10 @@ def _run_attn(s):
 EOS = 2
 
 
+def _alpha(c):
+    return float(np.float32(c["alpha"]))
+
+
 def _run_beam(s):
     c, o = s["case"], s["out"]
     B, K, V = c["batch"], c["beams"], c["vocab"]
@@ -408,7 +412,7 @@ def _run_beam(s):
     token = torch.arange(V, device=DEV)[None]
     total = torch.where(done, torch.where(token == EOS, score, -INF), total)
     length = s["len"].long()[:, None] + ~done
-    key = (total / length.double().pow(c["alpha"])).view(B, K * V)
+    key = (total / length.double().pow(_alpha(c))).view(B, K * V)
     best = torch.sort(key, dim=1, descending=True, stable=True).indices[:, :K]
     parent = torch.arange(B, device=DEV)[:, None] * K + best // V
     picked = (best % V).reshape(-1)
@@ -518,9 +522,9 @@ def exact(case, seed):
             found = []
             for r in range(b * K, (b + 1) * K):
                 if done[r]:
-                    found.append((score[r] / float(length[r]) ** c["alpha"], score[r]))
+                    found.append((score[r] / float(length[r]) ** _alpha(c), score[r]))
                 else:
-                    found += [((score[r] + p) / float(length[r] + 1) ** c["alpha"], score[r] + p) for p in kept[r]]
+                    found += [((score[r] + p) / float(length[r] + 1) ** _alpha(c), score[r] + p) for p in kept[r]]
             found.sort(key=lambda f: -f[0])
             out[b * K:(b + 1) * K] = [f[1] for f in found[:K]]
         return {"score": out, "len": None, "done": None, "parent": None, "token": None}
