@@ -1,0 +1,64 @@
+// What the attention kernels share: the layout of MFMA accumulators, reductions over
+// the half-waves and division by launch constants.
+#pragma once
+
+#include "common.h"
+
+namespace cdml {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Division by a launch-constant divisor d >= 1 for dividends 0 <= x < 2^31:
+// x / d = (x * m) >> l with l = 31 + ceil(log2 d) and m = ceil(2^l / d) < 2^32
+// (the error m * d - 2^l is below d, so x * error < 2^l for every such x).
+// Block-uniform dividends keep the division on the scalar unit.
+struct UDiv {
+  uint32_t m;
+  int l;
+  static UDiv make(uint32_t d) {
+    if (d == 0) d = 1;  // no launch divides by it
+    int s = 0;
+    while ((1ull << s) < d) ++s;
+    const int l = 31 + s;
+    return {(uint32_t)(((1ull << l) + d - 1) / d), l};
+  }
+  __device__ __forceinline__ int div(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> l); }
+};
+
+// max / sum of a value over the two half-waves (lanes l and l ^ 32) with
+// v_permlane32_swap: both results hold the value of lane l % 32 and of lane
+// l % 32 + 32.
+__device__ __forceinline__ float halves_max(float x) {
+#pragma float_control(precise, off)
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));  // scores: no signalling NaN
+}
+__device__ __forceinline__ float halves_sum(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// max of three scores.  The scores come from MFMA accumulators and are
+// never signalling NaNs, so the IEEE quieting that fmaxf otherwise adds to
+// each operand is dropped (one v_max3_f32 instead of five instructions).
+__device__ __forceinline__ float max3_scores(float a, float b, float c) {
+#pragma float_control(precise, off)
+  return __builtin_fmaxf(__builtin_fmaxf(a, b), c);
+}
+
+// Growth of the running max (log2 units) tolerated before the output is
+// rescaled: probabilities stay <= 2^8, far from fp32 overflow.
+constexpr float kRescaleThreshold = 8.0f;
+
+// Offset of accumulator register r's key inside its 32-key sub-block for a
+// lane of half-wave h: 8 * (r / 4) + 4 * h + r % 4 (the 32x32 MFMA D layout).
+__device__ __forceinline__ constexpr int acc_key(int r) { return 8 * (r >> 2) + (r & 3); }
+
+// A sub-block whose per-lane probability sum stays at or below this bound is
+// accumulated without looking at its maximum: no probability exceeds it, so
+// nothing overflows (the running sums stay below 2^32 times the key count).
+constexpr float kFastSumLimit = 4294967296.0f;  // 2^32
+
+}  // namespace
+}  // namespace cdml

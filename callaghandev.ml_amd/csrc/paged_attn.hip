@@ -1,0 +1,197 @@
+// Attention of a step's new tokens over a paged cache (cdml_paged_attn): the choice of
+// kernels and splits, and the join of a request's chunks.  The kernels are in
+// paged_attn.inc.h.
+#include "paged.h"
+
+namespace cdml {
+namespace {
+
+// One wave per (row, head): o = sum_s w_s o_s / sum_s w_s l_s with w_s = 2^(m_s - M) over
+// the chunks that hold a visible key.  Rows of one chunk are in o already.
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
+  const int row = blockIdx.x, lane = threadIdx.x & 63;
+  const int h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (h >= a.heads) return;
+  int b = 0;  // requests that end at or before the row
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const bool before = b0 + lane < a.batch && a.cu_new[b0 + lane + 1] <= row;
+    const int n = __popcll(__builtin_amdgcn_ballot_w64(before));
+    b += n;
+    if (n < 64) break;
+  }
+  if (b >= a.batch) return;
+  const PagedSeq s = paged_seq(a, b);
+  const int i = row - s.first;
+  if (i < 0 || i >= s.n) return;
+  const bool vec = s.n * a.group <= a.vec_rows;
+  const int chunk = vec ? a.vec_chunk : a.tile_chunk, seen = s.len - s.n + i + 1;
+  if (s.len <= chunk) return;
+  const int n = seen <= 0 ? 0 : (seen - 1) / chunk + 1, hk = a.by_group.div(h), stride = a.hd + 2;
+  const float *part =
+      vec ? a.vec_part + (((size_t)b * a.kv_heads + hk) * a.vec_rows + i * a.group + h - hk * a.group) * a.vec_splits * stride
+          : a.tile_part + ((size_t)row * a.heads + h) * a.tile_splits * stride;
+  float M = -3.0e38f;
+  for (int c = lane; c < n; c += 64) M = fmaxf(M, part[(size_t)c * stride + a.hd]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off));
+  float L = 0.f, acc[4] = {};
+  for (int c = 0; c < n; ++c) {
+    const float *p = part + (size_t)c * stride;
+    const float w = fast_exp2(p[a.hd] - M);
+    L = fmaf(p[a.hd + 1], w, L);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (lane + 64 * j < a.hd) acc[j] = fmaf(p[lane + 64 * j], w, acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (lane + 64 * j < a.hd)
+      a.o[(size_t)row * a.ldo + (size_t)h * a.hd + lane + 64 * j] = L == 0.f ? 0.f : acc[j] / L;
+}
+
+// Which kernels run and how keys are split, from the sizes alone.
+struct Plan {
+  bool vec, tile;
+  int vec_rows, vec_chunk, vec_splits, tile_chunk, tile_splits;
+  size_t vec_floats, tile_floats;
+};
+
+constexpr int kVecRows = 4;       // most rows a K/V head on the vector units
+constexpr int kComputeUnits = 256;
+
+int check_sizes(const char *what, int rows, int batch, int max_new, int max_len, int heads, int kv_heads, int hd) {
+  if (rows < 0 || batch < 0 || batch > kPagedMaxBatch || max_new < 0 || max_len < 0)
+    return fail(CDML_E_INVALID, "%s: bad size (rows %d, batch %d of at most %d, max_new %d, max_len %d)", what, rows,
+                batch, kPagedMaxBatch, max_new, max_len);
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || hd <= 0 || hd > 256)
+    return fail(CDML_E_INVALID, "%s: bad heads (%d over %d K/V heads, head_dim %d of at most 256)", what, heads,
+                kv_heads, hd);
+  const long long group = heads / kv_heads;
+  // the grids' limits, and room for key numbers past the last tile
+  const long long most = max_new * group;
+  const long long groups = (hd <= 128 && most > kVecRows ? kVecRows : most + kVecRows - 1) / kVecRows;
+  if (most > INT_MAX / 2 || max_len > INT_MAX / 2 || heads > 65535 || groups * kv_heads > 65535 ||
+      (long long)kv_heads * hd > INT_MAX / 4 ||
+      ((long long)rows * group / kPagedTileRows + batch) * kv_heads > INT_MAX / 2)
+    return fail(CDML_E_INVALID, "%s: problem too large", what);
+  return CDML_OK;
+}
+
+int round_up(int n, int m) { return (int)(((long long)n + m - 1) / m * m); }
+
+Plan make_plan(int rows, int batch, int max_new, int max_len, int heads, int kv_heads, int hd) {
+  Plan p{};
+  const int group = heads / kv_heads, most = max_new * group, len = max_len < 1 ? 1 : max_len;
+  p.tile = hd <= 128 && most > kVecRows;
+  p.vec = true;
+  p.vec_rows = p.tile ? kVecRows : most < 1 ? 1 : most;
+  // vector units: 512 keys a workgroup while there are four workgroups for every CU,
+  // else 256; rows without number (head dims above 128) are not split
+  const long long groups = (p.vec_rows + kVecRows - 1) / kVecRows;
+  if (groups > 2) {
+    p.vec_chunk = len > INT_MAX / 2 ? INT_MAX : round_up(len, kPagedSub);
+  } else {
+    const long long wide = (long long)((len - 1) / 512 + 1) * kv_heads * batch * groups;
+    p.vec_chunk = wide >= 4 * kComputeUnits ? 512 : 256;
+  }
+  p.vec_splits = (len - 1) / p.vec_chunk + 1;
+  if (p.vec_splits > 1) p.vec_floats = (size_t)batch * kv_heads * p.vec_rows * p.vec_splits * (hd + 2);
+  // matrix cores: keys are split where the tiles alone leave CUs without work
+  p.tile_chunk = INT_MAX;
+  p.tile_splits = 1;
+  if (p.tile) {
+    const long long tiles = ((long long)rows * group / kPagedTileRows + batch) * kv_heads;
+    long long splits = (2 * kComputeUnits + tiles - 1) / (tiles < 1 ? 1 : tiles);
+    const long long pieces = (len + 255) / 256;
+    if (splits > pieces) splits = pieces;
+    if (splits > 1) {
+      p.tile_chunk = round_up((int)((len + splits - 1) / splits), 64);
+      p.tile_splits = (len - 1) / p.tile_chunk + 1;
+      if (p.tile_splits > 1) p.tile_floats = (size_t)rows * heads * p.tile_splits * (hd + 2);
+    }
+  }
+  return p;
+}
+
+}  // namespace
+}  // namespace cdml
+
+using namespace cdml;
+
+extern "C" int cdml_paged_attn_workspace_size(int rows, int batch, int max_new, int max_len, int num_heads,
+                                              int num_kv_heads, int head_dim, size_t *bytes) {
+  if (!bytes) return fail(CDML_E_INVALID, "cdml_paged_attn_workspace_size: bytes is NULL");
+  int rc = check_sizes("cdml_paged_attn_workspace_size", rows, batch, max_new, max_len, num_heads, num_kv_heads,
+                       head_dim);
+  if (rc) return rc;
+  const Plan p = make_plan(rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
+  *bytes = sizeof(float) * (p.vec_floats + p.tile_floats);
+  return CDML_OK;
+}
+
+extern "C" int cdml_paged_attn(const float *q, int ldq, const void *kcache, const void *vcache, int cache_type,
+                               int n_pages, int page_size, const int *block_table, int max_blocks, const int *kv_len,
+                               const int *cu_new, float *o, int ldo, int rows, int batch, int max_new, int max_len,
+                               int num_heads, int num_kv_heads, int head_dim, float scale, int *bad, void *workspace,
+                               size_t workspace_bytes, cdml_stream stream) {
+  PagedArgs a{};
+  int rc = check_pool("cdml_paged_attn", n_pages, page_size, max_blocks, batch, &a.page_shift);
+  if (rc) return rc;
+  rc = check_sizes("cdml_paged_attn", rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
+  if (rc) return rc;
+  const int size = cache_type_bytes(cache_type);
+  if (!size) return fail(CDML_E_INVALID, "cdml_paged_attn: unknown cache type %d", cache_type);
+  if ((long long)max_len > (long long)max_blocks * page_size)
+    return fail(CDML_E_INVALID, "cdml_paged_attn: max_len %d above the table's %lld tokens", max_len,
+                (long long)max_blocks * page_size);
+  const long long dim = (long long)num_heads * head_dim;
+  if (ldq < dim || ldo < dim) return fail(CDML_E_INVALID, "cdml_paged_attn: row stride smaller than the heads");
+  if (rows == 0 || batch == 0 || max_new == 0) return CDML_OK;
+  if (!q || !kcache || !vcache || !block_table || !kv_len || !cu_new || !o)
+    return fail(CDML_E_INVALID, "cdml_paged_attn: NULL pointer");
+  const Plan p = make_plan(rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
+  const size_t need = sizeof(float) * (p.vec_floats + p.tile_floats);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(CDML_E_INVALID, "cdml_paged_attn: %zu bytes of 16-byte aligned workspace needed, %zu given", need,
+                workspace_bytes);
+  rc = ensure_device();
+  if (rc) return rc;
+  a.q = q;
+  a.kc = kcache;
+  a.vc = vcache;
+  a.table = block_table;
+  a.kv_len = kv_len;
+  a.cu_new = cu_new;
+  a.o = o;
+  a.bad = bad;
+  a.ldq = ldq;
+  a.ldo = ldo;
+  a.n_pages = n_pages;
+  a.max_blocks = max_blocks;
+  a.rows = rows;
+  a.batch = batch;
+  a.max_new = max_new;
+  a.max_len = max_len;
+  a.heads = num_heads;
+  a.kv_heads = num_kv_heads;
+  a.group = num_heads / num_kv_heads;
+  a.hd = head_dim;
+  a.scale_log2 = scale * kLog2e;
+  a.by_group = UDiv::make((uint32_t)a.group);
+  a.vec_rows = p.vec_rows;
+  a.vec_chunk = p.vec_chunk;
+  a.vec_splits = p.vec_splits;
+  a.tile_chunk = p.tile_chunk;
+  a.tile_splits = p.tile_splits;
+  a.vec_part = static_cast<float *>(workspace);
+  a.tile_part = a.vec_part + p.vec_floats;
+  const bool wide = (head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256) && ldq % 4 == 0 &&
+                    ldo % 4 == 0 && aligned16(q) && aligned16(o) && aligned16(kcache) && aligned16(vcache);
+  const hipStream_t st = as_hip(stream);
+  if (cache_type == CDML_CACHE_F32) rc = paged_attn_f32(a, p.vec, p.tile, wide, st);
+  else if (cache_type == CDML_CACHE_F16) rc = paged_attn_f16(a, p.vec, p.tile, wide, st);
+  else rc = paged_attn_bf16(a, p.vec, p.tile, wide, st);
+  if (rc || (p.vec_splits == 1 && p.tile_splits == 1)) return rc;
+  paged_join_kernel<<<dim3(rows, (num_heads + 3) / 4), 256, 0, st>>>(a);
+  return check_launch("paged_join_kernel");
+}

@@ -1,0 +1,843 @@
+// The attention kernels over a paged cache, for one cache type T (float, _Float16 or
+// __bf16; included by a file each).
+#pragma once
+
+#include "paged.h"
+
+namespace cdml {
+namespace {
+
+// Four cached values as they are loaded.
+template <typename T>
+struct Raw4 {
+  typedef vu2 type;
+};
+template <>
+struct Raw4<float> {
+  typedef vf4 type;
+};
+
+__device__ __forceinline__ float half_value(uint32_t w, int i, _Float16) {
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)(i ? w >> 16 : w & 0xffffu));
+}
+__device__ __forceinline__ float half_value(uint32_t w, int i, __bf16) {
+  return __uint_as_float(i ? w & 0xffff0000u : w << 16);
+}
+
+// ---- few rows: vector units ---------------------------------------------------
+
+constexpr int PR_THREADS = 256;
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+// Sum over groups of LPK (8 or 16) neighbouring lanes, in each of them: exchanges with
+// lane ^ 1, ^ 2, then the mirrored lane of 8 and of 16.
+template <int LPK>
+__device__ __forceinline__ float lanes_sum(float x) {
+  x += dpp<0xB1>(x);
+  x += dpp<0x4E>(x);
+  x += dpp<0x141>(x);
+  if constexpr (LPK == 16) x += dpp<0x140>(x);
+  return x;
+}
+
+// A lane's EPL values of one cached row: NV loads of VW values, LPK * VW apart.
+template <typename T, int VW, int NV, int LPK, bool VEC>
+struct RowSlice {
+  static constexpr int WORDS = VW * NV * (int)sizeof(T) / 4;
+  static_assert(VW * sizeof(T) % 4 == 0, "whole words");
+  uint32_t w[WORDS];
+
+  __device__ __forceinline__ void load(const T *p, int d0, int hd, bool zero) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      constexpr int LW = WORDS / NV;  // words per load
+      if constexpr (VEC) {
+        typedef uint32_t V __attribute__((ext_vector_type(LW)));
+        if constexpr (LW == 1) {
+          w[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p + LPK * VW * i));
+        } else {
+          const V t = __builtin_nontemporal_load(reinterpret_cast<const V *>(p + LPK * VW * i));
+#pragma unroll
+          for (int c = 0; c < LW; ++c) w[i * LW + c] = t[c];
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < LW; ++c) w[i * LW + c] = 0;
+#pragma unroll
+        for (int c = 0; c < VW; ++c) {
+          if (d0 + LPK * VW * i + c >= hd) continue;
+          if constexpr (sizeof(T) == 4) w[i * LW + c] = __builtin_bit_cast(uint32_t, p[LPK * VW * i + c]);
+          else w[i * LW + c / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[LPK * VW * i + c]) << 16 * (c & 1);
+        }
+      }
+    }
+    if (zero) {
+#pragma unroll
+      for (int c = 0; c < WORDS; ++c) w[c] = 0;
+    }
+  }
+  __device__ __forceinline__ float value(int e) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+    else return half_value(w[e / 2], e & 1, T{});
+  }
+};
+
+// One workgroup: R rows of a (request, K/V head) against one chunk of its keys; a cached
+// row goes through LPK lanes, its score through their sum, and every group of LPK lanes
+// keeps an online softmax of its own keys.  The four waves take 64 / LPK keys in turn.
+// Two sets of rows alternate, so that a step's loads are in flight while the step before
+// it is consumed.
+template <typename T, int HD, int R, bool VEC>
+__global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedArgs a) {
+  constexpr int LPK = HD >= 64 && R > 2 ? 16 : 8;
+  constexpr int EPL = HD / LPK;                                              // values per lane
+  constexpr int VW = EPL * sizeof(T) >= 16 ? 16 / (int)sizeof(T) : EPL;      // per load
+  constexpr int NV = EPL / VW, KPS = 64 / LPK;
+  typedef RowSlice<T, VW, NV, LPK, VEC> Slice;
+  constexpr float kNone = -3.0e38f;  // below every score that matters, and exp2 of it is 0
+  __shared__ int pages[kPagedSub + 1];
+  __shared__ float red_m[4][R], red_l[4][R];
+  __shared__ float red_o[4][R][HD];
+
+  const int b = blockIdx.z;
+  const PagedSeq s = paged_seq(a, b);
+  const int nr = s.n * a.group;
+  if (nr == 0 || nr > a.vec_rows) return;
+  const int hk = blockIdx.y % a.kv_heads, r0 = blockIdx.y / a.kv_heads * R;
+  if (r0 >= nr) return;
+  const int split = blockIdx.x, base = s.len - s.n;  // token i sees keys up to base + i
+  const bool single = s.len <= a.vec_chunk;
+  const int kend = base + a.by_group.div(min(r0 + R, nr) - 1) + 1;  // past the last visible key
+  const int c0 = split * a.vec_chunk, c1 = min(c0 + a.vec_chunk, kend);
+  if (c0 >= c1 && !(single && split == 0)) return;
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane / LPK, d0 = VW * (lane % LPK);
+  const int P1 = (1 << a.page_shift) - 1, kv_dim = a.kv_heads * a.hd;
+
+  float q[R][EPL], o[R][EPL], m[R], l[R];
+  int lim[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int rr = min(r0 + r, nr - 1), i = a.by_group.div(rr);
+    lim[r] = base + i;
+    const float *qr = a.q + (size_t)(s.first + i) * a.ldq + (size_t)(hk * a.group + rr - i * a.group) * a.hd;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      const int d = d0 + LPK * VW * (e / VW) + e % VW;
+      q[r][e] = VEC || d < a.hd ? qr[d] * a.scale_log2 : 0.f;
+      o[r][e] = 0.f;
+    }
+    m[r] = kNone;
+    l[r] = 0.f;
+  }
+
+  const T *kb = static_cast<const T *>(a.kc) + (size_t)hk * a.hd + d0;
+  const T *vb = static_cast<const T *>(a.vc) + (size_t)hk * a.hd + d0;
+  for (int sub = c0; sub < c1; sub += kPagedSub) {
+    const int end = min(sub + kPagedSub, c1), block0 = sub >> a.page_shift;
+    const int n_blocks = ((end - 1) >> a.page_shift) - block0 + 1;
+    if (sub > c0) __syncthreads();
+    int wrong = 0;
+    for (int i = threadIdx.x; i < n_blocks; i += PR_THREADS) {
+      const int page = a.table[(size_t)b * a.max_blocks + block0 + i];
+      const bool ok = (unsigned)page < (unsigned)a.n_pages;
+      pages[i] = ok ? page : -1;
+      wrong |= !ok;
+    }
+    const bool any_wrong = __syncthreads_or(wrong) != 0;
+    if (any_wrong && a.bad && threadIdx.x == 0) *a.bad = 1;
+
+    // keys past the end read the last one and are left out below
+    auto fetch = [&](int key, Slice &kr, Slice &vr) {
+      key = min(key, end - 1);
+      const int page = pages[(key >> a.page_shift) - block0];
+      const size_t at = ((size_t)(max(page, 0) << a.page_shift) + (key & P1)) * kv_dim;
+      kr.load(kb + at, d0, a.hd, any_wrong && page < 0);
+      vr.load(vb + at, d0, a.hd, any_wrong && page < 0);
+    };
+    auto step = [&](int key, const Slice &kr, const Slice &vr) {
+      float sc[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) sc[r] = 0.f;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const float x = kr.value(e);
+#pragma unroll
+        for (int r = 0; r < R; ++r) sc[r] = fmaf(q[r][e], x, sc[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) sc[r] = lanes_sum<LPK>(sc[r]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (key <= lim[r] && key < end) {
+          const float mn = fmaxf(m[r], sc[r]);
+          const float alpha = fast_exp2(m[r] - mn), p = fast_exp2(sc[r] - mn);
+          l[r] = fmaf(l[r], alpha, p);
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) o[r][e] = fmaf(p, vr.value(e), o[r][e] * alpha);
+          m[r] = mn;
+        }
+      }
+    };
+    Slice k0, v0, k1, v1;
+    const int key0 = sub + wave * KPS + g, steps = (end - sub + 4 * KPS - 1) / (4 * KPS);
+    fetch(key0, k0, v0);
+    for (int it = 0; it < steps; it += 2) {
+      const int key = key0 + it * 4 * KPS;
+      fetch(key + 4 * KPS, k1, v1);
+      step(key, k0, v0);
+      fetch(key + 8 * KPS, k0, v0);
+      step(key + 4 * KPS, k1, v1);
+    }
+  }
+
+  // the groups of a wave, then the waves
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int off = LPK; off < 64; off <<= 1) {
+      const float m2 = __shfl_xor(m[r], off), l2 = __shfl_xor(l[r], off);
+      const float mn = fmaxf(m[r], m2), w1 = fast_exp2(m[r] - mn), w2 = fast_exp2(m2 - mn);
+      l[r] = l[r] * w1 + l2 * w2;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[r][e] = o[r][e] * w1 + __shfl_xor(o[r][e], off) * w2;
+      m[r] = mn;
+    }
+    if (lane == 0) {
+      red_m[wave][r] = m[r];
+      red_l[wave][r] = l[r];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float M = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r]));
+    const float w = fast_exp2(m[r] - M);
+    if (g == 0) {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) red_o[wave][r][d0 + LPK * VW * (e / VW) + e % VW] = o[r][e] * w;
+    }
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < R * HD; t += PR_THREADS) {
+    const int r = t / HD, d = t % HD, rr = r0 + r;
+    if (rr >= nr || d >= a.hd) continue;
+    const float M = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r]));
+    float L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) L += red_l[w][r] * fast_exp2(red_m[w][r] - M);
+    const float x = red_o[0][r][d] + red_o[1][r][d] + red_o[2][r][d] + red_o[3][r][d];
+    if (single) {
+      const int i = a.by_group.div(rr), h = hk * a.group + rr - i * a.group;
+      a.o[(size_t)(s.first + i) * a.ldo + (size_t)h * a.hd + d] = L == 0.f ? 0.f : x / L;
+    } else {
+      float *part = a.vec_part + ((((size_t)b * a.kv_heads + hk) * a.vec_rows + rr) * a.vec_splits + split) * (a.hd + 2);
+      part[d] = x;
+      if (d == 0) {
+        part[a.hd] = M;
+        part[a.hd + 1] = L;
+      }
+    }
+  }
+}
+
+// ---- many rows: matrix cores --------------------------------------------------
+
+constexpr int PT_THREADS = 256;
+
+// Pieces of a cached value (common.h): fp32 has three, fp16's eleven bits lie in two,
+// bf16 is one; and the products of their pieces with the three of Q or of the
+// probabilities that reach fp32's accuracy, the main one last.
+template <typename T>
+struct Pieces;
+template <>
+struct Pieces<float> {
+  static constexpr int N = 3, PRODUCTS = 6;
+  static constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};
+};
+template <>
+struct Pieces<_Float16> {
+  static constexpr int N = 2, PRODUCTS = 5;
+  static constexpr int A[5] = {1, 0, 1, 0, 0}, B[5] = {1, 2, 0, 1, 0};
+};
+template <>
+struct Pieces<__bf16> {
+  static constexpr int N = 1, PRODUCTS = 3;
+  static constexpr int A[3] = {0, 0, 0}, B[3] = {2, 1, 0};
+};
+
+// Where a key's row lies in the cache, and whether its page is a page.
+struct Slot {
+  uint32_t at;
+  bool ok;
+};
+__device__ __forceinline__ Slot slot_in(const PagedArgs &a, int page, int key) {
+  const bool ok = (unsigned)page < (unsigned)a.n_pages;
+  return {((uint32_t)(ok ? page : 0) << a.page_shift) + (uint32_t)(key & ((1 << a.page_shift) - 1)), ok};
+}
+
+// Stages one tile of BN keys: K rows and V transposed, of one K/V head, from their pages
+// into registers and then, as bf16 pieces, into LDS (one plane per piece, rows of 16
+// values = 32 bytes).  The upper half of the workgroup's waves stages K, the lower half V,
+// four dims of a key per load.
+//   K: slab s holds dims 16 s .. 16 s + 15 of every key: rows are keys, even and odd ones
+//      in two clusters.
+//   V: slab s holds keys 16 s .. 16 s + 15 of every dim: rows are dims, in four clusters
+//      by d % 4.  A unit is four dims of two keys; key k of a slab sits at place
+//      8 (k / 4 % 2) + 4 (k / 8) + k % 4, the order the P.V product reads.
+// The pages of a tile are looked up a tile ahead of its rows.  Keys past the request's
+// last read that one: their scores are masked and their probabilities exactly 0.
+template <typename T, int HD, int BN, bool VEC>
+struct PagedStage {
+  typedef typename Raw4<T>::type Raw;
+  static constexpr int NP = Pieces<T>::N;
+  static constexpr int HALF = PT_THREADS / 2;
+  static constexpr int KROWB = BN / 2 * 32, VROWB = HD / 4 * 32;  // bytes of one row cluster
+  static constexpr int KSLAB = 2 * KROWB + 128, VSLAB = 4 * VROWB + 256;
+  static constexpr int KPLANE = HD / 16 * KSLAB, VPLANE = BN / 16 * VSLAB;
+  static constexpr int BYTES = NP * (KPLANE + VPLANE);   // K planes, then V planes
+  static constexpr int VU = (HD / 4) * (BN / 2) / HALF;  // V units per thread; twice as many K units
+  static constexpr int NV = 2 * VU;                      // loads of either
+  static_assert(VU >= 1 && (HD / 4) * (BN / 2) % HALF == 0, "tile units");
+  static __device__ __forceinline__ constexpr int kcluster(int c) { return c * (KROWB + 16); }
+  static __device__ __forceinline__ constexpr int vcluster(int c) {
+    return c * VROWB + (c & 1) * 16 + (c >> 1) * 128;
+  }
+  static constexpr int CH = HD / 4, KSTEP = HALF / CH;
+  static __device__ __forceinline__ constexpr int vgroups(int i) { return HALF / 8 * i % CH; }
+  static __device__ __forceinline__ constexpr int vslabs(int i) { return HALF / 8 * i / CH; }
+  Raw r[NV];
+  int page[NV];  // of the next tile's rows
+  uint32_t zero;  // bit i: load i's page is none
+  const T *base;  // of this thread's columns
+  const int *table;
+  int col, row, dst;  // first column, first row in a tile, LDS byte offset of the first unit
+  int kv_dim, last;   // the request's last key
+  bool kside;
+
+  __device__ __forceinline__ void init(const PagedArgs &a, int b, int hk, int last_key) {
+    kside = __builtin_amdgcn_readfirstlane(threadIdx.x) >= HALF;
+    const int t = threadIdx.x & (HALF - 1);
+    // K: the P keys of one load instruction share a cluster
+    constexpr int P = 64 / CH;
+    const int c = t % CH, j = t / CH, kkey = (j & ~(2 * P - 1)) | ((j & (P - 1)) << 1) | ((j / P) & 1);
+    const int sb = t & 7, g = (t >> 3) % CH, slab = (t >> 3) / CH;
+    const int place = ((sb >> 1) & 1) * 4 + (sb >> 2) * 2 + (sb & 1);  // of V's key pair
+    col = kside ? 4 * c : 4 * g;
+    row = kside ? kkey : 16 * slab + 2 * sb;
+    dst = kside ? (c >> 2) * KSLAB + kcluster(kkey & 1) + (kkey >> 1) * 32 + (c & 3) * 8
+                : NP * KPLANE + slab * VSLAB + g * 32 + place * 4;
+    base = static_cast<const T *>(kside ? a.kc : a.vc) + (size_t)hk * a.hd + col;
+    table = a.table + (size_t)b * a.max_blocks;
+    kv_dim = a.kv_heads * a.hd;
+    last = last_key;
+  }
+  __device__ __forceinline__ int key(int k0, int i) const {
+    return min(k0 + row + (kside ? KSTEP * i : 16 * vslabs(i / 2) + (i & 1)), last);
+  }
+  __device__ __forceinline__ void lookup(const PagedArgs &a, int k0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) page[i] = table[key(k0, i) >> a.page_shift];
+  }
+
+  __device__ __forceinline__ void load(const PagedArgs &a, int k0) {
+    zero = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const Slot s = slot_in(a, page[i], key(k0, i));
+      if (!s.ok) zero |= 1u << i;
+      const int dc = kside ? 0 : 4 * vgroups(i / 2);
+      const T *p = base + (size_t)s.at * kv_dim + dc;
+      if constexpr (VEC) {
+        r[i] = *reinterpret_cast<const Raw *>(p);
+      } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) r[i][c] = col + dc + c < a.hd ? (float)p[c] : 0.f;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t lo = col + dc + 2 * c < a.hd ? __builtin_bit_cast(uint16_t, p[2 * c]) : 0;
+          const uint32_t hi = col + dc + 2 * c + 1 < a.hd ? __builtin_bit_cast(uint16_t, p[2 * c + 1]) : 0;
+          r[i][c] = lo | hi << 16;
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void store(char *lds, int *bad) {
+    if (__builtin_amdgcn_ballot_w64(zero != 0)) {
+      if (zero && bad) *bad = 1;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (zero >> i & 1) r[i] = Raw{};
+    }
+    if (kside) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        char *d = lds + dst + KSTEP / 2 * 32 * i;
+        if constexpr (NP == 1) {
+          *reinterpret_cast<vu2 *>(d) = r[i];
+        } else {
+          float x[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if constexpr (NP == 3) x[c] = r[i][c];
+            else x[c] = half_value(r[i][c / 2], c & 1, T{});
+          }
+          uint32_t h0, m0, l0, h1, m1, l1;
+          split_bf16x3(x[0], x[1], h0, m0, l0);
+          split_bf16x3(x[2], x[3], h1, m1, l1);
+          *reinterpret_cast<vu2 *>(d) = vu2{h0, h1};
+          *reinterpret_cast<vu2 *>(d + KPLANE) = vu2{m0, m1};
+          if constexpr (NP == 3) *reinterpret_cast<vu2 *>(d + 2 * KPLANE) = vu2{l0, l1};
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VU; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          char *d = lds + dst + vslabs(i) * VSLAB + vgroups(i) * 32 + vcluster(c);
+          if constexpr (NP == 1) {
+            *reinterpret_cast<uint32_t *>(d) = __builtin_amdgcn_perm(r[2 * i + 1][c / 2], r[2 * i][c / 2],
+                                                                     c & 1 ? 0x07060302u : 0x05040100u);
+          } else {
+            uint32_t h, m, l;
+            if constexpr (NP == 3)
+              split_bf16x3(r[2 * i][c] * kSplitScale, r[2 * i + 1][c] * kSplitScale, h, m, l);
+            else
+              split_bf16x3(half_value(r[2 * i][c / 2], c & 1, T{}), half_value(r[2 * i + 1][c / 2], c & 1, T{}), h, m,
+                           l);
+            *reinterpret_cast<uint32_t *>(d) = h;
+            *reinterpret_cast<uint32_t *>(d + VPLANE) = m;
+            if constexpr (NP == 3) *reinterpret_cast<uint32_t *>(d + 2 * VPLANE) = l;
+          }
+        }
+    }
+  }
+
+  // Byte offsets of a lane's operands in a plane: dims 16 s + 8 hf + 0..7 of key
+  // row0 + li (row0 a multiple of 32), and eight keys of slab s for dim 32 db + li.
+  static __device__ __forceinline__ int koperand(int li, int hf) {
+    return kcluster(li & 1) + (li >> 1) * 32 + hf * 16;
+  }
+  static __device__ __forceinline__ int voperand(int li, int hf) {
+    return NP * KPLANE + vcluster(li & 3) + (li >> 2) * 32 + hf * 16;
+  }
+};
+
+// Q^T operand of a wave: the three bf16 pieces of this lane's row times scale_log2.
+// Scores start from the row's reference, so neither Q nor K takes the split's scale: what
+// a component below 2^-110 loses (2^-134) reaches a score only through a component of
+// 2^100 and more on the other side.  Returns whether Q holds one or the other
+// (wave-uniform); such rows are recomputed on the fp32 MFMA.
+template <int HD, bool VEC>
+__device__ __forceinline__ bool paged_load_q(bf16x8 (&q)[HD / 16][3], const float *qrow, int hd, float scale, int hf) {
+  uint32_t most = 0, least = ~0u;  // of |x|, and of 2 |x| - 1 as integers, which leaves zeros out
+#pragma unroll
+  for (int s = 0; s < HD / 16; ++s) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const int d = 16 * s + 8 * hf + e;
+      if constexpr (VEC) {
+        const vf4 t = *reinterpret_cast<const vf4 *>(qrow + d);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[e + c] = t[c] * scale;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[e + c] = d + c < hd ? qrow[d + c] * scale : 0.f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+      least = min(least, (__float_as_uint(x[e]) << 1) - 1u);
+    }
+    split_operand(x, 1.f, q[s]);
+  }
+  return __builtin_amdgcn_ballot_w64(most >= (100u + 127u) << 23 || least < (17u << 24) - 1u) != 0;  // 2^100, 2^-110
+}
+
+// The online softmax of one wave's 32 rows (one per lane % 32) over 32-key sub-blocks:
+// S^T = K Q^T puts one row per lane, O^T += V^T P^T consumes the probabilities in place.
+template <typename T, int HD, int BN, bool VEC>
+struct PagedRows {
+  typedef PagedStage<T, HD, BN, VEC> Tile;
+  typedef Pieces<T> PC;
+  static constexpr int NDB = HD / 32;  // 32-wide head-dim blocks of O^T
+  static constexpr int NS = HD / 16;   // MFMA k-steps of Q.K
+  floatx16 oacc[NDB], ocor[NDB];       // the main product, and its corrections
+  // -m_run in all 16 entries, what a block's scores start from (0 until the first
+  // visible key sets m_run): scores come out relative to the reference.
+  floatx16 negm;
+  float m_run, thr;  // thr: rescale threshold, any visible key until m_run is set
+  float l_sum;       // running sum over this half-wave's keys
+  bool warm;         // every lane of the wave has its reference (wave-uniform)
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) oacc[db][r] = ocor[db][r] = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) negm[r] = 0.f;
+    m_run = thr = -INFINITY;
+    l_sum = 0.f;
+    warm = false;
+  }
+
+  // -inf for the keys past this lane's last one (as an offset in its half's sub-block)
+  __device__ __forceinline__ void apply_mask(floatx16 &sacc, int last_vis) const {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sacc[r] = acc_key(r) <= last_vis ? sacc[r] : -INFINITY;
+  }
+
+  __device__ __forceinline__ void accumulate_pv(const floatx16 &p, const char *vt) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = p[8 * s + e];
+      bf16x8 pp[3];
+      split_operand(x, 1.f, pp);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        bf16x8 v[PC::N];
+#pragma unroll
+        for (int i = 0; i < PC::N; ++i)
+          v[i] = *reinterpret_cast<const bf16x8 *>(vt + i * Tile::VPLANE + s * Tile::VSLAB + db * 256);
+#pragma unroll
+        for (int i = 0; i < PC::PRODUCTS; ++i) {
+          floatx16 &c = i == PC::PRODUCTS - 1 ? oacc[db] : ocor[db];
+          c = mfma32x32x16(v[PC::A[i]], pp[PC::B[i]], c);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ floatx16 scores(const char *kt, const bf16x8 (&q)[NS][3]) const {
+    floatx16 sacc = negm, cor = {};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      bf16x8 k[PC::N];
+#pragma unroll
+      for (int i = 0; i < PC::N; ++i)
+        k[i] = *reinterpret_cast<const bf16x8 *>(kt + i * Tile::KPLANE + s * Tile::KSLAB);
+#pragma unroll
+      for (int i = 0; i < PC::PRODUCTS; ++i) {
+        floatx16 &c = i == PC::PRODUCTS - 1 ? sacc : cor;
+        c = mfma32x32x16(k[PC::A[i]], q[s][PC::B[i]], c);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sacc[r] += cor[r];
+    return sacc;
+  }
+
+  // The common sub-block once every row has its reference: probabilities and their
+  // per-lane sum first; false (nothing changed but sacc) if some lane's sum is above 2^32
+  // or NaN, and the caller takes consume() on recomputed scores.
+  __device__ __forceinline__ bool try_fast(floatx16 &sacc, const char *vt, bool masked, int last_vis) {
+    if (masked) apply_mask(sacc, last_vis);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sacc[r] = fast_exp2(sacc[r]);
+    float s8[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s8[i] = sacc[2 * i] + sacc[2 * i + 1];
+    const float ps = ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
+    if (__builtin_amdgcn_ballot_w64(!(ps <= kFastSumLimit))) return false;
+    l_sum += ps;
+    accumulate_pv(sacc, vt);
+    return true;
+  }
+
+  __device__ __forceinline__ void softmax(floatx16 &sacc, bool masked, int last_vis) {
+    if (masked) apply_mask(sacc, last_vis);
+    const float m0 = max3_scores(sacc[0], sacc[1], sacc[2]);
+    const float m1 = max3_scores(sacc[3], sacc[4], sacc[5]);
+    const float m2 = max3_scores(sacc[6], sacc[7], sacc[8]);
+    const float m3 = max3_scores(sacc[9], sacc[10], sacc[11]);
+    const float m4 = max3_scores(sacc[12], sacc[13], sacc[14]);
+    float smax = max3_scores(max3_scores(m0, m1, m2), max3_scores(m3, m4, sacc[15]), -INFINITY);
+    smax = halves_max(smax);
+    // Lazy rescale: the first visible key sets the reference, later only a rise of more
+    // than the threshold moves it (the scores shift with it).
+    const bool need = smax > thr;
+    if (__builtin_amdgcn_ballot_w64(need)) {
+      const bool first = m_run == -INFINITY;
+      const float shift = need ? smax : 0.f;
+      const float alpha = (need && !first) ? fast_exp2(-smax) : 1.0f;  // o and l are 0 before the first key
+      m_run = need ? (first ? smax : m_run + smax) : m_run;
+      thr = m_run == -INFINITY ? -INFINITY : kRescaleThreshold;
+      const float nref = m_run == -INFINITY ? 0.f : -m_run;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        sacc[r] -= shift;
+        negm[r] = nref;
+      }
+      if (__builtin_amdgcn_ballot_w64(need && !first)) {
+        l_sum *= alpha;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            oacc[db][r] *= alpha;
+            ocor[db][r] *= alpha;
+          }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      sacc[r] = fast_exp2(sacc[r]);
+      l_sum += sacc[r];
+    }
+    warm = !__builtin_amdgcn_ballot_w64(m_run == -INFINITY);
+  }
+
+  // Joins the two accumulators and undoes V's scale; whether some row came out
+  // non-finite (wave-uniform).
+  __device__ __forceinline__ bool finish() {
+    constexpr float unscale = PC::N == 3 ? kSplitUnscale : 1.f;
+    float wrong = l_sum * 0.f;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) oacc[db][r] = (oacc[db][r] + ocor[db][r]) * unscale;
+      wrong = nonfinite_sum(oacc[db], wrong);
+    }
+    return any_nonfinite(wrong);
+  }
+
+  // The wave's rows over keys [c0, c1) on the fp32 MFMA straight from the pages: only for
+  // rows that came out non-finite (common.h) or whose Q is out of the split's range.
+  // Where some row does not see all of a sub-block, V is summed per lane, without the keys
+  // that the lane's row does not see: a product with their probability 0 would let their
+  // infinities and NaNs through.
+  __device__ __forceinline__ void recompute(const PagedArgs &a, const float *qrow, const int *table, int hk, int li,
+                                            int hf, int c0, int c1, int lim, int lim_lo, int last) {
+    init();
+    const int kv_dim = a.kv_heads * a.hd;
+    const T *kb = static_cast<const T *>(a.kc) + (size_t)hk * a.hd, *vb = static_cast<const T *>(a.vc) + (size_t)hk * a.hd;
+#pragma unroll 1
+    for (int kb0 = c0; kb0 < c1; kb0 += 32) {
+      const int key = min(kb0 + li, last);
+      const Slot ks = slot_in(a, table[key >> a.page_shift], key);
+      const T *krow = kb + (size_t)ks.at * kv_dim;
+      floatx16 sacc = negm;
+#pragma unroll 1
+      for (int d = 0; d < HD; d += 2) {
+        const bool in = d + hf < a.hd;
+        sacc = mfma32x32x2(in && ks.ok ? (float)krow[d + hf] : 0.f, in ? qrow[d + hf] * a.scale_log2 : 0.f, sacc);
+      }
+      softmax(sacc, true, lim - kb0 - 4 * hf);
+      const bool whole = kb0 + 31 <= lim_lo;  // (wave-uniform)
+#pragma unroll 1
+      for (int i = 0; i < (whole ? 16 : 32); ++i) {
+        // whole: register i, whose key differs between the half-waves; else key i of the sub-block
+        const int r = whole ? i : (i >> 3) * 4 + (i & 3);
+        const int vk = kb0 + (whole ? acc_key(i) + 4 * hf : i), vkey = min(vk, last);
+        const Slot vs = slot_in(a, table[vkey >> a.page_shift], vkey);
+        const T *vrow = vb + (size_t)vs.at * kv_dim;
+        float p = 0.f;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) p = c == r ? sacc[c] : p;
+        if (whole) {
+#pragma unroll
+          for (int db = 0; db < NDB; ++db)
+            oacc[db] = mfma32x32x2(db * 32 + li < a.hd && vs.ok ? (float)vrow[db * 32 + li] : 0.f, p, oacc[db]);
+        } else {
+          p = __shfl(p, li + 32 * (i >> 2 & 1));
+          if (vk <= lim) {
+#pragma unroll
+            for (int db = 0; db < NDB; ++db)
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                const int d = db * 32 + acc_key(c) + 4 * hf;
+                oacc[db][c] = fmaf(p, d < a.hd && vs.ok ? (float)vrow[d] : 0.f, oacc[db][c]);
+              }
+          }
+        }
+      }
+    }
+  }
+};
+
+// One workgroup: 128 rows of a (request, K/V head) against one chunk of its keys, each
+// wave 32 rows.  Tiles of BN keys are double-buffered in LDS; the next tile's rows are in
+// flight while the current one is consumed.  Workgroup ids: the K/V head runs fastest, so
+// that tiles of one head meet on an XCD where the heads are a multiple of 8; a request's
+// last rows, which see the most keys, come first.
+template <typename T, int HD, int BN, bool VEC>
+__global__ void __launch_bounds__(PT_THREADS, HD <= 32 ? 3 : (HD <= 64 ? 2 : 1)) paged_tile_kernel(const PagedArgs a) {
+  constexpr int NKB = BN / 32;  // 32-key sub-blocks per tile
+  typedef PagedStage<T, HD, BN, VEC> Stage;
+  __shared__ __attribute__((aligned(16))) char lds[2][Stage::BYTES];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int li = lane & 31, hf = lane >> 5;
+  const int hk = blockIdx.x % a.kv_heads, flat = blockIdx.x / a.kv_heads, split = blockIdx.y;
+  // the request that the flat-th tile belongs to, 64 requests at a time
+  int b = -1, tile = 0;
+  for (int b0 = 0, before = 0; b0 < a.batch && b < 0; b0 += 64) {
+    int tiles = 0;
+    if (b0 + lane < a.batch) {
+      const int nr = paged_seq(a, b0 + lane).n * a.group;
+      tiles = nr > a.vec_rows ? (nr + kPagedTileRows - 1) / kPagedTileRows : 0;
+    }
+    int upto = tiles;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int y = __shfl_up(upto, off);
+      if (lane >= off) upto += y;
+    }
+    upto += before;
+    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > flat);
+    if (past) {
+      const int w = __builtin_ctzll(past);
+      b = b0 + w;
+      tile = __builtin_amdgcn_readlane(upto, w) - 1 - flat;  // from the request's last tile
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  if (b < 0) return;
+  b = __builtin_amdgcn_readfirstlane(b);
+  const PagedSeq s = paged_seq(a, b);
+  const int nr = s.n * a.group, base = s.len - s.n;
+  const int r0 = tile * kPagedTileRows, rw0 = r0 + wave * 32;
+  const int kend = base + a.by_group.div(min(r0 + kPagedTileRows, nr) - 1) + 1;
+  const bool single = s.len <= a.tile_chunk;
+  const int c0 = split * a.tile_chunk, c1 = min(c0 + a.tile_chunk, kend);
+  if (c0 >= c1 && !(single && split == 0)) return;
+
+  const int rr = min(rw0 + li, nr - 1), tok = a.by_group.div(rr), head = hk * a.group + rr - tok * a.group;
+  const int lim = base + tok;  // the last key this lane's row sees
+  const int lim_lo = base + a.by_group.div(min(rw0, nr - 1)), lim_hi = base + a.by_group.div(min(rw0 + 31, nr - 1));
+  const float *qrow = a.q + (size_t)(s.first + tok) * a.ldq + (size_t)head * a.hd;
+  PagedRows<T, HD, BN, VEC> rows;
+  rows.init();
+  if (c0 < c1) {
+    Stage st;
+    st.init(a, b, hk, s.len - 1);
+    st.lookup(a, c0);
+    st.load(a, c0);
+    st.lookup(a, c0 + BN);
+    bf16x8 q[HD / 16][3];
+    const bool wide = paged_load_q<HD, VEC>(q, qrow, a.hd, a.scale_log2, hf);
+    st.store(lds[0], a.bad);
+    __syncthreads();
+    const int ko = Stage::koperand(li, hf), vo = Stage::voperand(li, hf);
+    int cur = 0;
+    for (int k0 = c0; k0 < c1; k0 += BN, cur ^= 1) {
+      // (past the last tile the request's last rows are staged once more, unread)
+      st.load(a, k0 + BN);
+      st.lookup(a, k0 + 2 * BN);
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        const int kb0 = k0 + kb * 32;
+        if (kb0 >= c1 || kb0 > lim_hi || rw0 >= nr) continue;
+        const char *kop = lds[cur] + ko + kb * 512, *vop = lds[cur] + vo + 2 * kb * Stage::VSLAB;
+        floatx16 sacc = rows.scores(kop, q);
+        const bool masked = kb0 + 31 > lim_lo;
+        const int last_vis = lim - kb0 - 4 * hf;
+        bool done = false;
+        if (rows.warm) {
+          done = rows.try_fast(sacc, vop, masked, last_vis);
+          if (!done) {
+            // K is read from LDS again (the compiler may not keep the first scores)
+            asm volatile("" ::: "memory");
+            sacc = rows.scores(kop, q);
+          }
+        }
+        if (!done) {
+          rows.softmax(sacc, masked, last_vis);
+          rows.accumulate_pv(sacc, vop);
+        }
+      }
+      st.store(lds[cur ^ 1], a.bad);
+      __syncthreads();
+    }
+    if ((rows.finish() || wide) && rw0 < nr)
+      rows.recompute(a, qrow, a.table + (size_t)b * a.max_blocks, hk, li, hf, c0, min(c1, lim_hi + 1), lim, lim_lo,
+                     s.len - 1);
+  }
+  if (rw0 + li >= nr) return;
+  const float l = halves_sum(rows.l_sum);
+  float *out, f = 1.f;
+  if (single) {
+    out = a.o + (size_t)(s.first + tok) * a.ldo + (size_t)head * a.hd;
+    f = l == 0.f ? 0.f : 1.0f / l;
+  } else {
+    out = a.tile_part + (((size_t)(s.first + tok) * a.heads + head) * a.tile_splits + split) * (a.hd + 2);
+    if (hf == 0) {
+      out[a.hd] = fmaxf(rows.m_run, -3.0e38f);
+      out[a.hd + 1] = l;
+    }
+  }
+#pragma unroll
+  for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = db * 32 + 8 * g + 4 * hf;
+      const vf4 x = {rows.oacc[db][4 * g] * f, rows.oacc[db][4 * g + 1] * f, rows.oacc[db][4 * g + 2] * f,
+                     rows.oacc[db][4 * g + 3] * f};
+      if (VEC && single) {
+        *reinterpret_cast<vf4 *>(out + d) = x;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (d + r < a.hd) out[d + r] = x[r];
+      }
+    }
+}
+
+template <typename T, int HD, bool VEC>
+void launch_rows(const PagedArgs &a, hipStream_t st) {
+  const int most = min(a.vec_rows, a.max_new * a.group);
+  auto grid = [&](int r) { return dim3(a.vec_splits, a.kv_heads * ((most + r - 1) / r), a.batch); };
+  if (most <= 1) paged_rows_kernel<T, HD, 1, VEC><<<grid(1), PR_THREADS, 0, st>>>(a);
+  else if (most <= 2) paged_rows_kernel<T, HD, 2, VEC><<<grid(2), PR_THREADS, 0, st>>>(a);
+  else paged_rows_kernel<T, HD, 4, VEC><<<grid(4), PR_THREADS, 0, st>>>(a);
+}
+
+template <typename T, int HD>
+void launch_rows(const PagedArgs &a, bool wide, hipStream_t st) {
+  if (wide) launch_rows<T, HD, true>(a, st);
+  else launch_rows<T, HD, false>(a, st);
+}
+
+template <typename T, int HD, int BN>
+void launch_tile(const PagedArgs &a, bool wide, hipStream_t st) {
+  const long long tiles = (long long)a.rows * a.group / kPagedTileRows + a.batch;
+  const dim3 grid((unsigned)(tiles * a.kv_heads), a.tile_splits);
+  if (wide) paged_tile_kernel<T, HD, BN, true><<<grid, PT_THREADS, 0, st>>>(a);
+  else paged_tile_kernel<T, HD, BN, false><<<grid, PT_THREADS, 0, st>>>(a);
+}
+
+// wide: head dims of a template and 16-byte aligned rows.
+template <typename T>
+int paged_attn(const PagedArgs &a, bool vec, bool tile, bool wide, hipStream_t st) {
+  if (vec) {
+    if (a.hd <= 32) launch_rows<T, 32>(a, wide, st);
+    else if (a.hd <= 64) launch_rows<T, 64>(a, wide, st);
+    else if (a.hd <= 128) launch_rows<T, 128>(a, wide, st);
+    else launch_rows<T, 256>(a, wide, st);
+    const int rc = check_launch("paged_rows_kernel");
+    if (rc) return rc;
+  }
+  if (tile) {
+    if (a.hd <= 32) launch_tile<T, 32, 32>(a, wide, st);
+    else if (a.hd <= 64) launch_tile<T, 64, 32>(a, wide, st);
+    else launch_tile<T, 128, 32>(a, wide, st);
+    return check_launch("paged_tile_kernel");
+  }
+  return CDML_OK;
+}
+
+}  // namespace
+}  // namespace cdml

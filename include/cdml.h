@@ -593,6 +593,135 @@ int cdml_kv_cache_append(const float *k_new, const float *v_new,
                          float *kcache, float *vcache, const int *positions,
                          int batch, int t_max, int dim, cdml_stream stream);
 
+/* ---- serving from a cache in pages ----------------------------------------
+ * The reference keeps one contiguous K and V array per sequence
+ * (LanguageModel.cs:270-292,356-363) and has no counterpart of the entries
+ * below, which let requests of any lengths share one pool:
+ *   - a layer's cache is kcache and vcache [n_pages, page_size, kv_dim], kv_dim
+ *     = num_kv_heads * head_dim, of CDML_CACHE_* values (a contiguous cache
+ *     [batch, t_max, dim] is one whose pages follow each other);
+ *   - token t of request b lies in slot block_table[b][t / page_size] *
+ *     page_size + t % page_size; block_table is device int32 [batch,
+ *     max_blocks], kv_len (device int32[batch]) the tokens in the cache;
+ *   - page_refs (device int32[n_pages]) counts the requests a page belongs to,
+ *     0 for a free page.  All of them start as zeros.
+ * page_size is a power of two up to 4096, n_pages * page_size < 2^31 and batch
+ * <= 4096.  One step of a model: cdml_paged_plan; in every layer cdml_rope with
+ * the plan's positions, cdml_paged_append, cdml_paged_attn; then, in a beam
+ * search, cdml_beam_select, cdml_paged_reorder and cdml_paged_copy.  All of it
+ * may be captured into a graph: lengths stay on the device. */
+#define CDML_CACHE_F32 0
+#define CDML_CACHE_F16 1
+#define CDML_CACHE_BF16 2
+
+/* Makes room for new_len[b] (device int32, >= 0) more tokens of every request:
+ * takes the pages they need, the lowest free ones in the order of requests and
+ * tokens, into block_table, sets their page_refs to 1 and adds new_len to
+ * kv_len.  The new tokens of all requests follow each other in rows cu_new[b]
+ * .. cu_new[b + 1] (device int32[batch + 1]) of a step's activations; slots and
+ * positions (device int32[rows]) receive each row's cache slot and its position
+ * in its request, -1 and 0 for rows past the last request.
+ * status (device int32[3]): 0 or the sum of 1 (too few free pages), 2 (a
+ * negative length, or one that does not fit max_blocks pages) and 4 (more new
+ * tokens than rows); the pages and the tokens of the step, without requests
+ * that 2 stands for (INT32_MAX if more).  Unless status[0] is 0 nothing is
+ * taken: cu_new is zeros, every slot -1, tables and lengths stay. */
+int cdml_paged_plan(int *page_refs, int n_pages, int page_size,
+                    int *block_table, int max_blocks, int *kv_len,
+                    const int *new_len, int batch, int rows, int *cu_new,
+                    int *slots, int *positions, int *status,
+                    cdml_stream stream);
+
+/* Writes the rows of k_new and v_new (row strides ldk, ldv) to their slots of a
+ * layer's cache, rounded to its type (to nearest even; fp16 overflows to
+ * infinity).  Rows whose slot is outside [0, n_pages * page_size) are left out;
+ * the others' slots must differ from each other. */
+int cdml_paged_append(const float *k_new, int ldk, const float *v_new, int ldv,
+                      void *kcache, void *vcache, int cache_type,
+                      const int *slots, int rows, int n_pages, int page_size,
+                      int kv_dim, cdml_stream stream);
+
+/* Attention of every request's new tokens over its cached ones, its new ones
+ * among them (appended before): rows r = cu_new[b] + i of q (row stride ldq)
+ * and o (ldo), i < n = cu_new[b + 1] - cu_new[b], head h reads K/V head
+ * h / (num_heads / num_kv_heads) and
+ *   o[r] = softmax(scale * q[r] K^T) V over tokens j <= kv_len[b] - n + i.
+ * A row without a token is written as 0; rows of no request stay as they are.
+ * cu_new must not decrease and end within `rows`; max_new and max_len are upper
+ * bounds of n and kv_len (max_len <= max_blocks * page_size) that the launches
+ * are sized by; larger values are cut to them.  A page outside [0, n_pages)
+ * that a row would read counts as zeros; with bad non-NULL (device int32) it is
+ * then set to 1, and never cleared.  What masked or unused slots hold does not
+ * matter, infinities and NaNs included.  head_dim up to 256; up to 128 chunks
+ * run on the matrix cores (above, and for the rows of a few tokens, on the
+ * vector units).  Sums and statistics are fp32 whatever the cache's type.
+ * workspace: 16-byte aligned, cdml_paged_attn_workspace_size bytes of the same
+ * arguments (NULL when that is 0). */
+int cdml_paged_attn_workspace_size(int rows, int batch, int max_new,
+                                   int max_len, int num_heads,
+                                   int num_kv_heads, int head_dim,
+                                   size_t *bytes);
+int cdml_paged_attn(const float *q, int ldq, const void *kcache,
+                    const void *vcache, int cache_type, int n_pages,
+                    int page_size, const int *block_table, int max_blocks,
+                    const int *kv_len, const int *cu_new, float *o, int ldo,
+                    int rows, int batch, int max_new, int max_len,
+                    int num_heads, int num_kv_heads, int head_dim, float scale,
+                    int *bad, void *workspace, size_t workspace_bytes,
+                    cdml_stream stream);
+
+/* Gives every row b of the tables the state of row parents[b] (device
+ * int32[batch]; -1, and any value outside [0, batch), leaves it empty, which
+ * also releases a request): full pages become shared, a page that is not full
+ * stays with the lowest row that takes it, and every other such row gets the
+ * lowest free page, into which cdml_paged_copy has to copy page copy_src[b] to
+ * page copy_dst[b] (device int32[batch], -1 where there is nothing to copy).
+ * Pages that no row holds any more become free, before copies take theirs.
+ * status (device int32[3]): rows that found no free page (their kv_len is cut
+ * to their full pages), copies, parents outside [-1, batch).  workspace: 4-byte
+ * aligned, cdml_paged_reorder_workspace_size bytes. */
+int cdml_paged_reorder_workspace_size(int batch, int max_blocks, size_t *bytes);
+int cdml_paged_reorder(int *page_refs, int n_pages, int page_size,
+                       int *block_table, int max_blocks, int *kv_len,
+                       const int *parents, int batch, int *copy_src,
+                       int *copy_dst, int *status, void *workspace,
+                       size_t workspace_bytes, cdml_stream stream);
+
+/* The copies of a cdml_paged_reorder in `layers` caches that lie layer_stride
+ * elements apart: the first kv_len[b] % page_size tokens of page copy_src[b] go
+ * to page copy_dst[b].  Pages outside [0, n_pages) are left out. */
+int cdml_paged_copy(void *kcache, void *vcache, int cache_type, int layers,
+                    size_t layer_stride, int n_pages, int page_size,
+                    int kv_dim, const int *copy_src, const int *copy_dst,
+                    const int *kv_len, int batch, cdml_stream stream);
+
+/* One step of beam search, the beam counterpart of cdml_argmax_rows: `batch`
+ * requests with `beams` (<= 64) beams each, row b * beams + k of logits [rows,
+ * vocab] (row stride ldl), scores (sum of log-probabilities), lengths (tokens
+ * so far, >= 0) and finished.  A live beam offers every token t with total
+ * score + logit[t] - log(sum of exp(logit)) and length + 1, a finished one
+ * (finished != 0) only eos_token with its score and length unchanged.  The
+ * `beams` largest total / length^length_penalty become the request's next
+ * beams, in that order; equal ones in the order of beams, then tokens.
+ * parents: the row each comes from, for cdml_paged_reorder; tokens; new_scores
+ * / new_lengths / new_finished (1 once the token is eos_token; eos_token < 0:
+ * none is) may be the input arrays.  NaN and -infinite logits are no
+ * candidates; a beam whose score is not finite, or whose largest logit is
+ * +infinity, offers nothing.  Places that no candidate is left for keep their
+ * own row as parent, with score -infinity, finished 1 and token max(eos_token,
+ * 0).  Sums of exponentials and totals are kept in 64 bits, so that the choice
+ * between beams does not hang on their rounding.  workspace: 16-byte aligned,
+ * cdml_beam_select_workspace_size bytes. */
+int cdml_beam_select_workspace_size(int batch, int beams, int vocab,
+                                    size_t *bytes);
+int cdml_beam_select(const float *logits, int ldl, const float *scores,
+                     const int *lengths, const uint8_t *finished, int batch,
+                     int beams, int vocab, int eos_token, float length_penalty,
+                     float *new_scores, int *new_lengths,
+                     uint8_t *new_finished, int *parents, int *tokens,
+                     void *workspace, size_t workspace_bytes,
+                     cdml_stream stream);
+
 /* IAccelerationManager.ResidualLayerNorm (:132), replacing
  * AccelerationCPU.cs:1376-1438: y = gamma * (s - mean) / sqrt(var + eps) + beta
  * with s = a + b per row, biased variance.  a, b, y [rows, features]. */
