@@ -39,6 +39,47 @@ __device__ __forceinline__ float halves_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// A lane's neighbour by a DPP control, without a trip through LDS: quad_perm patterns
+// exchange lane ^ 1 (0xB1) and lane ^ 2 (0x4E); mirrors of 8 (0x141) and 16 lanes (0x140)
+// then pair the uniform quads and groups of 8.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __uint_as_float(dpp<CTRL>(__float_as_uint(x)));
+}
+// f over all 64 lanes, in each of them (f commutative and associative; every lane active).
+template <typename T, typename F>
+__device__ __forceinline__ T wave_reduce(T x, F f) {
+  static_assert(sizeof(T) == 4, "one register");
+  uint32_t w = __builtin_bit_cast(uint32_t, x);
+  auto with = [&](uint32_t o) {
+    w = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(T, w), __builtin_bit_cast(T, o)));
+  };
+  with(dpp<0xB1>(w));
+  with(dpp<0x4E>(w));
+  with(dpp<0x141>(w));
+  with(dpp<0x140>(w));
+  auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  w = r[0];
+  with(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  w = r[0];
+  with(r[1]);
+  return __builtin_bit_cast(T, w);
+}
+__device__ __forceinline__ float wave_max(float x) {
+  return wave_reduce(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  return wave_reduce(x, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ int wave_min(int x) {
+  return wave_reduce(x, [](int a, int b) { return min(a, b); });
+}
+
 // max of three scores.  The scores come from MFMA accumulators and are
 // never signalling NaNs, so the IEEE quieting that fmaxf otherwise adds to
 // each operand is dropped (one v_max3_f32 instead of five instructions).

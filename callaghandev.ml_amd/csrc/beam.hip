@@ -12,7 +12,7 @@
 // n = rint(x log2 e) and f = fma(x, log2 e, -n) (one rounding at 2^-25, whatever x), the
 // product with log2 e's low part added: 2^f is off by one rounding of fp32, and these
 // do not add up over a sum whose terms are independent.
-#include "common.h"
+#include "attn_common.h"
 
 namespace cdml {
 namespace {
@@ -39,12 +39,6 @@ struct BeamArgs {
   float *val;   // [beams] largest logits, -infinity where there are fewer
   int *tok;     // their tokens
 };
-
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off));
-  return x;
-}
 
 // exp(x - m) for m >= x, both finite: as 2^(n - n_m) 2^(f - f_m) while x log2 e has
 // fraction bits, else from the (then exact or huge) difference.

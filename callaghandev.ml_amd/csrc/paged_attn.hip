@@ -6,9 +6,58 @@
 namespace cdml {
 namespace {
 
-// One wave per (row, head): o = sum_s w_s o_s / sum_s w_s l_s with w_s = 2^(m_s - M) over
-// the chunks that hold a visible key.  Rows of one chunk are in o already.
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
+// o = sum_s w_s o_s / sum_s w_s l_s with w_s = 2^(m_s - M) over n chunks, one wave; the
+// chunks' statistics lie one to a lane, 64 chunks at a time.
+__device__ __forceinline__ void join_chunks(const PagedArgs &a, const float *part, int n, float *o) {
+  const int lane = threadIdx.x & 63, stride = a.hd + 2;
+  float M = -3.0e38f;
+  for (int c = lane; c < n; c += 64) M = fmaxf(M, part[(size_t)c * stride + a.hd]);
+  M = wave_max(M);
+  float L = 0.f, acc[4] = {};
+  for (int c0 = 0; c0 < n; c0 += 64) {
+    const float *p = part + (size_t)c0 * stride;
+    const int m = min(n - c0, 64);
+    const float w = lane < m ? fast_exp2(p[(size_t)lane * stride + a.hd] - M) : 0.f;
+    L += lane < m ? p[(size_t)lane * stride + a.hd + 1] * w : 0.f;
+    constexpr int U = 8;  // chunks in flight; past the last one it is read again and left out
+    for (int c = 0; c < m; c += U) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (lane + 64 * j >= a.hd) continue;
+        float x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = p[(size_t)min(c + u, m - 1) * stride + lane + 64 * j];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float wc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), min(c + u, m - 1)));
+          acc[j] = c + u < m ? fmaf(x[u], wc, acc[j]) : acc[j];
+        }
+      }
+    }
+  }
+  L = wave_sum(L);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (lane + 64 * j < a.hd) o[lane + 64 * j] = L == 0.f ? 0.f : acc[j] / L;
+}
+
+__device__ __forceinline__ int chunks_seen(int seen, int chunk) { return seen <= 0 ? 0 : (seen - 1) / chunk + 1; }
+
+// A wave per (new token, head) of the requests that ran on the vector units.
+__global__ void __launch_bounds__(256) paged_join_rows_kernel(const PagedArgs a, int tokens) {
+  const int b = blockIdx.x / tokens, i = blockIdx.x - b * tokens;
+  const int h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (h >= a.heads) return;
+  const PagedSeq s = paged_seq(a, b);
+  if (i >= s.n || s.n * a.group > a.vec_rows || s.len <= a.vec_chunk) return;
+  const int hk = a.by_group.div(h), rr = i * a.group + h - hk * a.group;
+  join_chunks(a, a.vec_part + (((size_t)b * a.kv_heads + hk) * a.vec_rows + rr) * a.vec_splits * (a.hd + 2),
+              chunks_seen(s.len - s.n + i + 1, a.vec_chunk),
+              a.o + (size_t)(s.first + i) * a.ldo + (size_t)h * a.hd);
+}
+
+// A wave per (row, head) of the requests that ran on the matrix cores.
+__global__ void __launch_bounds__(256) paged_join_tiles_kernel(const PagedArgs a) {
   const int row = blockIdx.x, lane = threadIdx.x & 63;
   const int h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (h >= a.heads) return;
@@ -22,31 +71,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
   if (b >= a.batch) return;
   const PagedSeq s = paged_seq(a, b);
   const int i = row - s.first;
-  if (i < 0 || i >= s.n) return;
-  const bool vec = s.n * a.group <= a.vec_rows;
-  const int chunk = vec ? a.vec_chunk : a.tile_chunk, seen = s.len - s.n + i + 1;
-  if (s.len <= chunk) return;
-  const int n = seen <= 0 ? 0 : (seen - 1) / chunk + 1, hk = a.by_group.div(h), stride = a.hd + 2;
-  const float *part =
-      vec ? a.vec_part + (((size_t)b * a.kv_heads + hk) * a.vec_rows + i * a.group + h - hk * a.group) * a.vec_splits * stride
-          : a.tile_part + ((size_t)row * a.heads + h) * a.tile_splits * stride;
-  float M = -3.0e38f;
-  for (int c = lane; c < n; c += 64) M = fmaxf(M, part[(size_t)c * stride + a.hd]);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off));
-  float L = 0.f, acc[4] = {};
-  for (int c = 0; c < n; ++c) {
-    const float *p = part + (size_t)c * stride;
-    const float w = fast_exp2(p[a.hd] - M);
-    L = fmaf(p[a.hd + 1], w, L);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (lane + 64 * j < a.hd) acc[j] = fmaf(p[lane + 64 * j], w, acc[j]);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (lane + 64 * j < a.hd)
-      a.o[(size_t)row * a.ldo + (size_t)h * a.hd + lane + 64 * j] = L == 0.f ? 0.f : acc[j] / L;
+  if (i < 0 || i >= s.n || s.n * a.group <= a.vec_rows || s.len <= a.tile_chunk) return;
+  join_chunks(a, a.tile_part + ((size_t)row * a.heads + h) * a.tile_splits * (a.hd + 2),
+              chunks_seen(s.len - s.n + i + 1, a.tile_chunk), a.o + (size_t)row * a.ldo + (size_t)h * a.hd);
 }
 
 // Which kernels run and how keys are split, from the sizes alone.
@@ -83,7 +110,7 @@ Plan make_plan(int rows, int batch, int max_new, int max_len, int heads, int kv_
   Plan p{};
   const int group = heads / kv_heads, most = max_new * group, len = max_len < 1 ? 1 : max_len;
   p.tile = hd <= 128 && most > kVecRows;
-  p.vec = true;
+  p.vec = !p.tile || group <= kVecRows;
   p.vec_rows = p.tile ? kVecRows : most < 1 ? 1 : most;
   // vector units: 512 keys a workgroup while there are four workgroups for every CU,
   // else 256; rows without number (head dims above 128) are not split
@@ -95,7 +122,7 @@ Plan make_plan(int rows, int batch, int max_new, int max_len, int heads, int kv_
     p.vec_chunk = wide >= 4 * kComputeUnits ? 512 : 256;
   }
   p.vec_splits = (len - 1) / p.vec_chunk + 1;
-  if (p.vec_splits > 1) p.vec_floats = (size_t)batch * kv_heads * p.vec_rows * p.vec_splits * (hd + 2);
+  if (p.vec && p.vec_splits > 1) p.vec_floats = (size_t)batch * kv_heads * p.vec_rows * p.vec_splits * (hd + 2);
   // matrix cores: keys are split where the tiles alone leave CUs without work
   p.tile_chunk = INT_MAX;
   p.tile_splits = 1;
@@ -191,7 +218,17 @@ extern "C" int cdml_paged_attn(const float *q, int ldq, const void *kcache, cons
   if (cache_type == CDML_CACHE_F32) rc = paged_attn_f32(a, p.vec, p.tile, wide, st);
   else if (cache_type == CDML_CACHE_F16) rc = paged_attn_f16(a, p.vec, p.tile, wide, st);
   else rc = paged_attn_bf16(a, p.vec, p.tile, wide, st);
-  if (rc || (p.vec_splits == 1 && p.tile_splits == 1)) return rc;
-  paged_join_kernel<<<dim3(rows, (num_heads + 3) / 4), 256, 0, st>>>(a);
-  return check_launch("paged_join_kernel");
+  if (rc) return rc;
+  const unsigned by_head = (unsigned)(num_heads + 3) / 4;
+  if (p.vec_floats) {
+    const int tokens = p.vec_rows / a.group;  // of a request on the vector units, at most
+    paged_join_rows_kernel<<<dim3(batch * tokens, by_head), 256, 0, st>>>(a, tokens);
+    rc = check_launch("paged_join_rows_kernel");
+    if (rc) return rc;
+  }
+  if (p.tile_floats) {
+    paged_join_tiles_kernel<<<dim3(rows, by_head), 256, 0, st>>>(a);
+    rc = check_launch("paged_join_tiles_kernel");
+  }
+  return rc;
 }

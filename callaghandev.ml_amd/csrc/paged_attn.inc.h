@@ -28,12 +28,7 @@ __device__ __forceinline__ float half_value(uint32_t w, int i, __bf16) {
 
 constexpr int PR_THREADS = 256;
 
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
-}
-// Sum over groups of LPK (8 or 16) neighbouring lanes, in each of them: exchanges with
-// lane ^ 1, ^ 2, then the mirrored lane of 8 and of 16.
+// Sum over groups of LPK (8 or 16) neighbouring lanes, in each of them.
 template <int LPK>
 __device__ __forceinline__ float lanes_sum(float x) {
   x += dpp<0xB1>(x);
@@ -289,9 +284,16 @@ __device__ __forceinline__ Slot slot_in(const PagedArgs &a, int page, int key) {
 //   V: slab s holds keys 16 s .. 16 s + 15 of every dim: rows are dims, in four clusters
 //      by d % 4.  A unit is four dims of two keys; key k of a slab sits at place
 //      8 (k / 4 % 2) + 4 (k / 8) + k % 4, the order the P.V product reads.
-// The pages of a tile are looked up a tile ahead of its rows.  Keys past the request's
-// last read that one: their scores are masked and their probabilities exactly 0.
-template <typename T, int HD, int BN, bool VEC>
+// The pages of a tile are looked up a tile ahead of its rows.  What masked keys hold never
+// matters to the scores; V's rows past the request's last key are staged as zeros, for the
+// probabilities that they meet are exactly 0.
+//   UNI (16-byte aligned rows, pages of 16 keys or more): the 16 keys of a block lie in one
+//      page and a wave's load touches one block, so a load's address is a scalar base plus
+//      an offset that the lane keeps throughout.  Lane l holds the base of block l of 64
+//      (1024 keys); a tile reads its blocks' from there.  Looking every row's page up
+//      instead costs some 50 vector instructions a tile, every block's a chain of 40 scalar
+//      ones ahead of the tile's loads.
+template <typename T, int HD, int BN, bool VEC, bool UNI>
 struct PagedStage {
   typedef typename Raw4<T>::type Raw;
   static constexpr int NP = Pieces<T>::N;
@@ -302,74 +304,144 @@ struct PagedStage {
   static constexpr int BYTES = NP * (KPLANE + VPLANE);   // K planes, then V planes
   static constexpr int VU = (HD / 4) * (BN / 2) / HALF;  // V units per thread; twice as many K units
   static constexpr int NV = 2 * VU;                      // loads of either
+  static constexpr int NB = BN / 16;                     // blocks of 16 keys
   static_assert(VU >= 1 && (HD / 4) * (BN / 2) % HALF == 0, "tile units");
   static __device__ __forceinline__ constexpr int kcluster(int c) { return c * (KROWB + 16); }
   static __device__ __forceinline__ constexpr int vcluster(int c) {
     return c * VROWB + (c & 1) * 16 + (c >> 1) * 128;
   }
   static constexpr int CH = HD / 4, KSTEP = HALF / CH;
+  static_assert(16 % KSTEP == 0, "a K load stays in a block of 16 keys");
   static __device__ __forceinline__ constexpr int vgroups(int i) { return HALF / 8 * i % CH; }
   static __device__ __forceinline__ constexpr int vslabs(int i) { return HALF / 8 * i / CH; }
   Raw r[NV];
-  int page[NV];  // of the next tile's rows
-  uint32_t zero;  // bit i: load i's page is none
-  const T *base;  // of this thread's columns
+  int page[UNI ? 1 : NV];  // UNI: lane's block in the next 64, else of the next tile's rows
+  uint32_t base_lo, base_hi;  // UNI: the lane's block in these 64
+  uint64_t none;              // UNI: those whose page is none
+  int group;                  // UNI: first key of these 64 blocks
+  uint32_t zero;              // bit i: load i's page is none
+  const T *base;            // the head's columns (UNI), this thread's columns
   const int *table;
   int col, row, dst;  // first column, first row in a tile, LDS byte offset of the first unit
+  int slab;           // V: the first unit's block (wave-uniform)
+  int loaded;         // first key of the tile in r
   int kv_dim, last;   // the request's last key
   bool kside;
 
   __device__ __forceinline__ void init(const PagedArgs &a, int b, int hk, int last_key) {
-    kside = __builtin_amdgcn_readfirstlane(threadIdx.x) >= HALF;
+    const int t0 = __builtin_amdgcn_readfirstlane(threadIdx.x);
+    kside = t0 >= HALF;
     const int t = threadIdx.x & (HALF - 1);
     // K: the P keys of one load instruction share a cluster
     constexpr int P = 64 / CH;
     const int c = t % CH, j = t / CH, kkey = (j & ~(2 * P - 1)) | ((j & (P - 1)) << 1) | ((j / P) & 1);
-    const int sb = t & 7, g = (t >> 3) % CH, slab = (t >> 3) / CH;
+    const int sb = t & 7, g = (t >> 3) % CH;
+    slab = ((t0 & (HALF - 1)) >> 3) / CH;
     const int place = ((sb >> 1) & 1) * 4 + (sb >> 2) * 2 + (sb & 1);  // of V's key pair
     col = kside ? 4 * c : 4 * g;
-    row = kside ? kkey : 16 * slab + 2 * sb;
+    row = kside ? kkey : 2 * sb + (UNI ? 0 : 16 * slab);
     dst = kside ? (c >> 2) * KSLAB + kcluster(kkey & 1) + (kkey >> 1) * 32 + (c & 3) * 8
                 : NP * KPLANE + slab * VSLAB + g * 32 + place * 4;
-    base = static_cast<const T *>(kside ? a.kc : a.vc) + (size_t)hk * a.hd + col;
+    base = static_cast<const T *>(kside ? a.kc : a.vc) + (size_t)hk * a.hd + (UNI ? 0 : col);
     table = a.table + (size_t)b * a.max_blocks;
     kv_dim = a.kv_heads * a.hd;
     last = last_key;
   }
-  __device__ __forceinline__ int key(int k0, int i) const {
-    return min(k0 + row + (kside ? KSTEP * i : 16 * vslabs(i / 2) + (i & 1)), last);
+  // Load i's row in the tile, without the lane's part
+  __device__ __forceinline__ int row_of(int i) const {
+    return kside ? KSTEP * i : 16 * vslabs(i / 2) + (i & 1);
+  }
+  // UNI: the block of a tile that load i lies in
+  __device__ __forceinline__ int block_of(int i) const {
+    return kside ? KSTEP * i / 16 : slab + vslabs(i / 2);
+  }
+  __device__ __forceinline__ int key(int k0, int i) const { return min(k0 + row + row_of(i), last); }
+  // UNI: pages of the 64 blocks from key k0 on, one to a lane
+  __device__ __forceinline__ int page_of_block(const PagedArgs &a, int k0) const {
+    return table[min(k0 + 16 * (int)(threadIdx.x & 63), last) >> a.page_shift];
+  }
+  __device__ __forceinline__ void start_group(const PagedArgs &a, int k0) {
+    const int mine = k0 + 16 * (int)(threadIdx.x & 63);
+    const Slot s = slot_in(a, page[0], mine);
+    const uint64_t at = reinterpret_cast<uint64_t>(base + (size_t)s.at * kv_dim);
+    base_lo = (uint32_t)at;
+    base_hi = (uint32_t)(at >> 32);
+    none = __builtin_amdgcn_ballot_w64(!s.ok);
+    group = k0;
+    page[0] = page_of_block(a, k0 + 1024);
+  }
+  // What load() of the first tile needs; then, after each load, of the next.
+  __device__ __forceinline__ void lookup_first(const PagedArgs &a, int k0) {
+    if constexpr (UNI) {
+      page[0] = page_of_block(a, k0);
+      start_group(a, k0);
+    } else {
+      lookup(a, k0);
+    }
   }
   __device__ __forceinline__ void lookup(const PagedArgs &a, int k0) {
+    if constexpr (!UNI) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) page[i] = table[key(k0, i) >> a.page_shift];
+      for (int i = 0; i < NV; ++i) page[i] = table[key(k0, i) >> a.page_shift];
+    }
   }
 
   __device__ __forceinline__ void load(const PagedArgs &a, int k0) {
-    zero = 0;
+    loaded = k0;
+    if constexpr (UNI) {
+      if (k0 - group >= 1024) start_group(a, k0);
+      const int first = (k0 - group) >> 4;
+      zero = (uint32_t)(none >> first) & ((1u << NB) - 1);  // (a tile's blocks lie in one group)
+      const char *block[NB];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const Slot s = slot_in(a, page[i], key(k0, i));
-      if (!s.ok) zero |= 1u << i;
-      const int dc = kside ? 0 : 4 * vgroups(i / 2);
-      const T *p = base + (size_t)s.at * kv_dim + dc;
-      if constexpr (VEC) {
-        r[i] = *reinterpret_cast<const Raw *>(p);
-      } else if constexpr (sizeof(T) == 4) {
+      for (int i = 0; i < NB; ++i)
+        block[i] = reinterpret_cast<const char *>((uint64_t)(uint32_t)__builtin_amdgcn_readlane(base_hi, first + i) << 32 |
+                                                  (uint32_t)__builtin_amdgcn_readlane(base_lo, first + i));
+      const uint32_t off = (uint32_t)(row * kv_dim + col) * (uint32_t)sizeof(T);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) r[i][c] = col + dc + c < a.hd ? (float)p[c] : 0.f;
-      } else {
+      for (int i = 0; i < NV; ++i) {
+        const char *p = nullptr;
+        const int at = block_of(i);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t lo = col + dc + 2 * c < a.hd ? __builtin_bit_cast(uint16_t, p[2 * c]) : 0;
-          const uint32_t hi = col + dc + 2 * c + 1 < a.hd ? __builtin_bit_cast(uint16_t, p[2 * c + 1]) : 0;
-          r[i][c] = lo | hi << 16;
+        for (int c = 0; c < NB; ++c)
+          if (at == c) p = block[c];
+        p += (size_t)(kside ? KSTEP * i % 16 : (i & 1)) * kv_dim * sizeof(T) + (kside ? 0 : 4 * vgroups(i / 2)) * sizeof(T);
+        r[i] = *reinterpret_cast<const Raw *>(p + off);
+      }
+    } else {
+      zero = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const Slot s = slot_in(a, page[i], key(k0, i));
+        if (!s.ok) zero |= 1u << i;
+        const int dc = kside ? 0 : 4 * vgroups(i / 2);
+        const T *p = base + (size_t)s.at * kv_dim + dc;
+        if constexpr (VEC) {
+          r[i] = *reinterpret_cast<const Raw *>(p);
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) r[i][c] = col + dc + c < a.hd ? (float)p[c] : 0.f;
+        } else {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t lo = col + dc + 2 * c < a.hd ? __builtin_bit_cast(uint16_t, p[2 * c]) : 0;
+            const uint32_t hi = col + dc + 2 * c + 1 < a.hd ? __builtin_bit_cast(uint16_t, p[2 * c + 1]) : 0;
+            r[i][c] = lo | hi << 16;
+          }
         }
       }
     }
   }
 
   __device__ __forceinline__ void store(char *lds, int *bad) {
-    if (__builtin_amdgcn_ballot_w64(zero != 0)) {
+    if constexpr (UNI) {
+      if (zero || loaded + BN - 1 > last) {  // (wave-uniform)
+        if (zero && bad) *bad = 1;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if ((zero >> block_of(i) & 1) || (!kside && loaded + 16 * slab + row + row_of(i) > last)) r[i] = Raw{};
+      }
+    } else if (__builtin_amdgcn_ballot_w64(zero != 0)) {
       if (zero && bad) *bad = 1;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -465,15 +537,20 @@ __device__ __forceinline__ bool paged_load_q(bf16x8 (&q)[HD / 16][3], const floa
 
 // The online softmax of one wave's 32 rows (one per lane % 32) over 32-key sub-blocks:
 // S^T = K Q^T puts one row per lane, O^T += V^T P^T consumes the probabilities in place.
-template <typename T, int HD, int BN, bool VEC>
+template <typename T, int HD, int BN, bool VEC, bool UNI>
 struct PagedRows {
-  typedef PagedStage<T, HD, BN, VEC> Tile;
+  typedef PagedStage<T, HD, BN, VEC, UNI> Tile;
   typedef Pieces<T> PC;
   static constexpr int NDB = HD / 32;  // 32-wide head-dim blocks of O^T
   static constexpr int NS = HD / 16;   // MFMA k-steps of Q.K
-  floatx16 oacc[NDB], ocor[NDB];       // the main product, and its corrections
+  // LEAN (head dims above 64): one accumulator for all products, the corrections before
+  // the main one, and the reference subtracted from finished scores: 96 registers less,
+  // which lets two workgroups share a CU.  A sum of 16 products is then rounded 2 *
+  // PRODUCTS times, as often as on the fp32 MFMA or less.
+  static constexpr bool LEAN = HD > 64;
+  floatx16 oacc[NDB], ocor[LEAN ? 1 : NDB];  // the main product, and its corrections
   // -m_run in all 16 entries, what a block's scores start from (0 until the first
-  // visible key sets m_run): scores come out relative to the reference.
+  // visible key sets m_run): scores come out relative to the reference.  LEAN: one.
   floatx16 negm;
   float m_run, thr;  // thr: rescale threshold, any visible key until m_run is set
   float l_sum;       // running sum over this half-wave's keys
@@ -483,7 +560,7 @@ struct PagedRows {
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) oacc[db][r] = ocor[db][r] = 0.f;
+      for (int r = 0; r < 16; ++r) oacc[db][r] = ocor[LEAN ? 0 : db][r] = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) negm[r] = 0.f;
     m_run = thr = -INFINITY;
@@ -513,7 +590,7 @@ struct PagedRows {
           v[i] = *reinterpret_cast<const bf16x8 *>(vt + i * Tile::VPLANE + s * Tile::VSLAB + db * 256);
 #pragma unroll
         for (int i = 0; i < PC::PRODUCTS; ++i) {
-          floatx16 &c = i == PC::PRODUCTS - 1 ? oacc[db] : ocor[db];
+          floatx16 &c = LEAN || i == PC::PRODUCTS - 1 ? oacc[db] : ocor[LEAN ? 0 : db];
           c = mfma32x32x16(v[PC::A[i]], pp[PC::B[i]], c);
         }
       }
@@ -521,7 +598,8 @@ struct PagedRows {
   }
 
   __device__ __forceinline__ floatx16 scores(const char *kt, const bf16x8 (&q)[NS][3]) const {
-    floatx16 sacc = negm, cor = {};
+    floatx16 sacc = {}, cor = {};
+    if constexpr (!LEAN) sacc = negm;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       bf16x8 k[PC::N];
@@ -530,12 +608,12 @@ struct PagedRows {
         k[i] = *reinterpret_cast<const bf16x8 *>(kt + i * Tile::KPLANE + s * Tile::KSLAB);
 #pragma unroll
       for (int i = 0; i < PC::PRODUCTS; ++i) {
-        floatx16 &c = i == PC::PRODUCTS - 1 ? sacc : cor;
+        floatx16 &c = LEAN || i == PC::PRODUCTS - 1 ? sacc : cor;
         c = mfma32x32x16(k[PC::A[i]], q[s][PC::B[i]], c);
       }
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sacc[r] += cor[r];
+    for (int r = 0; r < 16; ++r) sacc[r] += LEAN ? negm[0] : cor[r];
     return sacc;
   }
 
@@ -587,7 +665,7 @@ struct PagedRows {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             oacc[db][r] *= alpha;
-            ocor[db][r] *= alpha;
+            if (!LEAN) ocor[LEAN ? 0 : db][r] *= alpha;
           }
       }
     }
@@ -607,7 +685,7 @@ struct PagedRows {
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) oacc[db][r] = (oacc[db][r] + ocor[db][r]) * unscale;
+      for (int r = 0; r < 16; ++r) oacc[db][r] = (LEAN ? oacc[db][r] : oacc[db][r] + ocor[LEAN ? 0 : db][r]) * unscale;
       wrong = nonfinite_sum(oacc[db], wrong);
     }
     return any_nonfinite(wrong);
@@ -628,7 +706,9 @@ struct PagedRows {
       const int key = min(kb0 + li, last);
       const Slot ks = slot_in(a, table[key >> a.page_shift], key);
       const T *krow = kb + (size_t)ks.at * kv_dim;
-      floatx16 sacc = negm;
+      floatx16 sacc;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sacc[r] = negm[LEAN ? 0 : r];
 #pragma unroll 1
       for (int d = 0; d < HD; d += 2) {
         const bool in = d + hf < a.hd;
@@ -672,10 +752,10 @@ struct PagedRows {
 // flight while the current one is consumed.  Workgroup ids: the K/V head runs fastest, so
 // that tiles of one head meet on an XCD where the heads are a multiple of 8; a request's
 // last rows, which see the most keys, come first.
-template <typename T, int HD, int BN, bool VEC>
-__global__ void __launch_bounds__(PT_THREADS, HD <= 32 ? 3 : (HD <= 64 ? 2 : 1)) paged_tile_kernel(const PagedArgs a) {
+template <typename T, int HD, int BN, bool VEC, bool UNI>
+__global__ void __launch_bounds__(PT_THREADS, HD <= 32 ? 3 : (HD <= 64 || sizeof(T) == 2 ? 2 : 1)) paged_tile_kernel(const PagedArgs a) {
   constexpr int NKB = BN / 32;  // 32-key sub-blocks per tile
-  typedef PagedStage<T, HD, BN, VEC> Stage;
+  typedef PagedStage<T, HD, BN, VEC, UNI> Stage;
   __shared__ __attribute__((aligned(16))) char lds[2][Stage::BYTES];
 
   const int lane = threadIdx.x & 63;
@@ -719,12 +799,12 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 32 ? 3 : (HD <= 64 ? 2 : 1))
   const int lim = base + tok;  // the last key this lane's row sees
   const int lim_lo = base + a.by_group.div(min(rw0, nr - 1)), lim_hi = base + a.by_group.div(min(rw0 + 31, nr - 1));
   const float *qrow = a.q + (size_t)(s.first + tok) * a.ldq + (size_t)head * a.hd;
-  PagedRows<T, HD, BN, VEC> rows;
+  PagedRows<T, HD, BN, VEC, UNI> rows;
   rows.init();
   if (c0 < c1) {
     Stage st;
     st.init(a, b, hk, s.len - 1);
-    st.lookup(a, c0);
+    st.lookup_first(a, c0);
     st.load(a, c0);
     st.lookup(a, c0 + BN);
     bf16x8 q[HD / 16][3];
@@ -815,8 +895,11 @@ template <typename T, int HD, int BN>
 void launch_tile(const PagedArgs &a, bool wide, hipStream_t st) {
   const long long tiles = (long long)a.rows * a.group / kPagedTileRows + a.batch;
   const dim3 grid((unsigned)(tiles * a.kv_heads), a.tile_splits);
-  if (wide) paged_tile_kernel<T, HD, BN, true><<<grid, PT_THREADS, 0, st>>>(a);
-  else paged_tile_kernel<T, HD, BN, false><<<grid, PT_THREADS, 0, st>>>(a);
+  // offsets inside 16 rows of a page fit 32 bits
+  const bool uni = a.page_shift >= 4 && (long long)a.kv_heads * a.hd < (1 << 24);
+  if (wide && uni) paged_tile_kernel<T, HD, BN, true, true><<<grid, PT_THREADS, 0, st>>>(a);
+  else if (wide) paged_tile_kernel<T, HD, BN, true, false><<<grid, PT_THREADS, 0, st>>>(a);
+  else paged_tile_kernel<T, HD, BN, false, false><<<grid, PT_THREADS, 0, st>>>(a);
 }
 
 // wide: head dims of a template and 16-byte aligned rows.
