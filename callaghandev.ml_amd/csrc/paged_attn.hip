@@ -212,8 +212,8 @@ extern "C" int cdml_paged_attn(const float *q, int ldq, const void *kcache, cons
   a.tile_splits = p.tile_splits;
   a.vec_part = static_cast<float *>(workspace);
   a.tile_part = a.vec_part + p.vec_floats;
-  const bool wide = (head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256) && ldq % 4 == 0 &&
-                    ldo % 4 == 0 && aligned16(q) && aligned16(o) && aligned16(kcache) && aligned16(vcache);
+  const bool wide = head_dim % 8 == 0 && ldq % 4 == 0 && ldo % 4 == 0 && aligned16(q) && aligned16(o) &&
+                    aligned16(kcache) && aligned16(vcache);
   const hipStream_t st = as_hip(stream);
   if (cache_type == CDML_CACHE_F32) rc = paged_attn_f32(a, p.vec, p.tile, wide, st);
   else if (cache_type == CDML_CACHE_F16) rc = paged_attn_f16(a, p.vec, p.tile, wide, st);

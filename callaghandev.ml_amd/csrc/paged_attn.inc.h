@@ -38,8 +38,12 @@ __device__ __forceinline__ float lanes_sum(float x) {
   return x;
 }
 
+// How rows are read: value by value (any head dim, any alignment), in 16-byte aligned
+// vectors, or in vectors of which a lane's past the head dim (a multiple of 8) are zeros.
+enum { kScalar = 0, kVector = 1, kVectorCut = 2 };
+
 // A lane's EPL values of one cached row: NV loads of VW values, LPK * VW apart.
-template <typename T, int VW, int NV, int LPK, bool VEC>
+template <typename T, int VW, int NV, int LPK, int MODE>
 struct RowSlice {
   static constexpr int WORDS = VW * NV * (int)sizeof(T) / 4;
   static_assert(VW * sizeof(T) % 4 == 0, "whole words");
@@ -49,9 +53,12 @@ struct RowSlice {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       constexpr int LW = WORDS / NV;  // words per load
-      if constexpr (VEC) {
+      if constexpr (MODE != kScalar) {
         typedef uint32_t V __attribute__((ext_vector_type(LW)));
-        if constexpr (LW == 1) {
+        if (MODE == kVectorCut && d0 + LPK * VW * i >= hd) {
+#pragma unroll
+          for (int c = 0; c < LW; ++c) w[i * LW + c] = 0;
+        } else if constexpr (LW == 1) {
           w[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p + LPK * VW * i));
         } else {
           const V t = __builtin_nontemporal_load(reinterpret_cast<const V *>(p + LPK * VW * i));
@@ -83,15 +90,17 @@ struct RowSlice {
 // One workgroup: R rows of a (request, K/V head) against one chunk of its keys; a cached
 // row goes through LPK lanes, its score through their sum, and every group of LPK lanes
 // keeps an online softmax of its own keys.  The four waves take 64 / LPK keys in turn.
-// Two sets of rows alternate, so that a step's loads are in flight while the step before
-// it is consumed.
-template <typename T, int HD, int R, bool VEC>
+// U sets of rows go round, so that the loads of U - 1 steps are in flight while one is
+// consumed: four where 64 registers hold them (8 x 2048 keys of bf16, 16 heads of 64: U2_US ->
+// U4_US us).
+template <typename T, int HD, int R, int MODE>
 __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedArgs a) {
   constexpr int LPK = HD >= 64 && R > 2 ? 16 : 8;
   constexpr int EPL = HD / LPK;                                              // values per lane
   constexpr int VW = EPL * sizeof(T) >= 16 ? 16 / (int)sizeof(T) : EPL;      // per load
   constexpr int NV = EPL / VW, KPS = 64 / LPK;
-  typedef RowSlice<T, VW, NV, LPK, VEC> Slice;
+  typedef RowSlice<T, VW, NV, LPK, MODE> Slice;
+  constexpr int U = Slice::WORDS <= 8 ? 4 : 2;
   constexpr float kNone = -3.0e38f;  // below every score that matters, and exp2 of it is 0
   __shared__ int pages[kPagedSub + 1];
   __shared__ float red_m[4][R], red_l[4][R];
@@ -123,7 +132,7 @@ __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedArgs 
 #pragma unroll
     for (int e = 0; e < EPL; ++e) {
       const int d = d0 + LPK * VW * (e / VW) + e % VW;
-      q[r][e] = VEC || d < a.hd ? qr[d] * a.scale_log2 : 0.f;
+      q[r][e] = MODE == kVector || d < a.hd ? qr[d] * a.scale_log2 : 0.f;
       o[r][e] = 0.f;
     }
     m[r] = kNone;
@@ -178,15 +187,17 @@ __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedArgs 
         }
       }
     };
-    Slice k0, v0, k1, v1;
+    Slice k[U], v[U];
     const int key0 = sub + wave * KPS + g, steps = (end - sub + 4 * KPS - 1) / (4 * KPS);
-    fetch(key0, k0, v0);
-    for (int it = 0; it < steps; it += 2) {
-      const int key = key0 + it * 4 * KPS;
-      fetch(key + 4 * KPS, k1, v1);
-      step(key, k0, v0);
-      fetch(key + 8 * KPS, k0, v0);
-      step(key + 4 * KPS, k1, v1);
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u) fetch(key0 + u * 4 * KPS, k[u], v[u]);
+    for (int it = 0; it < steps; it += U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int key = key0 + (it + u) * 4 * KPS;
+        fetch(key + (U - 1) * 4 * KPS, k[(u + U - 1) % U], v[(u + U - 1) % U]);
+        step(key, k[u], v[u]);
+      }
     }
   }
 
@@ -397,7 +408,13 @@ struct PagedStage {
       for (int i = 0; i < NB; ++i)
         block[i] = reinterpret_cast<const char *>((uint64_t)(uint32_t)__builtin_amdgcn_readlane(base_hi, first + i) << 32 |
                                                   (uint32_t)__builtin_amdgcn_readlane(base_lo, first + i));
-      const uint32_t off = (uint32_t)(row * kv_dim + col) * (uint32_t)sizeof(T);
+      // (columns past the head dim read its last four again: Q is 0 there, and what they
+      // give O is not stored)
+      static_assert(vgroups(1) == 0 || vgroups(2) == 0, "two column offsets");
+      uint32_t off[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        off[i] = (uint32_t)(row * kv_dim + min(col + 4 * vgroups(i), a.hd - 4)) * (uint32_t)sizeof(T);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const char *p = nullptr;
@@ -405,8 +422,8 @@ struct PagedStage {
 #pragma unroll
         for (int c = 0; c < NB; ++c)
           if (at == c) p = block[c];
-        p += (size_t)(kside ? KSTEP * i % 16 : (i & 1)) * kv_dim * sizeof(T) + (kside ? 0 : 4 * vgroups(i / 2)) * sizeof(T);
-        r[i] = *reinterpret_cast<const Raw *>(p + off);
+        p += (size_t)(kside ? KSTEP * i % 16 : (i & 1)) * kv_dim * sizeof(T);
+        r[i] = *reinterpret_cast<const Raw *>(p + off[kside ? 0 : vgroups(i / 2) != 0]);
       }
     } else {
       zero = 0;
@@ -417,7 +434,7 @@ struct PagedStage {
         const int dc = kside ? 0 : 4 * vgroups(i / 2);
         const T *p = base + (size_t)s.at * kv_dim + dc;
         if constexpr (VEC) {
-          r[i] = *reinterpret_cast<const Raw *>(p);
+          r[i] = *reinterpret_cast<const Raw *>(p + min(0, a.hd - 4 - col - dc));
         } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) r[i][c] = col + dc + c < a.hd ? (float)p[c] : 0.f;
@@ -517,7 +534,7 @@ __device__ __forceinline__ bool paged_load_q(bf16x8 (&q)[HD / 16][3], const floa
     for (int e = 0; e < 8; e += 4) {
       const int d = 16 * s + 8 * hf + e;
       if constexpr (VEC) {
-        const vf4 t = *reinterpret_cast<const vf4 *>(qrow + d);
+        const vf4 t = d < hd ? *reinterpret_cast<const vf4 *>(qrow + d) : vf4{};
 #pragma unroll
         for (int c = 0; c < 4; ++c) x[e + c] = t[c] * scale;
       } else {
@@ -867,7 +884,7 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 32 ? 3 : (HD <= 64 || sizeof
       const vf4 x = {rows.oacc[db][4 * g] * f, rows.oacc[db][4 * g + 1] * f, rows.oacc[db][4 * g + 2] * f,
                      rows.oacc[db][4 * g + 3] * f};
       if (VEC && single) {
-        *reinterpret_cast<vf4 *>(out + d) = x;
+        if (d < a.hd) *reinterpret_cast<vf4 *>(out + d) = x;
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -876,19 +893,20 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 32 ? 3 : (HD <= 64 || sizeof
     }
 }
 
-template <typename T, int HD, bool VEC>
+template <typename T, int HD, int MODE>
 void launch_rows(const PagedArgs &a, hipStream_t st) {
   const int most = min(a.vec_rows, a.max_new * a.group);
   auto grid = [&](int r) { return dim3(a.vec_splits, a.kv_heads * ((most + r - 1) / r), a.batch); };
-  if (most <= 1) paged_rows_kernel<T, HD, 1, VEC><<<grid(1), PR_THREADS, 0, st>>>(a);
-  else if (most <= 2) paged_rows_kernel<T, HD, 2, VEC><<<grid(2), PR_THREADS, 0, st>>>(a);
-  else paged_rows_kernel<T, HD, 4, VEC><<<grid(4), PR_THREADS, 0, st>>>(a);
+  if (most <= 1) paged_rows_kernel<T, HD, 1, MODE><<<grid(1), PR_THREADS, 0, st>>>(a);
+  else if (most <= 2) paged_rows_kernel<T, HD, 2, MODE><<<grid(2), PR_THREADS, 0, st>>>(a);
+  else paged_rows_kernel<T, HD, 4, MODE><<<grid(4), PR_THREADS, 0, st>>>(a);
 }
 
 template <typename T, int HD>
 void launch_rows(const PagedArgs &a, bool wide, hipStream_t st) {
-  if (wide) launch_rows<T, HD, true>(a, st);
-  else launch_rows<T, HD, false>(a, st);
+  if (!wide) launch_rows<T, HD, kScalar>(a, st);
+  else if (a.hd == HD) launch_rows<T, HD, kVector>(a, st);
+  else launch_rows<T, HD, kVectorCut>(a, st);
 }
 
 template <typename T, int HD, int BN>
@@ -902,7 +920,7 @@ void launch_tile(const PagedArgs &a, bool wide, hipStream_t st) {
   else paged_tile_kernel<T, HD, BN, false, false><<<grid, PT_THREADS, 0, st>>>(a);
 }
 
-// wide: head dims of a template and 16-byte aligned rows.
+// wide: head dims that are multiples of 8, and 16-byte aligned rows.
 template <typename T>
 int paged_attn(const PagedArgs &a, bool vec, bool tile, bool wide, hipStream_t st) {
   if (vec) {
