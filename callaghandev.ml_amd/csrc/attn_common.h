@@ -70,6 +70,30 @@ __device__ __forceinline__ T wave_reduce(T x, F f) {
   with(r[1]);
   return __builtin_bit_cast(T, w);
 }
+// The same for a double, whose words travel together.
+template <typename F>
+__device__ __forceinline__ double wave_reduce64(double x, F f) {
+  auto with = [&](uint32_t lo, uint32_t hi) {
+    x = f(x, __builtin_bit_cast(double, (uint64_t)hi << 32 | lo));
+  };
+  auto lo = [&] { return (uint32_t)__builtin_bit_cast(uint64_t, x); };
+  auto hi = [&] { return (uint32_t)(__builtin_bit_cast(uint64_t, x) >> 32); };
+  with(dpp<0xB1>(lo()), dpp<0xB1>(hi()));
+  with(dpp<0x4E>(lo()), dpp<0x4E>(hi()));
+  with(dpp<0x141>(lo()), dpp<0x141>(hi()));
+  with(dpp<0x140>(lo()), dpp<0x140>(hi()));
+  // both results of a swap hold the own value in one half of the lanes and the partner's
+  // in the other: f of the two is the pair's
+  auto swap = [&](auto a, auto b) {
+    x = __builtin_bit_cast(double, (uint64_t)b[0] << 32 | a[0]);
+    with(a[1], b[1]);
+  };
+  swap(__builtin_amdgcn_permlane16_swap(lo(), lo(), false, false),
+       __builtin_amdgcn_permlane16_swap(hi(), hi(), false, false));
+  swap(__builtin_amdgcn_permlane32_swap(lo(), lo(), false, false),
+       __builtin_amdgcn_permlane32_swap(hi(), hi(), false, false));
+  return x;
+}
 __device__ __forceinline__ float wave_max(float x) {
   return wave_reduce(x, [](float a, float b) { return fmaxf(a, b); });
 }

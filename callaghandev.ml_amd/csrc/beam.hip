@@ -7,19 +7,27 @@
 // log-sum-exp and its `beams` best tokens, one wave per row, then merges the rows'
 // sorted lists, one lane per beam.
 //
+// A wave finds its largest logits by a threshold: the `beams`-th largest of its 64 lanes'
+// maxima, found without a look at the other values, is at most the `beams`-th largest of
+// all; the few values that reach it are ranked against each other, one to a lane.  Where
+// more than 64 do (equal logits), the largest is taken out `beams` times instead.
+//
 // The sum decides between tokens of different beams, whose totals lie arbitrarily close,
-// so it is kept in 64 bits, and so are totals and keys.  An exponential is 2^n 2^f with
-// n = rint(x log2 e) and f = fma(x, log2 e, -n) (one rounding at 2^-25, whatever x), the
-// product with log2 e's low part added: 2^f is off by one rounding of fp32, and these
-// do not add up over a sum whose terms are independent.
+// so it is kept in 64 bits, and so are totals and keys.  With L the fp32 value next to
+// log2 e and r = rint(m L) for a segment's maximum m, an exponential is 2^r 2^t with t =
+// fma(x, L, -r): one rounding, small where the term is large.  What L leaves out, k =
+// log2 e / L - 1, moves the whole sum: sum e^x = 2^r (s + k ln 2 (r s + sum t 2^t)) with s =
+// sum 2^t, to the first order of k; and segments of any r join exactly.  From |m| = 1024 on
+// the difference x - m is taken first: it is exact for every x whose term counts.
 #include "attn_common.h"
 
 namespace cdml {
 namespace {
 
 constexpr int BS_THREADS = 256;
-constexpr int BS_PER_LANE = 32;
-constexpr int BS_SEG = 64 * BS_PER_LANE;  // logits a wave holds
+// Logits a lane holds, and a wave with it: a segment.
+constexpr int BS_LONG = 32, BS_SHORT = 8;
+constexpr int BS_SHORT_VOCAB = 4096;  // up to here segments are short
 constexpr int BS_MAX_BEAMS = 64;
 
 struct BeamArgs {
@@ -34,194 +42,267 @@ struct BeamArgs {
   uint8_t *new_finished;
   int *parents, *tokens;
   // workspace, per row and segment
-  double *sum;  // sum of exp(x - max)
+  double *sum;  // sum of exponentials, relative to what the maximum says
   float *top;   // max
   float *val;   // [beams] largest logits, -infinity where there are fewer
   int *tok;     // their tokens
 };
 
-// exp(x - m) for m >= x, both finite: as 2^(n - n_m) 2^(f - f_m) while x log2 e has
-// fraction bits, else from the (then exact or huge) difference.
-struct ExpFrom {
-  float n, f, m;
-  bool small;
-  static constexpr float kL = 1.44269502162933349609375f;  // log2 e rounded to fp32
-  static constexpr float kLlo = 1.925963034e-08f;     // and the rest of it
-  __device__ __forceinline__ static void parts(float x, float &n, float &f) {
-    n = rintf(x * kL);
-    f = fmaf(x, kLlo, fmaf(x, kL, -n));
+constexpr float kL = 1.44269502162933349609375f;  // log2 e rounded to fp32
+constexpr double kLeft = 1.3349758349838184e-8;   // log2 e / kL - 1
+constexpr double kLn2 = 0.69314718055994531;
+
+// The exponent of two that a segment's sum is taken relative to, from its maximum; and
+// whether it is, or the maximum itself.
+__device__ __forceinline__ float ref_exponent(float m) { return rintf(m * kL); }
+__device__ __forceinline__ bool by_exponent(float m) { return fabsf(m) < 1024.f; }
+
+// Sum over this lane's E values of e^x / 2^ref_exponent(m), or of e^(x - m).
+template <int E>
+__device__ __forceinline__ double sum_exp(const float (&x)[E], float m) {
+  double s = 0;
+  if (by_exponent(m)) {
+    const float r = ref_exponent(m);
+    float s1 = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float t0 = fmaxf(fmaf(x[e], kL, -r), -200.f), t1 = fmaxf(fmaf(x[e + 1], kL, -r), -200.f);
+      const float e0 = fast_exp2(t0), e1 = fast_exp2(t1);  // (2^-200 is 0)
+      s1 = fmaf(t1, e1, fmaf(t0, e0, s1));
+      s += (double)(e0 + e1);
+    }
+    return s + kLeft * kLn2 * ((double)r * s + (double)s1);
   }
-  __device__ __forceinline__ explicit ExpFrom(float max) : m(max) {
-    parts(max, n, f);
-    small = fabsf(max) < 65536.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float d = fmaxf(x[e] - m, -200.f);
+    s += (double)fast_exp2(fmaf(d, (float)(kLeft * kL), d * kL));
   }
-  __device__ __forceinline__ float operator()(float x) const {
-    if (!small) return fast_exp2((x - m) * kL);
-    x = fmaxf(x, m - 200.f);  // e^-200 is nothing next to e^0, and -infinity has no fraction
-    float xn, xf;
-    parts(x, xn, xf);
-    return ldexpf(fast_exp2(xf - f), (int)(xn - n));
-  }
+  return s;
+}
+
+// A wave's list of candidates that reach its threshold.
+struct TopList {
+  float v[64];
+  int t[64];
 };
 
-__global__ void __launch_bounds__(BS_THREADS) beam_rows_kernel(const BeamArgs a, int vec) {
-  const int row = blockIdx.y, lane = threadIdx.x & 63;
-  const int seg = blockIdx.x * (BS_THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (seg >= a.n_seg) return;
-  // a finished beam's only candidate and a dead beam's none need no logits
-  if (a.finished[row] != 0 || !isfinite(a.scores[row])) return;
-  const float *x = a.x + (size_t)row * a.ld;
-  const int t0 = seg * BS_SEG;
-  // element 4 i + c of a lane is token t0 + 256 i + 4 lane + c
-  float v[BS_PER_LANE];
+// The K largest of the wave's values (E to a lane, none NaN, -infinity for none; best: the
+// lane's largest, m: the wave's), on ties the lowest token first, into val / tok in that
+// order; -infinity where there are fewer.  token_of(e): the token of the lane's value e.
+template <int E, typename F>
+__device__ __forceinline__ void select_top(float (&v)[E], float best, float m, int K, TopList &list, float *val, int *tok,
+                                           F token_of) {
+  const int lane = threadIdx.x & 63;
+  // the threshold: lanes' maxima leave one by one, equal ones together
+  float least = m, mine = best;
+  for (int out = 0;;) {
+    out += __popcll(__builtin_amdgcn_ballot_w64(mine == least));
+    if (least == -INFINITY || out >= K) break;
+    mine = mine == least ? -INFINITY : mine;
+    least = wave_max(mine);
+  }
+  // the values that reach it, in a list that lies one to a lane
+  int found = 0;
 #pragma unroll
-  for (int i = 0; i < BS_PER_LANE / 4; ++i) {
-    const int t = t0 + 256 * i + 4 * lane;
-    if (vec && t + 4 <= a.vocab) {
-      const vf4 w = *reinterpret_cast<const vf4 *>(x + t);
+  for (int e = 0; e < E; ++e) {
+    const bool reach = v[e] >= least && v[e] > -INFINITY;
+    const uint64_t who = __builtin_amdgcn_ballot_w64(reach);
+    if (who == 0) continue;
+    const int place =
+        found + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+    if (reach && place < 64) {
+      list.v[place] = v[e];
+      list.t[place] = token_of(e);
+    }
+    found += __popcll(who);
+  }
+  if (found <= 64) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the list is this wave's own)
+    const float x0 = lane < found ? list.v[lane] : -INFINITY;
+    const int x1 = lane < found ? list.t[lane] : INT32_MAX;
+    int rank = 0;
+    for (int i = 0; i < found; ++i) {
+      const float y0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x0), i));
+      const int y1 = __builtin_amdgcn_readlane(x1, i);
+      rank += y0 > x0 || (y0 == x0 && y1 < x1);
+    }
+    if (lane < found && rank < K) {
+      val[rank] = x0;
+      tok[rank] = x1;
+    }
+    for (int r = found + lane; r < K; r += 64) val[r] = -INFINITY;
+    return;
+  }
+  // K times: the wave's largest, on ties the lowest token, leaves its lane
+  for (int k = 0; k < K; ++k) {
+    const float w = k ? wave_max(best) : m;
+    if (w == -INFINITY) {  // (the same in every lane)
+      for (int r = k + lane; r < K; r += 64) val[r] = -INFINITY;
+      break;
+    }
+    int t = INT32_MAX;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v[4 * i + c] = w[c];
-    } else {
+    for (int e = 0; e < E; ++e) t = v[e] == w ? min(t, token_of(e)) : t;
+    const int low = wave_min(t);
+    if (lane == 0) {
+      val[k] = w;
+      tok[k] = low;
+    }
+    if (t == low) {
+      best = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v[4 * i + c] = t + c < a.vocab ? x[t + c] : -INFINITY;
+      for (int e = 0; e < E; ++e) {
+        v[e] = v[e] == w && token_of(e) == low ? -INFINITY : v[e];
+        best = fmaxf(best, v[e]);
+      }
     }
   }
-  float m = -INFINITY;
+}
+
+// A wave's values of segment seg of a row's logits: element e of a lane is token
+// 64 (E seg + e) + lane.  Those past the vocabulary, and NaNs, are no candidates.
+template <int E>
+__device__ __forceinline__ void load_segment(float (&v)[E], const float *x, int seg, int vocab) {
+  const int lane = threadIdx.x & 63, t0 = seg * 64 * E + lane;
+  x += seg * 64 * E;
+  if ((seg + 1) * 64 * E <= vocab) {
 #pragma unroll
-  for (int e = 0; e < BS_PER_LANE; ++e) {
-    v[e] = v[e] == v[e] ? v[e] : -INFINITY;  // a NaN is no candidate
-    m = fmaxf(m, v[e]);
+    for (int e = 0; e < E; ++e) v[e] = x[(uint32_t)(lane + 64 * e)];
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = t0 + 64 * e < vocab ? x[(uint32_t)(lane + 64 * e)] : -INFINITY;
   }
-  const float best0 = m;
-  m = wave_max(m);
+}
+template <int E>
+__device__ __forceinline__ float drop_nans(float (&v)[E]) {
+  float best = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    v[e] = v[e] == v[e] ? v[e] : -INFINITY;
+    best = fmaxf(best, v[e]);
+  }
+  return best;
+}
+
+template <int E>
+__global__ void __launch_bounds__(BS_THREADS) beam_rows_kernel(const BeamArgs a) {
+  __shared__ TopList lists[BS_THREADS / 64];
+  const int row = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int seg = blockIdx.x * (BS_THREADS / 64) + wave;
+  if (seg >= a.n_seg) return;
+  float v[E];
+  load_segment<E>(v, a.x + (size_t)row * a.ld, seg, a.vocab);
+  // a finished beam's only candidate and a dead beam's none need no logits
+  if (a.finished[row] != 0 || !isfinite(a.scores[row])) return;
+  const float best = drop_nans<E>(v);
+  const float m = wave_max(best);
   const size_t at = (size_t)row * a.n_seg + seg;
   double s = 0;
-  if (isfinite(m)) {
-    const ExpFrom e_of(m);
-#pragma unroll
-    for (int e = 0; e < BS_PER_LANE; ++e) s += (double)e_of(v[e]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
-  }
+  if (isfinite(m)) s = wave_reduce64(sum_exp<E>(v, m), [](double x, double y) { return x + y; });
   if (lane == 0) {
     a.sum[at] = s;
     a.top[at] = m;
   }
-  // `beams` times: the wave's largest, on ties the lowest token, leaves its lane
-  float best = best0;
-  for (int k = 0; k < a.beams; ++k) {
-    const float w = k ? wave_max(best) : m;
-    if (w == -INFINITY) {  // (the same in every lane)
-      for (int r = k + lane; r < a.beams; r += 64) a.val[at * a.beams + r] = -INFINITY;
-      break;
-    }
-    int e = BS_PER_LANE;
-#pragma unroll
-    for (int i = BS_PER_LANE - 1; i >= 0; --i) e = v[i] == w ? i : e;
-    int tok = e < BS_PER_LANE ? t0 + 256 * (e >> 2) + 4 * lane + (e & 3) : INT32_MAX;
-    int low = tok;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) low = min(low, __shfl_xor(low, off));
-    if (lane == 0) {
-      a.val[at * a.beams + k] = w;
-      a.tok[at * a.beams + k] = low;
-    }
-    if (tok == low) {
-      best = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < BS_PER_LANE; ++i) {
-        v[i] = i == e ? -INFINITY : v[i];
-        best = fmaxf(best, v[i]);
-      }
-    }
-  }
+  select_top<E>(v, best, m, a.beams, lists[wave], a.val + at * a.beams, a.tok + at * a.beams,
+                [&](int e) { return (seg * E + e) * 64 + lane; });
 }
 
-// The order of a merge: the larger key, on ties the lower beam.
-__device__ __forceinline__ bool ahead(double ka, int ba, double kb, int bb) {
-  return ka > kb || (ka == kb && ba < bb);
-}
-
-__global__ void __launch_bounds__(BS_THREADS) beam_pick_kernel(const BeamArgs a) {
-  extern __shared__ char smem[];  // per beam: [beams] logits, [beams] tokens; then the sums
+// ONE: the whole vocabulary is one short segment, and its row's wave reads the logits itself.
+template <bool ONE>
+__global__ void __launch_bounds__(1024) beam_pick_kernel(const BeamArgs a) {
+  extern __shared__ char smem[];  // per beam: [beams] logits, [beams] tokens
   float *val = reinterpret_cast<float *>(smem);
   int *tok = reinterpret_cast<int *>(val + a.beams * a.beams);
-  __shared__ double log_sum[BS_MAX_BEAMS];
-  __shared__ float row_max[BS_MAX_BEAMS];
+  __shared__ TopList lists[16];
+  __shared__ double log_sum[BS_MAX_BEAMS], log_ref[BS_MAX_BEAMS];  // their sum is the row's log-sum-exp
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int K = a.beams, row0 = blockIdx.x * K;
-  for (int k = wave; k < K; k += BS_THREADS / 64) {
-    const int row = row0 + k;
-    for (int r = lane; r < K; r += 64) val[k * K + r] = -INFINITY;
-    if (a.finished[row] != 0 || !isfinite(a.scores[row])) continue;
-    const size_t at = (size_t)row * a.n_seg;
+  // what the merge needs of lane k's beam, read ahead of everything that waits
+  const int row = row0 + min(lane, K - 1);
+  const float score32 = a.scores[row];
+  const bool done = a.finished[row] != 0;
+  const int len = a.lengths[row] + !done;
+  for (int k = wave; k < K; k += blockDim.x / 64) {
+    const bool offers = a.finished[row0 + k] == 0 && isfinite(a.scores[row0 + k]);
+    if constexpr (ONE) {
+      float v[BS_SHORT];
+      load_segment<BS_SHORT>(v, a.x + (size_t)(row0 + k) * a.ld, 0, a.vocab);
+      const float best = drop_nans<BS_SHORT>(v), m = wave_max(best);
+      if (!offers || !isfinite(m)) {
+        for (int r = lane; r < K; r += 64) val[k * K + r] = -INFINITY;
+        continue;
+      }
+      const double sum = wave_reduce64(sum_exp<BS_SHORT>(v, m), [](double x, double y) { return x + y; });
+      if (lane == 0) {
+        log_ref[k] = by_exponent(m) ? kLn2 * (double)ref_exponent(m) : (double)m;
+        log_sum[k] = log(sum);
+      }
+      select_top<BS_SHORT>(v, best, m, K, lists[wave], val + k * K, tok + k * K,
+                           [&](int e) { return 64 * e + lane; });
+      continue;
+    }
+    const size_t at = (size_t)(row0 + k) * a.n_seg;
+    // the row's candidates, seven a lane and pass, beside the best K of the passes before
+    constexpr int E = 8;
+    const int n_cand = a.n_seg * K;
+    float v[E];
+    int t[E];
+    auto load = [&](int from) {
+#pragma unroll
+      for (int e = 1; e < E; ++e) {
+        const int i = from + 64 * (e - 1) + lane;
+        v[e] = i < n_cand ? a.val[at * K + i] : -INFINITY;
+        t[e] = i < n_cand ? a.tok[at * K + i] : 0;
+      }
+    };
+    load(0);
     float m = -INFINITY;
     for (int s = lane; s < a.n_seg; s += 64) m = fmaxf(m, a.top[at + s]);
     m = wave_max(m);
-    if (!isfinite(m)) continue;
+    // (the lists and maxima of a row that offers nothing are whatever the workspace held)
+    if (!offers || !isfinite(m)) {
+      for (int r = lane; r < K; r += 64) val[k * K + r] = -INFINITY;
+      continue;
+    }
+    // segments relative to the row's own exponent, or its maximum
+    const bool pow2 = by_exponent(m);
+    const double ref = pow2 ? kLn2 * (double)ref_exponent(m) : (double)m;
     double sum = 0;
-    for (int s = lane; s < a.n_seg; s += 64)
-      if (a.top[at + s] > -INFINITY) sum += a.sum[at + s] * exp((double)a.top[at + s] - (double)m);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+    for (int s = lane; s < a.n_seg; s += 64) {
+      const float top = a.top[at + s];
+      const double part = a.sum[at + s];
+      if (top == -INFINITY) continue;
+      if (pow2 && by_exponent(top)) sum += ldexp(part, (int)(ref_exponent(top) - ref_exponent(m)));
+      else sum += part * exp((by_exponent(top) ? kLn2 * (double)ref_exponent(top) : (double)top) - ref);
+    }
+    sum = wave_reduce64(sum, [](double x, double y) { return x + y; });
     if (lane == 0) {
-      row_max[k] = m;
+      log_ref[k] = ref;
       log_sum[k] = log(sum);
     }
-    // the lists of the segments are sorted: lane l keeps a place in those of segments l, l + 64, ...;
-    // of equal logits the lowest token comes first
-    const int n_list = (a.n_seg + 63) / 64;
-    uint32_t taken = 0;  // with n_list == 1, the place in the lane's one list
-    for (int r = 0; r < K; ++r) {
-      float best = -INFINITY;
-      int low = INT32_MAX;
-      if (n_list == 1) {
-        if (lane < a.n_seg && (int)taken < K) {
-          best = a.val[(at + lane) * K + taken];
-          if (best > -INFINITY) low = a.tok[(at + lane) * K + taken];
-        }
-      } else {
-        // many segments: everything after the last pick (value, token) in the lists' order
-        const float lv = r ? val[k * K + r - 1] : INFINITY;
-        const int lt = r ? tok[k * K + r - 1] : -1;
-        for (int s = lane; s < a.n_seg; s += 64)
-          for (int i = 0; i < K; ++i) {
-            const float w = a.val[(at + s) * K + i];
-            if (w == -INFINITY) break;
-            const int t = a.tok[(at + s) * K + i];
-            if (w < lv || (w == lv && t > lt)) {
-              if (w > best || (w == best && t < low)) {
-                best = w;
-                low = t;
-              }
-              break;
-            }
-          }
+    v[0] = -INFINITY;
+    t[0] = 0;
+    for (int from = 0; from < n_cand; from += 64 * (E - 1)) {
+      if (from) {
+        load(from);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (val and tok: this wave's own)
+        v[0] = lane < K ? val[k * K + lane] : -INFINITY;
+        t[0] = lane < K ? tok[k * K + lane] : 0;
       }
-      const float w = wave_max(best);
-      if (w == -INFINITY) break;
-      const int mine = best == w ? low : INT32_MAX;
-      int t = mine;
+      float best = v[0];
 #pragma unroll
-      for (int off = 32; off > 0; off >>= 1) t = min(t, __shfl_xor(t, off));
-      if (mine == t) ++taken;
-      if (lane == 0) {
-        val[k * K + r] = w;
-        tok[k * K + r] = t;
-      }
-      __builtin_amdgcn_wave_barrier();
-      __threadfence_block();
+      for (int e = 1; e < E; ++e) best = fmaxf(best, v[e]);
+      select_top<E>(v, best, wave_max(best), K, lists[wave], val + k * K, tok + k * K, [&](int e) { return t[e]; });
     }
   }
   __syncthreads();
   if (wave) return;
-  // lane k: beam k's list, its keys falling along it
-  const int row = row0 + min(lane, K - 1);
-  const double score = a.scores[row];
-  const bool done = a.finished[row] != 0;
-  const int len = a.lengths[row] + !done;
-  const double div = pow((double)max(len, 1), (double)a.penalty);
-  const bool live = lane < K && isfinite(a.scores[row]);
+  // lane k: beam k's list, its keys falling along it; on equal keys the lowest lane wins
+  const double score = score32;
+  const double per = a.penalty == 0.f ? 1.0 : pow((double)max(len, 1), -(double)a.penalty);
+  const bool live = lane < K && isfinite(score32);
+  const int pad = max(a.eos, 0);
   int place = 0;
   double total = 0, key = -INFINITY;
   auto head = [&] {
@@ -232,24 +313,13 @@ __global__ void __launch_bounds__(BS_THREADS) beam_pick_kernel(const BeamArgs a)
       total = score;
     } else {
       if (place >= K || val[lane * K + place] == -INFINITY) return;
-      total = score + (((double)val[lane * K + place] - (double)row_max[lane]) - log_sum[lane]);
+      total = score + (((double)val[lane * K + place] - log_ref[lane]) - log_sum[lane]);
     }
-    key = total / div;
+    key = total * per;
   };
   head();
-  const int pad = max(a.eos, 0);
   for (int r = 0; r < K; ++r) {
-    double k = key;
-    int b = lane;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const double ok = __shfl_xor(k, off);
-      const int ob = __shfl_xor(b, off);
-      if (ahead(ok, ob, k, b)) {
-        k = ok;
-        b = ob;
-      }
-    }
+    const double k = wave_reduce64(key, [](double x, double y) { return y > x ? y : x; });
     const int out = row0 + r;
     if (!(k > -INFINITY)) {  // no candidate is left for this place
       if (lane == r) {
@@ -261,6 +331,7 @@ __global__ void __launch_bounds__(BS_THREADS) beam_pick_kernel(const BeamArgs a)
       }
       continue;
     }
+    const int b = __builtin_ctzll(__builtin_amdgcn_ballot_w64(key == k));
     if (lane == b) {
       const int t = done ? pad : tok[lane * K + place];
       a.parents[out] = row0 + b;
@@ -278,11 +349,13 @@ size_t align_up(size_t n) { return (n + 15) & ~(size_t)15; }
 
 struct Layout {
   size_t sum, top, val, tok, bytes;
-  int n_seg;
+  int n_seg, per_lane;
 };
 Layout layout(int batch, int beams, int vocab) {
   Layout l{};
-  l.n_seg = (int)(((long long)vocab + BS_SEG - 1) / BS_SEG);
+  l.per_lane = vocab <= BS_SHORT_VOCAB ? BS_SHORT : BS_LONG;
+  const int seg = 64 * l.per_lane;
+  l.n_seg = (int)(((long long)vocab + seg - 1) / seg);
   const size_t n = (size_t)batch * beams * l.n_seg;
   l.sum = 0;
   l.top = l.sum + align_up(n * sizeof(double));
@@ -299,7 +372,8 @@ using namespace cdml;
 
 extern "C" int cdml_beam_select_workspace_size(int batch, int beams, int vocab, size_t *bytes) {
   if (!bytes) return fail(CDML_E_INVALID, "cdml_beam_select_workspace_size: bytes is NULL");
-  if (batch < 0 || beams < 1 || beams > BS_MAX_BEAMS || vocab < 1 || (long long)batch * beams > 65535)
+  if (batch < 0 || beams < 1 || beams > BS_MAX_BEAMS || vocab < 1 || vocab > (1 << 30) ||
+      (long long)batch * beams > 65535)
     return fail(CDML_E_INVALID,
                 "cdml_beam_select: bad size (batch %d, beams %d of at most %d, vocab %d; at most 65535 rows)", batch,
                 beams, BS_MAX_BEAMS, vocab);
@@ -351,11 +425,18 @@ extern "C" int cdml_beam_select(const float *logits, int ldl, const float *score
   a.top = reinterpret_cast<float *>(ws + l.top);
   a.val = reinterpret_cast<float *>(ws + l.val);
   a.tok = reinterpret_cast<int *>(ws + l.tok);
-  const int vec = ldl % 4 == 0 && aligned16(logits);
+  // a wave for every beam, up to 16
+  const dim3 pick(64 * (beams < 16 ? beams : 16));
+  const size_t smem = 8 * (size_t)beams * beams;
+  if (vocab <= 64 * BS_SHORT) {
+    beam_pick_kernel<true><<<batch, pick, smem, as_hip(stream)>>>(a);
+    return check_launch("beam_pick_kernel");
+  }
   const dim3 grid((unsigned)((l.n_seg + 3) / 4), (unsigned)(batch * beams));
-  beam_rows_kernel<<<grid, BS_THREADS, 0, as_hip(stream)>>>(a, vec);
+  if (l.per_lane == BS_SHORT) beam_rows_kernel<BS_SHORT><<<grid, BS_THREADS, 0, as_hip(stream)>>>(a);
+  else beam_rows_kernel<BS_LONG><<<grid, BS_THREADS, 0, as_hip(stream)>>>(a);
   rc = check_launch("beam_rows_kernel");
   if (rc) return rc;
-  beam_pick_kernel<<<batch, BS_THREADS, 8 * beams * beams, as_hip(stream)>>>(a);
+  beam_pick_kernel<false><<<batch, pick, smem, as_hip(stream)>>>(a);
   return check_launch("beam_pick_kernel");
 }
