@@ -12,7 +12,9 @@ namespace cdml {
 namespace {
 
 constexpr int PC_THREADS = 1024;
-constexpr int PC_SCAN = 16;  // pages a thread looks at per round of a scan
+constexpr int PC_WAVES = PC_THREADS / 64;
+constexpr int PC_ROUNDS = 16;  // 256 pages a wave, of a span
+constexpr int PC_SPAN = PC_ROUNDS * 256 * PC_WAVES;
 
 struct PlanArgs {
   int *refs;
@@ -26,26 +28,46 @@ struct PlanArgs {
   int fill;  // whether the planning workgroup writes slots and positions itself
 };
 
-// Inclusive sum over the workgroup's threads; *total receives the sum of all.
-template <typename T>
-__device__ __forceinline__ T block_scan(T x, T *wave_sums, T *total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const T y = __shfl_up(x, off);
-    if (lane >= off) x += y;
-  }
-  __syncthreads();  // wave_sums may still be read from the call before
-  if (lane == 63) wave_sums[wave] = x;
+// Inclusive sum over the lanes of a wave: within rows of 16 lanes by shifts, then each row's
+// last lane to the rows after it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t shifted(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += shifted<0x111, 0xf>(x);
+  x += shifted<0x112, 0xf>(x);
+  x += shifted<0x114, 0xf>(x);
+  x += shifted<0x118, 0xf>(x);
+  x += shifted<0x142, 0xa>(x);
+  x += shifted<0x143, 0xc>(x);
+  return x;
+}
+
+// Inclusive sums of x and y (below 2^31) over the workgroup's threads, and their totals.
+// They are summed as halves of 16 bits, which 4096 terms cannot overflow.
+struct ScanScratch {
+  vu4 sums[PC_WAVES];
+};
+__device__ __forceinline__ void block_scan(int x, int y, ScanScratch &sc, long long *sum_x, long long *sum_y,
+                                           long long *all_x, long long *all_y) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  vu4 v = {wave_scan(x & 0xffff), wave_scan((uint32_t)x >> 16), wave_scan(y & 0xffff), wave_scan((uint32_t)y >> 16)};
+  __syncthreads();  // the scratch may still be read from the call before
+  if (lane == 63) sc.sums[wave] = v;
   __syncthreads();
-  T before = 0, all = 0;
+  vu4 all = {};
 #pragma unroll
-  for (int w = 0; w < PC_THREADS / 64; ++w) {
-    if (w < wave) before += wave_sums[w];
-    all += wave_sums[w];
+  for (int w = 0; w < PC_WAVES; ++w) {
+    const vu4 s = sc.sums[w];
+    if (w < wave) v += s;
+    all += s;
   }
-  *total = all;
-  return before + x;
+  auto whole = [](uint32_t lo, uint32_t hi) { return (long long)lo + ((long long)hi << 16); };
+  *sum_x = whole(v[0], v[1]);
+  *sum_y = whole(v[2], v[3]);
+  *all_x = whole(all[0], all[1]);
+  *all_y = whole(all[2], all[3]);
 }
 
 // Largest i in [0, n] with v[i] <= x, for v that does not decrease and v[0] <= x.
@@ -59,31 +81,86 @@ __device__ __forceinline__ int last_not_above(const int *v, int n, int x) {
   return lo;
 }
 
-// Calls take(page, rank) for free pages in increasing order, ranks 0 .. want - 1
-// (fewer if there are not as many), and returns how many free pages were seen, at
-// least want if there are.  A thread looks at PC_SCAN pages in a row per round.
-template <typename F>
-__device__ __forceinline__ int scan_free(const int *refs, int n_pages, int want, int *wave_sums, F take) {
-  int found = 0;
-  for (int p0 = 0; p0 < n_pages && found < want; p0 += PC_THREADS * PC_SCAN) {
-    const int mine = p0 + threadIdx.x * PC_SCAN;
-    uint32_t free = 0;
-#pragma unroll
-    for (int i = 0; i < PC_SCAN; ++i)
-      if (mine + i < n_pages && refs[mine + i] == 0) free |= 1u << i;
-    int total = 0;
-    int rank = found + block_scan<int>(__popc(free), wave_sums, &total) - (int)__popc(free);
-    for (; free && rank < want; free &= free - 1) take(mine + __ffs(free) - 1, rank++);
-    found += total;
+// The free pages among a wave's next 256, four to a lane: bit j for page p + 4 lane + j.
+__device__ __forceinline__ uint32_t free_of(const int *refs, int p, int n_pages) {
+  const int mine = p + 4 * (int)(threadIdx.x & 63);
+  if (mine + 4 <= n_pages) {
+    const int4 r = *reinterpret_cast<const int4 *>(refs + mine);
+    return (r.x == 0) | (r.y == 0) << 1 | (r.z == 0) << 2 | (r.w == 0) << 3;
   }
-  return found;
+  uint32_t f = 0;
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (mine + j < n_pages && refs[mine + j] == 0) f |= 1u << j;
+  return f;
 }
 
-__device__ __forceinline__ void write_row(const PlanArgs &a, int row, const int *cu) {
+// Free pages in increasing order, by one workgroup, a span of the pool at a time, of which
+// each wave has a run of its own and each lane, once counted, four bits for every 256 pages
+// of it.
+struct FreePages {
+  int *counts;    // LDS, [PC_WAVES]: free pages of a span's runs
+  uint64_t mask;  // this lane's of the span counted last
+  int span;       // its first page, or -1
+  int before, all;  // free pages of the runs before this wave's, and of the span
+
+  __device__ __forceinline__ explicit FreePages(int *lds) : counts(lds), mask(0), span(-1), before(0), all(0) {}
+  __device__ __forceinline__ int run(int n_pages, int *end) const {
+    const int len = min(n_pages - span, PC_SPAN), per = (len + PC_WAVES * 256 - 1) / (PC_WAVES * 256) * 256;
+    const int begin = span + (int)(threadIdx.x >> 6) * per;
+    *end = min(begin + per, span + len);
+    return begin;
+  }
+  // Counts the span from page s on (all threads), unless it is the one counted last.
+  __device__ __forceinline__ void count(const int *refs, int n_pages, int s) {
+    if (s == span) return;
+    span = s;
+    int end;
+    const int begin = run(n_pages, &end);
+    mask = 0;
+#pragma unroll 4
+    for (int i = 0; i < PC_ROUNDS; ++i)
+      if (begin + 256 * i < end) mask |= (uint64_t)free_of(refs, begin + 256 * i, end) << (4 * i);
+    const int c = wave_reduce((int)__popcll(mask), [](int a, int b) { return a + b; });
+    __syncthreads();  // counts may still be read
+    if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = c;
+    __syncthreads();
+    before = all = 0;
+#pragma unroll
+    for (int w = 0; w < PC_WAVES; ++w) {
+      if (w < (int)(threadIdx.x >> 6)) before += counts[w];
+      all += counts[w];
+    }
+  }
+  // list[r - from] = page for the span's free pages r = from .. upto - 1, counted from
+  // `first` on (what the spans before it held).
+  __device__ __forceinline__ void list_pages(int n_pages, int first, int from, int upto, int *list) const {
+    int end, rank = first + before;
+    int p = run(n_pages, &end);
+    for (uint64_t m = mask; p < end && rank < upto; p += 256, m >>= 4) {
+      int at = rank;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t who = __builtin_amdgcn_ballot_w64(m >> j & 1);
+        at += __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+        rank += __popcll(who);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (m >> j & 1) {
+          if (at >= from && at < upto) list[at - from] = p + 4 * (int)(threadIdx.x & 63) + j;
+          ++at;
+        }
+    }
+  }
+};
+
+// Slot and position of row `row`, which starts after `first` rows of its request, whose
+// cache held `len` tokens; or of a row of no request.
+__device__ __forceinline__ void write_row(const PlanArgs &a, int row, int b, int first, int len) {
   int slot = -1, pos = 0;
-  if (row < cu[a.batch]) {
-    const int b = last_not_above(cu, a.batch, row), end = cu[b + 1];
-    pos = a.kv_len[b] - end + row;  // kv_len holds the new tokens already
+  if (b >= 0) {
+    pos = len + row - first;
     const int page = a.table[(size_t)b * a.max_blocks + (pos >> a.page_shift)];
     slot = (page << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
   }
@@ -91,12 +168,17 @@ __device__ __forceinline__ void write_row(const PlanArgs &a, int row, const int 
   a.positions[row] = pos;
 }
 
-// One workgroup: sums of pages and tokens over the requests, a first scan that only
-// counts free pages up to the need, then the scan that takes them.
+constexpr int PLAN_LIST = 8192;  // pages that are handed out at a time
+
+// One workgroup: sums of pages and tokens over the requests, a count of free pages up to
+// the need, then the scan that takes them.  A chain of memory round trips bounds it: 64
+// requests over 40000 pages take PLAN_US us.
 __global__ void __launch_bounds__(PC_THREADS) paged_plan_kernel(const PlanArgs a) {
   __shared__ int pages[kPagedMaxBatch + 1], cu[kPagedMaxBatch + 1];  // exclusive sums
-  __shared__ long long sums64[PC_THREADS / 64];
-  __shared__ int sums[PC_THREADS / 64];
+  __shared__ int old[kPagedMaxBatch];                                // kv_len before
+  __shared__ ScanScratch scratch;
+  __shared__ int counts[PC_WAVES], list[PLAN_LIST];
+  FreePages pool(counts);
   const int t = threadIdx.x, P1 = (1 << a.page_shift) - 1;
   const long long room = (long long)a.max_blocks << a.page_shift;
   long long n_need = 0, n_new = 0;
@@ -106,57 +188,73 @@ __global__ void __launch_bounds__(PC_THREADS) paged_plan_kernel(const PlanArgs a
     int need = 0, fresh = 0;
     if (b < a.batch) {
       const int len = a.kv_len[b], add = a.new_len[b];
+      old[b] = len;
       if (len < 0 || add < 0 || (long long)len + add > room) {
         code = 2;
       } else {
         fresh = add;
-        need = (int)(((long long)len + add + P1) >> a.page_shift) - (int)(((long long)len + P1) >> a.page_shift);
+        need = (int)((((long long)len + add + P1) >> a.page_shift) - (((long long)len + P1) >> a.page_shift));
       }
     }
-    long long all = 0;
-    const long long p = n_need + block_scan<long long>(need, sums64, &all);
-    n_need += all;
-    const long long c = n_new + block_scan<long long>(fresh, sums64, &all);
-    n_new += all;
+    long long sum_need, sum_new, all_need, all_new;
+    block_scan(need, fresh, scratch, &sum_need, &sum_new, &all_need, &all_new);
     if (b < a.batch) {  // sums past 31 bits belong to a step that is refused below
-      pages[b + 1] = (int)p;
-      cu[b + 1] = (int)c;
+      pages[b + 1] = (int)(n_need + sum_need);
+      cu[b + 1] = (int)(n_new + sum_new);
     }
+    n_need += all_need;
+    n_new += all_new;
   }
   if (t == 0) pages[0] = cu[0] = 0;
   code = __syncthreads_or(code) ? 2 : 0;
   if (n_new > a.rows) code |= 4;
-  if (n_need > a.n_pages) {
-    code |= 1;
-  } else if (n_need > 0) {
-    if (scan_free(a.refs, a.n_pages, (int)n_need, sums, [](int, int) {}) < n_need) code |= 1;
+  long long n_free = 0;
+  for (int span = 0; span < a.n_pages && n_free < n_need; span += PC_SPAN) {
+    pool.count(a.refs, a.n_pages, span);
+    n_free += pool.all;
   }
+  if (n_free < n_need) code |= 1;
   if (t == 0) {
     a.status[0] = code;
     a.status[1] = (int)min(n_need, (long long)INT_MAX);
     a.status[2] = (int)min(n_new, (long long)INT_MAX);
   }
-  __syncthreads();
   if (code) {  // (the same in every thread)
-    for (int b = t; b <= a.batch; b += PC_THREADS) {
-      a.cu_new[b] = 0;
-      cu[b] = 0;
+    for (int b = t; b <= a.batch; b += PC_THREADS) a.cu_new[b] = 0;
+    if (a.fill)
+      for (int row = t; row < a.rows; row += PC_THREADS) write_row(a, row, -1, 0, 0);
+    return;
+  }
+  // a span's free pages by rank, then the rank's place: block have(b) + rank - pages[b] of
+  // the request that it falls to
+  const int want = (int)n_need;
+  for (int span = 0, first = 0; first < want; span += PC_SPAN) {
+    pool.count(a.refs, a.n_pages, span);
+    const int last = min(want, first + pool.all);
+    for (int from = first; from < last; from += PLAN_LIST) {
+      const int upto = min(last, from + PLAN_LIST);
+      pool.list_pages(a.n_pages, first, from, upto, list);
+      __syncthreads();
+      for (int rank = from + t; rank < upto; rank += PC_THREADS) {
+        const int b = last_not_above(pages, a.batch, rank), page = list[rank - from];
+        const int have = (int)(((long long)old[b] + P1) >> a.page_shift);
+        a.table[(size_t)b * a.max_blocks + have + rank - pages[b]] = page;
+        a.refs[page] = 1;
+      }
+      __syncthreads();
     }
-  } else {
-    // the i-th free page is block have(b) + i - pages[b] of the request it falls to
-    scan_free(a.refs, a.n_pages, (int)n_need, sums, [&](int page, int rank) {
-      const int b = last_not_above(pages, a.batch, rank);
-      const int have = (int)(((long long)a.kv_len[b] + P1) >> a.page_shift);
-      a.table[(size_t)b * a.max_blocks + have + rank - pages[b]] = page;
-      a.refs[page] = 1;
-    });
-    __syncthreads();
-    for (int b = t; b < a.batch; b += PC_THREADS) a.kv_len[b] += cu[b + 1] - cu[b];
-    for (int b = t; b <= a.batch; b += PC_THREADS) a.cu_new[b] = cu[b];
+    first += pool.all;
+  }
+  for (int b = t; b <= a.batch; b += PC_THREADS) {
+    a.cu_new[b] = cu[b];
+    if (b < a.batch) a.kv_len[b] = old[b] + cu[b + 1] - cu[b];
   }
   if (!a.fill) return;
   __syncthreads();
-  for (int row = t; row < a.rows; row += PC_THREADS) write_row(a, row, cu);
+  for (int row = t; row < a.rows; row += PC_THREADS) {
+    const int b = row < cu[a.batch] ? last_not_above(cu, a.batch, row) : -1;
+    write_row(a, row, b, b < 0 ? 0 : cu[b], b < 0 ? 0 : old[b]);
+  }
 }
 
 constexpr int SLOT_THREADS = 256, SLOT_ROWS = 4;  // rows per thread
@@ -167,8 +265,13 @@ __global__ void __launch_bounds__(SLOT_THREADS) paged_slots_kernel(const PlanArg
   __syncthreads();
   const int row0 = blockIdx.x * SLOT_THREADS * SLOT_ROWS + threadIdx.x;
 #pragma unroll
-  for (int i = 0; i < SLOT_ROWS; ++i)
-    if (row0 + i * SLOT_THREADS < a.rows) write_row(a, row0 + i * SLOT_THREADS, cu);
+  for (int i = 0; i < SLOT_ROWS; ++i) {
+    const int row = row0 + i * SLOT_THREADS;
+    if (row >= a.rows) break;
+    const int b = row < cu[a.batch] ? last_not_above(cu, a.batch, row) : -1;
+    // (kv_len holds the new tokens already)
+    write_row(a, row, b, b < 0 ? 0 : cu[b], b < 0 ? 0 : a.kv_len[b] - (cu[b + 1] - cu[b]));
+  }
 }
 
 // ---- append -----------------------------------------------------------------
@@ -263,78 +366,90 @@ __device__ __forceinline__ int parent_of(const ReorderArgs &a, int r) {
 __device__ __forceinline__ void add_ref(const ReorderArgs &a, int page, int d) {
   if ((unsigned)page < (unsigned)a.n_pages) atomicAdd(a.refs + page, d);
 }
-// Whether a lower row takes the state of p too (all threads of the workgroup call it).
+// Whether a lower row takes the state of p too (a wave's question).
 __device__ __forceinline__ bool taken_before(const ReorderArgs &a, int p, int r) {
-  int hit = 0;
-  for (int i = threadIdx.x; i < r; i += blockDim.x) hit |= a.parents[i] == p;
-  return __syncthreads_or(hit) != 0;
+  for (int i = threadIdx.x & 63; i - (int)(threadIdx.x & 63) < r; i += 64)
+    if (__builtin_amdgcn_ballot_w64(i < r && a.parents[i] == p)) return true;
+  return false;
+}
+__device__ __forceinline__ int length_of(const ReorderArgs &a, int r) {
+  return (int)min((long long)max(a.kv_len[r], 0), min((long long)a.max_blocks << a.page_shift, (long long)INT_MAX));
 }
 
-// Row r's old table and length into the workspace; its old pages lose a reference,
-// those it takes from its parent gain one (integer sums: any order gives the same).
-__global__ void __launch_bounds__(256) paged_refs_kernel(const ReorderArgs a) {
-  const int r = blockIdx.x, P1 = (1 << a.page_shift) - 1;
-  const int room = (int)min((long long)a.max_blocks << a.page_shift, (long long)INT_MAX);
-  const int len = min(max(a.kv_len[r], 0), room);
-  const int used = (int)(((long long)len + P1) >> a.page_shift);
-  const int p = parent_of(a, r);
+// A wave per row: its old table and length into the workspace; its old pages lose a
+// reference, those it takes from its parent gain one (integer sums: any order gives the
+// same).
+__device__ __forceinline__ void count_refs(const ReorderArgs &a, int r) {
+  const int lane = threadIdx.x & 63, P1 = (1 << a.page_shift) - 1;
+  const int len = length_of(a, r), used = (int)(((long long)len + P1) >> a.page_shift), p = parent_of(a, r);
   const bool second = p >= 0 && taken_before(a, p, r);
   const int *row = a.table + (size_t)r * a.max_blocks;
-  if (threadIdx.x == 0) a.old_len[r] = len;
-  for (int j = threadIdx.x; j < used; j += 256) {
-    const int page = row[j];
-    a.old_table[(size_t)r * a.max_blocks + j] = page;
-    // a row that stays where it is keeps its full pages, and its open one unless a lower row has it
-    if (p != r || (second && j == len >> a.page_shift)) add_ref(a, page, -1);
+  if (lane == 0) a.old_len[r] = len;
+  const int plen = p < 0 ? 0 : length_of(a, p), take = (plen >> a.page_shift) + ((plen & P1) != 0 && !second);
+  const int *from = a.table + (size_t)max(p, 0) * a.max_blocks;
+  // beams share most pages: one that the row has and takes again at the same place (all of
+  // them, if it stays where it is) is left alone
+  for (int j = lane; j < max(used, take); j += 64) {
+    const int had = j < used ? row[j] : -1, gets = j < take ? from[j] : -1;
+    if (j < used) a.old_table[(size_t)r * a.max_blocks + j] = had;
+    if (had == gets) continue;
+    add_ref(a, had, -1);
+    add_ref(a, gets, 1);
   }
-  if (p < 0 || p == r) return;
-  const int plen = min(max(a.kv_len[p], 0), room);
-  const int take = (plen >> a.page_shift) + ((plen & P1) != 0 && !second);
-  const int *from = a.table + (size_t)p * a.max_blocks;
-  for (int j = threadIdx.x; j < take; j += 256) add_ref(a, from[j], 1);
 }
 
-// Workgroup 0 finds pages for the copies; workgroup r + 1 writes row r's other entries.
-__global__ void __launch_bounds__(PC_THREADS) paged_tables_kernel(const ReorderArgs a) {
-  __shared__ int first[kPagedMaxBatch];  // lowest row that takes each row's state; then the pages found
-  __shared__ int sums[PC_THREADS / 64];
+// A wave per row: its length and entries but those of a copy.
+__device__ __forceinline__ void write_table(const ReorderArgs &a, int r) {
+  const int lane = threadIdx.x & 63, P1 = (1 << a.page_shift) - 1, p = parent_of(a, r);
+  const int len = p < 0 ? 0 : a.old_len[p];
+  const bool open = (len & P1) != 0, second = p >= 0 && taken_before(a, p, r);
+  if (lane == 0 && !(open && second)) a.kv_len[r] = len;
+  if (p == r) return;
+  const int n = (len >> a.page_shift) + (open && !second);
+  for (int j = lane; j < n; j += 64)
+    a.table[(size_t)r * a.max_blocks + j] = a.old_table[(size_t)p * a.max_blocks + j];
+}
+
+struct CopyScratch {
+  int first[kPagedMaxBatch];  // lowest row that takes each row's state; then the pages found
+  ScanScratch scan;
+  int counts[PC_WAVES];
+};
+
+// One workgroup: pages for the copies, and their rows' entries and lengths.
+__device__ __forceinline__ void place_copies(const ReorderArgs &a, CopyScratch &sc) {
   const int t = threadIdx.x, P1 = (1 << a.page_shift) - 1;
-  if (blockIdx.x > 0) {
-    const int r = blockIdx.x - 1, p = parent_of(a, r);
-    const int len = p < 0 ? 0 : a.old_len[p];
-    const bool open = (len & P1) != 0, second = p >= 0 && taken_before(a, p, r);
-    if (t == 0 && !(open && second)) a.kv_len[r] = len;
-    if (p == r) return;
-    const int n = (len >> a.page_shift) + (open && !second);
-    for (int j = t; j < n; j += PC_THREADS)
-      a.table[(size_t)r * a.max_blocks + j] = a.old_table[(size_t)p * a.max_blocks + j];
-    return;
-  }
+  int *first = sc.first;
   for (int r = t; r < a.batch; r += PC_THREADS) first[r] = INT_MAX;
   __syncthreads();
-  int wrong = 0;
   for (int r = t; r < a.batch; r += PC_THREADS) {
     const int p = parent_of(a, r);
     if (p >= 0) atomicMin(first + p, r);
-    else wrong += a.parents[r] != -1;
   }
-  int bad = 0, copies = 0;
-  block_scan(wrong, sums, &bad);
+  __syncthreads();
   // each thread's rows r = t + PC_THREADS * i, four of them at most: place among the copies, or -1
   constexpr int MINE = kPagedMaxBatch / PC_THREADS;
-  int turn[MINE];
+  int turn[MINE], copies = 0, wrong = 0;
 #pragma unroll
   for (int i = 0; i < MINE; ++i) {
+    turn[i] = -1;
+    if (i * PC_THREADS >= a.batch) continue;
     const int r = t + PC_THREADS * i, p = r < a.batch ? parent_of(a, r) : -1;
     const bool copy = p >= 0 && (a.old_len[p] & P1) != 0 && first[p] != r;
-    int all = 0;
-    const int at = copies + block_scan<int>(copy, sums, &all) - 1;
-    turn[i] = copy ? at : -1;
-    copies += all;
+    long long at, bad, all_copies, all_bad;
+    block_scan(copy, r < a.batch && p < 0 && a.parents[r] != -1, sc.scan, &at, &bad, &all_copies, &all_bad);
+    if (copy) turn[i] = copies + (int)at - 1;
+    copies += (int)all_copies;
+    wrong += (int)all_bad;
   }
   __syncthreads();  // the last read of `first` as such
-  const int found = copies ? scan_free(a.refs, a.n_pages, copies, sums, [&](int page, int rank) { first[rank] = page; })
-                           : 0;
+  FreePages pool(sc.counts);
+  int found = 0;
+  for (int span = 0; span < a.n_pages && found < copies; span += PC_SPAN) {
+    pool.count(a.refs, a.n_pages, span);
+    pool.list_pages(a.n_pages, found, 0, copies, first);
+    found += pool.all;
+  }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < MINE; ++i) {
@@ -346,7 +461,6 @@ __global__ void __launch_bounds__(PC_THREADS) paged_tables_kernel(const ReorderA
       if (turn[i] < found) {
         dst = first[turn[i]];
         src = a.old_table[(size_t)p * a.max_blocks + full];
-        // the full pages of the row are another workgroup's
         a.table[(size_t)r * a.max_blocks + full] = dst;
         a.refs[dst] = 1;
       }
@@ -358,8 +472,37 @@ __global__ void __launch_bounds__(PC_THREADS) paged_tables_kernel(const ReorderA
   if (t == 0) {
     a.status[0] = max(copies - found, 0);
     a.status[1] = min(copies, found);
-    a.status[2] = bad;
+    a.status[2] = wrong;
   }
+}
+
+constexpr int REFS_THREADS = 256;
+constexpr int REORDER_ONE = 32;  // rows up to which one workgroup does all
+
+__global__ void __launch_bounds__(REFS_THREADS) paged_refs_kernel(const ReorderArgs a) {
+  const int r = blockIdx.x * (REFS_THREADS / 64) + (threadIdx.x >> 6);
+  if (r < a.batch) count_refs(a, r);
+}
+
+// Workgroup 0 places the copies, the others write 16 rows each.
+__global__ void __launch_bounds__(PC_THREADS) paged_tables_kernel(const ReorderArgs a) {
+  __shared__ CopyScratch sc;
+  if (blockIdx.x == 0) {
+    place_copies(a, sc);
+    return;
+  }
+  const int r = (blockIdx.x - 1) * PC_WAVES + (threadIdx.x >> 6);
+  if (r < a.batch) write_table(a, r);
+}
+
+// All of it in one workgroup, for few rows.
+__global__ void __launch_bounds__(PC_THREADS) paged_reorder_kernel(const ReorderArgs a) {
+  __shared__ CopyScratch sc;
+  for (int r = threadIdx.x >> 6; r < a.batch; r += PC_WAVES) count_refs(a, r);
+  __threadfence();  // references are counted in L2
+  __syncthreads();
+  for (int r = threadIdx.x >> 6; r < a.batch; r += PC_WAVES) write_table(a, r);
+  place_copies(a, sc);
 }
 
 // Workgroup (row, 2 * layer + which): the open page's tokens, one contiguous run.
@@ -395,6 +538,7 @@ extern "C" int cdml_paged_plan(int *page_refs, int n_pages, int page_size, int *
   if (!cu_new || !status || (rows && (!slots || !positions)) ||
       (batch && (!page_refs || !block_table || !kv_len || !new_len)))
     return fail(CDML_E_INVALID, "cdml_paged_plan: NULL pointer");
+  if (!aligned16(page_refs)) return fail(CDML_E_INVALID, "cdml_paged_plan: page_refs is not 16-byte aligned");
   rc = ensure_device();
   if (rc) return rc;
   a.refs = page_refs;
@@ -460,6 +604,7 @@ extern "C" int cdml_paged_reorder(int *page_refs, int n_pages, int page_size, in
   if (rc) return rc;
   if (!status || (batch && (!page_refs || !block_table || !kv_len || !parents || !copy_src || !copy_dst)))
     return fail(CDML_E_INVALID, "cdml_paged_reorder: NULL pointer");
+  if (!aligned16(page_refs)) return fail(CDML_E_INVALID, "cdml_paged_reorder: page_refs is not 16-byte aligned");
   size_t need = 0;
   rc = cdml_paged_reorder_workspace_size(batch, max_blocks, &need);
   if (rc) return rc;
@@ -480,12 +625,15 @@ extern "C" int cdml_paged_reorder(int *page_refs, int n_pages, int page_size, in
   a.status = status;
   a.old_len = static_cast<int *>(workspace);
   a.old_table = a.old_len + batch;
-  if (batch) {
-    paged_refs_kernel<<<batch, 256, 0, as_hip(stream)>>>(a);
-    rc = check_launch("paged_refs_kernel");
-    if (rc) return rc;
+  const hipStream_t st = as_hip(stream);
+  if (batch <= REORDER_ONE) {
+    paged_reorder_kernel<<<1, PC_THREADS, 0, st>>>(a);
+    return check_launch("paged_reorder_kernel");
   }
-  paged_tables_kernel<<<batch + 1, PC_THREADS, 0, as_hip(stream)>>>(a);
+  paged_refs_kernel<<<(batch + 3) / 4, REFS_THREADS, 0, st>>>(a);
+  rc = check_launch("paged_refs_kernel");
+  if (rc) return rc;
+  paged_tables_kernel<<<1 + (batch + PC_WAVES - 1) / PC_WAVES, PC_THREADS, 0, st>>>(a);
   return check_launch("paged_tables_kernel");
 }
 

@@ -437,3 +437,23 @@ def test_two_streams_at_once():
                                             s.handle))
     for s, d, _, _, _, _, _, shape, (want, tol) in cases:
         assert (np.abs(d[6].download(shape, np.float32, s) - want) <= tol).all()
+
+
+def test_large_pools_in_spans():
+    # more pages than one count covers, more new pages than are handed out at a time, little free in front
+    r = rng(3)
+    n, P = 200_003, 2
+    refs = (r.random(n) < 0.9).astype(np.int32)
+    refs[70_000:] = r.random(n - 70_000) < 0.3
+    new = np.array([9000, 1, 0, 23_456, 40_000, 17], np.int32)
+    kv = np.array([3, 1, 8, 0, 11, 2], np.int32)
+    table = np.full((6, 21_000), -1, np.int32)
+    taken = np.flatnonzero(refs)
+    for b, m in enumerate(kv):
+        table[b, :-(-m // P)] = taken[10 * b:10 * b - (-m // P)]
+    same(M.call_plan(refs, table, kv, new, P, int(new.sum())), M.plan(refs, table, kv, new, P, int(new.sum())))
+    # copies that find their pages past the first span
+    refs[:66_000] = 1
+    parents = np.array([0, 0, 0, 1, 1, 5], np.int32)
+    want = M.reorder(refs, table, kv, parents, P)
+    same(M.call_reorder(refs, table, kv, parents, P), want)

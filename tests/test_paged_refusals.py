@@ -27,7 +27,7 @@ def test_plan_refusals():
     good = dict(refs=P, n_pages=8, page_size=16, table=P, max_blocks=4, kv_len=P, new_len=P, batch=2, rows=3, cu=P,
                 slots=P, positions=P, status=P, stream=None)
     refused("cdml_paged_plan", good, POOL + [
-        {"max_blocks": 0}, {"max_blocks": BIG}, {"batch": -1}, {"batch": 4097}, {"rows": -1}] + [
+        {"max_blocks": 0}, {"max_blocks": BIG}, {"batch": -1}, {"batch": 4097}, {"rows": -1}, {"refs": ODD}] + [
         {k: None} for k in ("refs", "table", "kv_len", "new_len", "cu", "slots", "positions", "status")])
 
 
@@ -75,7 +75,8 @@ def test_reorder_refusals():
     good = dict(refs=P, n_pages=8, page_size=16, table=P, max_blocks=7, kv_len=P, parents=P, batch=5, src=P, dst=P,
                 status=P, ws=P, bytes=160, stream=None)
     refused("cdml_paged_reorder", good, POOL + [
-        {"max_blocks": 0}, {"batch": -1}, {"batch": 4097}, {"bytes": 159}, {"ws": C.c_void_p(4097)}] + [
+        {"max_blocks": 0}, {"batch": -1}, {"batch": 4097}, {"bytes": 159}, {"ws": C.c_void_p(4097)},
+        {"refs": ODD}] + [
         {k: None} for k in ("refs", "table", "kv_len", "parents", "src", "dst", "status", "ws")])
 
 
