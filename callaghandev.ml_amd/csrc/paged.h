@@ -32,10 +32,10 @@ inline int check_pool(const char *what, int n_pages, int page_size, int max_bloc
 }  // namespace
 
 // A request's rows are numbered token-major: row rr of K/V head hk is head hk * group +
-// rr % group of its new token rr / group.  Those of requests with at most `vec_rows` rows
-// a K/V head run on the vector units, the others in tiles on the matrix cores.  Keys are
-// split into chunks of vec_chunk / tile_chunk; a request of one chunk is written to o,
-// the chunks of others leave [head_dim] sums, a maximum (log2) and a sum in *_part.
+// rr % group of its new token rr / group.  Requests with at most few_rows rows a K/V head
+// split their keys into chunks of few_chunk, those with more run in tiles of 128 rows and
+// chunks of tile_chunk.  A request of one chunk is written to o, the chunks of others
+// leave [head_dim] sums, a maximum (log2) and a sum in *_part.
 struct PagedArgs {
   const float *q;
   const void *kc, *vc;
@@ -45,8 +45,8 @@ struct PagedArgs {
   int ldq, ldo, n_pages, page_shift, max_blocks, rows, batch, max_new, max_len;
   int heads, kv_heads, group, hd;
   float scale_log2;
-  int vec_rows, vec_chunk, vec_splits, tile_chunk, tile_splits;
-  float *vec_part;   // [batch][kv_heads][vec_rows][vec_splits][hd + 2]
+  int few_rows, few_chunk, few_splits, tile_chunk, tile_splits;
+  float *few_part;   // [batch][kv_heads][few_rows][few_splits][hd + 2]
   float *tile_part;  // [rows][heads][tile_splits][hd + 2]
   UDiv by_group;
 };
@@ -64,10 +64,16 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &a, int b) {
   return s;
 }
 
+// The kernels of a call: for the requests of few rows either the vector units or a wave's
+// matrix operand, and tiles for the others.
+struct PagedKernels {
+  bool rows, span, tile;
+};
+
 // Enqueue the kernels of one cache type (the arguments are validated).
-int paged_attn_f32(const PagedArgs &a, bool vec, bool tile, bool wide, hipStream_t st);
-int paged_attn_f16(const PagedArgs &a, bool vec, bool tile, bool wide, hipStream_t st);
-int paged_attn_bf16(const PagedArgs &a, bool vec, bool tile, bool wide, hipStream_t st);
+int paged_attn_f32(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
+int paged_attn_f16(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
+int paged_attn_bf16(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
 
 constexpr int kPagedTileRows = 128;  // rows of a tile workgroup
 constexpr int kPagedSub = 512;       // keys whose pages a vector workgroup holds at a time

@@ -1,6 +1,8 @@
 // Attention of a step's new tokens over a paged cache (cdml_paged_attn): the choice of
 // kernels and splits, and the join of a request's chunks.  The kernels are in
 // paged_attn.inc.h.
+#include <algorithm>
+
 #include "paged.h"
 
 namespace cdml {
@@ -43,20 +45,20 @@ __device__ __forceinline__ void join_chunks(const PagedArgs &a, const float *par
 
 __device__ __forceinline__ int chunks_seen(int seen, int chunk) { return seen <= 0 ? 0 : (seen - 1) / chunk + 1; }
 
-// A wave per (new token, head) of the requests that ran on the vector units.
+// A wave per (new token, head) of the requests of few rows.
 __global__ void __launch_bounds__(256) paged_join_rows_kernel(const PagedArgs a, int tokens) {
   const int b = blockIdx.x / tokens, i = blockIdx.x - b * tokens;
   const int h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (h >= a.heads) return;
   const PagedSeq s = paged_seq(a, b);
-  if (i >= s.n || s.n * a.group > a.vec_rows || s.len <= a.vec_chunk) return;
+  if (i >= s.n || s.n * a.group > a.few_rows || s.len <= a.few_chunk) return;
   const int hk = a.by_group.div(h), rr = i * a.group + h - hk * a.group;
-  join_chunks(a, a.vec_part + (((size_t)b * a.kv_heads + hk) * a.vec_rows + rr) * a.vec_splits * (a.hd + 2),
-              chunks_seen(s.len - s.n + i + 1, a.vec_chunk),
+  join_chunks(a, a.few_part + (((size_t)b * a.kv_heads + hk) * a.few_rows + rr) * a.few_splits * (a.hd + 2),
+              chunks_seen(s.len - s.n + i + 1, a.few_chunk),
               a.o + (size_t)(s.first + i) * a.ldo + (size_t)h * a.hd);
 }
 
-// A wave per (row, head) of the requests that ran on the matrix cores.
+// A wave per (row, head) of the requests that ran in tiles.
 __global__ void __launch_bounds__(256) paged_join_tiles_kernel(const PagedArgs a) {
   const int row = blockIdx.x, lane = threadIdx.x & 63;
   const int h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -71,19 +73,23 @@ __global__ void __launch_bounds__(256) paged_join_tiles_kernel(const PagedArgs a
   if (b >= a.batch) return;
   const PagedSeq s = paged_seq(a, b);
   const int i = row - s.first;
-  if (i < 0 || i >= s.n || s.n * a.group <= a.vec_rows || s.len <= a.tile_chunk) return;
+  if (i < 0 || i >= s.n || s.n * a.group <= a.few_rows || s.len <= a.tile_chunk) return;
   join_chunks(a, a.tile_part + ((size_t)row * a.heads + h) * a.tile_splits * (a.hd + 2),
               chunks_seen(s.len - s.n + i + 1, a.tile_chunk), a.o + (size_t)row * a.ldo + (size_t)h * a.hd);
 }
 
 // Which kernels run and how keys are split, from the sizes alone.
 struct Plan {
-  bool vec, tile;
-  int vec_rows, vec_chunk, vec_splits, tile_chunk, tile_splits;
-  size_t vec_floats, tile_floats;
+  PagedKernels kernels;
+  int few_rows, few_chunk, few_splits, tile_chunk, tile_splits;
+  size_t few_floats, tile_floats;
 };
 
-constexpr int kVecRows = 4;       // most rows a K/V head on the vector units
+// Most rows a K/V head on the vector units: there a cached value is multiplied once for
+// every row, which 16-bit caches outrun first.  64 x 4096 keys, 4 rows, fp32 687 us against
+// 795 by paged_span_kernel, fp16 447 against 429; 2 rows, bf16 183 against 216.
+constexpr int kVecRows = 4, kVecRows16 = 2;
+constexpr int kSpanRows = 16;  // most rows a K/V head of an MFMA operand
 constexpr int kComputeUnits = 256;
 
 int check_sizes(const char *what, int rows, int batch, int max_new, int max_len, int heads, int kv_heads, int hd) {
@@ -96,7 +102,7 @@ int check_sizes(const char *what, int rows, int batch, int max_new, int max_len,
   const long long group = heads / kv_heads;
   // the grids' limits, and room for key numbers past the last tile
   const long long most = max_new * group;
-  const long long groups = (hd <= 128 && most > kVecRows ? kVecRows : most + kVecRows - 1) / kVecRows;
+  const long long groups = hd <= 128 ? 1 : (most + kVecRows - 1) / kVecRows;
   if (most > INT_MAX / 2 || max_len > INT_MAX / 2 || heads > 65535 || groups * kv_heads > 65535 ||
       (long long)kv_heads * hd > INT_MAX / 4 ||
       ((long long)rows * group / kPagedTileRows + batch) * kv_heads > INT_MAX / 2)
@@ -106,27 +112,36 @@ int check_sizes(const char *what, int rows, int batch, int max_new, int max_len,
 
 int round_up(int n, int m) { return (int)(((long long)n + m - 1) / m * m); }
 
-Plan make_plan(int rows, int batch, int max_new, int max_len, int heads, int kv_heads, int hd) {
+Plan make_plan(int size, int rows, int batch, int max_new, int max_len, int heads, int kv_heads, int hd) {
   Plan p{};
   const int group = heads / kv_heads, most = max_new * group, len = max_len < 1 ? 1 : max_len;
-  p.tile = hd <= 128 && most > kVecRows;
-  p.vec = !p.tile || group <= kVecRows;
-  p.vec_rows = p.tile ? kVecRows : most < 1 ? 1 : most;
-  // vector units: 512 keys a workgroup while there are four workgroups for every CU,
-  // else 256; rows without number (head dims above 128) are not split
-  const long long groups = (p.vec_rows + kVecRows - 1) / kVecRows;
-  if (groups > 2) {
-    p.vec_chunk = len > INT_MAX / 2 ? INT_MAX : round_up(len, kPagedSub);
+  PagedKernels &k = p.kernels;
+  k.tile = hd <= 128 && most > kSpanRows;
+  k.rows = hd > 128 || most <= (size == 4 ? kVecRows : kVecRows16);
+  k.span = !k.rows && (!k.tile || group <= kSpanRows);
+  p.few_rows = most < 1 ? 1 : k.tile ? kSpanRows : most;
+  const long long pairs = (long long)(batch < 1 ? 1 : batch) * kv_heads;
+  const long long groups = k.rows ? (p.few_rows + kVecRows - 1) / kVecRows : 1;
+  if (k.span) {
+    // a whole request to a workgroup where these fill the CUs (16 x 16 pairs of 4096 bf16 keys:
+    // 48.5 us, 55.3 in two chunks, 96 in chunks of 512), else two workgroups for every CU
+    long long splits = pairs >= kComputeUnits ? 1 : (2 * kComputeUnits + pairs - 1) / pairs;
+    if (splits > (len + 255) / 256) splits = (len + 255) / 256;
+    p.few_chunk = round_up((int)((len + splits - 1) / splits), 128);
+  } else if (groups > 2) {
+    p.few_chunk = round_up(len, kPagedSub);  // rows without number (head dims above 128) are not split
   } else {
-    const long long wide = (long long)((len - 1) / 512 + 1) * kv_heads * batch * groups;
-    p.vec_chunk = wide >= 4 * kComputeUnits ? 512 : 256;
+    // 512 keys a workgroup while there are four workgroups for every CU, else 256
+    const long long wide = (long long)((len - 1) / 512 + 1) * pairs * groups;
+    p.few_chunk = wide >= 4 * kComputeUnits ? 512 : 256;
   }
-  p.vec_splits = (len - 1) / p.vec_chunk + 1;
-  if (p.vec && p.vec_splits > 1) p.vec_floats = (size_t)batch * kv_heads * p.vec_rows * p.vec_splits * (hd + 2);
+  p.few_splits = (len - 1) / p.few_chunk + 1;
+  if ((k.rows || k.span) && p.few_splits > 1)
+    p.few_floats = (size_t)batch * kv_heads * p.few_rows * p.few_splits * (hd + 2);
   // matrix cores: keys are split where the tiles alone leave CUs without work
   p.tile_chunk = INT_MAX;
   p.tile_splits = 1;
-  if (p.tile) {
+  if (k.tile) {
     const long long tiles = ((long long)rows * group / kPagedTileRows + batch) * kv_heads;
     long long splits = (2 * kComputeUnits + tiles - 1) / (tiles < 1 ? 1 : tiles);
     const long long pieces = (len + 255) / 256;
@@ -151,8 +166,12 @@ extern "C" int cdml_paged_attn_workspace_size(int rows, int batch, int max_new, 
   int rc = check_sizes("cdml_paged_attn_workspace_size", rows, batch, max_new, max_len, num_heads, num_kv_heads,
                        head_dim);
   if (rc) return rc;
-  const Plan p = make_plan(rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
-  *bytes = sizeof(float) * (p.vec_floats + p.tile_floats);
+  size_t most = 0;
+  for (int size = 2; size <= 4; size += 2) {  // of either size of cached values
+    const Plan p = make_plan(size, rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
+    most = std::max(most, p.few_floats + p.tile_floats);
+  }
+  *bytes = sizeof(float) * most;
   return CDML_OK;
 }
 
@@ -176,8 +195,10 @@ extern "C" int cdml_paged_attn(const float *q, int ldq, const void *kcache, cons
   if (rows == 0 || batch == 0 || max_new == 0) return CDML_OK;
   if (!q || !kcache || !vcache || !block_table || !kv_len || !cu_new || !o)
     return fail(CDML_E_INVALID, "cdml_paged_attn: NULL pointer");
-  const Plan p = make_plan(rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
-  const size_t need = sizeof(float) * (p.vec_floats + p.tile_floats);
+  const Plan p = make_plan(size, rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
+  size_t need = 0;
+  rc = cdml_paged_attn_workspace_size(rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim, &need);
+  if (rc) return rc;
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(CDML_E_INVALID, "cdml_paged_attn: %zu bytes of 16-byte aligned workspace needed, %zu given", need,
                 workspace_bytes);
@@ -205,23 +226,23 @@ extern "C" int cdml_paged_attn(const float *q, int ldq, const void *kcache, cons
   a.hd = head_dim;
   a.scale_log2 = scale * kLog2e;
   a.by_group = UDiv::make((uint32_t)a.group);
-  a.vec_rows = p.vec_rows;
-  a.vec_chunk = p.vec_chunk;
-  a.vec_splits = p.vec_splits;
+  a.few_rows = p.few_rows;
+  a.few_chunk = p.few_chunk;
+  a.few_splits = p.few_splits;
   a.tile_chunk = p.tile_chunk;
   a.tile_splits = p.tile_splits;
-  a.vec_part = static_cast<float *>(workspace);
-  a.tile_part = a.vec_part + p.vec_floats;
+  a.few_part = static_cast<float *>(workspace);
+  a.tile_part = a.few_part + p.few_floats;
   const bool wide = head_dim % 8 == 0 && ldq % 4 == 0 && ldo % 4 == 0 && aligned16(q) && aligned16(o) &&
                     aligned16(kcache) && aligned16(vcache);
   const hipStream_t st = as_hip(stream);
-  if (cache_type == CDML_CACHE_F32) rc = paged_attn_f32(a, p.vec, p.tile, wide, st);
-  else if (cache_type == CDML_CACHE_F16) rc = paged_attn_f16(a, p.vec, p.tile, wide, st);
-  else rc = paged_attn_bf16(a, p.vec, p.tile, wide, st);
+  if (cache_type == CDML_CACHE_F32) rc = paged_attn_f32(a, p.kernels, wide, st);
+  else if (cache_type == CDML_CACHE_F16) rc = paged_attn_f16(a, p.kernels, wide, st);
+  else rc = paged_attn_bf16(a, p.kernels, wide, st);
   if (rc) return rc;
   const unsigned by_head = (unsigned)(num_heads + 3) / 4;
-  if (p.vec_floats) {
-    const int tokens = p.vec_rows / a.group;  // of a request on the vector units, at most
+  if (p.few_floats) {
+    const int tokens = p.few_rows / a.group;  // of a request of few rows, at most
     paged_join_rows_kernel<<<dim3(batch * tokens, by_head), 256, 0, st>>>(a, tokens);
     rc = check_launch("paged_join_rows_kernel");
     if (rc) return rc;

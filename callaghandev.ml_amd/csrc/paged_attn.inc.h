@@ -91,8 +91,8 @@ struct RowSlice {
 // row goes through LPK lanes, its score through their sum, and every group of LPK lanes
 // keeps an online softmax of its own keys.  The four waves take 64 / LPK keys in turn.
 // U sets of rows go round, so that the loads of U - 1 steps are in flight while one is
-// consumed: four where 64 registers hold them (8 x 2048 keys of bf16, 16 heads of 64: U2_US ->
-// U4_US us).
+// consumed: four where 64 registers hold them (8 x 2048 keys of bf16, 16 heads of 64: 15.0
+// -> 14.4 us).
 template <typename T, int HD, int R, int MODE>
 __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedArgs a) {
   constexpr int LPK = HD >= 64 && R > 2 ? 16 : 8;
@@ -109,13 +109,13 @@ __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedArgs 
   const int b = blockIdx.z;
   const PagedSeq s = paged_seq(a, b);
   const int nr = s.n * a.group;
-  if (nr == 0 || nr > a.vec_rows) return;
+  if (nr == 0 || nr > a.few_rows) return;
   const int hk = blockIdx.y % a.kv_heads, r0 = blockIdx.y / a.kv_heads * R;
   if (r0 >= nr) return;
   const int split = blockIdx.x, base = s.len - s.n;  // token i sees keys up to base + i
-  const bool single = s.len <= a.vec_chunk;
+  const bool single = s.len <= a.few_chunk;
   const int kend = base + a.by_group.div(min(r0 + R, nr) - 1) + 1;  // past the last visible key
-  const int c0 = split * a.vec_chunk, c1 = min(c0 + a.vec_chunk, kend);
+  const int c0 = split * a.few_chunk, c1 = min(c0 + a.few_chunk, kend);
   if (c0 >= c1 && !(single && split == 0)) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedArgs 
       const int i = a.by_group.div(rr), h = hk * a.group + rr - i * a.group;
       a.o[(size_t)(s.first + i) * a.ldo + (size_t)h * a.hd + d] = L == 0.f ? 0.f : x / L;
     } else {
-      float *part = a.vec_part + ((((size_t)b * a.kv_heads + hk) * a.vec_rows + rr) * a.vec_splits + split) * (a.hd + 2);
+      float *part = a.few_part + ((((size_t)b * a.kv_heads + hk) * a.few_rows + rr) * a.few_splits + split) * (a.hd + 2);
       part[d] = x;
       if (d == 0) {
         part[a.hd] = M;
@@ -284,6 +284,42 @@ struct Slot {
 __device__ __forceinline__ Slot slot_in(const PagedArgs &a, int page, int key) {
   const bool ok = (unsigned)page < (unsigned)a.n_pages;
   return {((uint32_t)(ok ? page : 0) << a.page_shift) + (uint32_t)(key & ((1 << a.page_shift) - 1)), ok};
+}
+
+// Puts dim c of two neighbouring keys of V (a's the lower one) at place d of its row in
+// every piece's plane.
+template <typename T>
+__device__ __forceinline__ void put_v(char *d, int plane, const typename Raw4<T>::type &a,
+                                      const typename Raw4<T>::type &b, int c) {
+  constexpr int NP = Pieces<T>::N;
+  if constexpr (NP == 1) {
+    *reinterpret_cast<uint32_t *>(d) = __builtin_amdgcn_perm(b[c / 2], a[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+  } else {
+    uint32_t h, m, l;
+    if constexpr (NP == 3) split_bf16x3(a[c] * kSplitScale, b[c] * kSplitScale, h, m, l);
+    else split_bf16x3(half_value(a[c / 2], c & 1, T{}), half_value(b[c / 2], c & 1, T{}), h, m, l);
+    *reinterpret_cast<uint32_t *>(d) = h;
+    *reinterpret_cast<uint32_t *>(d + plane) = m;
+    if constexpr (NP == 3) *reinterpret_cast<uint32_t *>(d + 2 * plane) = l;
+  }
+}
+
+// Four values of a row's columns d .. d + 3 at p, those past the head dim as zeros.
+template <typename T>
+__device__ __forceinline__ typename Raw4<T>::type load4_cut(const T *p, int d, int hd) {
+  typename Raw4<T>::type r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) r[c] = d + c < hd ? (float)p[c] : 0.f;
+  } else {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const uint32_t lo = d + 2 * c < hd ? __builtin_bit_cast(uint16_t, p[2 * c]) : 0;
+      const uint32_t hi = d + 2 * c + 1 < hd ? __builtin_bit_cast(uint16_t, p[2 * c + 1]) : 0;
+      r[c] = lo | hi << 16;
+    }
+  }
+  return r;
 }
 
 // Stages one tile of BN keys: K rows and V transposed, of one K/V head, from their pages
@@ -435,16 +471,8 @@ struct PagedStage {
         const T *p = base + (size_t)s.at * kv_dim + dc;
         if constexpr (VEC) {
           r[i] = *reinterpret_cast<const Raw *>(p + min(0, a.hd - 4 - col - dc));
-        } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) r[i][c] = col + dc + c < a.hd ? (float)p[c] : 0.f;
         } else {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t lo = col + dc + 2 * c < a.hd ? __builtin_bit_cast(uint16_t, p[2 * c]) : 0;
-            const uint32_t hi = col + dc + 2 * c + 1 < a.hd ? __builtin_bit_cast(uint16_t, p[2 * c + 1]) : 0;
-            r[i][c] = lo | hi << 16;
-          }
+          r[i] = load4_cut<T>(p, col + dc, a.hd);
         }
       }
     }
@@ -489,23 +517,8 @@ struct PagedStage {
 #pragma unroll
       for (int i = 0; i < VU; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          char *d = lds + dst + vslabs(i) * VSLAB + vgroups(i) * 32 + vcluster(c);
-          if constexpr (NP == 1) {
-            *reinterpret_cast<uint32_t *>(d) = __builtin_amdgcn_perm(r[2 * i + 1][c / 2], r[2 * i][c / 2],
-                                                                     c & 1 ? 0x07060302u : 0x05040100u);
-          } else {
-            uint32_t h, m, l;
-            if constexpr (NP == 3)
-              split_bf16x3(r[2 * i][c] * kSplitScale, r[2 * i + 1][c] * kSplitScale, h, m, l);
-            else
-              split_bf16x3(half_value(r[2 * i][c / 2], c & 1, T{}), half_value(r[2 * i + 1][c / 2], c & 1, T{}), h, m,
-                           l);
-            *reinterpret_cast<uint32_t *>(d) = h;
-            *reinterpret_cast<uint32_t *>(d + VPLANE) = m;
-            if constexpr (NP == 3) *reinterpret_cast<uint32_t *>(d + 2 * VPLANE) = l;
-          }
-        }
+        for (int c = 0; c < 4; ++c)
+          put_v<T>(lds + dst + vslabs(i) * VSLAB + vgroups(i) * 32 + vcluster(c), VPLANE, r[2 * i], r[2 * i + 1], c);
     }
   }
 
@@ -519,20 +532,22 @@ struct PagedStage {
   }
 };
 
-// Q^T operand of a wave: the three bf16 pieces of this lane's row times scale_log2.
+// Q^T operand of a wave: the three bf16 pieces of this lane's row times scale_log2, eight
+// values of every `step` (16 or 32, by the MFMA) from 8 * part on.
 // Scores start from the row's reference, so neither Q nor K takes the split's scale: what
 // a component below 2^-110 loses (2^-134) reaches a score only through a component of
 // 2^100 and more on the other side.  Returns whether Q holds one or the other
 // (wave-uniform); such rows are recomputed on the fp32 MFMA.
-template <int HD, bool VEC>
-__device__ __forceinline__ bool paged_load_q(bf16x8 (&q)[HD / 16][3], const float *qrow, int hd, float scale, int hf) {
+template <int N, bool VEC>
+__device__ __forceinline__ bool load_q_pieces(bf16x8 (&q)[N][3], const float *qrow, int hd, float scale, int step,
+                                              int part) {
   uint32_t most = 0, least = ~0u;  // of |x|, and of 2 |x| - 1 as integers, which leaves zeros out
 #pragma unroll
-  for (int s = 0; s < HD / 16; ++s) {
+  for (int s = 0; s < N; ++s) {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; e += 4) {
-      const int d = 16 * s + 8 * hf + e;
+      const int d = step * s + 8 * part + e;
       if constexpr (VEC) {
         const vf4 t = d < hd ? *reinterpret_cast<const vf4 *>(qrow + d) : vf4{};
 #pragma unroll
@@ -708,18 +723,18 @@ struct PagedRows {
     return any_nonfinite(wrong);
   }
 
-  // The wave's rows over keys [c0, c1) on the fp32 MFMA straight from the pages: only for
+  // The wave's rows over 32 keys of every `step` of [c0, c1) on the fp32 MFMA straight from the pages: only for
   // rows that came out non-finite (common.h) or whose Q is out of the split's range.
   // Where some row does not see all of a sub-block, V is summed per lane, without the keys
   // that the lane's row does not see: a product with their probability 0 would let their
   // infinities and NaNs through.
   __device__ __forceinline__ void recompute(const PagedArgs &a, const float *qrow, const int *table, int hk, int li,
-                                            int hf, int c0, int c1, int lim, int lim_lo, int last) {
+                                            int hf, int c0, int c1, int step, int lim, int lim_lo, int last) {
     init();
     const int kv_dim = a.kv_heads * a.hd;
     const T *kb = static_cast<const T *>(a.kc) + (size_t)hk * a.hd, *vb = static_cast<const T *>(a.vc) + (size_t)hk * a.hd;
 #pragma unroll 1
-    for (int kb0 = c0; kb0 < c1; kb0 += 32) {
+    for (int kb0 = c0; kb0 < c1; kb0 += step) {
       const int key = min(kb0 + li, last);
       const Slot ks = slot_in(a, table[key >> a.page_shift], key);
       const T *krow = kb + (size_t)ks.at * kv_dim;
@@ -785,7 +800,7 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 32 ? 3 : (HD <= 64 || sizeof
     int tiles = 0;
     if (b0 + lane < a.batch) {
       const int nr = paged_seq(a, b0 + lane).n * a.group;
-      tiles = nr > a.vec_rows ? (nr + kPagedTileRows - 1) / kPagedTileRows : 0;
+      tiles = nr > a.few_rows ? (nr + kPagedTileRows - 1) / kPagedTileRows : 0;
     }
     int upto = tiles;
 #pragma unroll
@@ -825,7 +840,7 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 32 ? 3 : (HD <= 64 || sizeof
     st.load(a, c0);
     st.lookup(a, c0 + BN);
     bf16x8 q[HD / 16][3];
-    const bool wide = paged_load_q<HD, VEC>(q, qrow, a.hd, a.scale_log2, hf);
+    const bool wide = load_q_pieces<HD / 16, VEC>(q, qrow, a.hd, a.scale_log2, 16, hf);
     st.store(lds[0], a.bad);
     __syncthreads();
     const int ko = Stage::koperand(li, hf), vo = Stage::voperand(li, hf);
@@ -860,7 +875,7 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 32 ? 3 : (HD <= 64 || sizeof
       __syncthreads();
     }
     if ((rows.finish() || wide) && rw0 < nr)
-      rows.recompute(a, qrow, a.table + (size_t)b * a.max_blocks, hk, li, hf, c0, min(c1, lim_hi + 1), lim, lim_lo,
+      rows.recompute(a, qrow, a.table + (size_t)b * a.max_blocks, hk, li, hf, c0, min(c1, lim_hi + 1), 32, lim, lim_lo,
                      s.len - 1);
   }
   if (rw0 + li >= nr) return;
@@ -893,10 +908,376 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 32 ? 3 : (HD <= 64 || sizeof
     }
 }
 
+// ---- 5 to 16 rows: matrix cores, a wave's own keys ------------------------------
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+// bf16 MFMA 16x16x32: D = A(16x32) * B(32x16) + C.  Lane l holds eight consecutive k,
+// 8 * (l / 16) + 0..7, of row (A) or column (B) l % 16; D: column l % 16, rows
+// 4 * (l / 16) + 0..3.
+__device__ __forceinline__ floatx4 mfma16x16x32(bf16x8 a, bf16x8 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// The keys of a block of 32 as one wave stages it: whole rows in 16-byte loads, CPR of them
+// a row.  K lies in LDS as it is, a row's chunks exchanged (chunk ^ turn(row)) so that the
+// 16 rows whose same chunk an operand read takes together lie in different banks.  fp32's V
+// lies as it is too, four floats between rows; V of a 16-bit type lies transposed, a dim's 32
+// keys in the order that the P.V product reads them (key k at 8 (k / 4 % 4) + 4 (k / 16) +
+// k % 4), as pairs put together on the way.
+template <typename T, int HD, bool VEC>
+struct SpanBlock {
+  static constexpr int NP = Pieces<T>::N, PER = 16 / (int)sizeof(T);  // values of a 16-byte load
+  static constexpr int CPR = HD / PER, NL = 32 * CPR / 64;            // loads a lane, of K and of V
+  static constexpr int ROWS = CPR >= 16 ? 1 : 16 / CPR;               // rows in 256 bytes
+  static constexpr int K_BYTES = 32 * HD * (int)sizeof(T);
+  static constexpr int V_STRIDE = HD + 4;                  // fp32: floats
+  static constexpr int V_ROW = 80;                         // 16-bit: bytes
+  static constexpr int BYTES = K_BYTES + (NP == 3 ? 32 * V_STRIDE * 4 : HD * V_ROW);
+  vu4 k[NL], v[NL];
+  uint32_t slot;  // of this lane's key (lane % 32) in the loaded block; ~0: no page
+
+  static __device__ __forceinline__ int turn(int row) { return row / ROWS & (CPR < 16 ? CPR - 1 : 15); }
+  // K: load i of a lane is chunk k_chunk of row k_row
+  static __device__ __forceinline__ int k_row(int i) { return ((threadIdx.x & 63) + 64 * i) / CPR; }
+  static __device__ __forceinline__ int k_chunk(int i) { return ((threadIdx.x & 63) + 64 * i) % CPR; }
+  // V: loads 2 u and 2 u + 1 are one chunk of two neighbouring rows (16-bit), or as K's (fp32)
+  static __device__ __forceinline__ int v_row(int i) {
+    if constexpr (NP == 3) return k_row(i);
+    const int x = (threadIdx.x & 63) + 64 * (i / 2);
+    return x / 8 / CPR * 16 + x % 8 * 2 + i % 2;
+  }
+  static __device__ __forceinline__ int v_chunk(int i) {
+    if constexpr (NP == 3) return k_chunk(i);
+    return ((threadIdx.x & 63) + 64 * (i / 2)) / 8 % CPR;
+  }
+  static __device__ __forceinline__ vu4 load16(const T *row, int chunk, int hd) {
+    if constexpr (VEC) return chunk * PER < hd ? *reinterpret_cast<const vu4 *>(row + chunk * PER) : vu4{};
+    vu4 w = {};
+#pragma unroll
+    for (int c = 0; c < PER; ++c)
+      if (chunk * PER + c < hd) {
+        if constexpr (NP == 3) w[c] = __builtin_bit_cast(uint32_t, (float)row[chunk * PER + c]);
+        else w[c / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, row[chunk * PER + c]) << 16 * (c & 1);
+      }
+    return w;
+  }
+  // Rows of a block, from the page and the number of this lane's key
+  __device__ __forceinline__ void load(const PagedArgs &a, const T *kc, const T *vc, int kv_dim, int page, int key) {
+    const Slot t = slot_in(a, page, key);
+    slot = t.ok ? t.at : ~0u;
+    const uint32_t at = t.at;  // (a page that is none reads page 0, and is zeroed below)
+#pragma unroll
+    for (int i = 0; i < NL; ++i) k[i] = load16(kc + (size_t)__shfl(at, k_row(i)) * kv_dim, k_chunk(i), a.hd);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) v[i] = load16(vc + (size_t)__shfl(at, v_row(i)) * kv_dim, v_chunk(i), a.hd);
+  }
+  // Rows of no page, and V's past the request's last key, become zeros
+  __device__ __forceinline__ void clean(int k0, int last, int *bad) {
+    const uint64_t none = __builtin_amdgcn_ballot_w64(slot == ~0u);
+    if (none == 0 && k0 + 31 <= last) return;
+    if (none && bad) *bad = 1;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      if (none >> k_row(i) & 1) k[i] = vu4{};
+      if ((none >> v_row(i) & 1) || k0 + v_row(i) > last) v[i] = vu4{};
+    }
+  }
+  __device__ __forceinline__ void store(char *lds) const {
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      *reinterpret_cast<vu4 *>(lds + (k_row(i) * CPR + (k_chunk(i) ^ turn(k_row(i)))) * 16) = k[i];
+    lds += K_BYTES;
+    if constexpr (NP == 3) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) *reinterpret_cast<vu4 *>(lds + v_row(i) * V_STRIDE * 4 + v_chunk(i) * 16) = v[i];
+    } else {
+#pragma unroll
+      for (int u = 0; u < NL / 2; ++u) {
+        const int row = v_row(2 * u);
+        char *d = lds + v_chunk(2 * u) * PER * V_ROW + (8 * (row / 4 % 4) + 4 * (row / 16) + row % 4) * 2;
+#pragma unroll
+        for (int c = 0; c < PER; ++c)
+          *reinterpret_cast<uint32_t *>(d + c * V_ROW) =
+              __builtin_amdgcn_perm(v[2 * u + 1][c / 2], v[2 * u][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+      }
+    }
+  }
+  // The pieces of dims 32 s + 8 q + 0..7 of a key
+  static __device__ __forceinline__ void k_operand(const char *lds, int s, int key, int q, bf16x8 (&p)[3]) {
+    auto chunk = [&](int c) { return *reinterpret_cast<const vu4 *>(lds + (key * CPR + (c ^ turn(key))) * 16); };
+    if constexpr (NP == 1) {
+      p[0] = __builtin_bit_cast(bf16x8, chunk(4 * s + q));
+    } else {
+      float x[8];
+      if constexpr (NP == 3) {
+        const vu4 a = chunk(8 * s + 2 * q), b = chunk(8 * s + 2 * q + 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = __uint_as_float(a[e]);
+          x[4 + e] = __uint_as_float(b[e]);
+        }
+      } else {
+        const vu4 a = chunk(4 * s + q);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = half_value(a[e / 2], e & 1, T{});
+      }
+      split_operand(x, 1.f, p);
+    }
+  }
+  // The pieces of a dim for the keys of quarter q: 4 q + 0..3 and 16 + 4 q + 0..3
+  static __device__ __forceinline__ void v_operand(const char *lds, int dim, int q, bf16x8 (&p)[3]) {
+    lds += K_BYTES;
+    if constexpr (NP == 3) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e] = reinterpret_cast<const float *>(lds)[(16 * (e / 4) + 4 * q + e % 4) * V_STRIDE + dim];
+      split_operand(x, kSplitScale, p);
+    } else {
+      const vu4 w = *reinterpret_cast<const vu4 *>(lds + dim * V_ROW + q * 16);
+      if constexpr (NP == 1) {
+        p[0] = __builtin_bit_cast(bf16x8, w);
+      } else {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = half_value(w[e / 2], e & 1, T{});
+        split_operand(x, 1.f, p);
+      }
+    }
+  }
+};
+
+// f over the four lanes of a row (l, l ^ 16, l ^ 32, l ^ 48), in each of them.
+template <typename F>
+__device__ __forceinline__ float quarters(float x, F f) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// The online softmax of up to 16 rows, one per lane % 16, over blocks of 32 keys: S^T = K Q^T
+// gives quarter q = lane / 16 of the wave the keys 4 q + 0..3 and 16 + 4 q + 0..3, the order
+// in which O^T += V^T P^T takes them.  Every sum has one accumulator, the corrections added
+// before the main product.
+template <typename T, int HD, bool VEC>
+struct SpanRows {
+  typedef SpanBlock<T, HD, VEC> Block;
+  typedef Pieces<T> PC;
+  static constexpr int NS = HD / 32, NDB = HD / 16;
+  floatx4 o[NDB];  // dims 16 db + 4 q + 0..3
+  float m, l;      // the reference (log2 units) and this quarter's sum
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[db] = floatx4{};
+    m = -INFINITY;
+    l = 0.f;
+  }
+  // Probabilities of the keys up to last_vis (counted from the quarter's first) in place of
+  // the scores; o and l follow a reference that rises.
+  __device__ __forceinline__ void softmax(float (&p)[8], int last_vis) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      p[e] = 16 * (e / 4) + e % 4 <= last_vis ? p[e] : -INFINITY;
+      top = fmaxf(top, p[e]);
+    }
+    top = quarters(top, [](float a, float b) { return fmaxf(a, b); });
+    if (__builtin_amdgcn_ballot_w64(top > m)) {
+      const float to = fmaxf(m, top), w = m == -INFINITY ? 0.f : fast_exp2(m - to);
+      m = to;
+      l *= w;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) o[db] *= w;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      p[e] = fast_exp2(p[e] - ref);
+      l += p[e];
+    }
+  }
+  __device__ __forceinline__ void add(const char *lds, const bf16x8 (&q)[NS][3], int row, int quarter, int last_vis) {
+    float p[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // keys 16 h .. 16 h + 15
+      floatx4 s = {};
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        bf16x8 k[3];
+        Block::k_operand(lds, i, 16 * h + row, quarter, k);
+#pragma unroll
+        for (int c = 0; c < PC::PRODUCTS; ++c) s = mfma16x16x32(k[PC::A[c]], q[i][PC::B[c]], s);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[4 * h + e] = s[e];
+    }
+    softmax(p, last_vis);
+    bf16x8 pp[3];
+    split_operand(p, 1.f, pp);
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      bf16x8 v[3];
+      Block::v_operand(lds, 16 * db + row, quarter, v);
+#pragma unroll
+      for (int c = 0; c < PC::PRODUCTS; ++c) o[db] = mfma16x16x32(v[PC::A[c]], pp[PC::B[c]], o[db]);
+    }
+  }
+  // Undoes V's scale; whether some row came out non-finite (wave-uniform)
+  __device__ __forceinline__ bool finish() {
+    constexpr float unscale = PC::N == 3 ? kSplitUnscale : 1.f;
+    float wrong = l * 0.f;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      o[db] *= unscale;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) wrong = fmaf(o[db][e], 0.f, wrong);
+    }
+    return any_nonfinite(wrong);
+  }
+  // The rows over the wave's blocks in fp32 straight from the pages, without the keys that
+  // a row does not see: for rows that came out non-finite or whose Q is out of the split's
+  // range.
+  __device__ __forceinline__ void recompute(const PagedArgs &a, const float *qrow, const int *table, const T *kc,
+                                            const T *vc, int quarter, int first, int c1, int lim, int last) {
+    init();
+    const int kv_dim = a.kv_heads * a.hd;
+    auto row_of = [&](const T *cache, int key) -> const T * {
+      const Slot s = slot_in(a, table[key >> a.page_shift], key);
+      return s.ok ? cache + (size_t)s.at * kv_dim : nullptr;
+    };
+#pragma unroll 1
+    for (int k0 = first; k0 < c1; k0 += 128) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const T *k = row_of(kc, min(k0 + 16 * (e / 4) + 4 * quarter + e % 4, last));
+        p[e] = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < a.hd; ++d) p[e] = fmaf(k ? (float)k[d] : 0.f, qrow[d] * a.scale_log2, p[e]);
+      }
+      softmax(p, lim - k0 - 4 * quarter);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          const float w = __shfl(p[e], (threadIdx.x & 15) + 16 * q);
+          const int key = k0 + 16 * (e / 4) + 4 * q + e % 4;
+          if (key > lim) continue;
+          const T *v = row_of(vc, key);
+#pragma unroll
+          for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int d = 16 * db + 4 * quarter + c;
+              if (v && d < a.hd) o[db][c] = fmaf(w, (float)v[d], o[db][c]);
+            }
+        }
+    }
+  }
+};
+
+// One workgroup: the up to 16 rows of a (request, K/V head) against one chunk of its keys.
+// Reading the cache bounds this, and rows fill one small MFMA operand at most, so the four
+// waves split the keys: each walks blocks of 32 through LDS of its own, with no barrier until
+// the waves' sums are joined.  The next block is loaded into registers while one is
+// multiplied; two workgroups a CU keep 128 KB on the way at head dim 128.
+template <typename T, int HD, bool VEC>
+__global__ void __launch_bounds__(PT_THREADS, sizeof(T) == 2 || HD <= 64 ? 2 : 1) paged_span_kernel(const PagedArgs a) {
+  typedef SpanRows<T, HD, VEC> Rows;
+  typedef SpanBlock<T, HD, VEC> Block;
+  constexpr int NS = HD / 32, NDB = HD / 16, ROW = HD + 4;  // floats between rows of the join
+  constexpr int WAVE_O = 16 * ROW * 4, WAVE = Block::BYTES > WAVE_O ? Block::BYTES : WAVE_O;
+  __shared__ __attribute__((aligned(16))) char lds[4][WAVE];
+  __shared__ float red_m[4][16], red_l[4][16];
+
+  const int b = blockIdx.z, hk = blockIdx.y, split = blockIdx.x;
+  const PagedSeq s = paged_seq(a, b);
+  const int nr = s.n * a.group;
+  if (nr == 0 || nr > a.few_rows) return;
+  const int base = s.len - s.n;
+  const bool single = s.len <= a.few_chunk;
+  const int c0 = split * a.few_chunk, c1 = min(c0 + a.few_chunk, s.len);  // the last row sees all keys
+  if (c0 >= c1 && !(single && split == 0)) return;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = lane & 15, quarter = lane >> 4;
+  const int rr = min(row, nr - 1), tok = a.by_group.div(rr), head = hk * a.group + rr - tok * a.group;
+  const int lim = base + tok, last = s.len - 1;
+  const float *qrow = a.q + (size_t)(s.first + tok) * a.ldq + (size_t)head * a.hd;
+  const int *table = a.table + (size_t)b * a.max_blocks;
+  const int kv_dim = a.kv_heads * a.hd;
+  const T *kc = static_cast<const T *>(a.kc) + (size_t)hk * a.hd, *vc = static_cast<const T *>(a.vc) + (size_t)hk * a.hd;
+
+  Rows rows;
+  rows.init();
+  const int first = c0 + wave * 32;
+  if (first < c1) {
+    char *mine = lds[wave];
+    // this lane's key (lane % 32 of the block) and its page, a block ahead of its rows
+    auto key_at = [&](int k0) { return min(k0 + (lane & 31), last); };
+    auto page_at = [&](int k0) { return table[key_at(k0) >> a.page_shift]; };
+    Block blk;
+    blk.load(a, kc, vc, kv_dim, page_at(first), key_at(first));
+    int page = page_at(first + 128);
+    bf16x8 q[NS][3];
+    const bool wide = load_q_pieces<NS, VEC>(q, qrow, a.hd, a.scale_log2, 32, quarter);
+#pragma unroll 1
+    for (int k0 = first; k0 < c1; k0 += 128) {
+      blk.clean(k0, last, a.bad);
+      blk.store(mine);
+      blk.load(a, kc, vc, kv_dim, page, key_at(k0 + 128));
+      page = page_at(k0 + 256);
+      // the LDS writes above are this wave's own: in order, but not for the compiler
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      rows.add(mine, q, row, quarter, lim - k0 - 4 * quarter);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    if (rows.finish() || wide) rows.recompute(a, qrow, table, kc, vc, quarter, first, c1, lim, last);
+  }
+  // the waves' sums: rows' statistics, then each wave's O scaled to the common maximum
+  const float m = fmaxf(rows.m, -3.0e38f), l = quarters(rows.l, [](float x, float y) { return x + y; });
+  if (quarter == 0) {
+    red_m[wave][row] = m;
+    red_l[wave][row] = l;
+  }
+  __syncthreads();
+  const float w = fast_exp2(m - fmaxf(fmaxf(red_m[0][row], red_m[1][row]), fmaxf(red_m[2][row], red_m[3][row])));
+  float *part_o = reinterpret_cast<float *>(lds[wave]) + row * ROW;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) *reinterpret_cast<floatx4 *>(part_o + db * 16 + 4 * quarter) = rows.o[db] * w;
+  __syncthreads();
+  for (int t = threadIdx.x; t < nr * HD; t += PT_THREADS) {
+    const int r = t / HD, d = t % HD;
+    if (d >= a.hd) continue;
+    float x = 0.f, L = 0.f;
+    const float M = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r]));
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      x += reinterpret_cast<const float *>(lds[v])[r * ROW + d];
+      L += red_l[v][r] * fast_exp2(red_m[v][r] - M);
+    }
+    if (single) {
+      const int i = a.by_group.div(r), h = hk * a.group + r - i * a.group;
+      a.o[(size_t)(s.first + i) * a.ldo + (size_t)h * a.hd + d] = L == 0.f ? 0.f : x / L;
+    } else {
+      float *part = a.few_part + ((((size_t)b * a.kv_heads + hk) * a.few_rows + r) * a.few_splits + split) * (a.hd + 2);
+      part[d] = x;
+      if (d == 0) {
+        part[a.hd] = M;
+        part[a.hd + 1] = L;
+      }
+    }
+  }
+}
+
 template <typename T, int HD, int MODE>
 void launch_rows(const PagedArgs &a, hipStream_t st) {
-  const int most = min(a.vec_rows, a.max_new * a.group);
-  auto grid = [&](int r) { return dim3(a.vec_splits, a.kv_heads * ((most + r - 1) / r), a.batch); };
+  const int most = a.few_rows;
+  auto grid = [&](int r) { return dim3(a.few_splits, a.kv_heads * ((most + r - 1) / r), a.batch); };
   if (most <= 1) paged_rows_kernel<T, HD, 1, MODE><<<grid(1), PR_THREADS, 0, st>>>(a);
   else if (most <= 2) paged_rows_kernel<T, HD, 2, MODE><<<grid(2), PR_THREADS, 0, st>>>(a);
   else paged_rows_kernel<T, HD, 4, MODE><<<grid(4), PR_THREADS, 0, st>>>(a);
@@ -920,10 +1301,17 @@ void launch_tile(const PagedArgs &a, bool wide, hipStream_t st) {
   else paged_tile_kernel<T, HD, BN, false, false><<<grid, PT_THREADS, 0, st>>>(a);
 }
 
+template <typename T, int HD>
+void launch_span(const PagedArgs &a, bool wide, hipStream_t st) {
+  const dim3 grid(a.few_splits, a.kv_heads, a.batch);
+  if (wide) paged_span_kernel<T, HD, true><<<grid, PT_THREADS, 0, st>>>(a);
+  else paged_span_kernel<T, HD, false><<<grid, PT_THREADS, 0, st>>>(a);
+}
+
 // wide: head dims that are multiples of 8, and 16-byte aligned rows.
 template <typename T>
-int paged_attn(const PagedArgs &a, bool vec, bool tile, bool wide, hipStream_t st) {
-  if (vec) {
+int paged_attn(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st) {
+  if (k.rows) {
     if (a.hd <= 32) launch_rows<T, 32>(a, wide, st);
     else if (a.hd <= 64) launch_rows<T, 64>(a, wide, st);
     else if (a.hd <= 128) launch_rows<T, 128>(a, wide, st);
@@ -931,7 +1319,14 @@ int paged_attn(const PagedArgs &a, bool vec, bool tile, bool wide, hipStream_t s
     const int rc = check_launch("paged_rows_kernel");
     if (rc) return rc;
   }
-  if (tile) {
+  if (k.span) {
+    if (a.hd <= 32) launch_span<T, 32>(a, wide, st);
+    else if (a.hd <= 64) launch_span<T, 64>(a, wide, st);
+    else launch_span<T, 128>(a, wide, st);
+    const int rc = check_launch("paged_span_kernel");
+    if (rc) return rc;
+  }
+  if (k.tile) {
     if (a.hd <= 32) launch_tile<T, 32, 32>(a, wide, st);
     else if (a.hd <= 64) launch_tile<T, 64, 32>(a, wide, st);
     else launch_tile<T, 128, 32>(a, wide, st);

@@ -3,8 +3,8 @@
 
 namespace cdml {
 
-int paged_attn_f16(const PagedArgs &a, bool vec, bool tile, bool wide, hipStream_t st) {
-  return paged_attn<_Float16>(a, vec, tile, wide, st);
+int paged_attn_f16(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st) {
+  return paged_attn<_Float16>(a, k, wide, st);
 }
 
 }  // namespace cdml
