@@ -944,6 +944,35 @@ PYBIND11_MODULE(_cdml_host, m) {
              std::memcpy(r.mutable_data(), out.data(), out.size() * sizeof(int));
              return r;
            })
+      .def("GenerateBeam",
+           // prompts: token id arrays of any lengths -> (tokens, scores): per
+           // prompt the list of its beams' token arrays, and [prompts, beams]
+           [](DeviceLanguageModel &d, py::list prompts, int beams, int maxNew, int eos, float lengthPenalty) {
+             std::vector<std::vector<int>> in;
+             for (py::handle h : prompts) {
+               I32 a = I32::ensure(py::reinterpret_borrow<py::object>(h));
+               if (!a || a.ndim() != 1) throw ArgumentException("each prompt must be a token id array", "prompts");
+               in.emplace_back(a.data(), a.data() + a.size());
+             }
+             BeamHypotheses found;
+             {
+               py::gil_scoped_release nogil;
+               found = d.GenerateBeam(in, beams, maxNew, eos, lengthPenalty);
+             }
+             py::list tokens;
+             for (size_t r = 0; r < found.tokens.size(); ++r) {
+               const std::vector<int> &t = found.tokens[r];
+               if (r % beams == 0) tokens.append(py::list());
+               py::array_t<int> a((py::ssize_t)t.size());
+               std::memcpy(a.mutable_data(), t.data(), t.size() * sizeof(int));
+               tokens[r / beams].cast<py::list>().append(std::move(a));
+             }
+             py::array_t<float> scores({(py::ssize_t)in.size(), (py::ssize_t)beams});
+             std::memcpy(scores.mutable_data(), found.scores.data(), found.scores.size() * sizeof(float));
+             return py::make_tuple(tokens, scores);
+           },
+           py::arg("prompts"), py::arg("beams"), py::arg("max_new"), py::arg("eos") = -1,
+           py::arg("length_penalty") = 0.0f)
       .def("time_forward",
            // Device-resident forward of `batch` sequences of `seqLen` inputs
            // that are already in HBM: returns the mean ms of `steps` launches

@@ -627,6 +627,13 @@ class LanguageModel {
   HipAccelerationManager *accel_;
 };
 
+// What GenerateBeam found: for every prompt its beams, best first.
+struct BeamHypotheses {
+  int beams = 0;
+  std::vector<std::vector<int>> tokens;  // [prompts * beams]: the prompt, then the new tokens up to eosToken
+  std::vector<float> scores;             // total log-probability of the new tokens; -infinity where no beam is left
+};
+
 // ---- device-resident engine ----------------------------------------------
 class DeviceLanguageModel {
  public:
@@ -648,6 +655,16 @@ class DeviceLanguageModel {
   // MaxSequenceLength), the count the reference's Generate produces.
   std::vector<int> GenerateGreedy(const std::vector<int> &prompts, int batch, int promptLen,
                                   int maxNewTokens, int *outLen);
+  // Beam search for decoder-only models over prompts of any lengths, prompts *
+  // beams rows within the batch capacity: n = min(maxNewTokens,
+  // MaxSequenceLength - longest prompt) steps of `beams` beams each, ranked by
+  // total log-probability / length^lengthPenalty (lengths count new tokens).
+  // A beam that chooses eosToken (>= 0) is finished and keeps its score.  The
+  // cache lies in pages that beams share (cdml_paged_*); selection and
+  // reordering stay on the device.  No counterpart in the reference, whose
+  // Generate samples one sequence (LanguageModel.cs:482-584).
+  BeamHypotheses GenerateBeam(const std::vector<std::vector<int>> &prompts, int beams, int maxNewTokens,
+                              int eosToken, float lengthPenalty);
   // Enqueue-only forms over device pointers for benchmarking.
   void forward_device(const int *dev_ids, const float *dev_x, int batch, int seqLen,
                       float *dev_out);
@@ -677,8 +694,13 @@ class DeviceLanguageModel {
   float *alloc(size_t floats);
   float *upload(const float *host, size_t floats);
   void hidden_pass(float *x, int batch, int seqLen, bool fill_cache);
+  void finish_block(const Layer &L, float *x, int rows);
   void decode_step(const int *dev_tok, int batch, int pos, float *x);
   void generate_device(int batch, int promptLen, int n);
+  struct BeamState;
+  void prepare_beams();
+  void *beam_workspace(size_t bytes);
+  void paged_pass(float *x, int rows, int seqs, int longest, int max_len, int *status);
 
   TransformerConfig cfg_;
   int cap_, device_;
@@ -697,6 +719,9 @@ class DeviceLanguageModel {
   std::map<std::tuple<int, int, int, bool>, cdml_graph> graphs_;  // (batch, promptLen, n, fused decode)
   cdml_tiny_model tiny_{};  // descriptors for cdml_tiny_decode (layers in device memory)
   bool tiny_ok_ = false;
+  std::unique_ptr<BeamState> beam_;
+  void *beam_ws_ = nullptr;
+  size_t beam_ws_bytes_ = 0;
 };
 
 // ---- the reference's trainer on the manager -------------------------------

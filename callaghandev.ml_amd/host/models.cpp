@@ -378,6 +378,21 @@ std::vector<int> LanguageModel::Generate(const std::vector<int> &prompt, int max
 }
 
 // ---- DeviceLanguageModel -------------------------------------------------------
+// Allocated on the first GenerateBeam: every layer's pages (enough for a row of its own per
+// capacity slot) and the tables, and the state and history of the search.
+struct DeviceLanguageModel::BeamState {
+  static constexpr int kPage = 16;
+  int blocks, pages;
+  size_t layer_floats;  // of K, and of V
+  float *k, *v;
+  int *refs, *table, *kv, *new_len, *cu, *slots, *pos, *src, *dst, *gather;
+  float *scores;
+  int *lengths;
+  uint8_t *finished;
+  int *parents, *tokens;  // [MaxSequenceLength][capacity]
+  int *status;            // [MaxSequenceLength][2][3]: plan, reorder
+};
+
 float *DeviceLanguageModel::alloc(size_t floats) {
   void *p = nullptr;
   check(cdml_malloc(&p, std::max<size_t>(floats, 1) * sizeof(float)), "cdml_malloc");
@@ -523,6 +538,26 @@ DeviceLanguageModel::~DeviceLanguageModel() {
 
 void DeviceLanguageModel::synchronize() { check(cdml_stream_synchronize(stream_), "cdml_stream_synchronize"); }
 
+// What follows the attention in a block (TransformerBlock.cs:38-44): output projection of
+// att_, residual LayerNorm, FFN and its residual LayerNorm, on x [rows, D] in place.
+void DeviceLanguageModel::finish_block(const Layer &L, float *x, int rows) {
+  const int D = cfg_.EmbeddingDim;
+  check(cdml_linear(att_, D, L.wo, L.bo, proj_, D, rows, D, D, CDML_ACT_NONE, stream_), "cdml_linear");
+  check(cdml_residual_layernorm(x, proj_, L.ln1g, L.ln1b, h_, rows, D, 1e-5f, stream_), "layernorm");
+  const float *in = h_;
+  int width = D;
+  float *bufs[2] = {ff_, ff2_};
+  for (size_t l = 0; l < L.ffw.size(); ++l) {
+    float *out = bufs[l & 1];
+    check(cdml_linear(in, width, L.ffw[l], L.ffb[l], out, L.ffrows[l], rows, width, L.ffrows[l],
+                      L.ffact[l], stream_),
+          "cdml_linear");
+    in = out;
+    width = L.ffrows[l];
+  }
+  check(cdml_residual_layernorm(h_, in, L.ln2g, L.ln2b, x, rows, D, 1e-5f, stream_), "layernorm");
+}
+
 // The blocks over x [batch * seqLen, D] in place (LanguageModel.cs:210-223 /
 // TransformerBlock.cs:35-44), every sequence at positions 0..seqLen-1.  With
 // fill_cache the post-RoPE K and V rows are also written to each layer's
@@ -544,20 +579,7 @@ void DeviceLanguageModel::hidden_pass(float *x, int batch, int seqLen, bool fill
     check(cdml_sdpa_fwd(q_, D, k_, D, v_, D, att_, D, batch, seqLen, seqLen, D, H, scale,
                         cfg_.UseDecoderOnly ? 1 : 0, nullptr, stream_),
           "cdml_sdpa_fwd");
-    check(cdml_linear(att_, D, L.wo, L.bo, proj_, D, rows, D, D, CDML_ACT_NONE, stream_), "cdml_linear");
-    check(cdml_residual_layernorm(x, proj_, L.ln1g, L.ln1b, h_, rows, D, 1e-5f, stream_), "layernorm");
-    const float *in = h_;
-    int width = D;
-    float *bufs[2] = {ff_, ff2_};
-    for (size_t l = 0; l < L.ffw.size(); ++l) {
-      float *out = bufs[l & 1];
-      check(cdml_linear(in, width, L.ffw[l], L.ffb[l], out, L.ffrows[l], rows, width, L.ffrows[l],
-                        L.ffact[l], stream_),
-            "cdml_linear");
-      in = out;
-      width = L.ffrows[l];
-    }
-    check(cdml_residual_layernorm(h_, in, L.ln2g, L.ln2b, x, rows, D, 1e-5f, stream_), "layernorm");
+    finish_block(L, x, rows);
   }
 }
 
@@ -634,20 +656,7 @@ void DeviceLanguageModel::decode_step(const int *dev_tok, int batch, int pos, fl
     check(cdml_decode_attn(q_, L.kcache, L.vcache, kvlen_, att_, batch, S, D, H, scale, ws_, ws_bytes_,
                            stream_),
           "cdml_decode_attn");
-    check(cdml_linear(att_, D, L.wo, L.bo, proj_, D, batch, D, D, CDML_ACT_NONE, stream_), "cdml_linear");
-    check(cdml_residual_layernorm(x, proj_, L.ln1g, L.ln1b, h_, batch, D, 1e-5f, stream_), "layernorm");
-    const float *in = h_;
-    int width = D;
-    float *bufs[2] = {ff_, ff2_};
-    for (size_t l = 0; l < L.ffw.size(); ++l) {
-      float *out = bufs[l & 1];
-      check(cdml_linear(in, width, L.ffw[l], L.ffb[l], out, L.ffrows[l], batch, width, L.ffrows[l],
-                        L.ffact[l], stream_),
-            "cdml_linear");
-      in = out;
-      width = L.ffrows[l];
-    }
-    check(cdml_residual_layernorm(h_, in, L.ln2g, L.ln2b, x, batch, D, 1e-5f, stream_), "layernorm");
+    finish_block(L, x, batch);
   }
 }
 
@@ -762,6 +771,186 @@ std::vector<int> DeviceLanguageModel::GenerateGreedy(const std::vector<int> &pro
       out[(size_t)b * total + len] = next[b];
     }
     cur.swap(grown);
+  }
+  return out;
+}
+
+// ---- beam search over a paged cache ---------------------------------------------
+
+void DeviceLanguageModel::prepare_beams() {
+  if (beam_) return;
+  auto st = std::make_unique<BeamState>();
+  const int S = cfg_.MaxSequenceLength;
+  const size_t cap = cap_, rows = cap * S;
+  st->blocks = (S + BeamState::kPage - 1) / BeamState::kPage;
+  st->pages = cap_ * st->blocks;
+  st->layer_floats = (size_t)st->pages * BeamState::kPage * cfg_.EmbeddingDim;
+  auto ints = [&](size_t n) { return reinterpret_cast<int *>(alloc(n)); };
+  st->k = alloc(st->layer_floats * layers_.size());
+  st->v = alloc(st->layer_floats * layers_.size());
+  st->refs = ints(st->pages);
+  st->table = ints(cap * st->blocks);
+  st->kv = ints(cap);
+  st->new_len = ints(cap);
+  st->cu = ints(cap + 1);
+  st->slots = ints(rows);
+  st->pos = ints(rows);
+  st->src = ints(cap);
+  st->dst = ints(cap);
+  st->gather = ints(cap);
+  st->scores = alloc(cap);
+  st->lengths = ints(cap);
+  st->finished = reinterpret_cast<uint8_t *>(alloc((cap + 3) / 4));
+  st->parents = ints(rows);
+  st->tokens = ints(rows);
+  st->status = ints((size_t)S * 6);
+  beam_ = std::move(st);
+}
+
+// Grow-only workspace of the paged entries.
+void *DeviceLanguageModel::beam_workspace(size_t bytes) {
+  if (bytes > beam_ws_bytes_) {
+    // (the smaller one stays with allocs_ until the model goes: launches may still use it)
+    beam_ws_ = alloc((bytes + 3) / sizeof(float));
+    beam_ws_bytes_ = bytes;
+  }
+  return beam_ws_;
+}
+
+// One pass of the blocks over the new tokens x [rows, D] of `seqs` requests: the plan's
+// pages, then in every layer Q/K/V, RoPE at the plan's positions, the append and the
+// attention over what each request's cache holds.
+void DeviceLanguageModel::paged_pass(float *x, int rows, int seqs, int longest, int max_len, int *status) {
+  BeamState &s = *beam_;
+  const int D = cfg_.EmbeddingDim, H = cfg_.NumHeads, hd = D / H, P = BeamState::kPage;
+  const float scale = 1.0f / std::sqrt((float)hd);
+  check(cdml_paged_plan(s.refs, s.pages, P, s.table, s.blocks, s.kv, s.new_len, seqs, rows, s.cu, s.slots, s.pos,
+                        status, stream_),
+        "cdml_paged_plan");
+  size_t ws = 0;
+  check(cdml_paged_attn_workspace_size(rows, seqs, longest, max_len, H, H, hd, &ws), "cdml_paged_attn_workspace_size");
+  void *work = beam_workspace(ws);
+  for (size_t i = 0; i < layers_.size(); ++i) {
+    const Layer &L = layers_[i];
+    float *k = s.k + i * s.layer_floats, *v = s.v + i * s.layer_floats;
+    check(cdml_project_qkv(x, L.wq, L.bq, L.wk, L.bk, L.wv, L.bv, q_, k_, v_, rows, D, D, stream_),
+          "cdml_project_qkv");
+    check(cdml_rope(q_, rows, D, 0, hd, H, 10000.0f, 0, 0, 0, s.pos, stream_), "cdml_rope");
+    check(cdml_rope(k_, rows, D, 0, hd, H, 10000.0f, 0, 0, 0, s.pos, stream_), "cdml_rope");
+    check(cdml_paged_append(k_, D, v_, D, k, v, CDML_CACHE_F32, s.slots, rows, s.pages, P, D, stream_),
+          "cdml_paged_append");
+    check(cdml_paged_attn(q_, D, k, v, CDML_CACHE_F32, s.pages, P, s.table, s.blocks, s.kv, s.cu, att_, D, rows, seqs,
+                          longest, max_len, H, H, hd, scale, nullptr, work, ws, stream_),
+          "cdml_paged_attn");
+    finish_block(L, x, rows);
+  }
+}
+
+BeamHypotheses DeviceLanguageModel::GenerateBeam(const std::vector<std::vector<int>> &prompts, int beams,
+                                                 int maxNewTokens, int eosToken, float lengthPenalty) {
+  if (!cfg_.UsesDiscreteTokens)
+    throw InvalidOperationException("Generate is only supported for discrete token data types.");
+  if (!cfg_.UseDecoderOnly) throw InvalidOperationException("GenerateBeam needs a decoder-only model.");
+  const int batch = (int)prompts.size(), S = cfg_.MaxSequenceLength, D = cfg_.EmbeddingDim, V = cfg_.VocabSize;
+  if (beams <= 0 || beams > 64) throw ArgumentOutOfRangeException("beams");
+  if (batch == 0 || (long long)batch * beams > cap_ || (long long)batch * beams > 4096)
+    throw ArgumentOutOfRangeException("prompts", "prompts * beams must lie within the batch capacity and 4096.");
+  if (maxNewTokens < 0) throw ArgumentOutOfRangeException("maxNewTokens", "maxNewTokens must be non-negative.");
+  if (eosToken >= V) throw ArgumentOutOfRangeException("eosToken");
+  if (!(lengthPenalty >= -16.0f && lengthPenalty <= 16.0f)) throw ArgumentOutOfRangeException("lengthPenalty");
+  const int R = batch * beams;
+  std::vector<int> ids, news(R, 0), last(R, -1);
+  size_t longest = 0;
+  for (int b = 0; b < batch; ++b) {
+    const std::vector<int> &p = prompts[b];
+    if (p.empty()) throw ArgumentException("Token sequence must contain at least one token.", "tokenIds");
+    if (p.size() > (size_t)S) throw ArgumentException("Token sequence length exceeds MaxSequenceLength.", "tokenIds");
+    for (int t : p)
+      if ((unsigned)t >= (unsigned)V) throw ArgumentOutOfRangeException("tokenIds");
+    ids.insert(ids.end(), p.begin(), p.end());
+    news[(size_t)b * beams] = (int)p.size();
+    last[(size_t)b * beams] = (int)ids.size() - 1;
+    longest = std::max(longest, p.size());
+  }
+  const int n = std::min(maxNewTokens, S - (int)longest), rows = (int)ids.size();
+  BeamHypotheses out;
+  out.beams = beams;
+  if (n == 0) {  // no room, or none wanted: the prompts alone
+    for (int r = 0; r < R; ++r) out.tokens.push_back(prompts[r / beams]);
+    out.scores.assign(R, 0.0f);
+    return out;
+  }
+  prepare_beams();
+  BeamState &s = *beam_;
+  // a search starts from an empty pool; only the first beam of a prompt holds it
+  std::vector<float> scores(R, -INFINITY);
+  for (int b = 0; b < batch; ++b) scores[(size_t)b * beams] = 0.0f;
+  const std::vector<uint8_t> open(R, 0);
+  check(cdml_fill_i32_async(s.refs, s.pages, 0, stream_), "page references");
+  check(cdml_fill_i32_async(s.kv, R, 0, stream_), "kv lengths");
+  check(cdml_fill_i32_async(s.lengths, R, 0, stream_), "lengths");
+  auto put = [&](void *dst, const void *src, size_t bytes) {
+    check(cdml_memcpy_h2d_async(dst, src, bytes, stream_), "cdml_memcpy_h2d_async");
+  };
+  put(ids_, ids.data(), ids.size() * sizeof(int));
+  put(s.new_len, news.data(), news.size() * sizeof(int));
+  put(s.gather, last.data(), last.size() * sizeof(int));
+  put(s.scores, scores.data(), scores.size() * sizeof(float));
+  put(s.finished, open.data(), open.size());
+  size_t select = 0, reorder = 0;
+  check(cdml_beam_select_workspace_size(batch, beams, V, &select), "cdml_beam_select_workspace_size");
+  check(cdml_paged_reorder_workspace_size(R, s.blocks, &reorder), "cdml_paged_reorder_workspace_size");
+  const float *hidden = h_;
+  for (int step = 0; step < n; ++step) {
+    int *status = s.status + (size_t)step * 6;
+    if (step == 0) {
+      check(cdml_embed_tokens(ids_, rows, emb_, V, D, x_, nullptr, stream_), "embed");
+      paged_pass(x_, rows, R, (int)longest, (int)longest, status);
+      // each prompt's last row for its first beam; the others' (-1) are zeros and offer nothing
+      check(cdml_embed_tokens(s.gather, R, x_, rows, D, h_, nullptr, stream_), "gather");
+      check(cdml_fill_i32_async(s.new_len, R, 1, stream_), "new tokens");
+    } else {
+      check(cdml_embed_tokens(s.tokens + (size_t)(step - 1) * R, R, emb_, V, D, x_, nullptr, stream_), "embed");
+      paged_pass(x_, R, R, 1, (int)longest + step, status);
+      hidden = x_;
+    }
+    check(cdml_linear(hidden, D, outproj_, outbias_, logits_, V, R, D, V, CDML_ACT_NONE, stream_), "output projection");
+    int *parents = s.parents + (size_t)step * R, *tokens = s.tokens + (size_t)step * R;
+    check(cdml_beam_select(logits_, V, s.scores, s.lengths, s.finished, batch, beams, V, eosToken, lengthPenalty,
+                           s.scores, s.lengths, s.finished, parents, tokens, beam_workspace(select), select, stream_),
+          "cdml_beam_select");
+    check(cdml_paged_reorder(s.refs, s.pages, BeamState::kPage, s.table, s.blocks, s.kv, parents, R, s.src, s.dst,
+                             status + 3, beam_workspace(reorder), reorder, stream_),
+          "cdml_paged_reorder");
+    check(cdml_paged_copy(s.k, s.v, CDML_CACHE_F32, (int)layers_.size(), s.layer_floats, s.pages, BeamState::kPage, D,
+                          s.src, s.dst, s.kv, R, stream_),
+          "cdml_paged_copy");
+  }
+  std::vector<int> parents((size_t)n * R), tokens((size_t)n * R), status((size_t)n * 6);
+  out.scores.resize(R);
+  auto get = [&](void *dst, const void *src, size_t bytes) {
+    check(cdml_memcpy_d2h_async(dst, src, bytes, stream_), "download");
+  };
+  get(parents.data(), s.parents, parents.size() * sizeof(int));
+  get(tokens.data(), s.tokens, tokens.size() * sizeof(int));
+  get(status.data(), s.status, status.size() * sizeof(int));
+  get(out.scores.data(), s.scores, out.scores.size() * sizeof(float));
+  synchronize();
+  for (int step = 0; step < n; ++step)
+    if (status[(size_t)step * 6] || status[(size_t)step * 6 + 3] || status[(size_t)step * 6 + 5])
+      throw InvalidOperationException("The paged cache ran out of pages.");
+  for (int r = 0; r < R; ++r) {
+    std::vector<int> tail(n);
+    for (int step = n - 1, at = r; step >= 0; --step) {
+      tail[step] = tokens[(size_t)step * R + at];
+      at = parents[(size_t)step * R + at];
+    }
+    // a finished beam repeats eosToken
+    const auto eos = eosToken < 0 ? tail.end() : std::find(tail.begin(), tail.end(), eosToken);
+    if (eos != tail.end()) tail.erase(eos + 1, tail.end());
+    std::vector<int> all(prompts[r / beams]);
+    all.insert(all.end(), tail.begin(), tail.end());
+    out.tokens.push_back(std::move(all));
   }
   return out;
 }
