@@ -19,7 +19,8 @@ inline int cache_type_bytes(int cache_type) {
 inline int check_pool(const char *what, int n_pages, int page_size, int max_blocks, int batch, int *shift) {
   if (page_size < 1 || page_size > 4096 || (page_size & (page_size - 1)))
     return fail(CDML_E_INVALID, "%s: page_size %d is no power of two up to 4096", what, page_size);
-  if (n_pages < 1 || (long long)n_pages * page_size > INT_MAX)
+  // (scans of page_refs step past the last page by less than 2^30)
+  if (n_pages < 1 || n_pages > (1 << 30) || (long long)n_pages * page_size > INT_MAX)
     return fail(CDML_E_INVALID, "%s: n_pages %d out of range", what, n_pages);
   if (max_blocks < 1 || (long long)max_blocks * page_size > INT_MAX)
     return fail(CDML_E_INVALID, "%s: max_blocks %d out of range", what, max_blocks);

@@ -206,7 +206,7 @@ def call_reorder(refs, table, kv, parents, P):
 
 
 def call_attention(q, kbits, vbits, kind, table, kv, cu, P, H, HK, scale, o, max_new=None, max_len=None, ldq=None,
-                   n_pages=None):
+                   n_pages=None, ldo=None):
     """q, o [rows, H * hd]; returns (o, bad)."""
     rows, B, hd = len(q), len(kv), q.shape[1] // H
     ldq = ldq or q.shape[1]
@@ -214,13 +214,18 @@ def call_attention(q, kbits, vbits, kind, table, kv, cu, P, H, HK, scale, o, max
     wide[:, :q.shape[1]] = q
     max_new = int(np.max(np.diff(cu), initial=0)) if max_new is None else max_new
     max_len = int(np.max(kv, initial=0)) if max_len is None else max_len
-    dq, dk, dv, do = up(wide), up(kbits, raw_dtype(kind)), up(vbits, raw_dtype(kind)), up(o)
+    ldo = ldo or o.shape[1]
+    out = np.full((rows, ldo), 7.0, np.float32)
+    out[:, :o.shape[1]] = o
+    dq, dk, dv, do = up(wide), up(kbits, raw_dtype(kind)), up(vbits, raw_dtype(kind)), up(out)
     dt, dl, dc, bad = ints(table), ints(kv), ints(cu), ints(np.zeros(1))
     w, n = ws("cdml_paged_attn_workspace_size", rows, B, max_new, max_len, H, HK, hd)
     N.check(N.lib().cdml_paged_attn(dq.ptr, ldq, dk.ptr, dv.ptr, N.CACHE[kind], n_pages or len(kbits), P, dt.ptr,
-                                    table.shape[1], dl.ptr, dc.ptr, do.ptr, H * hd, rows, B, max_new, max_len, H, HK,
+                                    table.shape[1], dl.ptr, dc.ptr, do.ptr, ldo, rows, B, max_new, max_len, H, HK,
                                     hd, scale, bad.ptr, w.ptr, n, stream().handle))
-    return down(do, o.shape), int(down(bad, (1,), np.int32)[0])
+    out = down(do, out.shape)
+    assert (out[:, o.shape[1]:] == 7.0).all()
+    return out[:, :o.shape[1]], int(down(bad, (1,), np.int32)[0])
 
 
 def call_beam(x, scores, lengths, done, K, eos, alpha, in_place=False, ldl=None):

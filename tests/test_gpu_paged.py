@@ -125,8 +125,9 @@ def attention_case(r, kind, lens, news, P, H, HK, hd, pad=0, blocks=None):
     return q, bits, table, np.array(lens, np.int32), cu, o
 
 
-def check_attention(kind, q, bits, table, kv, cu, o, P, H, HK, **more):
-    scale = float(np.float32(1) / np.sqrt(np.float32(q.shape[1] // H)))
+def check_attention(kind, q, bits, table, kv, cu, o, P, H, HK, scale=None, **more):
+    if scale is None:
+        scale = float(np.float32(1) / np.sqrt(np.float32(q.shape[1] // H)))
     k, v = (M.from_bits(b, kind).astype(np.float64) for b in bits)
     want, tol = M.attention(q, k, v, table, kv, cu, P, H, HK, scale, o)
     got, bad = M.call_attention(q, *bits, kind, table, kv, cu, P, H, HK, scale, o, **more)
@@ -265,11 +266,93 @@ def test_bounds_cut_lengths():
     np.testing.assert_array_equal(got[2:6], o[2:6])
 
 
-def test_strided_rows():
+@pytest.mark.parametrize("news", [[30, 1], [3, 1], [1, 1]])
+def test_strided_rows(news):
     r = rng(14)
-    for ldq in (130, 132):
-        q, bits, table, kv, cu, o = attention_case(r, "bf16", [100, 60], [30, 1], 16, 2, 1, 64)
-        check_attention("bf16", q, bits, table, kv, cu, o, 16, 2, 1, ldq=ldq)
+    for ldq, ldo in ((130, 128), (132, 140), (128, 129)):
+        q, bits, table, kv, cu, o = attention_case(r, "bf16", [100, 60], news, 16, 2, 1, 64)
+        check_attention("bf16", q, bits, table, kv, cu, o, 16, 2, 1, ldq=ldq, ldo=ldo)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("news", [[1, 1], [7, 2], [50, 1]])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 40.0])
+def test_scales(kind, news, scale):
+    # no weight on the scores at all, a negative one, and one that leaves a single key
+    r = rng(15)
+    q, bits, table, kv, cu, o = attention_case(r, kind, [100, 60], news, 16, 2, 1, 32)
+    check_attention(kind, q, bits, table, kv, cu, o, 16, 2, 1, scale=scale)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [4, 60])
+def test_a_broken_key_or_query_stays_in_its_rows(kind, n):
+    r = rng(16)
+    q, bits, table, kv, cu, o = attention_case(r, kind, [90], [n], 16, 2, 2, 64)
+    first_seen = 90 - n
+    bits[0].reshape(-1, 128)[table[0, (first_seen + 2) // 16] * 16 + (first_seen + 2) % 16] = M.to_bits(np.full(1, np.nan), kind)[0]
+    q[1, :64] = np.inf
+    got = check_attention(kind, q, bits, table, kv, cu, o, 16, 2, 2)
+    assert np.isfinite(got[0]).all() and np.isfinite(got[1, 64:]).all() and np.isnan(got[1, :64]).all()
+    assert np.isnan(got[2:]).all()
+
+
+def test_queries_out_of_the_split_range():
+    # components below 2^-110 beside ordinary ones, and large ones against small keys
+    r = rng(17)
+    for news in ([7], [60]):
+        q, bits, table, kv, cu, o = attention_case(r, "f32", [90], news, 16, 1, 1, 64)
+        q[:, ::3] *= np.float32(2.0 ** -118)
+        check_attention("f32", q, bits, table, kv, cu, o, 16, 1, 1)
+        q *= np.float32(2.0 ** 105)
+        bits[0] *= np.float32(2.0 ** -105)
+        check_attention("f32", q, bits, table, kv, cu, o, 16, 1, 1)
+
+
+@pytest.mark.parametrize("kind,news", [("f32", 1), ("bf16", 1), ("bf16", 6), ("f32", 40), ("bf16", 40)])
+def test_offsets_past_32_bits(kind, news):
+    """Pages at the end of a cache of over 2^32 bytes (and, in fp32, 2^31 elements) a tensor: written by
+    cdml_paged_append, read back by the attention.  Only the pages in use are ever touched."""
+    r = rng(18)
+    P, H, hd = 16, 8, 128
+    D, n_pages = H * hd, 140_000
+    size = n_pages * P * D * (4 if kind == "f32" else 2)
+    assert size > 2 ** 32
+    lens = np.array([70, 45], np.int32)
+    table = np.array([[n_pages - 1, 3, n_pages - 9, n_pages - 2, n_pages // 2 + 1], [n_pages - 5, n_pages - 4, 0, -1, -1]],
+                     np.int32)
+    k, v = (r.standard_normal((lens.sum(), D)).astype(np.float32) for _ in range(2))
+    slots = np.concatenate([table[b, np.arange(m) // P] * P + np.arange(m) % P for b, m in enumerate(lens)])
+    kc, vc = N.DeviceBuffer(size), N.DeviceBuffer(size)
+    dk, dv, ds = up(k), up(v), M.ints(slots)
+    N.check(N.lib().cdml_paged_append(dk.ptr, D, dv.ptr, D, kc.ptr, vc.ptr, N.CACHE[kind], ds.ptr, len(slots), n_pages,
+                                      P, D, stream().handle))
+    rows = 2 * news
+    q, cu = r.standard_normal((rows, D)).astype(np.float32), np.array([0, news, rows], np.int32)
+    dq, do, dt, dl, dc, bad = up(q), N.DeviceBuffer(4 * rows * D), M.ints(table), M.ints(lens), M.ints(cu), M.ints([0])
+    args = (rows, 2, news, 80, H, H, hd)
+    w, n = M.ws("cdml_paged_attn_workspace_size", *args)
+    N.check(N.lib().cdml_paged_attn(dq.ptr, D, kc.ptr, vc.ptr, N.CACHE[kind], n_pages, P, dt.ptr, 5, dl.ptr, dc.ptr,
+                                    do.ptr, D, *args, 0.09, bad.ptr, w.ptr, n, stream().handle))
+    got = down(do, (rows, D))
+    small = np.concatenate([[0], np.cumsum(lens)])
+    rounded = [M.from_bits(M.to_bits(x, kind), kind).astype(np.float64) for x in (k, v)]
+    for b in range(2):
+        own = [x[small[b]:small[b + 1]][:, None] for x in rounded]
+        want, tol = M.attention(q[b * news:(b + 1) * news], *own, np.arange(lens[b])[None], lens[b:b + 1],
+                                np.array([0, news]), 1, H, H, 0.09, np.zeros((news, D)))
+        assert (np.abs(got[b * news:(b + 1) * news] - want) <= tol).all()
+    assert down(bad, (1,), np.int32)[0] == 0
+
+
+def test_many_requests():
+    r = rng(19)
+    B = 700
+    lens = r.integers(0, 40, B).tolist()
+    news = [min(int(n), m) for n, m in zip(r.integers(0, 4, B), lens)]
+    news[333], lens[333] = 30, 37
+    case = attention_case(r, "bf16", lens, news, 8, 2, 1, 16, pad=3)
+    check_attention("bf16", *case, 8, 2, 1)
 
 
 # ---- reorder and copies ------------------------------------------------------------------
@@ -299,6 +382,30 @@ def test_reorder_follows_the_plain_form(R, P, blocks, steps):
         got = M.call_plan(refs, table, kv, new, P, R)
         same(got, want)
         refs, table, kv = got[:3]
+
+
+@pytest.mark.parametrize("R", [6, 50])
+def test_released_pages_are_taken_again(R):
+    r = rng(22, R)
+    P, blocks = 4, 6
+    lens = r.integers(1, 16, R).astype(np.int32)
+    refs, table = pool(r, R, blocks, P, lens, held=0)
+    kv = lens
+    for turn in range(4):
+        parents = np.where(np.arange(R) % 3 == turn % 3, -1, np.arange(R)).astype(np.int32)
+        want = M.reorder(refs, table, kv, parents, P)
+        got = M.call_reorder(refs, table, kv, parents, P)
+        same(got, want)
+        refs, table, kv = got[:3]
+        assert (kv[parents < 0] == 0).all() and refs.sum() == sum(-(-m // P) for m in kv)
+        new = np.where(parents < 0, 9, 0).astype(np.int32)
+        want = M.plan(refs, table, kv, new, P, int(new.sum()))
+        got = M.call_plan(refs, table, kv, new, P, int(new.sum()))
+        assert got[-1][0] == 0
+        same(got, want)
+        refs, table, kv = got[:3]
+    nobody = np.full(R, -1, np.int32)
+    assert not M.call_reorder(refs, table, kv, nobody, P)[0].any()
 
 
 def test_reorder_without_room_cuts_to_full_pages():

@@ -20,7 +20,8 @@ def refused(name, good, changes):
         assert name.encode() in N.lib().cdml_last_error(), change
 
 
-POOL = [{"page_size": n} for n in (0, -1, 3, 24, 8192)] + [{"n_pages": 0}, {"n_pages": -4}, {"n_pages": BIG}]
+POOL = [{"page_size": n} for n in (0, -1, 3, 24, 8192)] + [
+    {"n_pages": 0}, {"n_pages": -4}, {"n_pages": BIG}, {"n_pages": 2 ** 30 + 1, "page_size": 1}]
 
 
 def test_plan_refusals():
