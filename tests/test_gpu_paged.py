@@ -284,6 +284,42 @@ def test_scales(kind, news, scale):
     check_attention(kind, q, bits, table, kv, cu, o, 16, 2, 1, scale=scale)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [4, 60, 200])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("where", [5, 239])
+def test_a_huge_key_or_value_among_ordinary_ones(kind, n, which, where):
+    # one token's K or V is 10^30 in a few dims; the rows that do not see it, or give it no weight, are exact
+    r = rng(23)
+    q, bits, table, kv, cu, o = attention_case(r, kind, [240, 30], [n, 30], 16, 2, 2, 64)
+    x = M.from_bits(bits[which], kind).reshape(-1, 128).copy()
+    at = table[0, where // 16] * 16 + where % 16
+    x[at, 5:9] = 1e30
+    bits[which] = M.to_bits(x, kind).reshape(bits[which].shape)
+    if which == 1:
+        k = M.from_bits(bits[0], kind).reshape(-1, 128).copy()
+        k[at] = -50 * np.sign(q[0])  # the first row's head gives the token no weight
+        bits[0] = M.to_bits(k, kind).reshape(bits[0].shape)
+    check_attention(kind, q, bits, table, kv, cu, o, 16, 2, 2)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_magnitudes_that_change_along_the_keys(kind):
+    # V grows and shrinks by tens along the request, some dims are always small, some keys zero
+    r = rng(24)
+    q, bits, table, kv, cu, o = attention_case(r, kind, [600, 333], [70, 333], 16, 2, 1, 64)
+    k, v = (M.from_bits(b, kind).copy() for b in bits)
+    for b, m in enumerate((600, 333)):
+        at = np.arange(m)
+        v[table[b, at // 16], at % 16] *= (10.0 ** np.sin(at / 40))[:, None].astype(np.float32)
+        v[table[b, at[::17] // 16], at[::17] % 16] = 0
+        k[table[b, at[::13] // 16], at[::13] % 16] = 0
+    v[..., 7:13] *= np.float32(1 / 64)
+    k[..., 20:24] *= np.float32(1 / 64)
+    bits = [M.to_bits(x, kind) for x in (k, v)]
+    check_attention(kind, q, bits, table, kv, cu, o, 16, 2, 1)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n", [4, 60])
 def test_a_broken_key_or_query_stays_in_its_rows(kind, n):
