@@ -540,14 +540,21 @@ struct PagedStage {
       }
       return;
     }
-    // a value that the scale does not hold moves it (infinities and NaNs do not)
+    // a value that the scale does not hold moves it (infinities and NaNs do not: beside one,
+    // K's largest finite value would otherwise overflow and its key could vanish)
     float most = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       most = fmaxf(most, fmaxf(fmaxf(fabsf(value(i, 0)), fabsf(value(i, 1))), fmaxf(fabsf(value(i, 2)), fabsf(value(i, 3)))));
     auto low = [&] { return __float_as_uint(most) - 1u < below; };  // (not 0)
     if (__builtin_amdgcn_ballot_w64(most >= above || low())) {
-      most = most < INFINITY ? most : 0.f;
+      if (__builtin_amdgcn_ballot_w64(most == INFINITY)) {
+        most = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) most = fmaxf(most, fabsf(value(i, c)) < INFINITY ? fabsf(value(i, c)) : 0.f);
+      }
       const float top = wave_max(most);
       if (top >= above) set_expo(min(expo_of(top), 126));
       if (low()) *coarse = 1;

@@ -333,6 +333,23 @@ def test_a_broken_key_or_query_stays_in_its_rows(kind, n):
     assert np.isnan(got[2:]).all()
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("first", [0.02, 0.021, 0.022])
+def test_a_large_key_beside_unseen_infinities(kind, hd, first):
+    # K's largest values stand next to infinite ones that the rows do not see
+    r = rng(29)
+    q, bits, table, kv, cu, o = attention_case(r, kind, [73], [64], 16, 1, 1, hd)
+    k = M.from_bits(bits[0], kind).copy()
+    k[table[0, 33 // 16], 33 % 16, 0] = -100
+    at = np.arange(41, 73)  # row 31 sees keys up to 40
+    k[table[0, at // 16], at % 16] = np.inf
+    bits[0] = M.to_bits(k, kind)
+    q[:, 0] = first
+    got = check_attention(kind, q, bits, table, kv, cu, o, 16, 1, 1)
+    assert np.isfinite(got[:32]).all()
+
+
 def test_queries_out_of_the_split_range():
     # components below 2^-110 beside ordinary ones, and large ones against small keys
     r = rng(17)
