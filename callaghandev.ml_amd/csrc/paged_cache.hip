@@ -534,7 +534,9 @@ extern "C" int cdml_paged_plan(int *page_refs, int n_pages, int page_size, int *
   PlanArgs a{};
   int rc = check_pool("cdml_paged_plan", n_pages, page_size, max_blocks, batch, &a.page_shift);
   if (rc) return rc;
-  if (rows < 0) return fail(CDML_E_INVALID, "cdml_paged_plan: rows %d is negative", rows);
+  // (row numbers step past the last row by less than 2^30)
+  if (rows < 0 || rows > (1 << 30))
+    return fail(CDML_E_INVALID, "cdml_paged_plan: rows %d outside [0, 2^30]", rows);
   if (!cu_new || !status || (rows && (!slots || !positions)) ||
       (batch && (!page_refs || !block_table || !kv_len || !new_len)))
     return fail(CDML_E_INVALID, "cdml_paged_plan: NULL pointer");

@@ -606,10 +606,12 @@ int cdml_kv_cache_append(const float *k_new, const float *v_new,
  *   - page_refs (device int32[n_pages], 16-byte aligned) counts the requests a
  *     page belongs to, 0 for a free page.  All of them start as zeros.
  * page_size is a power of two up to 4096, n_pages <= 2^30, n_pages * page_size
- * < 2^31 and batch <= 4096.  One step of a model: cdml_paged_plan; in every layer cdml_rope with
- * the plan's positions, cdml_paged_append, cdml_paged_attn; then, in a beam
- * search, cdml_beam_select, cdml_paged_reorder and cdml_paged_copy.  All of it
- * may be captured into a graph: lengths stay on the device. */
+ * < 2^31, batch <= 4096 and a step's rows <= 2^30.  One step of a model:
+ * cdml_paged_plan; in every layer cdml_rope with the plan's positions,
+ * cdml_paged_append, cdml_paged_attn; then, in a beam search, cdml_beam_select,
+ * cdml_paged_reorder and cdml_paged_copy.  All of it may be captured into a
+ * graph: lengths stay on the device.  Calls that may run at the same time need
+ * workspaces of their own; a workspace holds nothing from one call to the next. */
 #define CDML_CACHE_F32 0
 #define CDML_CACHE_F16 1
 #define CDML_CACHE_BF16 2

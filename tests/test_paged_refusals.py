@@ -28,7 +28,8 @@ def test_plan_refusals():
     good = dict(refs=P, n_pages=8, page_size=16, table=P, max_blocks=4, kv_len=P, new_len=P, batch=2, rows=3, cu=P,
                 slots=P, positions=P, status=P, stream=None)
     refused("cdml_paged_plan", good, POOL + [
-        {"max_blocks": 0}, {"max_blocks": BIG}, {"batch": -1}, {"batch": 4097}, {"rows": -1}, {"refs": ODD}] + [
+        {"max_blocks": 0}, {"max_blocks": BIG}, {"batch": -1}, {"batch": 4097}, {"rows": -1}, {"rows": BIG},
+        {"refs": ODD}] + [
         {k: None} for k in ("refs", "table", "kv_len", "new_len", "cu", "slots", "positions", "status")])
 
 
