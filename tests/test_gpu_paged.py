@@ -2,6 +2,8 @@
 against plain numpy and float64 restatements (paged_model.py)."""
 from __future__ import annotations
 
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -554,7 +556,6 @@ def test_serving_run_in_a_graph(kind):
         if graph is None:
             e.step(s)  # the first step runs eagerly; a second run of it would append again
             s.synchronize()
-            import ctypes as C
             graph = C.c_void_p()
             N.check(N.lib().cdml_graph_capture_begin(s.handle))
             e.step(s)
@@ -617,3 +618,67 @@ def test_large_pools_in_spans():
     parents = np.array([0, 0, 0, 1, 1, 5], np.int32)
     want = M.reorder(refs, table, kv, parents, P)
     same(M.call_reorder(refs, table, kv, parents, P), want)
+
+
+@pytest.mark.parametrize("B,K,V", [(3, 4, 300), (10, 5, 6000)])
+def test_beam_steps_in_a_graph(B, K, V):
+    """Plan, append, selection in place, reordering and copies, captured once: every replay equals the plain forms,
+    with work and synchronisation of other kinds between the replays."""
+    r = rng(32, B)
+    R, P, blocks, dim, steps = B * K, 4, 7, 8, 6
+    pages, L, s = R * blocks, N.lib(), N.Stream()
+    refs, table, kv = np.zeros(pages, np.int32), np.full((R, blocks), -1, np.int32), np.zeros(R, np.int32)
+    cache = [np.zeros((pages, P, dim), np.float32) for _ in range(2)]
+    scores = -np.abs(r.standard_normal(R)).astype(np.float32)
+    lengths, done = np.ones(R, np.int32), np.zeros(R, np.uint8)
+    d_refs, d_table, d_kv, d_len, d_new = (M.ints(a) for a in (refs, table, kv, lengths, np.ones(R)))
+    d_cu, d_slots, d_pos, d_par, d_tok, d_src, d_dst, st1, st2 = (M.ints(np.zeros(R + 3)) for _ in range(9))
+    d_k, d_v, d_scores, d_x = up(cache[0]), up(cache[1]), up(scores), up(np.zeros((R, V)))
+    d_done, d_nk, d_nv = up(done, np.uint8), up(np.zeros((R, dim))), up(np.zeros((R, dim)))
+    w1, n1 = M.ws("cdml_beam_select_workspace_size", B, K, V)
+    w2, n2 = M.ws("cdml_paged_reorder_workspace_size", R, blocks)
+    h = s.handle
+
+    def step():
+        N.check(L.cdml_paged_plan(d_refs.ptr, pages, P, d_table.ptr, blocks, d_kv.ptr, d_new.ptr, R, R, d_cu.ptr,
+                                  d_slots.ptr, d_pos.ptr, st1.ptr, h))
+        N.check(L.cdml_paged_append(d_nk.ptr, dim, d_nv.ptr, dim, d_k.ptr, d_v.ptr, 0, d_slots.ptr, R, pages, P, dim, h))
+        N.check(L.cdml_beam_select(d_x.ptr, V, d_scores.ptr, d_len.ptr, d_done.ptr, B, K, V, 2, 0.5, d_scores.ptr,
+                                   d_len.ptr, d_done.ptr, d_par.ptr, d_tok.ptr, w1.ptr, n1, h))
+        N.check(L.cdml_paged_reorder(d_refs.ptr, pages, P, d_table.ptr, blocks, d_kv.ptr, d_par.ptr, R, d_src.ptr,
+                                     d_dst.ptr, st2.ptr, w2.ptr, n2, h))
+        N.check(L.cdml_paged_copy(d_k.ptr, d_v.ptr, 0, 1, 0, pages, P, dim, d_src.ptr, d_dst.ptr, d_kv.ptr, R, h))
+
+    graph = C.c_void_p()
+    N.check(L.cdml_graph_capture_begin(h))
+    step()
+    N.check(L.cdml_graph_capture_end(h, C.byref(graph)))
+    for _ in range(steps):
+        x = (r.standard_normal((R, V)) * 2).astype(np.float32)
+        nk, nv = r.standard_normal((2, R, dim)).astype(np.float32)
+        for buf, a in ((d_x, x), (d_nk, nk), (d_nv, nv)):
+            buf.upload(a, s)
+        N.check(L.cdml_graph_launch(graph, h))
+        refs, table, kv, _, slots, _, _ = M.plan(refs, table, kv, np.ones(R, np.int64), P, R)
+        for c, a in zip(cache, (nk, nv)):
+            c.reshape(-1, dim)[slots] = a
+        want = M.beam(x, scores, lengths, done, K, 2, 0.5)
+        refs, table, kv, src, dst, status = M.reorder(refs, table, kv, want[3], P)
+        for c in cache:
+            for b in np.flatnonzero(dst >= 0):
+                c[dst[b], :kv[b] % P] = c[src[b], :kv[b] % P]
+        lengths, done = want[1], want[2]
+        scores = d_scores.download((R,), np.float32, s)
+        assert np.allclose(scores, want[0], rtol=2.0 ** -23, atol=2.0 ** -23)
+        same([d.download((R,), t, s) for d, t in ((d_len, np.int32), (d_done, np.uint8), (d_par, np.int32),
+                                                  (d_tok, np.int32), (d_kv, np.int32), (d_src, np.int32))],
+             (lengths, done, want[3], want[4], kv, src))
+        same([d_refs.download((pages,), np.int32, s), st2.download((3,), np.int32, s)], (refs, status))
+        got = d_table.download((R, blocks), np.int32, s)
+        for b in range(R):
+            used = -(-int(kv[b]) // P)
+            np.testing.assert_array_equal(got[b, :used], table[b, :used])
+        used = refs > 0
+        for d, c in zip((d_k, d_v), cache):
+            np.testing.assert_array_equal(d.download(c.shape, np.float32, s)[used], c[used])
+    N.check(L.cdml_graph_destroy(graph))
