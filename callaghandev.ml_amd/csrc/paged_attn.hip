@@ -131,14 +131,22 @@ Plan make_plan(int size, int rows, int batch, int max_new, int max_len, int head
   } else if (groups > 2) {
     p.few_chunk = round_up(len, kPagedSub);  // rows without number (head dims above 128) are not split
   } else {
-    // 512 keys a workgroup while there are four workgroups for every CU, else 256
+    // One chunk, which needs no join, up to 512 keys, or up to 1024 where requests and heads
+    // fill the CUs: 16 heads of 64, bf16, 64 x 500 keys 25.7 us, 30.4 in chunks of 256; 4 x
+    // 1000 keys 13.8 in one, 9.6 in 256s; 64 x 1000 keys 49.8 in one, 55.0.  Else 256 keys, or
+    // 512 of fp32 where that leaves four workgroups for every CU: 16 heads of 128, fp32, 64 x
+    // 8000 keys 1248 us, 1286 in 256s, but 1 x 2000 keys 15.8, 12.8 in 256s; 16 heads of 64,
+    // bf16, 64 x 2000 keys 103.6, 91.5 in 256s.
     const long long wide = (long long)((len - 1) / 512 + 1) * pairs * groups;
-    p.few_chunk = wide >= 4 * kComputeUnits ? 512 : 256;
+    const bool one = len <= 512 || (len <= 1024 && pairs * groups >= kComputeUnits);
+    p.few_chunk = one ? round_up(len, 256) : size == 4 && wide >= 4 * kComputeUnits ? 512 : 256;
   }
   p.few_splits = (len - 1) / p.few_chunk + 1;
   if ((k.rows || k.span) && p.few_splits > 1)
     p.few_floats = (size_t)batch * kv_heads * p.few_rows * p.few_splits * (hd + 2);
-  // matrix cores: keys are split where the tiles alone leave CUs without work
+  // Matrix cores: keys are split where the tiles alone leave CUs without work, to two
+  // workgroups for every CU.  16 heads of 64, bf16: 256 tokens over 8192 keys 69.9 us, 66.5
+  // with twice the splits, 338 with none; 4 x 512 over 4096 146, 154, 195.
   p.tile_chunk = INT_MAX;
   p.tile_splits = 1;
   if (k.tile) {
