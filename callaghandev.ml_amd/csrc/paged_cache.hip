@@ -172,7 +172,7 @@ constexpr int PLAN_LIST = 8192;  // pages that are handed out at a time
 
 // One workgroup: sums of pages and tokens over the requests, a count of free pages up to
 // the need, then the scan that takes them.  A chain of memory round trips bounds it: 64
-// requests over 40000 pages take PLAN_US us.
+// requests over 40000 pages take 10.8 us.
 __global__ void __launch_bounds__(PC_THREADS) paged_plan_kernel(const PlanArgs a) {
   __shared__ int pages[kPagedMaxBatch + 1], cu[kPagedMaxBatch + 1];  // exclusive sums
   __shared__ int old[kPagedMaxBatch];                                // kv_len before
@@ -477,7 +477,9 @@ __device__ __forceinline__ void place_copies(const ReorderArgs &a, CopyScratch &
 }
 
 constexpr int REFS_THREADS = 256;
-constexpr int REORDER_ONE = 32;  // rows up to which one workgroup does all
+// Rows up to which one workgroup does all, a wave each: 16 rows of two layers, copies
+// included, 11.7 us in one launch, 12.2 in two; 32 rows 13.9, 12.4.
+constexpr int REORDER_ONE = PC_WAVES;
 
 __global__ void __launch_bounds__(REFS_THREADS) paged_refs_kernel(const ReorderArgs a) {
   const int r = blockIdx.x * (REFS_THREADS / 64) + (threadIdx.x >> 6);
@@ -498,10 +500,13 @@ __global__ void __launch_bounds__(PC_THREADS) paged_tables_kernel(const ReorderA
 // All of it in one workgroup, for few rows.
 __global__ void __launch_bounds__(PC_THREADS) paged_reorder_kernel(const ReorderArgs a) {
   __shared__ CopyScratch sc;
-  for (int r = threadIdx.x >> 6; r < a.batch; r += PC_WAVES) count_refs(a, r);
-  __threadfence();  // references are counted in L2
+  const int r = threadIdx.x >> 6;
+  if (r < a.batch) count_refs(a, r);
+  // References are counted in L2, and nothing has read them into the CU's cache: once the
+  // sums are done (this wait; a fence for the whole device takes 2.6 us), place_copies sees them.
+  __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  for (int r = threadIdx.x >> 6; r < a.batch; r += PC_WAVES) write_table(a, r);
+  if (r < a.batch) write_table(a, r);
   place_copies(a, sc);
 }
 
@@ -555,7 +560,9 @@ extern "C" int cdml_paged_plan(int *page_refs, int n_pages, int page_size, int *
   a.slots = slots;
   a.positions = positions;
   a.status = status;
-  a.fill = rows <= 4 * PC_THREADS;
+  // (8 x 256 rows 10.0 us so, 13.0 with a launch of their own; 8 x 1021 10.4, 12.9; 32 x 1021
+  // 19.7 so, 14.6)
+  a.fill = rows <= 8 * PC_THREADS;
   paged_plan_kernel<<<1, PC_THREADS, 0, as_hip(stream)>>>(a);
   rc = check_launch("paged_plan_kernel");
   if (rc || a.fill) return rc;
