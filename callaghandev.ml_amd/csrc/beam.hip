@@ -27,8 +27,14 @@ namespace {
 constexpr int BS_THREADS = 256;
 // Logits a lane holds, and a wave with it: a segment.
 constexpr int BS_LONG = 32, BS_SHORT = 8;
-constexpr int BS_SHORT_VOCAB = 4096;  // up to here segments are short
+constexpr int BS_PICK = 8;  // values a lane of the pick kernel holds, one for those picked before
 constexpr int BS_MAX_BEAMS = 64;
+// Short segments, while they leave a wave or so for every place on the card and a row's
+// candidates to one pass of the pick kernel.  8 beams of 64 requests over 2048 logits (2048
+// segments) 15.7 us in long ones, 14.4 in short, over 8192 (8192) 16.5, 19.2; of 4 requests
+// over 16000 (252 candidates) 16.2, 14.6, over 50021 (784) 16.1, 19.7; 4 of 4 over 50021 (392)
+// 12.1, 11.5.
+constexpr int BS_SHORT_SEGMENTS = 4096, BS_SHORT_CANDIDATES = 64 * (BS_PICK - 1);
 
 struct BeamArgs {
   const float *x;
@@ -185,6 +191,8 @@ __device__ __forceinline__ float drop_nans(float (&v)[E]) {
   return best;
 }
 
+// Reading the logits bounds it: 512 rows of 50021 (102 MB) take 25 us, 4.1 TB/s; a wave
+// reads once and then computes, and others' reads hide that.
 template <int E>
 __global__ void __launch_bounds__(BS_THREADS) beam_rows_kernel(const BeamArgs a) {
   __shared__ TopList lists[BS_THREADS / 64];
@@ -208,7 +216,10 @@ __global__ void __launch_bounds__(BS_THREADS) beam_rows_kernel(const BeamArgs a)
                 [&](int e) { return (seg * E + e) * 64 + lane; });
 }
 
-// ONE: the whole vocabulary is one short segment, and its row's wave reads the logits itself.
+// ONE: the whole vocabulary is one short segment, and its row's wave reads the logits itself
+// (8 beams of 64 requests, vocabulary 512: 9.6 us; 14.2 with a launch for the rows).  Chains of
+// reductions over a wave bound it, the merge's one for each of the beams: 8 x 8 beams with 25
+// segments 10 us.
 template <bool ONE>
 __global__ void __launch_bounds__(1024) beam_pick_kernel(const BeamArgs a) {
   extern __shared__ char smem[];  // per beam: [beams] logits, [beams] tokens
@@ -244,7 +255,7 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(const BeamArgs a) {
     }
     const size_t at = (size_t)(row0 + k) * a.n_seg;
     // the row's candidates, seven a lane and pass, beside the best K of the passes before
-    constexpr int E = 8;
+    constexpr int E = BS_PICK;
     const int n_cand = a.n_seg * K;
     float v[E];
     int t[E];
@@ -353,7 +364,9 @@ struct Layout {
 };
 Layout layout(int batch, int beams, int vocab) {
   Layout l{};
-  l.per_lane = vocab <= BS_SHORT_VOCAB ? BS_SHORT : BS_LONG;
+  const long long shorts = ((long long)vocab + 64 * BS_SHORT - 1) / (64 * BS_SHORT);
+  const bool few = (long long)batch * beams * shorts <= BS_SHORT_SEGMENTS && beams * shorts <= BS_SHORT_CANDIDATES;
+  l.per_lane = few ? BS_SHORT : BS_LONG;
   const int seg = 64 * l.per_lane;
   l.n_seg = (int)(((long long)vocab + seg - 1) / seg);
   const size_t n = (size_t)batch * beams * l.n_seg;
