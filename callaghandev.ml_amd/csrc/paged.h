@@ -32,6 +32,22 @@ inline int check_pool(const char *what, int n_pages, int page_size, int max_bloc
 
 }  // namespace
 
+// Inclusive sum over the lanes of a wave: within rows of 16 lanes by shifts, then each row's
+// last lane to the rows after it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t shifted(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += shifted<0x111, 0xf>(x);
+  x += shifted<0x112, 0xf>(x);
+  x += shifted<0x114, 0xf>(x);
+  x += shifted<0x118, 0xf>(x);
+  x += shifted<0x142, 0xa>(x);
+  x += shifted<0x143, 0xc>(x);
+  return x;
+}
+
 // A request's rows are numbered token-major: row rr of K/V head hk is head hk * group +
 // rr % group of its new token rr / group.  Requests with at most few_rows rows a K/V head
 // split their keys into chunks of few_chunk, those with more run in tiles of 128 rows and

@@ -28,22 +28,6 @@ struct PlanArgs {
   int fill;  // whether the planning workgroup writes slots and positions itself
 };
 
-// Inclusive sum over the lanes of a wave: within rows of 16 lanes by shifts, then each row's
-// last lane to the rows after it.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t shifted(uint32_t x) {
-  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-  x += shifted<0x111, 0xf>(x);
-  x += shifted<0x112, 0xf>(x);
-  x += shifted<0x114, 0xf>(x);
-  x += shifted<0x118, 0xf>(x);
-  x += shifted<0x142, 0xa>(x);
-  x += shifted<0x143, 0xc>(x);
-  return x;
-}
-
 // Inclusive sums of x and y (below 2^31) over the workgroup's threads, and their totals.
 // They are summed as halves of 16 bits, which 4096 terms cannot overflow.
 struct ScanScratch {

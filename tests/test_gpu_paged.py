@@ -410,6 +410,18 @@ def test_many_requests():
     check_attention("bf16", *case, 8, 2, 1)
 
 
+@pytest.mark.parametrize("B", [2, 64, 65, 140])
+def test_tiles_of_many_ragged_requests(B):
+    # every tile of every request is met once, whatever the order: long and short, few rows, none, rows without a key
+    r = rng(33, B)
+    news = np.where(r.random(B) < 0.2, r.integers(0, 5, B), r.integers(0, 100, B))
+    lens = np.where(r.random(B) < 0.3, news, news + r.integers(0, 500, B))
+    news[B // 2], lens[B // 2] = 260, 300
+    news[1], lens[1] = 70, 10
+    case = attention_case(r, "bf16", lens.tolist(), news.tolist(), 16, 4, 1, 16, pad=5, blocks=48)
+    check_attention("bf16", *case, 16, 4, 1)
+
+
 # ---- reorder and copies ------------------------------------------------------------------
 
 @pytest.mark.parametrize("R,P,blocks,steps", [(1, 16, 4, 3), (8, 4, 6, 6), (40, 16, 5, 5), (300, 2, 9, 3),
