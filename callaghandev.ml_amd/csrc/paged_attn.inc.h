@@ -92,7 +92,7 @@ struct RowSlice {
 // keeps an online softmax of its own keys.  The four waves take 64 / LPK keys in turn.
 // U sets of rows go round, so that the loads of U - 1 steps are in flight while one is
 // consumed: four where 64 registers hold them (8 x 2048 keys of bf16, 16 heads of 64: 15.0
-// -> 14.4 us).
+// -> 14.4 us).  HBM bounds it: 64 x 8192 keys, 16 heads of 128, fp32 1248 us, 6.9 TB/s.
 template <typename T, int HD, int R, int MODE>
 __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedArgs a) {
   constexpr int LPK = HD >= 64 && R > 2 ? 16 : 8;
@@ -289,8 +289,8 @@ __device__ __forceinline__ typename Raw4<T>::type load4_cut(const T *p, int d, i
 // hh + hl + lh leave out 2^-24 of a product, so three products of fp16 pieces are as good as
 // fp32's own; a 16-bit cached value is one piece (bf16's eight bits, too, but for values below
 // 2^-32 of the largest) and takes two.  bf16 pieces need no scale but three of them, and six
-// products (or three): 4 x 4096 tokens, 16 heads of 64, fp32 776 us, now 495; ragged
-// chunks over bf16, head dim 128, 794 us, now 711.
+// products (or three): 4 x 4096 tokens, 16 heads of 64, fp32 776 us, 495 so; ragged chunks
+// over bf16, head dim 128, 794 us, 711 so.
 //   The scales.  Q: each row has its own.  K and V: each of the four staging waves has one
 // for what it stages (K: the even or the odd keys; V: every other 32 dims, or 16 of head dim
 // 32), which only grows, by the largest value it meets.  Every tile in LDS says which; scores
@@ -883,11 +883,11 @@ struct PagedRows {
 // 64 requests, the tiles that see the most keys come first, so that short ones fill the end:
 // by classes, eighths of the most keys, within which a request's tiles follow each other and
 // share its keys in L2.  One request after the other, 4 x 4096 tokens (fp32, 16 heads of 64)
-// 538 us, now 511; 64 x 512 (8 heads of 32) 87, now 69.  With 16 classes ragged chunks lose
-// what they gained (738 us one by one, 732 in 8, 747 in 16).
-//   The matrix cores are busy 38% of that time (head dim 64; 31% at 128, bf16): beside each of
-// their instructions run nine others of a vector unit, half of them for the softmax, half to
-// scale, round and split what is staged.
+// 507 us, now 492 (279 TFLOP/s); 64 x 512 (8 heads of 32) 87, now 69; ragged chunks (bf16, 32
+// heads over 8 of 128) 716, now 714 (353 TFLOP/s), 2% more with 16 classes.
+//   Vector instructions bound it: nine run beside each MFMA, half of them for the softmax, half
+// to scale, round and split what is staged, and the matrix cores are busy 41% of the time (head
+// dim 64, fp32; 31% at 128, bf16, where registers leave two workgroups a CU).
 constexpr int kTileClasses = 8;
 template <typename T, int HD, int BN, bool VEC, bool UNI>
 __global__ void __launch_bounds__(PT_THREADS, HD <= 64 ? 3 : 2) paged_tile_kernel(const PagedArgs a) {
@@ -1362,7 +1362,8 @@ struct SpanRows {
 // Reading the cache bounds this, and rows fill one small MFMA operand at most, so the four
 // waves split the keys: each walks blocks of 32 through LDS of its own, with no barrier until
 // the waves' sums are joined.  The next block is loaded into registers while one is
-// multiplied; two workgroups a CU keep 128 KB on the way at head dim 128.
+// multiplied; two workgroups a CU keep 128 KB on the way at head dim 128.  64 x 8192 keys of
+// bf16, 64 heads over 8 of 128: 373 us, 5.8 TB/s.
 template <typename T, int HD, bool VEC>
 __global__ void __launch_bounds__(PT_THREADS, sizeof(T) == 2 || HD <= 64 ? 2 : 1) paged_span_kernel(const PagedArgs a) {
   typedef SpanRows<T, HD, VEC> Rows;
