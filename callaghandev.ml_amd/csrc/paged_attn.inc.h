@@ -358,6 +358,9 @@ __device__ __forceinline__ float power_of_2(int e) { return ldexpf(1.f, e); }
 template <typename T, int HD, int BN, bool VEC, bool UNI>
 struct PagedStage {
   typedef typename Raw4<T>::type Raw;
+  // Global memory, said so: a load through a pointer made of numbers would be a flat one, and
+  // every wait for LDS a wait for it too.
+  typedef const __attribute__((address_space(1))) char *GlobalBytes;
   static constexpr int NP = sizeof(T) == 4 ? 2 : 1;  // pieces
   // fp16 values are staged as they are, at a scale of 1 that holds them all
   static constexpr bool RAW = __is_same(T, _Float16);
@@ -466,11 +469,11 @@ struct PagedStage {
       if (k0 - group >= 1024) start_group(a, k0);
       const int first = (k0 - group) >> 4;
       zero = (uint32_t)(none >> first) & ((1u << NB) - 1);  // (a tile's blocks lie in one group)
-      const char *block[NB];
+      GlobalBytes block[NB];
 #pragma unroll
       for (int i = 0; i < NB; ++i)
-        block[i] = reinterpret_cast<const char *>((uint64_t)(uint32_t)__builtin_amdgcn_readlane(base_hi, first + i) << 32 |
-                                                  (uint32_t)__builtin_amdgcn_readlane(base_lo, first + i));
+        block[i] = (GlobalBytes)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(base_hi, first + i) << 32 |
+                                 (uint32_t)__builtin_amdgcn_readlane(base_lo, first + i));
       // (columns past the head dim read its last four again: Q is 0 there, and what they
       // give O is not stored)
       static_assert(vgroups(1) == 0 || vgroups(2) == 0, "two column offsets");
@@ -480,12 +483,12 @@ struct PagedStage {
         off[i] = (uint32_t)(row * kv_dim + min(col + 4 * vgroups(i), a.hd - 4)) * (uint32_t)sizeof(T);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const char *p = nullptr;
+        GlobalBytes p = nullptr;
         const int at = block_of(i);
 #pragma unroll
         for (int c = 0; c < NB; ++c) p = at == c ? block[c] : p;
         p += (size_t)(kside ? KSTEP * i % 16 : (i & 1)) * kv_dim * sizeof(T);
-        r[i] = *reinterpret_cast<const Raw *>(p + off[kside ? 0 : vgroups(i / 2) != 0]);
+        r[i] = *(const __attribute__((address_space(1))) Raw *)(p + off[kside ? 0 : vgroups(i / 2) != 0]);
       }
     } else {
       zero = 0;
