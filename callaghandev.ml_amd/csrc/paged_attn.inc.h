@@ -665,6 +665,7 @@ struct PagedRows {
   static constexpr int A[3] = {NP - 1, 0, 0}, B[3] = {NP == 2 ? 0 : 1, NP == 2 ? 1 : 0, 0};  // pieces of K or V, of Q or P
   static constexpr int NDB = HD / 32;  // 32-wide head-dim blocks of O^T
   static constexpr int NS = HD / 16;   // MFMA k-steps of Q.K
+  static constexpr int kAhead = NP == 1 ? 4 : HD <= 64 ? 2 : 1;
   floatx16 oacc[NDB];
   float m_run, thr;  // the reference (log2), and the score from which it moves: any until it is set
   float lift;        // log2 of the probability of a score at the row's maximum
@@ -719,37 +720,65 @@ struct PagedRows {
     for (int r = 0; r < 16; ++r) sacc[r] = acc_key(r) <= last_vis ? sacc[r] : -INFINITY;
   }
 
+  // Operands are read AHEAD steps before their products, and kept there: left to itself, the
+  // compiler reads each right before its use and waits (ragged chunks over bf16 730 us, 700 so).
+  // As far ahead as the registers go.
+  static __device__ __forceinline__ void hold() { __builtin_amdgcn_sched_barrier(0x6); }  // (vector and scalar units may pass)
+  typedef halfx8 Operand[NP];
+
+  static __device__ __forceinline__ void read_v(Operand &v, const char *vt, int j) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      v[i] = *reinterpret_cast<const halfx8 *>(vt + i * Tile::VPLANE + j / NDB * Tile::VSLAB + j % NDB * 256);
+  }
+  static __device__ __forceinline__ void read_k(Operand &k, const char *kt, int s) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) k[i] = *reinterpret_cast<const halfx8 *>(kt + i * Tile::KPLANE + s * Tile::KSLAB);
+  }
+
   __device__ __forceinline__ void accumulate_pv(const floatx16 &p, const char *vt) {
+    constexpr int N = 2 * NDB, AHEAD = N < kAhead ? N : kAhead;
+    Operand v[AHEAD];
+    halfx8 pp[2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      float x[8];
+    for (int j = 0; j < AHEAD; ++j) read_v(v[j], vt, j);
+    hold();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = p[8 * s + e];
-      halfx8 pp[2];
-      split_halves(x, pp);
+    for (int j = 0; j < N; ++j) {
+      const int s = j / NDB, db = j % NDB;
+      if (db == 0) {
+        float x[8];
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        halfx8 v[2];
+        for (int e = 0; e < 8; ++e) x[e] = p[8 * s + e];
+        split_halves(x, pp);
+      }
 #pragma unroll
-        for (int i = 0; i < NP; ++i)
-          v[i] = *reinterpret_cast<const halfx8 *>(vt + i * Tile::VPLANE + s * Tile::VSLAB + db * 256);
-#pragma unroll
-        for (int i = 0; i < PRODUCTS; ++i) oacc[db] = mfma_f16(v[A[i]], pp[B[i]], oacc[db]);
+      for (int i = 0; i < PRODUCTS; ++i) oacc[db] = mfma_f16(v[j % AHEAD][A[i]], pp[B[i]], oacc[db]);
+      hold();
+      if (j + AHEAD < N) {
+        read_v(v[j % AHEAD], vt, j + AHEAD);
+        hold();
       }
     }
   }
 
   // Scores in log2 units, relative to the reference (absolute until there is one).
   __device__ __forceinline__ floatx16 scores(const char *kt, const halfx8 (&q)[NS][2]) const {
+    constexpr int AHEAD = NS < kAhead ? NS : kAhead;
     floatx16 sacc = {};
+    Operand k[AHEAD];
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) read_k(k[s], kt, s);
+    hold();
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      halfx8 k[2];
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
-        k[i] = *reinterpret_cast<const halfx8 *>(kt + i * Tile::KPLANE + s * Tile::KSLAB);
-#pragma unroll
-      for (int i = 0; i < PRODUCTS; ++i) sacc = mfma_f16(k[A[i]], q[s][B[i]], sacc);
+      for (int i = 0; i < PRODUCTS; ++i) sacc = mfma_f16(k[s % AHEAD][A[i]], q[s][B[i]], sacc);
+      hold();
+      if (s + AHEAD < NS) {
+        read_k(k[s % AHEAD], kt, s + AHEAD);
+        hold();
+      }
     }
     const float ref = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
@@ -886,11 +915,14 @@ struct PagedRows {
 // 64 requests, the tiles that see the most keys come first, so that short ones fill the end:
 // by classes, eighths of the most keys, within which a request's tiles follow each other and
 // share its keys in L2.  One request after the other, 4 x 4096 tokens (fp32, 16 heads of 64)
-// 507 us, now 492 (279 TFLOP/s); 64 x 512 (8 heads of 32) 87, now 69; ragged chunks (bf16, 32
-// heads over 8 of 128) 716, now 714 (353 TFLOP/s), 2% more with 16 classes.
-//   Vector instructions bound it: nine run beside each MFMA, half of them for the softmax, half
-// to scale, round and split what is staged, and the matrix cores are busy 41% of the time (head
-// dim 64, fp32; 31% at 128, bf16, where registers leave two workgroups a CU).
+// 507 us, 492 so; 64 x 512 (8 heads of 32) 87, 69 so; ragged chunks (bf16, 32 heads over 8 of
+// 128) 716, 714 so, 2% more with 16 classes.
+//   What bounds it: 4 x 4096 tokens take 490 us, 280 TFLOP/s, which is 0.84 PFLOP/s of fp16
+// products where the library's largest plain ones reach 1.13; ragged chunks 707 us, 357.  The
+// matrix cores are busy 43% of the cycles (33% at head dim 128, where registers leave two
+// workgroups a CU) beside nine vector instructions for each of theirs, half for the softmax, half
+// to scale, round and split what is staged; and cycles are long: the clock falls to 1.8 GHz (2.0)
+// under their power, so that a step that saves 5% of the cycles saves 1 to 3% of the time.
 constexpr int kTileClasses = 8;
 template <typename T, int HD, int BN, bool VEC, bool UNI>
 __global__ void __launch_bounds__(PT_THREADS, HD <= 64 ? 3 : 2) paged_tile_kernel(const PagedArgs a) {
