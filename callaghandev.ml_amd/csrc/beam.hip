@@ -19,6 +19,8 @@
 // log2 e / L - 1, moves the whole sum: sum e^x = 2^r (s + k ln 2 (r s + sum t 2^t)) with s =
 // sum 2^t, to the first order of k; and segments of any r join exactly.  From |m| = 1024 on
 // the difference x - m is taken first: it is exact for every x whose term counts.
+#include <cfloat>
+
 #include "attn_common.h"
 
 namespace cdml {
@@ -93,7 +95,7 @@ struct TopList {
   int t[64];
 };
 
-// The K largest of the wave's values (E to a lane, none NaN, -infinity for none; best: the
+// The K largest of the wave's values (E to a lane; NaNs and -infinity are none; best: the
 // lane's largest, m: the wave's), on ties the lowest token first, into val / tok in that
 // order; -infinity where there are fewer.  token_of(e): the token of the lane's value e.
 template <int E, typename F>
@@ -109,10 +111,11 @@ __device__ __forceinline__ void select_top(float (&v)[E], float best, float m, i
     least = wave_max(mine);
   }
   // the values that reach it, in a list that lies one to a lane
+  least = fmaxf(least, -FLT_MAX);
   int found = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const bool reach = v[e] >= least && v[e] > -INFINITY;
+    const bool reach = v[e] >= least;
     const uint64_t who = __builtin_amdgcn_ballot_w64(reach);
     if (who == 0) continue;
     const int place =
@@ -167,7 +170,7 @@ __device__ __forceinline__ void select_top(float (&v)[E], float best, float m, i
 }
 
 // A wave's values of segment seg of a row's logits: element e of a lane is token
-// 64 (E seg + e) + lane.  Those past the vocabulary, and NaNs, are no candidates.
+// 64 (E seg + e) + lane.  Those past the vocabulary are no candidates.
 template <int E>
 __device__ __forceinline__ void load_segment(float (&v)[E], const float *x, int seg, int vocab) {
   const int lane = threadIdx.x & 63, t0 = seg * 64 * E + lane;
@@ -181,18 +184,16 @@ __device__ __forceinline__ void load_segment(float (&v)[E], const float *x, int 
   }
 }
 template <int E>
-__device__ __forceinline__ float drop_nans(float (&v)[E]) {
+__device__ __forceinline__ float largest(const float (&v)[E]) {
   float best = -INFINITY;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    v[e] = v[e] == v[e] ? v[e] : -INFINITY;
-    best = fmaxf(best, v[e]);
-  }
+  for (int e = 0; e < E; ++e) best = fmaxf(best, v[e]);  // (of a NaN, the other)
   return best;
 }
 
-// Reading the logits bounds it: 512 rows of 50021 (102 MB) take 25 us, 4.1 TB/s; a wave
-// reads once and then computes, and others' reads hide that.
+// Reading the logits and the instructions for each bound it alike: 512 rows of 50021 (102 MB)
+// take 22 us, 4.6 TB/s.  (25 us while NaNs were taken out one by one; 28 and 30 with segments of
+// half and twice the length; 16-byte loads change nothing.)
 template <int E>
 __global__ void __launch_bounds__(BS_THREADS) beam_rows_kernel(const BeamArgs a) {
   __shared__ TopList lists[BS_THREADS / 64];
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(BS_THREADS) beam_rows_kernel(const BeamArgs a)
   load_segment<E>(v, a.x + (size_t)row * a.ld, seg, a.vocab);
   // a finished beam's only candidate and a dead beam's none need no logits
   if (a.finished[row] != 0 || !isfinite(a.scores[row])) return;
-  const float best = drop_nans<E>(v);
+  const float best = largest<E>(v);
   const float m = wave_max(best);
   const size_t at = (size_t)row * a.n_seg + seg;
   double s = 0;
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(const BeamArgs a) {
     if constexpr (ONE) {
       float v[BS_SHORT];
       load_segment<BS_SHORT>(v, a.x + (size_t)(row0 + k) * a.ld, 0, a.vocab);
-      const float best = drop_nans<BS_SHORT>(v), m = wave_max(best);
+      const float best = largest<BS_SHORT>(v), m = wave_max(best);
       if (!offers || !isfinite(m)) {
         for (int r = lane; r < K; r += 64) val[k * K + r] = -INFINITY;
         continue;
