@@ -654,9 +654,10 @@ int cdml_paged_append(const float *k_new, int ldk, const float *v_new, int ldv,
  * are sized by; larger values are cut to them.  A page outside [0, n_pages)
  * that a row would read counts as zeros; with bad non-NULL (device int32) it is
  * then set to 1, and never cleared.  What masked or unused slots hold does not
- * matter, infinities and NaNs included.  head_dim up to 256; up to 128 chunks
- * run on the matrix cores (above, and for the rows of a few tokens, on the
- * vector units).  Sums and statistics are fp32 whatever the cache's type.
+ * matter, infinities and NaNs included.  head_dim up to 256; up to 128 more
+ * than a few rows a K/V head run on the matrix cores (above, and for single
+ * tokens, on the vector units).  Sums and statistics are fp32 whatever the
+ * cache's type.
  * workspace: 16-byte aligned, cdml_paged_attn_workspace_size bytes of the same
  * arguments (NULL when that is 0). */
 int cdml_paged_attn_workspace_size(int rows, int batch, int max_new,
