@@ -153,12 +153,16 @@ Plan make_plan(int size, int rows, int batch, int max_new, int max_len, int head
   // Matrix cores: keys are split where the tiles alone leave CUs without work, to two
   // workgroups for every CU.  16 heads of 64, bf16: 256 tokens over 8192 keys 69.9 us, 66.5
   // with twice the splits, 338 with none; 4 x 512 over 4096 146, 154, 195.
+  // Pieces of 256 keys at least, or of 128 where those leave half the CUs without work: 5
+  // heads of 96, fp32, 30 tokens over 500 keys 29.6 us, 21.8 so; 7 heads over 1 of 128 over 4000
+  // 37.4, 32.4; but 16 over 2 of 40, fp16, 120 tokens over 4000 (256 workgroups) 23.3, 27.9.
   p.tile_chunk = INT_MAX;
   p.tile_splits = 1;
   if (k.tile) {
     const long long tiles = ((long long)rows * group / kPagedTileRows + batch) * kv_heads;
     long long splits = (2 * kComputeUnits + tiles - 1) / (tiles < 1 ? 1 : tiles);
-    const long long pieces = (len + 255) / 256;
+    long long pieces = (len + 255) / 256;
+    if (pieces > 1 && tiles * pieces < kComputeUnits / 2) pieces = (len + 127) / 128;
     if (splits > pieces) splits = pieces;
     if (splits > 1) {
       p.tile_chunk = round_up((int)((len + splits - 1) / splits), 64);
