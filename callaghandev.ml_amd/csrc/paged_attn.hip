@@ -75,7 +75,7 @@ __device__ __forceinline__ void join_tile(const PagedArgs &a, int row, int h) {
 
 // A wave per (new token, head): the first few_tokens * batch workgroups for the requests of few
 // rows, the others, one a row, for those that ran in tiles.  One launch for both: 30 tokens over
-// 4000 keys, 16 heads over 2 of 40, fp16 21.6 us with two, 19.9 with one.
+// 4000 keys, 16 heads over 2 of 40, fp16 take 21.2 us, 1.7 more with two.
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a, int few_tokens) {
   const int h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (h >= a.heads) return;
@@ -151,11 +151,11 @@ Plan make_plan(int size, int rows, int batch, int max_new, int max_len, int head
   if ((k.rows || k.span) && p.few_splits > 1)
     p.few_floats = (size_t)batch * kv_heads * p.few_rows * p.few_splits * (hd + 2);
   // Matrix cores: keys are split where the tiles alone leave CUs without work, to two
-  // workgroups for every CU.  16 heads of 64, bf16: 256 tokens over 8192 keys 69.9 us, 66.5
-  // with twice the splits, 338 with none; 4 x 512 over 4096 146, 154, 195.
+  // workgroups for every CU.  16 heads of 64, bf16: 256 tokens over 8192 keys 59 us, 62
+  // with twice the splits, 260 with none; 4 x 512 over 4096 152, 159, 160.
   // Pieces of 256 keys at least, or of 128 where those leave half the CUs without work: 5
-  // heads of 96, fp32, 30 tokens over 500 keys 29.6 us, 21.8 so; 7 heads over 1 of 128 over 4000
-  // 37.4, 32.4; but 16 over 2 of 40, fp16, 120 tokens over 4000 (256 workgroups) 23.3, 27.9.
+  // heads of 96, fp32, 30 tokens over 500 keys 36.9 us, 26.2 so; 7 heads over 1 of 128 over 4000
+  // 44.7, 36.9; but 16 over 2 of 40, fp16, 120 tokens over 4000 (256 workgroups) 29.2, 32.7.
   p.tile_chunk = INT_MAX;
   p.tile_splits = 1;
   if (k.tile) {

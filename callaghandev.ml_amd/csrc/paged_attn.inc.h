@@ -255,6 +255,27 @@ __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedArgs 
 
 constexpr int PT_THREADS = 256;
 
+// Pieces of a cached value (common.h): fp32 has three, fp16's eleven bits lie in two,
+// bf16 is one; and the products of their pieces with the three of Q or of the
+// probabilities that reach fp32's accuracy, the main one last.
+template <typename T>
+struct Pieces;
+template <>
+struct Pieces<float> {
+  static constexpr int N = 3, PRODUCTS = 6;
+  static constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};
+};
+template <>
+struct Pieces<_Float16> {
+  static constexpr int N = 2, PRODUCTS = 5;
+  static constexpr int A[5] = {1, 0, 1, 0, 0}, B[5] = {1, 2, 0, 1, 0};
+};
+template <>
+struct Pieces<__bf16> {
+  static constexpr int N = 1, PRODUCTS = 3;
+  static constexpr int A[3] = {0, 0, 0}, B[3] = {2, 1, 0};
+};
+
 // Where a key's row lies in the cache, and whether its page is a page.
 struct Slot {
   uint32_t at;
@@ -263,6 +284,24 @@ struct Slot {
 __device__ __forceinline__ Slot slot_in(const PagedArgs &a, int page, int key) {
   const bool ok = (unsigned)page < (unsigned)a.n_pages;
   return {((uint32_t)(ok ? page : 0) << a.page_shift) + (uint32_t)(key & ((1 << a.page_shift) - 1)), ok};
+}
+
+// Puts dim c of two neighbouring keys of V (a's the lower one) at place d of its row in
+// every piece's plane.
+template <typename T>
+__device__ __forceinline__ void put_v(char *d, int plane, const typename Raw4<T>::type &a,
+                                      const typename Raw4<T>::type &b, int c) {
+  constexpr int NP = Pieces<T>::N;
+  if constexpr (NP == 1) {
+    *reinterpret_cast<uint32_t *>(d) = __builtin_amdgcn_perm(b[c / 2], a[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+  } else {
+    uint32_t h, m, l;
+    if constexpr (NP == 3) split_bf16x3(a[c] * kSplitScale, b[c] * kSplitScale, h, m, l);
+    else split_bf16x3(half_value(a[c / 2], c & 1, T{}), half_value(b[c / 2], c & 1, T{}), h, m, l);
+    *reinterpret_cast<uint32_t *>(d) = h;
+    *reinterpret_cast<uint32_t *>(d + plane) = m;
+    if constexpr (NP == 3) *reinterpret_cast<uint32_t *>(d + 2 * plane) = l;
+  }
 }
 
 // Four values of a row's columns d .. d + 3 at p, those past the head dim as zeros.
@@ -283,62 +322,8 @@ __device__ __forceinline__ typename Raw4<T>::type load4_cut(const T *p, int d, i
   return r;
 }
 
-// Products on the fp16 matrix cores.  An fp32 value of a power-of-two range, scaled so that
-// the largest lies in [2^14, 2^15), is the sum of two fp16 values h = fp16(x), l = fp16(x - h)
-// but for 2^-24 of itself, or 2^-40 of the largest where l runs into fp16's last bit (2^-24).
-// hh + hl + lh leave out 2^-24 of a product, so three products of fp16 pieces are as good as
-// fp32's own; a 16-bit cached value is one piece (bf16's eight bits, too, but for values below
-// 2^-32 of the largest) and takes two.  bf16 pieces need no scale but three of them, and six
-// products (or three): 4 x 4096 tokens, 16 heads of 64, fp32 776 us, 495 so; ragged chunks
-// over bf16, head dim 128, 794 us, 711 so.
-//   The scales.  Q: each row has its own.  K and V: each of the four staging waves has one
-// for what it stages (K: the even or the odd keys; V: every other 32 dims, or 16 of head dim
-// 32), which only grows, by the largest value it meets.  Every tile in LDS says which; scores
-// take K's and Q's as a factor, O is kept in V's and follows a change.  Probabilities are
-// lifted by 2^kLift: they reach 2^14 to 2^15.
-//   What that does not cover is recomputed in fp32: rows that come out non-finite, from
-// infinities, NaNs and sums past fp32; and the rows of a workgroup that met values too small
-// for their scale, where all that a lane of a staging wave holds (four dims of a few keys),
-// or eight neighbours of Q, lie below 2^-kRange of the largest and above 0.  A single huge
-// key among ordinary ones is found that way.
-//   fp16 caches are staged as they are (the scale 1 holds whatever fp16 holds): 4 x 2048 tokens
-// over 4096 keys, 16 heads of 128, 551 us scaled, 514 so.
-typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
-
-__device__ __forceinline__ floatx16 mfma_f16(halfx8 a, halfx8 b, floatx16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-// (fp16(a), fp16(b)) in the low and high half, rounded to nearest even.
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  typedef float vf2 __attribute__((ext_vector_type(2)));
-  typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((vf2{a, b}), halfx2));
-}
-__device__ __forceinline__ void split_f16x2(float a, float b, uint32_t &h, uint32_t &l) {
-  h = pack_f16(a, b);
-  l = pack_f16(a - half_value(h, 0, _Float16{}), b - half_value(h, 1, _Float16{}));
-}
-__device__ __forceinline__ void split_halves(const float (&x)[8], halfx8 (&p)[2]) {
-  uint32_t h[4], l[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) split_f16x2(x[2 * i], x[2 * i + 1], h[i], l[i]);
-  p[0] = __builtin_bit_cast(halfx8, (vu4{h[0], h[1], h[2], h[3]}));
-  p[1] = __builtin_bit_cast(halfx8, (vu4{l[0], l[1], l[2], l[3]}));
-}
-
-constexpr int kLowestExpo = -110;   // scales stay within fp32
-constexpr int kRange = 16;
-constexpr float kLift = 10.f;       // log2
-constexpr float kTileRise = 14.f;   // log2 of a lifted probability from which the reference moves
-constexpr float kTileSum = 32768.f; // a lane's sum up to which no probability overflows fp16
-
-__device__ __forceinline__ int expo_of(float x) {
-  return max((int)(__float_as_uint(x) >> 23 & 255) - 127, kLowestExpo);
-}
-__device__ __forceinline__ float power_of_2(int e) { return ldexpf(1.f, e); }
-
 // Stages one tile of BN keys: K rows and V transposed, of one K/V head, from their pages
-// into registers and then, as fp16 pieces, into LDS (one plane per piece, rows of 16
+// into registers and then, as bf16 pieces, into LDS (one plane per piece, rows of 16
 // values = 32 bytes).  The upper half of the workgroup's waves stages K, the lower half V,
 // four dims of a key per load.
 //   K: slab s holds dims 16 s .. 16 s + 15 of every key: rows are keys, even and odd ones
@@ -346,9 +331,9 @@ __device__ __forceinline__ float power_of_2(int e) { return ldexpf(1.f, e); }
 //   V: slab s holds keys 16 s .. 16 s + 15 of every dim: rows are dims, in four clusters
 //      by d % 4.  A unit is four dims of two keys; key k of a slab sits at place
 //      8 (k / 4 % 2) + 4 (k / 8) + k % 4, the order the P.V product reads.
-// The pages of a tile are looked up a tile ahead of its rows.  Rows past the request's last
-// key are staged as zeros (UNI) or read that key: the probabilities that V's meet are exactly
-// 0, and neither may move a scale.
+// The pages of a tile are looked up a tile ahead of its rows.  What masked keys hold never
+// matters to the scores; V's rows past the request's last key are staged as zeros, for the
+// probabilities that they meet are exactly 0.
 //   UNI (16-byte aligned rows, pages of 16 keys or more): the 16 keys of a block lie in one
 //      page and a wave's load touches one block, so a load's address is a scalar base plus
 //      an offset that the lane keeps throughout.  Lane l holds the base of block l of 64
@@ -361,9 +346,7 @@ struct PagedStage {
   // Global memory, said so: a load through a pointer made of numbers would be a flat one, and
   // every wait for LDS a wait for it too.
   typedef const __attribute__((address_space(1))) char *GlobalBytes;
-  static constexpr int NP = sizeof(T) == 4 ? 2 : 1;  // pieces
-  // fp16 values are staged as they are, at a scale of 1 that holds them all
-  static constexpr bool RAW = __is_same(T, _Float16);
+  static constexpr int NP = Pieces<T>::N;
   static constexpr int HALF = PT_THREADS / 2;
   static constexpr int KROWB = BN / 2 * 32, VROWB = HD / 4 * 32;  // bytes of one row cluster
   static constexpr int KSLAB = 2 * KROWB + 128, VSLAB = 4 * VROWB + 256;
@@ -390,10 +373,7 @@ struct PagedStage {
   const T *base;            // the head's columns (UNI), this thread's columns
   const int *table;
   int col, row, dst;  // first column, first row in a tile, LDS byte offset of the first unit
-  int slab;           // V: the first unit's block (wave-uniform but at head dim 32)
-  int expo;           // this wave's scale: values below 2^(expo + 1) times 2^(14 - expo)
-  float above;        // 2^(expo + 1)
-  uint32_t below;     // the bits of 2^(expo - kRange), less one
+  int slab;           // V: the first unit's block (wave-uniform)
   int loaded;         // first key of the tile in r
   int kv_dim, last;   // the request's last key
   bool kside;
@@ -405,10 +385,8 @@ struct PagedStage {
     // K: the P keys of one load instruction share a cluster
     constexpr int P = 64 / CH;
     const int c = t % CH, j = t / CH, kkey = (j & ~(2 * P - 1)) | ((j & (P - 1)) << 1) | ((j / P) & 1);
-    // V: a wave keeps to its dims
-    const int sb = t & 7, g = HD == 32 ? (t >> 3 & 3) + (t >> 6 << 2) : (t >> 3) % CH;
-    slab = HD == 32 ? t >> 5 & 1 : ((t0 & (HALF - 1)) >> 3) / CH;
-    set_expo(RAW ? 14 : kLowestExpo);
+    const int sb = t & 7, g = (t >> 3) % CH;
+    slab = ((t0 & (HALF - 1)) >> 3) / CH;
     const int place = ((sb >> 1) & 1) * 4 + (sb >> 2) * 2 + (sb & 1);  // of V's key pair
     col = kside ? 4 * c : 4 * g;
     row = kside ? kkey : 2 * sb + (UNI ? 0 : 16 * slab);
@@ -418,11 +396,6 @@ struct PagedStage {
     table = a.table + (size_t)b * a.max_blocks;
     kv_dim = a.kv_heads * a.hd;
     last = last_key;
-  }
-  __device__ __forceinline__ void set_expo(int e) {
-    expo = e;
-    above = power_of_2(e + 1);
-    below = __float_as_uint(power_of_2(max(e - kRange, -126))) - 1u;
   }
   // Load i's row in the tile, without the lane's part
   __device__ __forceinline__ int row_of(int i) const {
@@ -507,20 +480,13 @@ struct PagedStage {
     }
   }
 
-  __device__ __forceinline__ float value(int i, int c) const {
-    if constexpr (NP == 2) return r[i][c];
-    else return half_value(r[i][c / 2], c & 1, T{});
-  }
-
-  // expos: of the four waves, a byte each, beside the tile; *coarse (LDS) is set where the
-  // scale is too large for some of the values.
-  __device__ __forceinline__ void store(char *lds, uint32_t *expos, int *coarse, int *bad) {
+  __device__ __forceinline__ void store(char *lds, int *bad) {
     if constexpr (UNI) {
       if (zero || loaded + BN - 1 > last) {  // (wave-uniform)
         if (zero && bad) *bad = 1;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-          if ((zero >> block_of(i) & 1) || loaded + (kside ? 0 : 16 * slab) + row + row_of(i) > last) r[i] = Raw{};
+          if ((zero >> block_of(i) & 1) || (!kside && loaded + 16 * slab + row + row_of(i) > last)) r[i] = Raw{};
       }
     } else if (__builtin_amdgcn_ballot_w64(zero != 0)) {
       if (zero && bad) *bad = 1;
@@ -528,80 +494,33 @@ struct PagedStage {
       for (int i = 0; i < NV; ++i)
         if (zero >> i & 1) r[i] = Raw{};
     }
-    if constexpr (RAW) {
-      if ((threadIdx.x & 63) == 0) reinterpret_cast<int8_t *>(expos)[threadIdx.x >> 6] = (int8_t)expo;
-      if (kside) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) *reinterpret_cast<vu2 *>(lds + dst + KSTEP / 2 * 32 * i) = r[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < VU; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint32_t *>(lds + dst + vslabs(i) * VSLAB + vgroups(i) * 32 + vcluster(c)) =
-                __builtin_amdgcn_perm(r[2 * i + 1][c / 2], r[2 * i][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
-      }
-      return;
-    }
-    // a value that the scale does not hold moves it (infinities and NaNs do not: beside one,
-    // K's largest finite value would otherwise overflow and its key could vanish)
-    float most = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      most = fmaxf(most, fmaxf(fmaxf(fabsf(value(i, 0)), fabsf(value(i, 1))), fmaxf(fabsf(value(i, 2)), fabsf(value(i, 3)))));
-    auto low = [&] { return __float_as_uint(most) - 1u < below; };  // (not 0)
-    if (__builtin_amdgcn_ballot_w64(most >= above || low())) {
-      if (__builtin_amdgcn_ballot_w64(most == INFINITY)) {
-        most = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) most = fmaxf(most, fabsf(value(i, c)) < INFINITY ? fabsf(value(i, c)) : 0.f);
-      }
-      const float top = wave_max(most);
-      if (top >= above) set_expo(min(expo_of(top), 126));
-      if (low()) *coarse = 1;
-    }
-    if ((threadIdx.x & 63) == 0) reinterpret_cast<int8_t *>(expos)[threadIdx.x >> 6] = (int8_t)expo;
-    const float scale = power_of_2(14 - expo);
     if (kside) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         char *d = lds + dst + KSTEP / 2 * 32 * i;
-        float x[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) x[c] = value(i, c) * scale;
         if constexpr (NP == 1) {
-          *reinterpret_cast<vu2 *>(d) = vu2{pack_f16(x[0], x[1]), pack_f16(x[2], x[3])};
+          *reinterpret_cast<vu2 *>(d) = r[i];
         } else {
-          vu2 h, l;
+          float x[4];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t hc, lc;
-            split_f16x2(x[2 * c], x[2 * c + 1], hc, lc);
-            h[c] = hc;
-            l[c] = lc;
+          for (int c = 0; c < 4; ++c) {
+            if constexpr (NP == 3) x[c] = r[i][c];
+            else x[c] = half_value(r[i][c / 2], c & 1, T{});
           }
-          *reinterpret_cast<vu2 *>(d) = h;
-          *reinterpret_cast<vu2 *>(d + KPLANE) = l;
+          uint32_t h0, m0, l0, h1, m1, l1;
+          split_bf16x3(x[0], x[1], h0, m0, l0);
+          split_bf16x3(x[2], x[3], h1, m1, l1);
+          *reinterpret_cast<vu2 *>(d) = vu2{h0, h1};
+          *reinterpret_cast<vu2 *>(d + KPLANE) = vu2{m0, m1};
+          if constexpr (NP == 3) *reinterpret_cast<vu2 *>(d + 2 * KPLANE) = vu2{l0, l1};
         }
       }
     } else {
 #pragma unroll
       for (int i = 0; i < VU; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          char *d = lds + dst + vslabs(i) * VSLAB + vgroups(i) * 32 + vcluster(c);
-          const float x = value(2 * i, c) * scale, y = value(2 * i + 1, c) * scale;
-          if constexpr (NP == 1) {
-            *reinterpret_cast<uint32_t *>(d) = pack_f16(x, y);
-          } else {
-            uint32_t h, l;
-            split_f16x2(x, y, h, l);
-            *reinterpret_cast<uint32_t *>(d) = h;
-            *reinterpret_cast<uint32_t *>(d + VPLANE) = l;
-          }
-        }
+        for (int c = 0; c < 4; ++c)
+          put_v<T>(lds + dst + vslabs(i) * VSLAB + vgroups(i) * 32 + vcluster(c), VPLANE, r[2 * i], r[2 * i + 1], c);
     }
   }
 
@@ -615,103 +534,66 @@ struct PagedStage {
   }
 };
 
-// Q^T operand of a wave: two fp16 pieces of this lane's row times scale, scaled by the power
-// of two that brings the row's largest to [2^14, 2^15); returns that largest's exponent, and
-// sets *coarse where that leaves too little of some of its values.
-template <int HD, bool VEC>
-__device__ __forceinline__ int load_q_halves(halfx8 (&q)[HD / 16][2], const float *qrow, int hd, float scale, int hf,
-                                             int *coarse) {
-  float x[HD / 16][8], most = 0.f, least = INFINITY;
+// Q^T operand of a wave: the three bf16 pieces of this lane's row times scale_log2, eight
+// values of every `step` (16 or 32, by the MFMA) from 8 * part on.
+// Scores start from the row's reference, so neither Q nor K takes the split's scale: what
+// a component below 2^-110 loses (2^-134) reaches a score only through a component of
+// 2^100 and more on the other side.  Returns whether Q holds one or the other
+// (wave-uniform); such rows are recomputed on the fp32 MFMA.
+template <int N, bool VEC>
+__device__ __forceinline__ bool load_q_pieces(bf16x8 (&q)[N][3], const float *qrow, int hd, float scale, int step,
+                                              int part) {
+  uint32_t most = 0, least = ~0u;  // of |x|, and of 2 |x| - 1 as integers, which leaves zeros out
 #pragma unroll
-  for (int s = 0; s < HD / 16; ++s) {
-    float here = 0.f;
+  for (int s = 0; s < N; ++s) {
+    float x[8];
 #pragma unroll
     for (int e = 0; e < 8; e += 4) {
-      const int d = 16 * s + 8 * hf + e;
+      const int d = step * s + 8 * part + e;
       if constexpr (VEC) {
         const vf4 t = d < hd ? *reinterpret_cast<const vf4 *>(qrow + d) : vf4{};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) x[s][e + c] = t[c] * scale;
+        for (int c = 0; c < 4; ++c) x[e + c] = t[c] * scale;
       } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) x[s][e + c] = d + c < hd ? qrow[d + c] * scale : 0.f;
+        for (int c = 0; c < 4; ++c) x[e + c] = d + c < hd ? qrow[d + c] * scale : 0.f;
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) here = fmaxf(here, fabsf(x[s][e + c]));
     }
-    most = fmaxf(most, here);
-    least = here > 0.f ? fminf(least, here) : least;
-  }
-  const int expo = min(expo_of(halves_max(most)), 126);
-  if (__builtin_amdgcn_ballot_w64(least < power_of_2(max(expo - kRange, -126)))) *coarse = 1;
-  const float f = power_of_2(14 - expo);
 #pragma unroll
-  for (int s = 0; s < HD / 16; ++s) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[s][e] *= f;
-    split_halves(x[s], q[s]);
+    for (int e = 0; e < 8; ++e) {
+      most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+      least = min(least, (__float_as_uint(x[e]) << 1) - 1u);
+    }
+    split_operand(x, 1.f, q[s]);
   }
-  return expo;
+  return __builtin_amdgcn_ballot_w64(most >= (100u + 127u) << 23 || least < (17u << 24) - 1u) != 0;  // 2^100, 2^-110
 }
 
 // The online softmax of one wave's 32 rows (one per lane % 32) over 32-key sub-blocks:
 // S^T = K Q^T puts one row per lane, O^T += V^T P^T consumes the probabilities in place.
 // Each sum has one accumulator, the corrections before the main product: a sum of 16
-// products is rounded six (four) times, where the fp32 MFMA rounds it 16 times.
+// products is rounded 12 times (fp16 10, bf16 6), where the fp32 MFMA rounds it 16 times.
 template <typename T, int HD, int BN, bool VEC, bool UNI>
 struct PagedRows {
   typedef PagedStage<T, HD, BN, VEC, UNI> Tile;
-  static constexpr int NP = Tile::NP, PRODUCTS = NP + 1;
-  static constexpr int A[3] = {NP - 1, 0, 0}, B[3] = {NP == 2 ? 0 : 1, NP == 2 ? 1 : 0, 0};  // pieces of K or V, of Q or P
+  typedef Pieces<T> PC;
+  static constexpr int NP = PC::N;
   static constexpr int NDB = HD / 32;  // 32-wide head-dim blocks of O^T
   static constexpr int NS = HD / 16;   // MFMA k-steps of Q.K
-  static constexpr int kAhead = NP == 1 ? 4 : HD <= 64 ? 2 : 1;
+  static constexpr int kAhead = NP == 1 ? (HD <= 64 ? 4 : 2) : NP == 3 && HD <= 64 ? 2 : 1;
   floatx16 oacc[NDB];
   float m_run, thr;  // the reference (log2), and the score from which it moves: any until it is set
-  float lift;        // log2 of the probability of a score at the row's maximum
   float l_sum;       // running sum over this half-wave's keys
-  float fk[2];       // from accumulated scores to log2 units, of even and odd keys
-  int ek[2], ev[2];  // the scales of the tiles so far, and
-  uint32_t expos;    // as the tile wrote them
-  int eq;            // of this lane's Q
   bool warm;         // every lane of the wave has its reference (wave-uniform)
 
-  __device__ __forceinline__ void init(int q_expo, float lifted) {
+  __device__ __forceinline__ void init() {
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) oacc[db][r] = 0.f;
     m_run = thr = -INFINITY;
-    lift = lifted;
     l_sum = 0.f;
-    eq = q_expo;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      ek[i] = ev[i] = kLowestExpo;
-      fk[i] = power_of_2(ek[i] + eq - 28);
-    }
-    expos = (uint32_t)(uint8_t)kLowestExpo * 0x01010101u;
     warm = false;
-  }
-  // Which of V's two scales register r of block db is in
-  static __device__ __forceinline__ constexpr int v_class(int db, int r) { return HD == 32 ? r >> 3 : db & 1; }
-
-  // Follows the scales of a tile (wave-uniform; mostly those of the one before).
-  __device__ __forceinline__ void follow(uint32_t e) {
-    if (e == expos) return;
-    expos = e;
-    auto byte = [&](int i) { return (int)(int8_t)(e >> 8 * i); };
-    const float w[2] = {power_of_2(ev[0] - byte(0)), power_of_2(ev[1] - byte(1))};
-#pragma unroll
-    for (int db = 0; db < NDB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) oacc[db][r] *= w[v_class(db, r)];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      ev[i] = byte(i);
-      ek[i] = byte(2 + i);
-      fk[i] = power_of_2(ek[i] + eq - 28);
-    }
   }
 
   // -inf for the keys past this lane's last one (as an offset in its half's sub-block)
@@ -721,25 +603,25 @@ struct PagedRows {
   }
 
   // Operands are read AHEAD steps before their products, and kept there: left to itself, the
-  // compiler reads each right before its use and waits (ragged chunks over bf16 730 us, 700 so).
-  // As far ahead as the registers go.
+  // compiler reads each right before its use and waits (ragged chunks over bf16 857 us, 837 so;
+  // 4 x 2048 of 4096 tokens, 16 heads of 64, fp32 620, 598).  As far ahead as the registers go.
   static __device__ __forceinline__ void hold() { __builtin_amdgcn_sched_barrier(0x6); }  // (vector and scalar units may pass)
-  typedef halfx8 Operand[NP];
+  typedef bf16x8 Operand[NP];
 
   static __device__ __forceinline__ void read_v(Operand &v, const char *vt, int j) {
 #pragma unroll
     for (int i = 0; i < NP; ++i)
-      v[i] = *reinterpret_cast<const halfx8 *>(vt + i * Tile::VPLANE + j / NDB * Tile::VSLAB + j % NDB * 256);
+      v[i] = *reinterpret_cast<const bf16x8 *>(vt + i * Tile::VPLANE + j / NDB * Tile::VSLAB + j % NDB * 256);
   }
   static __device__ __forceinline__ void read_k(Operand &k, const char *kt, int s) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) k[i] = *reinterpret_cast<const halfx8 *>(kt + i * Tile::KPLANE + s * Tile::KSLAB);
+    for (int i = 0; i < NP; ++i) k[i] = *reinterpret_cast<const bf16x8 *>(kt + i * Tile::KPLANE + s * Tile::KSLAB);
   }
 
   __device__ __forceinline__ void accumulate_pv(const floatx16 &p, const char *vt) {
     constexpr int N = 2 * NDB, AHEAD = N < kAhead ? N : kAhead;
     Operand v[AHEAD];
-    halfx8 pp[2];
+    bf16x8 pp[3];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) read_v(v[j], vt, j);
     hold();
@@ -750,10 +632,10 @@ struct PagedRows {
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = p[8 * s + e];
-        split_halves(x, pp);
+        split_operand(x, 1.f, pp);
       }
 #pragma unroll
-      for (int i = 0; i < PRODUCTS; ++i) oacc[db] = mfma_f16(v[j % AHEAD][A[i]], pp[B[i]], oacc[db]);
+      for (int i = 0; i < PC::PRODUCTS; ++i) oacc[db] = mfma32x32x16(v[j % AHEAD][PC::A[i]], pp[PC::B[i]], oacc[db]);
       hold();
       if (j + AHEAD < N) {
         read_v(v[j % AHEAD], vt, j + AHEAD);
@@ -763,7 +645,7 @@ struct PagedRows {
   }
 
   // Scores in log2 units, relative to the reference (absolute until there is one).
-  __device__ __forceinline__ floatx16 scores(const char *kt, const halfx8 (&q)[NS][2]) const {
+  __device__ __forceinline__ floatx16 scores(const char *kt, const bf16x8 (&q)[NS][3]) const {
     constexpr int AHEAD = NS < kAhead ? NS : kAhead;
     floatx16 sacc = {};
     Operand k[AHEAD];
@@ -773,7 +655,7 @@ struct PagedRows {
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
 #pragma unroll
-      for (int i = 0; i < PRODUCTS; ++i) sacc = mfma_f16(k[s % AHEAD][A[i]], q[s][B[i]], sacc);
+      for (int i = 0; i < PC::PRODUCTS; ++i) sacc = mfma32x32x16(k[s % AHEAD][PC::A[i]], q[s][PC::B[i]], sacc);
       hold();
       if (s + AHEAD < NS) {
         read_k(k[s % AHEAD], kt, s + AHEAD);
@@ -782,12 +664,12 @@ struct PagedRows {
     }
     const float ref = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sacc[r] = fmaf(sacc[r], fk[r & 1], -ref);  // (acc_key(r) is odd where r is)
+    for (int r = 0; r < 16; ++r) sacc[r] -= ref;
     return sacc;
   }
 
   // The common sub-block once every row has its reference: probabilities and their
-  // per-lane sum first; false (nothing changed but sacc) if some lane's sum is too large or
+  // per-lane sum first; false (nothing changed but sacc) if some lane's sum is above 2^32 or
   // NaN, and the caller takes softmax() on recomputed scores.
   __device__ __forceinline__ bool try_fast(floatx16 &sacc, const char *vt, bool masked, int last_vis) {
     if (masked) apply_mask(sacc, last_vis);
@@ -797,7 +679,7 @@ struct PagedRows {
 #pragma unroll
     for (int i = 0; i < 8; ++i) s8[i] = sacc[2 * i] + sacc[2 * i + 1];
     const float ps = ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
-    if (__builtin_amdgcn_ballot_w64(!(ps <= kTileSum))) return false;
+    if (__builtin_amdgcn_ballot_w64(!(ps <= kFastSumLimit))) return false;
     l_sum += ps;
     accumulate_pv(sacc, vt);
     return true;
@@ -812,15 +694,15 @@ struct PagedRows {
     const float m4 = max3_scores(sacc[12], sacc[13], sacc[14]);
     float smax = max3_scores(max3_scores(m0, m1, m2), max3_scores(m3, m4, sacc[15]), -INFINITY);
     smax = halves_max(smax);
-    // Lazy rescale: the first visible key sets the reference (lift below it), later only a
-    // rise of more than the threshold moves it (the scores shift with it).
+    // Lazy rescale: the first visible key sets the reference, later only a rise of more
+    // than the threshold moves it (the scores shift with it).
     const bool need = smax > thr;
     if (__builtin_amdgcn_ballot_w64(need)) {
       const bool first = m_run == -INFINITY;
-      const float shift = need ? smax - lift : 0.f;
+      const float shift = need ? smax : 0.f;
       const float alpha = (need && !first) ? fast_exp2(-shift) : 1.0f;  // o and l are 0 before the first key
       m_run = need ? (first ? shift : m_run + shift) : m_run;
-      thr = m_run == -INFINITY ? -INFINITY : kTileRise;
+      thr = m_run == -INFINITY ? -INFINITY : kRescaleThreshold;
 #pragma unroll
       for (int r = 0; r < 16; ++r) sacc[r] -= shift;
       if (__builtin_amdgcn_ballot_w64(need && !first)) {
@@ -839,27 +721,27 @@ struct PagedRows {
     warm = !__builtin_amdgcn_ballot_w64(m_run == -INFINITY);
   }
 
-  // Undoes V's scales; whether some row came out non-finite (wave-uniform).
+  // Undoes V's scale; whether some row came out non-finite (wave-uniform).
   __device__ __forceinline__ bool finish() {
+    constexpr float unscale = NP == 3 ? kSplitUnscale : 1.f;
     float wrong = l_sum * 0.f;
-    const float w[2] = {power_of_2(ev[0] - 14), power_of_2(ev[1] - 14)};
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) oacc[db][r] *= w[v_class(db, r)];
+      for (int r = 0; r < 16; ++r) oacc[db][r] *= unscale;
       wrong = nonfinite_sum(oacc[db], wrong);
     }
     return any_nonfinite(wrong);
   }
 
   // The wave's rows over keys [c0, c1) on the fp32 MFMA straight from the pages: only for
-  // rows that came out non-finite.
+  // rows that came out non-finite (common.h) or whose Q is out of the split's range.
   // Where some row does not see all of a sub-block, V is summed per lane, without the keys
   // that the lane's row does not see: a product with their probability 0 would let their
   // infinities and NaNs through.
   __device__ __forceinline__ void recompute(const PagedArgs &a, const float *qrow, const int *table, int hk, int li,
                                             int hf, int c0, int c1, int lim, int lim_lo, int last) {
-    init(0, 0.f);
+    init();
     const int kv_dim = a.kv_heads * a.hd;
     const T *kb = static_cast<const T *>(a.kc) + (size_t)hk * a.hd, *vb = static_cast<const T *>(a.vc) + (size_t)hk * a.hd;
 #pragma unroll 1
@@ -914,23 +796,32 @@ struct PagedRows {
 // that tiles of one head meet on an XCD where the heads are a multiple of 8.  Then, of every
 // 64 requests, the tiles that see the most keys come first, so that short ones fill the end:
 // by classes, eighths of the most keys, within which a request's tiles follow each other and
-// share its keys in L2.  One request after the other, 4 x 4096 tokens (fp32, 16 heads of 64)
-// 507 us, 492 so; 64 x 512 (8 heads of 32) 87, 69 so; ragged chunks (bf16, 32 heads over 8 of
-// 128) 716, 714 so, 2% more with 16 classes.
-//   What bounds it: 4 x 4096 tokens take 490 us, 280 TFLOP/s, which is 0.84 PFLOP/s of fp16
-// products where the library's largest plain ones reach 1.13; ragged chunks 707 us, 357.  The
-// matrix cores are busy 43% of the cycles (33% at head dim 128, where registers leave two
-// workgroups a CU) beside nine vector instructions for each of theirs, half for the softmax, half
-// to scale, round and split what is staged; and cycles are long: the clock falls to 1.8 GHz (2.0)
-// under their power, so that a step that saves 5% of the cycles saves 1 to 3% of the time.
+// share its keys in L2.  One request after the other, 64 x 512 tokens (fp32, 8 heads of 32)
+// 110 us, 81 so; 4 x 4096 tokens and ragged chunks the same within 1%, as with 16 classes.
+//   Every value is held in bf16 pieces, which together have fp32's bits and its range: no
+// scale, so no key, dim or probability is too small beside others.  Two fp16 pieces, three
+// products for fp32 and two for 16-bit caches, would be 1.1 (bf16) to 1.8 times as fast, but
+// they need a scale: a probability then loses what lies below 2^-35 of its row's largest, and
+// a value what lies below 2^-40 of the largest beside it, while its part in the sum, the
+// product of the two, may be as large as any.
+//   What bounds it: 4 x 4096 tokens (fp32, 16 heads of 64) take 755 to 840 us by card, 1.0
+// PFLOP/s of bf16 products where the library's largest plain ones reach 1.13; ragged chunks
+// (bf16, 32 heads over 8 of 128) 765 to 830 us, as much.  The matrix cores are busy 51% of the
+// cycles (46% at head dim 128) beside six (four) vector instructions for each of theirs; and
+// cycles are long: the clock falls to 1.9 GHz (2.0) under their power.
 constexpr int kTileClasses = 8;
+// Waves a SIMD that registers are kept for; LDS holds as many.  16-bit caches, 16 heads of 64,
+// 4 x 2048 of 4096 tokens: three 331 us (bf16) and 506 (fp16), two 348 and 530.
+template <typename T>
+constexpr int tile_waves(int hd) {
+  if (hd <= 32 || (hd <= 64 && sizeof(T) == 2)) return 3;
+  return hd <= 64 || sizeof(T) == 2 ? 2 : 1;
+}
 template <typename T, int HD, int BN, bool VEC, bool UNI>
-__global__ void __launch_bounds__(PT_THREADS, HD <= 64 ? 3 : 2) paged_tile_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kernel(const PagedArgs a) {
   constexpr int NKB = BN / 32;  // 32-key sub-blocks per tile
   typedef PagedStage<T, HD, BN, VEC, UNI> Stage;
   __shared__ __attribute__((aligned(16))) char lds[2][Stage::BYTES];
-  __shared__ uint32_t expos[2];
-  __shared__ int coarse;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -986,27 +877,23 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 64 ? 3 : 2) paged_tile_kerne
   const int lim_lo = base + a.by_group.div(min(rw0, nr - 1)), lim_hi = base + a.by_group.div(min(rw0 + 31, nr - 1));
   const float *qrow = a.q + (size_t)(s.first + tok) * a.ldq + (size_t)head * a.hd;
   PagedRows<T, HD, BN, VEC, UNI> rows;
-  rows.init(0, kLift);
+  rows.init();
   if (c0 < c1) {
     Stage st;
     st.init(a, b, hk, s.len - 1);
     st.lookup_first(a, c0);
     st.load(a, c0);
     st.lookup(a, c0 + BN);
-    halfx8 q[HD / 16][2];
-    if (threadIdx.x == 0) coarse = 0;
-    __syncthreads();
-    rows.init(load_q_halves<HD, VEC>(q, qrow, a.hd, a.scale_log2, hf, &coarse), kLift);
-    st.store(lds[0], &expos[0], &coarse, a.bad);
+    bf16x8 q[HD / 16][3];
+    const bool wide = load_q_pieces<HD / 16, VEC>(q, qrow, a.hd, a.scale_log2, 16, hf);
+    st.store(lds[0], a.bad);
     __syncthreads();
     const int ko = Stage::koperand(li, hf), vo = Stage::voperand(li, hf);
     int cur = 0;
     for (int k0 = c0; k0 < c1; k0 += BN, cur ^= 1) {
-      // (past the last tile the request's last rows are staged once more, unread)
-      const uint32_t scales = expos[cur];
+      // (past the last tile the request's last rows are loaded once more, and left there)
       st.load(a, k0 + BN);
       st.lookup(a, k0 + 2 * BN);
-      rows.follow(__builtin_amdgcn_readfirstlane(scales));
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
         const int kb0 = k0 + kb * 32;
@@ -1029,10 +916,10 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 64 ? 3 : 2) paged_tile_kerne
           rows.accumulate_pv(sacc, vop);
         }
       }
-      st.store(lds[cur ^ 1], &expos[cur ^ 1], &coarse, a.bad);
+      if (k0 + BN < c1) st.store(lds[cur ^ 1], a.bad);
       __syncthreads();
     }
-    if ((rows.finish() || coarse) && rw0 < nr)
+    if ((rows.finish() || wide) && rw0 < nr)
       rows.recompute(a, qrow, a.table + (size_t)b * a.max_blocks, hk, li, hf, c0, min(c1, lim_hi + 1), lim, lim_lo,
                      s.len - 1);
   }
@@ -1067,27 +954,6 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 64 ? 3 : 2) paged_tile_kerne
 }
 
 // ---- 5 to 16 rows: matrix cores, a wave's own keys ------------------------------
-
-// Pieces of a cached value (common.h): fp32 has three, fp16's eleven bits lie in two,
-// bf16 is one; and the products of their pieces with the three of Q or of the
-// probabilities that reach fp32's accuracy, the main one last.
-template <typename T>
-struct Pieces;
-template <>
-struct Pieces<float> {
-  static constexpr int N = 3, PRODUCTS = 6;
-  static constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};
-};
-template <>
-struct Pieces<_Float16> {
-  static constexpr int N = 2, PRODUCTS = 5;
-  static constexpr int A[5] = {1, 0, 1, 0, 0}, B[5] = {1, 2, 0, 1, 0};
-};
-template <>
-struct Pieces<__bf16> {
-  static constexpr int N = 1, PRODUCTS = 3;
-  static constexpr int A[3] = {0, 0, 0}, B[3] = {2, 1, 0};
-};
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
@@ -1226,41 +1092,6 @@ struct SpanBlock {
     }
   }
 };
-
-// Q^T operand of a wave: the three bf16 pieces of this lane's row times scale_log2, eight
-// values of every `step` (16 or 32, by the MFMA) from 8 * part on.
-// Scores start from the row's reference, so neither Q nor K takes the split's scale: what
-// a component below 2^-110 loses (2^-134) reaches a score only through a component of
-// 2^100 and more on the other side.  Returns whether Q holds one or the other
-// (wave-uniform); such rows are recomputed on the fp32 MFMA.
-template <int N, bool VEC>
-__device__ __forceinline__ bool load_q_pieces(bf16x8 (&q)[N][3], const float *qrow, int hd, float scale, int step,
-                                              int part) {
-  uint32_t most = 0, least = ~0u;  // of |x|, and of 2 |x| - 1 as integers, which leaves zeros out
-#pragma unroll
-  for (int s = 0; s < N; ++s) {
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      const int d = step * s + 8 * part + e;
-      if constexpr (VEC) {
-        const vf4 t = d < hd ? *reinterpret_cast<const vf4 *>(qrow + d) : vf4{};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) x[e + c] = t[c] * scale;
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) x[e + c] = d + c < hd ? qrow[d + c] * scale : 0.f;
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
-      least = min(least, (__float_as_uint(x[e]) << 1) - 1u);
-    }
-    split_operand(x, 1.f, q[s]);
-  }
-  return __builtin_amdgcn_ballot_w64(most >= (100u + 127u) << 23 || least < (17u << 24) - 1u) != 0;  // 2^100, 2^-110
-}
 
 // f over the four lanes of a row (l, l ^ 16, l ^ 32, l ^ 48), in each of them.
 template <typename F>
