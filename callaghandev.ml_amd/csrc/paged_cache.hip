@@ -66,22 +66,43 @@ __device__ __forceinline__ int last_not_above(const int *v, int n, int x) {
 }
 
 // The free pages among a wave's next 256, four to a lane: bit j for page p + 4 lane + j.
+// COUNTED: the references were counted by this kernel's atomics, which add in L2; loads of
+// the device's scope read there, whatever the CU's cache holds of their lines (tables and
+// lengths may lie next to the references, and were read before).
+template <bool COUNTED>
 __device__ __forceinline__ uint32_t free_of(const int *refs, int p, int n_pages) {
   const int mine = p + 4 * (int)(threadIdx.x & 63);
   if (mine + 4 <= n_pages) {
-    const int4 r = *reinterpret_cast<const int4 *>(refs + mine);
-    return (r.x == 0) | (r.y == 0) << 1 | (r.z == 0) << 2 | (r.w == 0) << 3;
+    int r[4];
+    if constexpr (COUNTED) {
+      const uint64_t *two = reinterpret_cast<const uint64_t *>(refs + mine);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint64_t w = __hip_atomic_load(two + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        r[2 * i] = (int)(uint32_t)w;
+        r[2 * i + 1] = (int)(w >> 32);
+      }
+    } else {
+      const int4 w = *reinterpret_cast<const int4 *>(refs + mine);
+      r[0] = w.x, r[1] = w.y, r[2] = w.z, r[3] = w.w;
+    }
+    return (r[0] == 0) | (r[1] == 0) << 1 | (r[2] == 0) << 2 | (r[3] == 0) << 3;
   }
   uint32_t f = 0;
 #pragma unroll
-  for (int j = 0; j < 3; ++j)
-    if (mine + j < n_pages && refs[mine + j] == 0) f |= 1u << j;
+  for (int j = 0; j < 3; ++j) {
+    if (mine + j >= n_pages) continue;
+    const int r = COUNTED ? __hip_atomic_load(refs + mine + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                          : refs[mine + j];
+    if (r == 0) f |= 1u << j;
+  }
   return f;
 }
 
 // Free pages in increasing order, by one workgroup, a span of the pool at a time, of which
 // each wave has a run of its own and each lane, once counted, four bits for every 256 pages
 // of it.
+template <bool COUNTED>
 struct FreePages {
   int *counts;    // LDS, [PC_WAVES]: free pages of a span's runs
   uint64_t mask;  // this lane's of the span counted last
@@ -104,7 +125,7 @@ struct FreePages {
     mask = 0;
 #pragma unroll 4
     for (int i = 0; i < PC_ROUNDS; ++i)
-      if (begin + 256 * i < end) mask |= (uint64_t)free_of(refs, begin + 256 * i, end) << (4 * i);
+      if (begin + 256 * i < end) mask |= (uint64_t)free_of<COUNTED>(refs, begin + 256 * i, end) << (4 * i);
     const int c = wave_reduce((int)__popcll(mask), [](int a, int b) { return a + b; });
     __syncthreads();  // counts may still be read
     if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = c;
@@ -162,7 +183,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_plan_kernel(const PlanArgs a
   __shared__ int old[kPagedMaxBatch];                                // kv_len before
   __shared__ ScanScratch scratch;
   __shared__ int counts[PC_WAVES], list[PLAN_LIST];
-  FreePages pool(counts);
+  FreePages<false> pool(counts);
   const int t = threadIdx.x, P1 = (1 << a.page_shift) - 1;
   const long long room = (long long)a.max_blocks << a.page_shift;
   long long n_need = 0, n_new = 0;
@@ -402,6 +423,7 @@ struct CopyScratch {
 };
 
 // One workgroup: pages for the copies, and their rows' entries and lengths.
+template <bool COUNTED>
 __device__ __forceinline__ void place_copies(const ReorderArgs &a, CopyScratch &sc) {
   const int t = threadIdx.x, P1 = (1 << a.page_shift) - 1;
   int *first = sc.first;
@@ -428,7 +450,7 @@ __device__ __forceinline__ void place_copies(const ReorderArgs &a, CopyScratch &
     wrong += (int)all_bad;
   }
   __syncthreads();  // the last read of `first` as such
-  FreePages pool(sc.counts);
+  FreePages<COUNTED> pool(sc.counts);
   int found = 0;
   for (int span = 0; span < a.n_pages && found < copies; span += PC_SPAN) {
     pool.count(a.refs, a.n_pages, span);
@@ -477,7 +499,7 @@ __global__ void __launch_bounds__(REFS_THREADS) paged_refs_kernel(const ReorderA
 __global__ void __launch_bounds__(PC_THREADS) paged_tables_kernel(const ReorderArgs a) {
   __shared__ CopyScratch sc;
   if (blockIdx.x == 0) {
-    place_copies(a, sc);
+    place_copies<false>(a, sc);
     return;
   }
   const int r = (blockIdx.x - 1) * PC_WAVES + (threadIdx.x >> 6);
@@ -489,12 +511,12 @@ __global__ void __launch_bounds__(PC_THREADS) paged_reorder_kernel(const Reorder
   __shared__ CopyScratch sc;
   const int r = threadIdx.x >> 6;
   if (r < a.batch) count_refs(a, r);
-  // References are counted in L2, and nothing has read them into the CU's cache: once the
-  // sums are done (this wait; a fence for the whole device takes 2.6 us), place_copies sees them.
+  // Once the sums are done in L2 (this wait; a fence for the whole device takes 2.6 us),
+  // place_copies reads them there.
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   if (r < a.batch) write_table(a, r);
-  place_copies(a, sc);
+  place_copies<true>(a, sc);
 }
 
 // Workgroup (row, 2 * layer + which): the open page's tokens, one contiguous run (512 rows,
