@@ -973,6 +973,7 @@ PYBIND11_MODULE(_cdml_host, m) {
            },
            py::arg("prompts"), py::arg("beams"), py::arg("max_new"), py::arg("eos") = -1,
            py::arg("length_penalty") = 0.0f)
+      .def_property_readonly("allocations", &DeviceLanguageModel::allocations)
       .def("time_forward",
            // Device-resident forward of `batch` sequences of `seqLen` inputs
            // that are already in HBM: returns the mean ms of `steps` launches

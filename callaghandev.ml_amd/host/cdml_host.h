@@ -665,6 +665,8 @@ class DeviceLanguageModel {
   // Generate samples one sequence (LanguageModel.cs:482-584).
   BeamHypotheses GenerateBeam(const std::vector<std::vector<int>> &prompts, int beams, int maxNewTokens,
                               int eosToken, float lengthPenalty);
+  // Device allocations that the engine holds.
+  size_t allocations() const { return allocs_.size(); }
   // Enqueue-only forms over device pointers for benchmarking.
   void forward_device(const int *dev_ids, const float *dev_x, int batch, int seqLen,
                       float *dev_out);
@@ -699,7 +701,7 @@ class DeviceLanguageModel {
   void generate_device(int batch, int promptLen, int n);
   struct BeamState;
   void prepare_beams();
-  void *beam_workspace(size_t bytes);
+  void reserve_beam_workspace(int batch, int beams, int promptRows, int longest, int n);
   void paged_pass(float *x, int rows, int seqs, int longest, int max_len, int *status);
 
   TransformerConfig cfg_;

@@ -807,14 +807,32 @@ void DeviceLanguageModel::prepare_beams() {
   beam_ = std::move(st);
 }
 
-// Grow-only workspace of the paged entries.
-void *DeviceLanguageModel::beam_workspace(size_t bytes) {
-  if (bytes > beam_ws_bytes_) {
-    // (the smaller one stays with allocs_ until the model goes: launches may still use it)
-    beam_ws_ = alloc((bytes + 3) / sizeof(float));
-    beam_ws_bytes_ = bytes;
+// The workspace of all paged entries of a search: the largest that any of them needs, in
+// the prefill or in a step, before the first launch. It only grows, and the smaller one is
+// freed, so that the engine holds one whatever the lengths of its searches.
+void DeviceLanguageModel::reserve_beam_workspace(int batch, int beams, int promptRows, int longest, int n) {
+  const int R = batch * beams, H = cfg_.NumHeads, hd = cfg_.EmbeddingDim / H;
+  size_t most = 0, bytes = 0;
+  check(cdml_beam_select_workspace_size(batch, beams, cfg_.VocabSize, &bytes), "cdml_beam_select_workspace_size");
+  most = std::max(most, bytes);
+  check(cdml_paged_reorder_workspace_size(R, beam_->blocks, &bytes), "cdml_paged_reorder_workspace_size");
+  most = std::max(most, bytes);
+  for (int step = 0; step < n; ++step) {  // (the split of the keys does not grow with every length)
+    check(cdml_paged_attn_workspace_size(step ? R : promptRows, R, step ? 1 : longest, longest + step, H, H, hd, &bytes),
+          "cdml_paged_attn_workspace_size");
+    most = std::max(most, bytes);
   }
-  return beam_ws_;
+  if (most <= beam_ws_bytes_) return;
+  if (beam_ws_) {
+    synchronize();  // (a search that threw may have left launches behind)
+    allocs_.erase(std::find(allocs_.begin(), allocs_.end(), beam_ws_));
+    void *old = beam_ws_;
+    beam_ws_ = nullptr;
+    beam_ws_bytes_ = 0;
+    check(cdml_free(old), "cdml_free");
+  }
+  beam_ws_ = alloc((most + 3) / sizeof(float));
+  beam_ws_bytes_ = most;
 }
 
 // One pass of the blocks over the new tokens x [rows, D] of `seqs` requests: the plan's
@@ -827,9 +845,6 @@ void DeviceLanguageModel::paged_pass(float *x, int rows, int seqs, int longest, 
   check(cdml_paged_plan(s.refs, s.pages, P, s.table, s.blocks, s.kv, s.new_len, seqs, rows, s.cu, s.slots, s.pos,
                         status, stream_),
         "cdml_paged_plan");
-  size_t ws = 0;
-  check(cdml_paged_attn_workspace_size(rows, seqs, longest, max_len, H, H, hd, &ws), "cdml_paged_attn_workspace_size");
-  void *work = beam_workspace(ws);
   for (size_t i = 0; i < layers_.size(); ++i) {
     const Layer &L = layers_[i];
     float *k = s.k + i * s.layer_floats, *v = s.v + i * s.layer_floats;
@@ -840,7 +855,7 @@ void DeviceLanguageModel::paged_pass(float *x, int rows, int seqs, int longest, 
     check(cdml_paged_append(k_, D, v_, D, k, v, CDML_CACHE_F32, s.slots, rows, s.pages, P, D, stream_),
           "cdml_paged_append");
     check(cdml_paged_attn(q_, D, k, v, CDML_CACHE_F32, s.pages, P, s.table, s.blocks, s.kv, s.cu, att_, D, rows, seqs,
-                          longest, max_len, H, H, hd, scale, nullptr, work, ws, stream_),
+                          longest, max_len, H, H, hd, scale, nullptr, beam_ws_, beam_ws_bytes_, stream_),
           "cdml_paged_attn");
     finish_block(L, x, rows);
   }
@@ -881,6 +896,7 @@ BeamHypotheses DeviceLanguageModel::GenerateBeam(const std::vector<std::vector<i
     return out;
   }
   prepare_beams();
+  reserve_beam_workspace(batch, beams, rows, (int)longest, n);
   BeamState &s = *beam_;
   // a search starts from an empty pool; only the first beam of a prompt holds it
   std::vector<float> scores(R, -INFINITY);
@@ -897,9 +913,6 @@ BeamHypotheses DeviceLanguageModel::GenerateBeam(const std::vector<std::vector<i
   put(s.gather, last.data(), last.size() * sizeof(int));
   put(s.scores, scores.data(), scores.size() * sizeof(float));
   put(s.finished, open.data(), open.size());
-  size_t select = 0, reorder = 0;
-  check(cdml_beam_select_workspace_size(batch, beams, V, &select), "cdml_beam_select_workspace_size");
-  check(cdml_paged_reorder_workspace_size(R, s.blocks, &reorder), "cdml_paged_reorder_workspace_size");
   const float *hidden = h_;
   for (int step = 0; step < n; ++step) {
     int *status = s.status + (size_t)step * 6;
@@ -917,10 +930,10 @@ BeamHypotheses DeviceLanguageModel::GenerateBeam(const std::vector<std::vector<i
     check(cdml_linear(hidden, D, outproj_, outbias_, logits_, V, R, D, V, CDML_ACT_NONE, stream_), "output projection");
     int *parents = s.parents + (size_t)step * R, *tokens = s.tokens + (size_t)step * R;
     check(cdml_beam_select(logits_, V, s.scores, s.lengths, s.finished, batch, beams, V, eosToken, lengthPenalty,
-                           s.scores, s.lengths, s.finished, parents, tokens, beam_workspace(select), select, stream_),
+                           s.scores, s.lengths, s.finished, parents, tokens, beam_ws_, beam_ws_bytes_, stream_),
           "cdml_beam_select");
     check(cdml_paged_reorder(s.refs, s.pages, BeamState::kPage, s.table, s.blocks, s.kv, parents, R, s.src, s.dst,
-                             status + 3, beam_workspace(reorder), reorder, stream_),
+                             status + 3, beam_ws_, beam_ws_bytes_, stream_),
           "cdml_paged_reorder");
     check(cdml_paged_copy(s.k, s.v, CDML_CACHE_F32, (int)layers_.size(), s.layer_floats, s.pages, BeamState::kPage, D,
                           s.src, s.dst, s.kv, R, stream_),
