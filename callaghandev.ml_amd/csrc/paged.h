@@ -2,6 +2,7 @@
 // the attention kernels, whose cache types are built in files of their own.
 #pragma once
 
+#include <cfloat>
 #include <climits>
 
 #include "attn_common.h"
@@ -92,6 +93,9 @@ int paged_attn_f32(const PagedArgs &a, const PagedKernels &k, bool wide, hipStre
 int paged_attn_f16(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
 int paged_attn_bf16(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
 
+// The maximum (log2) of no key at all: no finite score lies below it, and beside any other its
+// weight, with the sum 0 that it comes with, changes nothing.
+constexpr float kNoKey = -FLT_MAX;
 constexpr int kPagedTileRows = 128;  // rows of a tile workgroup
 constexpr int kPagedSub = 512;       // keys whose pages a vector workgroup holds at a time
 

@@ -12,7 +12,7 @@ namespace {
 // chunks' statistics lie one to a lane, 64 chunks at a time.
 __device__ __forceinline__ void join_chunks(const PagedArgs &a, const float *part, int n, float *o) {
   const int lane = threadIdx.x & 63, stride = a.hd + 2;
-  float M = -3.0e38f;
+  float M = kNoKey;
   for (int c = lane; c < n; c += 64) M = fmaxf(M, part[(size_t)c * stride + a.hd]);
   M = wave_max(M);
   float L = 0.f, acc[4] = {};

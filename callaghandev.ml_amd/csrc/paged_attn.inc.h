@@ -101,7 +101,6 @@ __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedArgs 
   constexpr int NV = EPL / VW, KPS = 64 / LPK;
   typedef RowSlice<T, VW, NV, LPK, MODE> Slice;
   constexpr int U = Slice::WORDS <= 8 ? 4 : 2;
-  constexpr float kNone = -3.0e38f;  // below every score that matters, and exp2 of it is 0
   __shared__ int pages[kPagedSub + 1];
   __shared__ float red_m[4][R], red_l[4][R];
   __shared__ float red_o[4][R][HD];
@@ -135,7 +134,7 @@ __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedArgs 
       q[r][e] = MODE == kVector || d < a.hd ? qr[d] * a.scale_log2 : 0.f;
       o[r][e] = 0.f;
     }
-    m[r] = kNone;
+    m[r] = kNoKey;
     l[r] = 0.f;
   }
 
@@ -932,7 +931,7 @@ __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kern
   } else {
     out = a.tile_part + (((size_t)(s.first + tok) * a.heads + head) * a.tile_splits + split) * (a.hd + 2);
     if (hf == 0) {
-      out[a.hd] = fmaxf(rows.m_run, -3.0e38f);
+      out[a.hd] = fmaxf(rows.m_run, kNoKey);
       out[a.hd + 1] = l;
     }
   }
@@ -1285,7 +1284,7 @@ __global__ void __launch_bounds__(PT_THREADS, sizeof(T) == 2 || HD <= 64 ? 2 : 1
     if (rows.finish() || wide) rows.recompute(a, qrow, table, kc, vc, quarter, first, c1, lim, last);
   }
   // the waves' sums: rows' statistics, then each wave's O scaled to the common maximum
-  const float m = fmaxf(rows.m, -3.0e38f), l = quarters(rows.l, [](float x, float y) { return x + y; });
+  const float m = fmaxf(rows.m, kNoKey), l = quarters(rows.l, [](float x, float y) { return x + y; });
   if (quarter == 0) {
     red_m[wave][row] = m;
     red_l[wave][row] = l;

@@ -116,3 +116,22 @@ def test_rows_of_any_number_agree(kind, which):
     for n in (1, 8, 40):
         for m in (64, 60, 49):
             check_attention(kind, q[:n], bits, table, np.array([m], np.int32), np.array([0, n], np.int32), o[:n], 16, 1, 1)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("T,n", [(60, 1), (3000, 1), (60, 8), (3000, 8), (60, 40), (3000, 40)])
+def test_the_lowest_finite_scores(kind, T, n):
+    """Scores of -3.17e38 and -3.25e38 in log2 units, next to -FLT_MAX: the latter's keys, every one from the
+    middle on, have no weight, and the former's are equal, so that o is the mean of their V, all 3."""
+    r = rng(45)
+    q, bits, table, kv, cu, o = attention_case(r, kind, [T], [n], 16, 1, 1, 8)
+    k, v = (np.zeros_like(M.from_bits(b, kind)) for b in bits)
+    at = np.arange(T)
+    low = np.where(at < T // 2, np.float32(-1e19), np.float32(-1.025e19))
+    k[table[0, at // 16], at % 16, 0] = low
+    v[table[0, at // 16], at % 16] = np.where(at < T // 2, 3, 7)[:, None]
+    bits = [M.to_bits(x, kind) for x in (k, v)]
+    q[:] = 0
+    q[:, 0] = np.float32(2.2e19)
+    got, _ = M.call_attention(q, *bits, kind, table, kv, cu, 16, 1, 1, 1.0, o)
+    np.testing.assert_allclose(got, 3, rtol=(2 * T + 32) * 2.0 ** -24)
