@@ -648,7 +648,8 @@ int cdml_paged_append(const float *k_new, int ldk, const float *v_new, int ldv,
  * and o (ldo), i < n = cu_new[b + 1] - cu_new[b], head h reads K/V head
  * h / (num_heads / num_kv_heads) and
  *   o[r] = softmax(scale * q[r] K^T) V over tokens j <= kv_len[b] - n + i.
- * A row without a token is written as 0; rows of no request stay as they are.
+ * A row without a token is written as 0, and so is one whose scores are all
+ * -infinity; rows of no request stay as they are.
  * cu_new must not decrease and end within `rows`; max_new and max_len are upper
  * bounds of n and kv_len (max_len <= max_blocks * page_size) that the launches
  * are sized by; larger values are cut to them.  A page outside [0, n_pages)

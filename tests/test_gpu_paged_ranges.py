@@ -135,3 +135,22 @@ def test_the_lowest_finite_scores(kind, T, n):
     q[:, 0] = np.float32(2.2e19)
     got, _ = M.call_attention(q, *bits, kind, table, kv, cu, 16, 1, 1, 1.0, o)
     np.testing.assert_allclose(got, 3, rtol=(2 * T + 32) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("T,n", [(60, 1), (3000, 1), (60, 8), (3000, 8), (60, 40), (3000, 40)])
+def test_scores_of_minus_infinity(kind, T, n):
+    # a row that sees such scores alone is 0, as one that sees no token; beside others they have no weight
+    r = rng(46)
+    q, bits, table, kv, cu, o = attention_case(r, kind, [T], [n], 16, 1, 1, 64)
+    k, v = (M.from_bits(b, kind).copy() for b in bits)
+    at = np.arange(T)
+    q[:, 0] = 1
+    for some in (0, 3, T):  # finite ones: the last of them
+        k[table[0, at // 16], at % 16, 0] = np.where(at >= T - some, 0, -np.inf)
+        v[table[0, at // 16], at % 16] = 3
+        got, _ = M.call_attention(q, M.to_bits(k, kind), M.to_bits(v, kind), kind, table, kv, cu, 16, 1, 1, 0.125, o)
+        seen = np.minimum(T, T - n + 1 + np.arange(n))
+        none = seen <= T - some
+        assert not got[none].any()
+        np.testing.assert_allclose(got[~none], 3, rtol=(2 * T + 32) * 2.0 ** -24)
