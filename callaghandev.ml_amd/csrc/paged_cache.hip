@@ -167,7 +167,8 @@ __device__ __forceinline__ void write_row(const PlanArgs &a, int row, int b, int
   if (b >= 0) {
     pos = len + row - first;
     const int page = a.table[(size_t)b * a.max_blocks + (pos >> a.page_shift)];
-    slot = (page << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+    // (an entry that is no page, shifted, could pass 32 bits into another page's slots)
+    if ((unsigned)page < (unsigned)a.n_pages) slot = (page << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
   }
   a.slots[row] = slot;
   a.positions[row] = pos;

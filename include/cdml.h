@@ -622,7 +622,8 @@ int cdml_kv_cache_append(const float *k_new, const float *v_new,
  * kv_len.  The new tokens of all requests follow each other in rows cu_new[b]
  * .. cu_new[b + 1] (device int32[batch + 1]) of a step's activations; slots and
  * positions (device int32[rows]) receive each row's cache slot and its position
- * in its request, -1 and 0 for rows past the last request.
+ * in its request, -1 and 0 for rows past the last request; the slot is -1, too,
+ * where the request's open page, taken before, is not in [0, n_pages).
  * status (device int32[3]): 0 or the sum of 1 (too few free pages), 2 (a
  * negative length, or one that does not fit max_blocks pages) and 4 (more new
  * tokens than rows); the pages and the tokens of the step, without requests

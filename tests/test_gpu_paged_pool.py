@@ -40,3 +40,19 @@ def test_references_beside_tables_in_one_buffer(R, odd):
         same([got[:n_pages], got[n_pages:n_pages + R * blocks].reshape(R, blocks), got[-2 * R:-R], got[-R:]],
              [*want[:3], parents])
         same([down(x, (m,), np.int32) for x, m in ((src, R), (dst, R), (status, 3))], want[3:])
+
+
+@pytest.mark.parametrize("rows", [40, 9000])
+def test_an_open_page_that_is_none_has_no_slots(rows):
+    # entries that pass 32 bits once shifted would else name slots of other requests
+    P, n_pages = 16, 40
+    refs, kv = np.zeros(n_pages, np.int32), np.array([5, 20, 3, 7], np.int32)
+    table = np.full((4, 3), -1, np.int32)
+    table[0, 0], table[1, :2], table[2, 0], table[3, 0] = 2 ** 28, [0, n_pages], 2 ** 28 + 7, -2 ** 28
+    refs[0] = 1
+    new = np.array([13, 2, 1, 1], np.int32)
+    got = M.call_plan(refs, table, kv, new, P, rows)
+    assert list(got[6]) == [0, 1, 17]
+    slots = got[4]
+    assert (slots[:11] == -1).all() and list(slots[11:13]) == [16, 17] and (slots[13:] == -1).all()
+    assert list(got[5][:17]) == [*range(5, 18), 20, 21, 3, 7]
