@@ -106,12 +106,13 @@ int check_sizes(const char *what, int rows, int batch, int max_new, int max_len,
     return fail(CDML_E_INVALID, "%s: bad heads (%d over %d K/V heads, head_dim %d of at most 256)", what, heads,
                 kv_heads, hd);
   const long long group = heads / kv_heads;
-  // the grids' limits, and room for key numbers past the last tile
+  // the grids' limits (a launch has less than 2^32 threads along x, 2^24 workgroups of tiles),
+  // and room for key numbers past the last tile
   const long long most = max_new * group;
   const long long groups = hd <= 128 ? 1 : (most + kVecRows - 1) / kVecRows;
   if (most > INT_MAX / 2 || max_len > INT_MAX / 2 || heads > 65535 || groups * kv_heads > 65535 ||
       (long long)kv_heads * hd > INT_MAX / 4 ||
-      ((long long)rows * group / kPagedTileRows + batch) * kv_heads > INT_MAX / 2)
+      (hd <= 128 && most > kSpanRows && ((long long)rows * group / kPagedTileRows + batch) * kv_heads >= 1 << 24))
     return fail(CDML_E_INVALID, "%s: problem too large", what);
   return CDML_OK;
 }
