@@ -1,7 +1,8 @@
 // Selection of the next beams over beams and vocabulary (cdml_beam_select).
 //
-// Two launches.  beam_rows_kernel reads every live row's logits once: each wave holds a
-// segment of BS_SEG of them in registers and leaves the segment's maximum, its sum of
+// Two launches, or one up to 512 logits, which the second kernel then reads itself.
+// beam_rows_kernel reads every live row's logits once: each wave holds a segment of them in
+// registers (64 * BS_LONG, or 64 * BS_SHORT) and leaves the segment's maximum, its sum of
 // exponentials and its `beams` largest logits (no beam can give more to the result).
 // beam_pick_kernel, one workgroup per request, joins a row's segments into its
 // log-sum-exp and its `beams` best tokens, one wave per row, then merges the rows'

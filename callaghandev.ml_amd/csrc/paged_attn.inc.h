@@ -24,7 +24,7 @@ __device__ __forceinline__ float half_value(uint32_t w, int i, __bf16) {
   return __uint_as_float(i ? w & 0xffff0000u : w << 16);
 }
 
-// ---- few rows: vector units ---------------------------------------------------
+// ---- one to four rows: vector units -------------------------------------------
 
 constexpr int PR_THREADS = 256;
 
@@ -952,7 +952,7 @@ __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kern
     }
 }
 
-// ---- 5 to 16 rows: matrix cores, a wave's own keys ------------------------------
+// ---- few rows: matrix cores, a wave's own keys -----------------------------------
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 

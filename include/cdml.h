@@ -707,7 +707,8 @@ int cdml_paged_copy(void *kcache, void *vcache, int cache_type, int layers,
  * score + logit[t] - log(sum of exp(logit)) and length + 1, a finished one
  * (finished != 0) only eos_token with its score and length unchanged.  The
  * `beams` largest total / length^length_penalty become the request's next
- * beams, in that order; equal ones in the order of beams, then tokens.
+ * beams, in that order; equal ones in the order of beams, those of one beam by
+ * their logits, then in the order of tokens.
  * parents: the row each comes from, for cdml_paged_reorder; tokens; new_scores
  * / new_lengths / new_finished (1 once the token is eos_token; eos_token < 0:
  * none is) may be the input arrays.  NaN and -infinite logits are no
