@@ -58,7 +58,8 @@ HBM_PEAK_GBS = 8000.0           # MI355X HBM3E, AMD published
 # sources they were measured on; a record measured on other sources is not used.
 TRAFFIC_PROFILE = os.path.join("profiles", "mha_c3_decode_c4_hbm_traffic.md")
 TRAFFIC_SOURCES = {
-    "flash_c3": ("callaghandev.ml_amd/csrc/flash_attn.hip", "callaghandev.ml_amd/csrc/common.h"),
+    "flash_c3": ("callaghandev.ml_amd/csrc/flash_attn.hip", "callaghandev.ml_amd/csrc/attn_common.h",
+                 "callaghandev.ml_amd/csrc/common.h"),
     "decode_c4": ("callaghandev.ml_amd/csrc/decode_attn.hip", "callaghandev.ml_amd/csrc/common.h"),
 }
 
