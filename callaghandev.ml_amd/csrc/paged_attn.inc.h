@@ -734,7 +734,8 @@ struct PagedRows {
   }
 
   // The wave's rows over keys [c0, c1) on the fp32 MFMA straight from the pages: only for
-  // rows that came out non-finite (common.h) or whose Q is out of the split's range.
+  // rows that came out non-finite (common.h) or whose Q is out of the split's range (one NaN in
+  // V of one head of 4 x 4096 tokens, fp32, 16 heads of 64: 798 -> 2980 us).
   // Where some row does not see all of a sub-block, V is summed per lane, without the keys
   // that the lane's row does not see: a product with their probability 0 would let their
   // infinities and NaNs through.

@@ -655,8 +655,8 @@ class DeviceLanguageModel {
   // MaxSequenceLength), the count the reference's Generate produces.
   std::vector<int> GenerateGreedy(const std::vector<int> &prompts, int batch, int promptLen,
                                   int maxNewTokens, int *outLen);
-  // Beam search for decoder-only models over prompts of any lengths, prompts *
-  // beams rows within the batch capacity: n = min(maxNewTokens,
+  // Beam search for decoder-only models with head dims up to 256, over prompts
+  // of any lengths, prompts * beams rows within the batch capacity: n = min(maxNewTokens,
   // MaxSequenceLength - longest prompt) steps of `beams` beams each, ranked by
   // total log-probability / length^lengthPenalty (lengths count new tokens).
   // A beam that chooses eosToken (>= 0) is finished and keeps its score.  The

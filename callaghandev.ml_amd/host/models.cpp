@@ -866,6 +866,8 @@ BeamHypotheses DeviceLanguageModel::GenerateBeam(const std::vector<std::vector<i
   if (!cfg_.UsesDiscreteTokens)
     throw InvalidOperationException("Generate is only supported for discrete token data types.");
   if (!cfg_.UseDecoderOnly) throw InvalidOperationException("GenerateBeam needs a decoder-only model.");
+  if (cfg_.EmbeddingDim / cfg_.NumHeads > 256)  // (cdml_paged_attn's limit)
+    throw InvalidOperationException("GenerateBeam needs head dims of at most 256.");
   const int batch = (int)prompts.size(), S = cfg_.MaxSequenceLength, D = cfg_.EmbeddingDim, V = cfg_.VocabSize;
   if (beams <= 0 || beams > 64) throw ArgumentOutOfRangeException("beams");
   if (batch == 0 || (long long)batch * beams > cap_ || (long long)batch * beams > 4096)

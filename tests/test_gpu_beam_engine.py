@@ -32,3 +32,17 @@ def test_memory_does_not_grow_with_the_steps():
             np.testing.assert_array_equal(x, y)
     np.testing.assert_array_equal(first[1], again[1])
     assert all(len(t) == 1505 for t in long[0][0])
+
+
+def test_models_that_cannot_be_searched():
+    m = host.module()
+    dev = engine({"vocab": 20, "dim": 288, "heads": 1, "layers": 1, "ff": 16, "max_seq": 16}, 4)
+    held = dev.allocations
+    with pytest.raises(m.InvalidOperationException, match="256"):
+        dev.GenerateBeam([np.array([1, 2])], 2, 3)
+    assert dev.allocations == held  # refused before its pool is allocated
+    wide = engine({"vocab": 20, "dim": 256, "heads": 1, "layers": 1, "ff": 16, "max_seq": 16}, 4)
+    tokens, scores = wide.GenerateBeam([np.array([1, 2]), np.array([3])], 2, 3)
+    assert np.isfinite(scores).all()
+    np.testing.assert_array_equal([t[0] for t in wide.GenerateBeam([np.array([1, 2])], 1, 3)[0]],
+                                  wide.GenerateGreedy(np.array([[1, 2]]), 3))
