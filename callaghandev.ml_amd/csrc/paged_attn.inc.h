@@ -806,7 +806,7 @@ struct PagedRows {
 // product of the two, may be as large as any.
 //   What bounds it: 4 x 4096 tokens (fp32, 16 heads of 64) take 755 to 840 us by card, 1.0
 // PFLOP/s of bf16 products where the library's largest plain ones reach 1.13; ragged chunks
-// (bf16, 32 heads over 8 of 128) 765 to 830 us, as much.  The matrix cores are busy 51% of the
+// (bf16, 32 heads over 8 of 128) 765 to 840 us, as much.  The matrix cores are busy 51% of the
 // cycles (46% at head dim 128) beside six (four) vector instructions for each of theirs; and
 // cycles are long: the clock falls to 1.9 GHz (2.0) under their power.
 constexpr int kTileClasses = 8;
