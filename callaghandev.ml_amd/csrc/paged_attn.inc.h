@@ -804,7 +804,7 @@ struct PagedRows {
 // they need a scale: a probability then loses what lies below 2^-35 of its row's largest, and
 // a value what lies below 2^-40 of the largest beside it, while its part in the sum, the
 // product of the two, may be as large as any.
-//   What bounds it: 4 x 4096 tokens (fp32, 16 heads of 64) take 755 to 840 us by card, 1.0
+//   What bounds it: 4 x 4096 tokens (fp32, 16 heads of 64) take 745 to 840 us by card, 1.0
 // PFLOP/s of bf16 products where the library's largest plain ones reach 1.13; ragged chunks
 // (bf16, 32 heads over 8 of 128) 765 to 840 us, as much.  The matrix cores are busy 51% of the
 // cycles (46% at head dim 128) beside six (four) vector instructions for each of theirs; and
