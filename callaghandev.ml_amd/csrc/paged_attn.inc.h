@@ -535,8 +535,8 @@ struct PagedStage {
 
 // Q^T operand of a wave: the three bf16 pieces of this lane's row times scale_log2, eight
 // values of every `step` (16 or 32, by the MFMA) from 8 * part on.
-// Scores start from the row's reference, so neither Q nor K takes the split's scale: what
-// a component below 2^-110 loses (2^-134) reaches a score only through a component of
+// Neither Q nor K takes the split's scale, so that scores come out as they are: what a
+// component below 2^-110 loses (2^-134) reaches a score only through a component of
 // 2^100 and more on the other side.  Returns whether Q holds one or the other
 // (wave-uniform); such rows are recomputed on the fp32 MFMA.
 template <int N, bool VEC>
