@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(PKG, "_build", "libcdml_hip.so")
 HEADER = os.path.join(ROOT, "include", "cdml.h")
 
 OK, E_INVALID, E_NODEVICE, E_HIP, E_CAUSAL = 0, -1, -2, -3, -4
-CACHE = {"f32": 0, "f16": 1, "bf16": 2}  # CDML_CACHE_*
+CACHE = {"f32": 0, "f16": 1, "bf16": 2, "i8": 3, "f8": 4}  # CDML_CACHE_*
 ACT = {"none": 0, "sigmoid": 1, "tanh": 2, "relu": 3, "leakyrelu": 4, "swish": 5}
 
 
@@ -106,6 +106,9 @@ SIGNATURES = {
     "cdml_paged_reorder_workspace_size": [_i, _i, C.POINTER(_sz)],
     "cdml_paged_reorder": [_vp, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp],
     "cdml_paged_copy": [_vp, _vp, _i, _i, _sz, _i, _i, _i, _vp, _vp, _vp, _i, _vp],
+    "cdml_paged_append_q8": [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp],
+    "cdml_paged_copy_q8": [_vp, _vp, _vp, _vp, _i, _sz, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp],
+    "cdml_paged_read": [_vp] * 4 + [_i, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp],
     "cdml_beam_select_workspace_size": [_i, _i, _i, C.POINTER(_sz)],
     "cdml_beam_select": [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _f] + [_vp] * 6 + [_sz, _vp],
     "cdml_residual_layernorm": [_vp, _vp, _vp, _vp, _vp, _i, _i, _f, _vp],

@@ -16,6 +16,20 @@ inline int cache_type_bytes(int cache_type) {
   return cache_type == CDML_CACHE_F32 ? 4 : cache_type == CDML_CACHE_F16 || cache_type == CDML_CACHE_BF16 ? 2 : 0;
 }
 
+inline bool q8_cache_type(int cache_type) { return cache_type == CDML_CACHE_I8 || cache_type == CDML_CACHE_F8; }
+
+// Bytes of a K/V head's row of an 8-bit cache.
+__host__ __device__ constexpr int q8_width(int hd) { return (hd + 15) & ~15; }
+
+// The checks of an 8-bit cache's arrays.
+inline int check_q8(const char *what, const void *kcache, const void *vcache, const float *kscale,
+                    const float *vscale) {
+  if (!kcache || !vcache || !kscale || !vscale) return fail(CDML_E_INVALID, "%s: NULL pointer", what);
+  if (!aligned16(kcache) || !aligned16(vcache))
+    return fail(CDML_E_INVALID, "%s: the cache is not 16-byte aligned", what);
+  return CDML_OK;
+}
+
 // The checks of a pool and its tables; the page size's log2 in *shift.
 inline int check_pool(const char *what, int n_pages, int page_size, int max_blocks, int batch, int *shift) {
   if (page_size < 1 || page_size > 4096 || (page_size & (page_size - 1)))

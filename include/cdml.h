@@ -616,6 +616,23 @@ int cdml_kv_cache_append(const float *k_new, const float *v_new,
 #define CDML_CACHE_F16 1
 #define CDML_CACHE_BF16 2
 
+/* Caches of 8 bits, for the entries that name them: a row of a K/V head (a
+ * token's head_dim values) is one fp32 scale s and a byte c for each value, which
+ * stands for c * s:
+ *   CDML_CACHE_I8  c in [-127, 127] (two's complement), s = max|x| / 127 rounded
+ *                  to fp32, 2^-126 at least, c the whole number nearest to x / s
+ *                  (ties to even);
+ *   CDML_CACHE_F8  c an e4m3 value (of [-448, 448]), s the least power of two,
+ *                  2^-126 at least, with max|x| <= 448 s, c = e4m3(x / s).
+ * (rounded to fp32 where it is read: a value next to FLT_MAX may become infinite).
+ * A row of zeros has s = 0; one that holds an infinity or a NaN has s = NaN and c =
+ * 0, and reads as NaN.  A layer's cache is kcache and vcache [n_pages, num_kv_heads,
+ * page_size, W] bytes, W = head_dim rounded up to a multiple of 16, 16-byte aligned,
+ * the bytes behind head_dim zeros, and kscale and vscale [n_pages, num_kv_heads,
+ * page_size] fp32; slots, tables and page_refs are as above, head_dim up to 256. */
+#define CDML_CACHE_I8 3
+#define CDML_CACHE_F8 4
+
 /* Makes room for new_len[b] (device int32, >= 0) more tokens of every request:
  * takes the pages they need, the lowest free ones in the order of requests and
  * tokens, into block_table, sets their page_refs to 1 and adds new_len to
@@ -643,6 +660,28 @@ int cdml_paged_append(const float *k_new, int ldk, const float *v_new, int ldv,
                       void *kcache, void *vcache, int cache_type,
                       const int *slots, int rows, int n_pages, int page_size,
                       int kv_dim, cdml_stream stream);
+
+/* cdml_paged_append into an 8-bit cache (CDML_CACHE_I8, CDML_CACHE_F8). */
+int cdml_paged_append_q8(const float *k_new, int ldk, const float *v_new,
+                         int ldv, void *kcache, void *vcache, float *kscale,
+                         float *vscale, int cache_type, const int *slots,
+                         int rows, int n_pages, int page_size,
+                         int num_kv_heads, int head_dim, cdml_stream stream);
+
+/* Reads cached tokens of any cache type back as fp32 rows: row cu_rows[b] + i of
+ * k_out (row stride ldk) and v_out (ldv) is token kv_len[b] - n + i of request b, n
+ * = cu_rows[b + 1] - cu_rows[b]: a request's last n tokens, all of them where n is
+ * kv_len[b].  cu_rows must not decrease.  Rows of tokens before the first, or of a
+ * page outside [0, n_pages), are written as zeros; the latter sets bad, if that is
+ * given, to 1.  Rows of no request stay as they are.  kscale and vscale are for 8-bit
+ * caches, and NULL for others. */
+int cdml_paged_read(const void *kcache, const void *vcache,
+                    const float *kscale, const float *vscale, int cache_type,
+                    int n_pages, int page_size, const int *block_table,
+                    int max_blocks, const int *kv_len, const int *cu_rows,
+                    float *k_out, int ldk, float *v_out, int ldv, int rows,
+                    int batch, int num_kv_heads, int head_dim, int *bad,
+                    cdml_stream stream);
 
 /* Attention of every request's new tokens over its cached ones, its new ones
  * among them (appended before): rows r = cu_new[b] + i of q (row stride ldq)
@@ -699,6 +738,14 @@ int cdml_paged_copy(void *kcache, void *vcache, int cache_type, int layers,
                     size_t layer_stride, int n_pages, int page_size,
                     int kv_dim, const int *copy_src, const int *copy_dst,
                     const int *kv_len, int batch, cdml_stream stream);
+
+/* The same in 8-bit caches, whose layers lie layer_stride slots apart (codes at
+ * layer_stride * num_kv_heads * W bytes, scales at layer_stride * num_kv_heads). */
+int cdml_paged_copy_q8(void *kcache, void *vcache, float *kscale,
+                       float *vscale, int layers, size_t layer_stride,
+                       int n_pages, int page_size, int num_kv_heads,
+                       int head_dim, const int *copy_src, const int *copy_dst,
+                       const int *kv_len, int batch, cdml_stream stream);
 
 /* One step of beam search, the beam counterpart of cdml_argmax_rows: `batch`
  * requests with `beams` (<= 64) beams each, row b * beams + k of logits [rows,

@@ -1,0 +1,111 @@
+"""Plain restatements of the 8-bit paged cache in numpy and float64 (test helper), and
+numpy-in, numpy-out calls of its C-ABI entries."""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from abi_ops import down, stream, up
+from cdml import native as N
+from paged_model import from_bits, ints, raw_dtype, to_bits
+
+
+def width(hd):
+    return -(-hd // 16) * 16
+
+
+def quantise(x, kind):
+    """fp32 [..., hd] -> (codes uint8 [..., width], scales fp32 [...])."""
+    x = np.asarray(x, np.float32)
+    codes = np.zeros(x.shape[:-1] + (width(x.shape[-1]),), np.uint8)
+    finite = np.isfinite(x).all(-1)
+    x = np.where(finite[..., None], x, 0).astype(np.float64)
+    most = np.abs(x).max(-1)
+    if kind == "i8":
+        s = np.maximum((most / 127).astype(np.float32), np.float32(2.0 ** -126)).astype(np.float64)
+        c = np.rint(x / s[..., None]).astype(np.int8).view(np.uint8)  # (a quotient that is no tie is 2^-33 from one)
+    else:
+        s = np.full(most.shape, 2.0 ** -126)
+        while (448 * s < most).any():
+            s = np.where(448 * s < most, 2 * s, s)
+        q = torch.from_numpy((x / s[..., None]).astype(np.float32))  # exact, or below 2^-10 and rounded to 0
+        c = q.to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    codes[..., :x.shape[-1]] = c
+    codes[most == 0] = 0
+    return codes, np.where(finite, np.where(most > 0, s, 0), np.nan).astype(np.float32)
+
+
+def values(codes, scales, kind, hd):
+    """float64 values [..., hd]."""
+    c = np.ascontiguousarray(codes[..., :hd])
+    c = c.view(np.int8).astype(np.float64) if kind == "i8" else (
+        torch.from_numpy(c).view(torch.float8_e4m3fn).to(torch.float64).numpy())
+    with np.errstate(invalid="ignore"):
+        return c * np.asarray(scales, np.float64)[..., None]
+
+
+def in_place(cache, slots, P):
+    """Rows [len(slots), heads, ...] of a cache [pages, heads, P, ...]."""
+    return cache[slots // P, :, slots % P]
+
+
+def random_rows(r, n, heads, hd):
+    """Rows of very different sizes, a few channels larger than the others."""
+    x = r.standard_normal((n, heads, hd)) * 10.0 ** r.integers(-3, 3, (n, heads, 1))
+    x[..., 3::16] *= 8
+    return x.astype(np.float32)
+
+
+def random_cache(r, kind, pages, P, heads, hd):
+    """{"kind", "k", "v": raw arrays, "ks", "vs": scales or None, "kx", "vx": float64 [pages, P, heads * hd]}."""
+    c = {"kind": kind, "P": P, "heads": heads, "hd": hd}
+    for side in "kv":
+        x = random_rows(r, pages * P, heads, hd) if kind in ("i8", "f8") else r.standard_normal(
+            (pages * P, heads, hd)).astype(np.float32)
+        put(c, side, x.reshape(pages, P, heads, hd))
+    return c
+
+
+def put(c, side, x):
+    """Fills a side of a cache from fp32 [pages, P, heads, hd]."""
+    pages, P, heads, hd = x.shape
+    if c["kind"] in ("i8", "f8"):
+        codes, scales = quantise(np.moveaxis(x, 2, 1), c["kind"])
+        c[side], c[side + "s"] = np.ascontiguousarray(codes), np.ascontiguousarray(scales)
+        val = np.moveaxis(values(codes, scales, c["kind"], hd), 1, 2)
+    else:
+        c[side], c[side + "s"] = to_bits(x.reshape(pages, P, heads * hd), c["kind"]), None
+        val = from_bits(c[side], c["kind"]).astype(np.float64)
+    c[side + "x"] = np.ascontiguousarray(val).reshape(pages, P, heads * hd)
+
+
+def upload(c):
+    """(k, v, kscale, vscale) as device buffers, None for the scales that a type has not."""
+    raw = np.uint8 if c["kind"] in ("i8", "f8") else raw_dtype(c["kind"])
+    return [up(c["k"], raw), up(c["v"], raw)] + [None if c[s] is None else up(c[s]) for s in ("ks", "vs")]
+
+
+def ptr(b):
+    return None if b is None else b.ptr
+
+
+# ---- calls -------------------------------------------------------------------------
+
+def call_append(k, ldk, v, ldv, codes, scales, kind, slots, P, heads, hd):
+    """codes, scales: pairs of the caches' arrays before; returns them after."""
+    d = [up(a, a.dtype) for a in (k, v, *codes, *scales, slots)]
+    N.check(N.lib().cdml_paged_append_q8(d[0].ptr, ldk, d[1].ptr, ldv, *(b.ptr for b in d[2:6]), N.CACHE[kind],
+                                         d[6].ptr, len(slots), len(codes[0]), P, heads, hd, stream().handle))
+    return ([down(b, a.shape, np.uint8) for b, a in zip(d[2:4], codes)],
+            [down(b, a.shape) for b, a in zip(d[4:6], scales)])
+
+
+def call_read(c, table, kv, cu, rows, ldk, ldv, fill=7.0, n_pages=None):
+    """([rows, ldk], [rows, ldv], bad)."""
+    d = upload(c)
+    out = [up(np.full((rows, ld), fill, np.float32)) for ld in (ldk, ldv)]
+    t, l, u, bad = ints(table), ints(kv), ints(cu), ints(np.zeros(1))
+    N.check(N.lib().cdml_paged_read(*(ptr(b) for b in d), N.CACHE[c["kind"]], n_pages or len(c["k"]), c["P"], t.ptr,
+                                    table.shape[1], l.ptr, u.ptr, out[0].ptr, ldk, out[1].ptr, ldv, rows, len(kv),
+                                    c["heads"], c["hd"], bad.ptr, stream().handle))
+    return down(out[0], (rows, ldk)), down(out[1], (rows, ldv)), int(down(bad, (1,), np.int32)[0])
