@@ -4,6 +4,7 @@
 
 #include <cfloat>
 #include <climits>
+#include <type_traits>
 
 #include "attn_common.h"
 
@@ -71,6 +72,8 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 struct PagedArgs {
   const float *q;
   const void *kc, *vc;
+  const float *ks, *vs;  // scales and bytes of a head's row of an 8-bit cache
+  int width;
   const int *table, *kv_len, *cu_new;
   float *o;
   int *bad;
@@ -96,6 +99,16 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &a, int b) {
   return s;
 }
 
+// A cached value of 8 bits, without its scale.
+struct I8 {
+  uint8_t c;
+};
+struct F8 {
+  uint8_t c;
+};
+template <typename T>
+constexpr bool kQ8 = std::is_same<T, I8>::value || std::is_same<T, F8>::value;
+
 // The kernels of a call: for the requests of few rows either the vector units or a wave's
 // matrix operand, and tiles for the others.
 struct PagedKernels {
@@ -106,6 +119,8 @@ struct PagedKernels {
 int paged_attn_f32(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
 int paged_attn_f16(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
 int paged_attn_bf16(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
+int paged_attn_i8(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
+int paged_attn_f8(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
 
 // The maximum (log2) of no key at all: no finite score lies below it, and beside any other its
 // weight, with the sum 0 that it comes with, changes nothing.

@@ -124,15 +124,16 @@ Plan make_plan(int size, int rows, int batch, int max_new, int max_len, int head
   const int group = heads / kv_heads, most = max_new * group, len = max_len < 1 ? 1 : max_len;
   PagedKernels &k = p.kernels;
   k.tile = hd <= 128 && most > kSpanRows;
-  k.rows = hd > 128 || most <= (size == 4 ? kVecRows : kVecRows16);
+  k.rows = size > 1 && (hd > 128 || most <= (size == 4 ? kVecRows : kVecRows16));
   k.span = !k.rows && (!k.tile || group <= kSpanRows);
   p.few_rows = most < 1 ? 1 : k.tile ? kSpanRows : most;
   const long long pairs = (long long)(batch < 1 ? 1 : batch) * kv_heads;
-  const long long groups = k.rows ? (p.few_rows + kVecRows - 1) / kVecRows : 1;
+  const long long groups = k.rows ? (p.few_rows + kVecRows - 1) / kVecRows : (p.few_rows + kSpanRows - 1) / kSpanRows;
   if (k.span) {
     // a whole request to a workgroup where these fill the CUs (16 x 16 pairs of 4096 bf16 keys:
     // 48.5 us, 55.3 in two chunks, 96 in chunks of 512), else two workgroups for every CU
-    long long splits = pairs >= kComputeUnits ? 1 : (2 * kComputeUnits + pairs - 1) / pairs;
+    const long long many = pairs * groups;
+    long long splits = many >= kComputeUnits ? 1 : (2 * kComputeUnits + many - 1) / many;
     if (splits > (len + 255) / 256) splits = (len + 255) / 256;
     p.few_chunk = round_up((int)((len + splits - 1) / splits), 128);
   } else if (groups > 2) {
@@ -174,19 +175,13 @@ Plan make_plan(int size, int rows, int batch, int max_new, int max_len, int head
   return p;
 }
 
-}  // namespace
-}  // namespace cdml
-
-using namespace cdml;
-
-extern "C" int cdml_paged_attn_workspace_size(int rows, int batch, int max_new, int max_len, int num_heads,
-                                              int num_kv_heads, int head_dim, size_t *bytes) {
-  if (!bytes) return fail(CDML_E_INVALID, "cdml_paged_attn_workspace_size: bytes is NULL");
-  int rc = check_sizes("cdml_paged_attn_workspace_size", rows, batch, max_new, max_len, num_heads, num_kv_heads,
-                       head_dim);
+int workspace_size(const char *what, bool q8, int rows, int batch, int max_new, int max_len, int num_heads,
+                   int num_kv_heads, int head_dim, size_t *bytes) {
+  if (!bytes) return fail(CDML_E_INVALID, "%s: bytes is NULL", what);
+  int rc = check_sizes(what, rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
   if (rc) return rc;
   size_t most = 0;
-  for (int size = 2; size <= 4; size += 2) {  // of either size of cached values
+  for (int size = q8 ? 1 : 2; size <= (q8 ? 1 : 4); size *= 2) {  // of any size of cached values
     const Plan p = make_plan(size, rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
     most = std::max(most, p.few_floats + p.tile_floats);
   }
@@ -194,38 +189,45 @@ extern "C" int cdml_paged_attn_workspace_size(int rows, int batch, int max_new, 
   return CDML_OK;
 }
 
-extern "C" int cdml_paged_attn(const float *q, int ldq, const void *kcache, const void *vcache, int cache_type,
-                               int n_pages, int page_size, const int *block_table, int max_blocks, const int *kv_len,
-                               const int *cu_new, float *o, int ldo, int rows, int batch, int max_new, int max_len,
-                               int num_heads, int num_kv_heads, int head_dim, float scale, int *bad, void *workspace,
-                               size_t workspace_bytes, cdml_stream stream) {
+int attention(const char *what, bool q8, const float *q, int ldq, const void *kcache, const void *vcache,
+              const float *kscale, const float *vscale, int cache_type, int n_pages, int page_size,
+              const int *block_table, int max_blocks, const int *kv_len, const int *cu_new, float *o, int ldo, int rows,
+              int batch, int max_new, int max_len, int num_heads, int num_kv_heads, int head_dim, float scale, int *bad,
+              void *workspace, size_t workspace_bytes, cdml_stream stream) {
   PagedArgs a{};
-  int rc = check_pool("cdml_paged_attn", n_pages, page_size, max_blocks, batch, &a.page_shift);
+  int rc = check_pool(what, n_pages, page_size, max_blocks, batch, &a.page_shift);
   if (rc) return rc;
-  rc = check_sizes("cdml_paged_attn", rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
+  rc = check_sizes(what, rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
   if (rc) return rc;
-  const int size = cache_type_bytes(cache_type);
-  if (!size) return fail(CDML_E_INVALID, "cdml_paged_attn: unknown cache type %d", cache_type);
+  const int size = q8 ? (int)q8_cache_type(cache_type) : cache_type_bytes(cache_type);
+  if (!size) return fail(CDML_E_INVALID, "%s: unknown cache type %d", what, cache_type);
   if ((long long)max_len > (long long)max_blocks * page_size)
-    return fail(CDML_E_INVALID, "cdml_paged_attn: max_len %d above the table's %lld tokens", max_len,
+    return fail(CDML_E_INVALID, "%s: max_len %d above the table's %lld tokens", what, max_len,
                 (long long)max_blocks * page_size);
   const long long dim = (long long)num_heads * head_dim;
-  if (ldq < dim || ldo < dim) return fail(CDML_E_INVALID, "cdml_paged_attn: row stride smaller than the heads");
+  if (ldq < dim || ldo < dim) return fail(CDML_E_INVALID, "%s: row stride smaller than the heads", what);
   if (rows == 0 || batch == 0 || max_new == 0) return CDML_OK;
   if (!q || !kcache || !vcache || !block_table || !kv_len || !cu_new || !o)
-    return fail(CDML_E_INVALID, "cdml_paged_attn: NULL pointer");
+    return fail(CDML_E_INVALID, "%s: NULL pointer", what);
+  if (q8) {
+    rc = check_q8(what, kcache, vcache, kscale, vscale);
+    if (rc) return rc;
+  }
   const Plan p = make_plan(size, rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
   size_t need = 0;
-  rc = cdml_paged_attn_workspace_size(rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim, &need);
+  rc = workspace_size(what, q8, rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim, &need);
   if (rc) return rc;
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
-    return fail(CDML_E_INVALID, "cdml_paged_attn: %zu bytes of 16-byte aligned workspace needed, %zu given", need,
+    return fail(CDML_E_INVALID, "%s: %zu bytes of 16-byte aligned workspace needed, %zu given", what, need,
                 workspace_bytes);
   rc = ensure_device();
   if (rc) return rc;
   a.q = q;
   a.kc = kcache;
   a.vc = vcache;
+  a.ks = kscale;
+  a.vs = vscale;
+  a.width = q8_width(head_dim);
   a.table = block_table;
   a.kv_len = kv_len;
   a.cu_new = cu_new;
@@ -255,13 +257,55 @@ extern "C" int cdml_paged_attn(const float *q, int ldq, const void *kcache, cons
   const bool wide = head_dim % 8 == 0 && ldq % 4 == 0 && ldo % 4 == 0 && aligned16(q) && aligned16(o) &&
                     aligned16(kcache) && aligned16(vcache);
   const hipStream_t st = as_hip(stream);
-  if (cache_type == CDML_CACHE_F32) rc = paged_attn_f32(a, p.kernels, wide, st);
-  else if (cache_type == CDML_CACHE_F16) rc = paged_attn_f16(a, p.kernels, wide, st);
-  else rc = paged_attn_bf16(a, p.kernels, wide, st);
+  switch (cache_type) {
+    case CDML_CACHE_F32: rc = paged_attn_f32(a, p.kernels, wide, st); break;
+    case CDML_CACHE_F16: rc = paged_attn_f16(a, p.kernels, wide, st); break;
+    case CDML_CACHE_BF16: rc = paged_attn_bf16(a, p.kernels, wide, st); break;
+    case CDML_CACHE_I8: rc = paged_attn_i8(a, p.kernels, wide, st); break;
+    default: rc = paged_attn_f8(a, p.kernels, wide, st);
+  }
   if (rc) return rc;
   if (!p.few_floats && !p.tile_floats) return CDML_OK;
   const int few_tokens = p.few_floats ? p.few_rows / a.group : 0;  // of a request of few rows, at most
   const unsigned joins = (unsigned)batch * few_tokens + (p.tile_floats ? (unsigned)rows : 0u);
   paged_join_kernel<<<dim3(joins, (unsigned)(num_heads + 3) / 4), 256, 0, st>>>(a, few_tokens);
   return check_launch("paged_join_kernel");
+}
+
+}  // namespace
+}  // namespace cdml
+
+using namespace cdml;
+
+extern "C" int cdml_paged_attn_workspace_size(int rows, int batch, int max_new, int max_len, int num_heads,
+                                              int num_kv_heads, int head_dim, size_t *bytes) {
+  return workspace_size("cdml_paged_attn_workspace_size", false, rows, batch, max_new, max_len, num_heads, num_kv_heads,
+                        head_dim, bytes);
+}
+
+extern "C" int cdml_paged_attn_q8_workspace_size(int rows, int batch, int max_new, int max_len, int num_heads,
+                                                 int num_kv_heads, int head_dim, size_t *bytes) {
+  return workspace_size("cdml_paged_attn_q8_workspace_size", true, rows, batch, max_new, max_len, num_heads,
+                        num_kv_heads, head_dim, bytes);
+}
+
+extern "C" int cdml_paged_attn(const float *q, int ldq, const void *kcache, const void *vcache, int cache_type,
+                               int n_pages, int page_size, const int *block_table, int max_blocks, const int *kv_len,
+                               const int *cu_new, float *o, int ldo, int rows, int batch, int max_new, int max_len,
+                               int num_heads, int num_kv_heads, int head_dim, float scale, int *bad, void *workspace,
+                               size_t workspace_bytes, cdml_stream stream) {
+  return attention("cdml_paged_attn", false, q, ldq, kcache, vcache, nullptr, nullptr, cache_type, n_pages, page_size,
+                   block_table, max_blocks, kv_len, cu_new, o, ldo, rows, batch, max_new, max_len, num_heads,
+                   num_kv_heads, head_dim, scale, bad, workspace, workspace_bytes, stream);
+}
+
+extern "C" int cdml_paged_attn_q8(const float *q, int ldq, const void *kcache, const void *vcache, const float *kscale,
+                                  const float *vscale, int cache_type, int n_pages, int page_size,
+                                  const int *block_table, int max_blocks, const int *kv_len, const int *cu_new,
+                                  float *o, int ldo, int rows, int batch, int max_new, int max_len, int num_heads,
+                                  int num_kv_heads, int head_dim, float scale, int *bad, void *workspace,
+                                  size_t workspace_bytes, cdml_stream stream) {
+  return attention("cdml_paged_attn_q8", true, q, ldq, kcache, vcache, kscale, vscale, cache_type, n_pages, page_size,
+                   block_table, max_blocks, kv_len, cu_new, o, ldo, rows, batch, max_new, max_len, num_heads,
+                   num_kv_heads, head_dim, scale, bad, workspace, workspace_bytes, stream);
 }

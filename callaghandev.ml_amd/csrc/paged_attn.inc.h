@@ -1,5 +1,5 @@
 // The attention kernels over a paged cache, for one cache type T (float, _Float16 or
-// __bf16; included by a file each).
+// __bf16, and of the tiles I8 or F8; included by a file each).
 #pragma once
 
 #include "paged.h"
@@ -15,6 +15,14 @@ struct Raw4 {
 template <>
 struct Raw4<float> {
   typedef vf4 type;
+};
+template <>
+struct Raw4<I8> {
+  typedef uint32_t type;
+};
+template <>
+struct Raw4<F8> {
+  typedef uint32_t type;
 };
 
 __device__ __forceinline__ float half_value(uint32_t w, int i, _Float16) {
@@ -274,6 +282,34 @@ struct Pieces<__bf16> {
   static constexpr int N = 1, PRODUCTS = 3;
   static constexpr int A[3] = {0, 0, 0}, B[3] = {2, 1, 0};
 };
+// A code of 8 bits is one bf16 value; its key's scale meets the score (K) or the probability (V).
+template <>
+struct Pieces<I8> : Pieces<__bf16> {};
+template <>
+struct Pieces<F8> : Pieces<__bf16> {};
+
+// Of the probabilities times V's scales: as small as 2^-150 they keep fp32's bits in bf16 pieces
+// (common.h); those of 2^87 and more over V's codes come out infinite, and are recomputed.
+constexpr float kCodeScale = 1099511627776.f, kCodeUnscale = 1.f / kCodeScale;  // 2^40
+
+// Codes (dims 2 i, 2 i + 1 of four in w) as a pair of bf16 values, which hold them exactly.
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, I8) {
+  const float a = (float)(int8_t)(w >> 16 * i), b = (float)(int8_t)(w >> (16 * i + 8));
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, F8) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 r = i ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true)
+                     : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false);
+  return __builtin_bit_cast(uint32_t, r);
+}
+__device__ __forceinline__ float code_value(I8 x) { return (float)(int8_t)x.c; }
+__device__ __forceinline__ float code_value(F8 x) { return __builtin_amdgcn_cvt_f32_fp8(x.c, 0); }
+__device__ __forceinline__ float cached(float x, float) { return x; }
+__device__ __forceinline__ float cached(_Float16 x, float) { return (float)x; }
+__device__ __forceinline__ float cached(__bf16 x, float) { return (float)x; }
+template <typename T>
+__device__ __forceinline__ float cached(T x, float scale) { return code_value(x) * scale; }
 
 // Where a key's row lies in the cache, and whether its page is a page.
 struct Slot {
@@ -285,13 +321,39 @@ __device__ __forceinline__ Slot slot_in(const PagedArgs &a, int page, int key) {
   return {((uint32_t)(ok ? page : 0) << a.page_shift) + (uint32_t)(key & ((1 << a.page_shift) - 1)), ok};
 }
 
+// Elements before a slot's row in a head's cache; of an 8-bit cache, rows of the head's scales.
+template <typename T>
+__device__ __forceinline__ size_t row_at(const PagedArgs &a, uint32_t slot) {
+  if constexpr (kQ8<T>) {
+    const uint32_t page = slot >> a.page_shift;
+    return ((size_t)page * a.kv_heads << a.page_shift) + (slot & ((1u << a.page_shift) - 1));
+  }
+  return (size_t)slot * (uint32_t)(a.kv_heads * a.hd);
+}
+template <typename T>
+__device__ __forceinline__ const T *head_of(const PagedArgs &a, const void *cache, int hk) {
+  return static_cast<const T *>(cache) + (kQ8<T> ? ((size_t)hk << a.page_shift) * a.width : (size_t)hk * a.hd);
+}
+template <typename T>
+__device__ __forceinline__ int row_step(const PagedArgs &a) {
+  return kQ8<T> ? a.width : a.kv_heads * a.hd;
+}
+
 // Puts dim c of two neighbouring keys of V (a's the lower one) at place d of its row in
 // every piece's plane.
 template <typename T>
 __device__ __forceinline__ void put_v(char *d, int plane, const typename Raw4<T>::type &a,
                                       const typename Raw4<T>::type &b, int c) {
   constexpr int NP = Pieces<T>::N;
-  if constexpr (NP == 1) {
+  if constexpr (kQ8<T>) {
+    if constexpr (std::is_same<T, I8>::value) {
+      const float x = code_value(I8{(uint8_t)(a >> 8 * c)}), y = code_value(I8{(uint8_t)(b >> 8 * c)});
+      *reinterpret_cast<uint32_t *>(d) = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+    } else {
+      *reinterpret_cast<uint32_t *>(d) = __builtin_amdgcn_perm(code_pair(b, c / 2, T{}), code_pair(a, c / 2, T{}),
+                                                               c & 1 ? 0x07060302u : 0x05040100u);
+    }
+  } else if constexpr (NP == 1) {
     *reinterpret_cast<uint32_t *>(d) = __builtin_amdgcn_perm(b[c / 2], a[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
   } else {
     uint32_t h, m, l;
@@ -350,7 +412,9 @@ struct PagedStage {
   static constexpr int KROWB = BN / 2 * 32, VROWB = HD / 4 * 32;  // bytes of one row cluster
   static constexpr int KSLAB = 2 * KROWB + 128, VSLAB = 4 * VROWB + 256;
   static constexpr int KPLANE = HD / 16 * KSLAB, VPLANE = BN / 16 * VSLAB;
-  static constexpr int BYTES = NP * (KPLANE + VPLANE);   // K planes, then V planes
+  static constexpr bool Q8 = kQ8<T>;
+  static constexpr int SCALES = NP * (KPLANE + VPLANE);  // K planes, V planes, then K's and V's scales
+  static constexpr int BYTES = SCALES + (Q8 ? 2 * BN * 4 : 0);
   static constexpr int VU = (HD / 4) * (BN / 2) / HALF;  // V units per thread; twice as many K units
   static constexpr int NV = 2 * VU;                      // loads of either
   static constexpr int NB = BN / 16;                     // blocks of 16 keys
@@ -374,8 +438,11 @@ struct PagedStage {
   int col, row, dst;  // first column, first row in a tile, LDS byte offset of the first unit
   int slab;           // V: the first unit's block (wave-uniform)
   int loaded;         // first key of the tile in r
-  int kv_dim, last;   // the request's last key
+  int kv_dim, last;   // elements from row to row, the request's last key
   bool kside;
+  const float *scales;  // 8 bits: the head's, of this side
+  int scale_page;       // the page of key lane % 32 of the next tile
+  float scale;          // and its scale in the loaded one
 
   __device__ __forceinline__ void init(const PagedArgs &a, int b, int hk, int last_key) {
     const int t0 = __builtin_amdgcn_readfirstlane(threadIdx.x);
@@ -391,10 +458,32 @@ struct PagedStage {
     row = kside ? kkey : 2 * sb + (UNI ? 0 : 16 * slab);
     dst = kside ? (c >> 2) * KSLAB + kcluster(kkey & 1) + (kkey >> 1) * 32 + (c & 3) * 8
                 : NP * KPLANE + slab * VSLAB + g * 32 + place * 4;
-    base = static_cast<const T *>(kside ? a.kc : a.vc) + (size_t)hk * a.hd + (UNI ? 0 : col);
+    base = head_of<T>(a, kside ? a.kc : a.vc, hk) + (UNI ? 0 : col);
     table = a.table + (size_t)b * a.max_blocks;
-    kv_dim = a.kv_heads * a.hd;
+    kv_dim = row_step<T>(a);
     last = last_key;
+    if constexpr (Q8) scales = (kside ? a.ks : a.vs) + ((size_t)hk << a.page_shift);
+  }
+  // 8 bits: the first wave of either half has the tile's scales, a key's to two lanes
+  static __device__ __forceinline__ bool has_scales() {
+    return (__builtin_amdgcn_readfirstlane(threadIdx.x) & 64) == 0;
+  }
+  __device__ __forceinline__ int scale_key(int k0) const { return min(k0 + (int)(threadIdx.x & 31), last); }
+  __device__ __forceinline__ void lookup_scale(const PagedArgs &a, int k0) {
+    static_assert(!Q8 || BN == 32, "a key to a lane");
+    if constexpr (Q8)
+      if (has_scales()) scale_page = table[scale_key(k0) >> a.page_shift];
+  }
+  __device__ __forceinline__ void load_scale(const PagedArgs &a, int k0) {
+    if constexpr (Q8)
+      if (has_scales()) {
+        const Slot s = slot_in(a, scale_page, scale_key(k0));
+        scale = s.ok ? scales[row_at<T>(a, s.at)] * (kside ? 1.f : kCodeScale) : 0.f;
+      }
+  }
+  __device__ __forceinline__ void store_scale(char *lds) const {
+    if constexpr (Q8)
+      if (has_scales()) reinterpret_cast<float *>(lds + SCALES)[(kside ? 0 : BN) + (threadIdx.x & 31)] = scale;
   }
   // Load i's row in the tile, without the lane's part
   __device__ __forceinline__ int row_of(int i) const {
@@ -412,7 +501,7 @@ struct PagedStage {
   __device__ __forceinline__ void start_group(const PagedArgs &a, int k0) {
     const int mine = k0 + 16 * (int)(threadIdx.x & 63);
     const Slot s = slot_in(a, page[0], mine);
-    const uint64_t at = reinterpret_cast<uint64_t>(base + (size_t)s.at * kv_dim);
+    const uint64_t at = reinterpret_cast<uint64_t>(base + row_at<T>(a, s.at) * (Q8 ? a.width : 1));
     base_lo = (uint32_t)at;
     base_hi = (uint32_t)(at >> 32);
     none = __builtin_amdgcn_ballot_w64(!s.ok);
@@ -421,6 +510,7 @@ struct PagedStage {
   }
   // What load() of the first tile needs; then, after each load, of the next.
   __device__ __forceinline__ void lookup_first(const PagedArgs &a, int k0) {
+    lookup_scale(a, k0);
     if constexpr (UNI) {
       page[0] = page_of_block(a, k0);
       start_group(a, k0);
@@ -433,10 +523,13 @@ struct PagedStage {
 #pragma unroll
       for (int i = 0; i < NV; ++i) page[i] = table[key(k0, i) >> a.page_shift];
     }
+    lookup_scale(a, k0);
   }
 
   __device__ __forceinline__ void load(const PagedArgs &a, int k0) {
     loaded = k0;
+    load_scale(a, k0);
+    const int columns = Q8 ? a.width : a.hd;
     if constexpr (UNI) {
       if (k0 - group >= 1024) start_group(a, k0);
       const int first = (k0 - group) >> 4;
@@ -452,7 +545,7 @@ struct PagedStage {
       uint32_t off[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        off[i] = (uint32_t)(row * kv_dim + min(col + 4 * vgroups(i), a.hd - 4)) * (uint32_t)sizeof(T);
+        off[i] = (uint32_t)(row * kv_dim + min(col + 4 * vgroups(i), columns - 4)) * (uint32_t)sizeof(T);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         GlobalBytes p = nullptr;
@@ -469,9 +562,9 @@ struct PagedStage {
         const Slot s = slot_in(a, page[i], key(k0, i));
         if (!s.ok) zero |= 1u << i;
         const int dc = kside ? 0 : 4 * vgroups(i / 2);
-        const T *p = base + (size_t)s.at * kv_dim + dc;
-        if constexpr (VEC) {
-          r[i] = *reinterpret_cast<const Raw *>(p + min(0, a.hd - 4 - col - dc));
+        const T *p = base + row_at<T>(a, s.at) * (Q8 ? a.width : 1) + dc;
+        if constexpr (VEC || Q8) {
+          r[i] = *reinterpret_cast<const Raw *>(p + min(0, columns - 4 - col - dc));
         } else {
           r[i] = load4_cut<T>(p, col + dc, a.hd);
         }
@@ -480,6 +573,7 @@ struct PagedStage {
   }
 
   __device__ __forceinline__ void store(char *lds, int *bad) {
+    store_scale(lds);
     if constexpr (UNI) {
       if (zero || loaded + BN - 1 > last) {  // (wave-uniform)
         if (zero && bad) *bad = 1;
@@ -497,7 +591,9 @@ struct PagedStage {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         char *d = lds + dst + KSTEP / 2 * 32 * i;
-        if constexpr (NP == 1) {
+        if constexpr (Q8) {
+          *reinterpret_cast<vu2 *>(d) = vu2{code_pair(r[i], 0, T{}), code_pair(r[i], 1, T{})};
+        } else if constexpr (NP == 1) {
           *reinterpret_cast<vu2 *>(d) = r[i];
         } else {
           float x[4];
@@ -534,21 +630,21 @@ struct PagedStage {
 };
 
 // Q^T operand of a wave: the three bf16 pieces of this lane's row times scale_log2, eight
-// values of every `step` (16 or 32, by the MFMA) from 8 * part on.
+// values of every `step` from `from` on.
 // Neither Q nor K takes the split's scale, so that scores come out as they are: what a
 // component below 2^-110 loses (2^-134) reaches a score only through a component of
 // 2^100 and more on the other side.  Returns whether Q holds one or the other
 // (wave-uniform); such rows are recomputed on the fp32 MFMA.
 template <int N, bool VEC>
 __device__ __forceinline__ bool load_q_pieces(bf16x8 (&q)[N][3], const float *qrow, int hd, float scale, int step,
-                                              int part) {
+                                              int from) {
   uint32_t most = 0, least = ~0u;  // of |x|, and of 2 |x| - 1 as integers, which leaves zeros out
 #pragma unroll
   for (int s = 0; s < N; ++s) {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; e += 4) {
-      const int d = step * s + 8 * part + e;
+      const int d = step * s + from + e;
       if constexpr (VEC) {
         const vf4 t = d < hd ? *reinterpret_cast<const vf4 *>(qrow + d) : vf4{};
 #pragma unroll
@@ -617,7 +713,12 @@ struct PagedRows {
     for (int i = 0; i < NP; ++i) k[i] = *reinterpret_cast<const bf16x8 *>(kt + i * Tile::KPLANE + s * Tile::KSLAB);
   }
 
-  __device__ __forceinline__ void accumulate_pv(const floatx16 &p, const char *vt) {
+  // The scales of the four keys of a sub-block that accumulator registers 4 g .. 4 g + 3 hold.
+  static __device__ __forceinline__ vf4 scales_of(const char *sc, int g) {
+    return *reinterpret_cast<const vf4 *>(sc + 32 * g);
+  }
+
+  __device__ __forceinline__ void accumulate_pv(const floatx16 &p, const char *vt, const char *sc) {
     constexpr int N = 2 * NDB, AHEAD = N < kAhead ? N : kAhead;
     Operand v[AHEAD];
     bf16x8 pp[3];
@@ -631,6 +732,14 @@ struct PagedRows {
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = p[8 * s + e];
+        if constexpr (kQ8<T>) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const vf4 w = scales_of(sc + BN * 4, 2 * s + g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * g + e] *= w[e];
+          }
+        }
         split_operand(x, 1.f, pp);
       }
 #pragma unroll
@@ -644,7 +753,7 @@ struct PagedRows {
   }
 
   // Scores in log2 units, relative to the reference (absolute until there is one).
-  __device__ __forceinline__ floatx16 scores(const char *kt, const bf16x8 (&q)[NS][3]) const {
+  __device__ __forceinline__ floatx16 scores(const char *kt, const bf16x8 (&q)[NS][3], const char *sc) const {
     constexpr int AHEAD = NS < kAhead ? NS : kAhead;
     floatx16 sacc = {};
     Operand k[AHEAD];
@@ -662,15 +771,24 @@ struct PagedRows {
       }
     }
     const float ref = m_run == -INFINITY ? 0.f : m_run;
+    if constexpr (kQ8<T>) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sacc[r] -= ref;
+      for (int g = 0; g < 4; ++g) {
+        const vf4 w = scales_of(sc, g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sacc[4 * g + e] = fmaf(sacc[4 * g + e], w[e], -ref);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sacc[r] -= ref;
+    }
     return sacc;
   }
 
   // The common sub-block once every row has its reference: probabilities and their
   // per-lane sum first; false (nothing changed but sacc) if some lane's sum is above 2^32 or
   // NaN, and the caller takes softmax() on recomputed scores.
-  __device__ __forceinline__ bool try_fast(floatx16 &sacc, const char *vt, bool masked, int last_vis) {
+  __device__ __forceinline__ bool try_fast(floatx16 &sacc, const char *vt, const char *sc, bool masked, int last_vis) {
     if (masked) apply_mask(sacc, last_vis);
 #pragma unroll
     for (int r = 0; r < 16; ++r) sacc[r] = fast_exp2(sacc[r]);
@@ -680,7 +798,7 @@ struct PagedRows {
     const float ps = ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
     if (__builtin_amdgcn_ballot_w64(!(ps <= kFastSumLimit))) return false;
     l_sum += ps;
-    accumulate_pv(sacc, vt);
+    accumulate_pv(sacc, vt, sc);
     return true;
   }
 
@@ -722,7 +840,7 @@ struct PagedRows {
 
   // Undoes V's scale; whether some row came out non-finite (wave-uniform).
   __device__ __forceinline__ bool finish() {
-    constexpr float unscale = NP == 3 ? kSplitUnscale : 1.f;
+    constexpr float unscale = NP == 3 ? kSplitUnscale : kQ8<T> ? kCodeUnscale : 1.f;
     float wrong = l_sum * 0.f;
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
@@ -742,20 +860,22 @@ struct PagedRows {
   __device__ __forceinline__ void recompute(const PagedArgs &a, const float *qrow, const int *table, int hk, int li,
                                             int hf, int c0, int c1, int lim, int lim_lo, int last) {
     init();
-    const int kv_dim = a.kv_heads * a.hd;
-    const T *kb = static_cast<const T *>(a.kc) + (size_t)hk * a.hd, *vb = static_cast<const T *>(a.vc) + (size_t)hk * a.hd;
+    const size_t unit = kQ8<T> ? a.width : 1, head = kQ8<T> ? (size_t)hk << a.page_shift : 0;
+    const T *kb = head_of<T>(a, a.kc, hk), *vb = head_of<T>(a, a.vc, hk);
 #pragma unroll 1
     for (int kb0 = c0; kb0 < c1; kb0 += 32) {
       const int key = min(kb0 + li, last);
       const Slot ks = slot_in(a, table[key >> a.page_shift], key);
-      const T *krow = kb + (size_t)ks.at * kv_dim;
+      const size_t kat = row_at<T>(a, ks.at);
+      const T *krow = kb + kat * unit;
+      const float kscale = kQ8<T> ? a.ks[head + kat] : 1.f;
       floatx16 sacc;
 #pragma unroll
       for (int r = 0; r < 16; ++r) sacc[r] = m_run == -INFINITY ? 0.f : -m_run;
 #pragma unroll 1
       for (int d = 0; d < HD; d += 2) {
         const bool in = d + hf < a.hd;
-        sacc = mfma32x32x2(in && ks.ok ? (float)krow[d + hf] : 0.f, in ? qrow[d + hf] * a.scale_log2 : 0.f, sacc);
+        sacc = mfma32x32x2(in && ks.ok ? cached(krow[d + hf], kscale) : 0.f, in ? qrow[d + hf] * a.scale_log2 : 0.f, sacc);
       }
       softmax(sacc, true, lim - kb0 - 4 * hf);
       const bool whole = kb0 + 31 <= lim_lo;  // (wave-uniform)
@@ -765,14 +885,16 @@ struct PagedRows {
         const int r = whole ? i : (i >> 3) * 4 + (i & 3);
         const int vk = kb0 + (whole ? acc_key(i) + 4 * hf : i), vkey = min(vk, last);
         const Slot vs = slot_in(a, table[vkey >> a.page_shift], vkey);
-        const T *vrow = vb + (size_t)vs.at * kv_dim;
+        const size_t vat = row_at<T>(a, vs.at);
+        const T *vrow = vb + vat * unit;
+        const float vscale = kQ8<T> ? a.vs[head + vat] : 1.f;
         float p = 0.f;
 #pragma unroll
         for (int c = 0; c < 16; ++c) p = c == r ? sacc[c] : p;
         if (whole) {
 #pragma unroll
           for (int db = 0; db < NDB; ++db)
-            oacc[db] = mfma32x32x2(db * 32 + li < a.hd && vs.ok ? (float)vrow[db * 32 + li] : 0.f, p, oacc[db]);
+            oacc[db] = mfma32x32x2(db * 32 + li < a.hd && vs.ok ? cached(vrow[db * 32 + li], vscale) : 0.f, p, oacc[db]);
         } else {
           p = __shfl(p, li + 32 * (i >> 2 & 1));
           if (vk <= lim) {
@@ -781,7 +903,7 @@ struct PagedRows {
 #pragma unroll
               for (int c = 0; c < 16; ++c) {
                 const int d = db * 32 + acc_key(c) + 4 * hf;
-                oacc[db][c] = fmaf(p, d < a.hd && vs.ok ? (float)vrow[d] : 0.f, oacc[db][c]);
+                oacc[db][c] = fmaf(p, d < a.hd && vs.ok ? cached(vrow[d], vscale) : 0.f, oacc[db][c]);
               }
           }
         }
@@ -814,8 +936,8 @@ constexpr int kTileClasses = 8;
 // 4 x 2048 of 4096 tokens: three 331 us (bf16) and 506 (fp16), two 348 and 530.
 template <typename T>
 constexpr int tile_waves(int hd) {
-  if (hd <= 32 || (hd <= 64 && sizeof(T) == 2)) return 3;
-  return hd <= 64 || sizeof(T) == 2 ? 2 : 1;
+  if (hd <= 32 || (hd <= 64 && sizeof(T) <= 2)) return 3;
+  return hd <= 64 || sizeof(T) <= 2 ? 2 : 1;
 }
 template <typename T, int HD, int BN, bool VEC, bool UNI>
 __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kernel(const PagedArgs a) {
@@ -885,7 +1007,7 @@ __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kern
     st.load(a, c0);
     st.lookup(a, c0 + BN);
     bf16x8 q[HD / 16][3];
-    const bool wide = load_q_pieces<HD / 16, VEC>(q, qrow, a.hd, a.scale_log2, 16, hf);
+    const bool wide = load_q_pieces<HD / 16, VEC>(q, qrow, a.hd, a.scale_log2, 16, 8 * hf);
     st.store(lds[0], a.bad);
     __syncthreads();
     const int ko = Stage::koperand(li, hf), vo = Stage::voperand(li, hf);
@@ -899,21 +1021,22 @@ __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kern
         const int kb0 = k0 + kb * 32;
         if (kb0 >= c1 || kb0 > lim_hi || rw0 >= nr) continue;
         const char *kop = lds[cur] + ko + kb * 512, *vop = lds[cur] + vo + 2 * kb * Stage::VSLAB;
-        floatx16 sacc = rows.scores(kop, q);
+        const char *sc = Stage::Q8 ? lds[cur] + Stage::SCALES + kb * 128 + hf * 16 : nullptr;
+        floatx16 sacc = rows.scores(kop, q, sc);
         const bool masked = kb0 + 31 > lim_lo;
         const int last_vis = lim - kb0 - 4 * hf;
         bool done = false;
         if (rows.warm) {
-          done = rows.try_fast(sacc, vop, masked, last_vis);
+          done = rows.try_fast(sacc, vop, sc, masked, last_vis);
           if (!done) {
             // K is read from LDS again (the compiler may not keep the first scores)
             asm volatile("" ::: "memory");
-            sacc = rows.scores(kop, q);
+            sacc = rows.scores(kop, q, sc);
           }
         }
         if (!done) {
           rows.softmax(sacc, masked, last_vis);
-          rows.accumulate_pv(sacc, vop);
+          rows.accumulate_pv(sacc, vop, sc);
         }
       }
       if (k0 + BN < c1) st.store(lds[cur ^ 1], a.bad);
@@ -1270,7 +1393,7 @@ __global__ void __launch_bounds__(PT_THREADS, sizeof(T) == 2 || HD <= 64 ? 2 : 1
     blk.load(a, kc, vc, kv_dim, page_at(first), key_at(first));
     int page = page_at(first + 128);
     bf16x8 q[NS][3];
-    const bool wide = load_q_pieces<NS, VEC>(q, qrow, a.hd, a.scale_log2, 32, quarter);
+    const bool wide = load_q_pieces<NS, VEC>(q, qrow, a.hd, a.scale_log2, 32, 8 * quarter);
 #pragma unroll 1
     for (int k0 = first; k0 < c1; k0 += 128) {
       blk.clean(k0, last, a.bad);

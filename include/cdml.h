@@ -714,6 +714,23 @@ int cdml_paged_attn(const float *q, int ldq, const void *kcache,
                     int *bad, void *workspace, size_t workspace_bytes,
                     cdml_stream stream);
 
+/* cdml_paged_attn over an 8-bit cache (CDML_CACHE_I8, CDML_CACHE_F8), which stands
+ * for the values c * s: the codes are multiplied as they are, a key's scale meets its
+ * scores and its probabilities.  A row of s = NaN counts as NaNs. */
+int cdml_paged_attn_q8_workspace_size(int rows, int batch, int max_new,
+                                      int max_len, int num_heads,
+                                      int num_kv_heads, int head_dim,
+                                      size_t *bytes);
+int cdml_paged_attn_q8(const float *q, int ldq, const void *kcache,
+                       const void *vcache, const float *kscale,
+                       const float *vscale, int cache_type, int n_pages,
+                       int page_size, const int *block_table, int max_blocks,
+                       const int *kv_len, const int *cu_new, float *o, int ldo,
+                       int rows, int batch, int max_new, int max_len,
+                       int num_heads, int num_kv_heads, int head_dim,
+                       float scale, int *bad, void *workspace,
+                       size_t workspace_bytes, cdml_stream stream);
+
 /* Gives every row b of the tables the state of row parents[b] (device
  * int32[batch]; -1, and any value outside [0, batch), leaves it empty, which
  * also releases a request): full pages become shared, a page that is not full

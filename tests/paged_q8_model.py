@@ -7,7 +7,7 @@ import torch
 
 from abi_ops import down, stream, up
 from cdml import native as N
-from paged_model import from_bits, ints, raw_dtype, to_bits
+from paged_model import from_bits, ints, raw_dtype, to_bits, ws
 
 
 def width(hd):
@@ -109,3 +109,49 @@ def call_read(c, table, kv, cu, rows, ldk, ldv, fill=7.0, n_pages=None):
                                     table.shape[1], l.ptr, u.ptr, out[0].ptr, ldk, out[1].ptr, ldv, rows, len(kv),
                                     c["heads"], c["hd"], bad.ptr, stream().handle))
     return down(out[0], (rows, ldk)), down(out[1], (rows, ldv)), int(down(bad, (1,), np.int32)[0])
+
+
+def call_attention(q, c, table, kv, cu, H, scale, o, max_new=None, max_len=None, ldq=None, ldo=None, n_pages=None,
+                   filth=True):
+    """cdml_paged_attn_q8; q, o [rows, H * hd]; returns (o, bad)."""
+    rows, B, hd = len(q), len(kv), c["hd"]
+    ldq, ldo = ldq or q.shape[1], ldo or o.shape[1]
+    wide = np.full((rows, ldq), np.nan, np.float32)
+    wide[:, :q.shape[1]] = q
+    out = np.full((rows, ldo), 7.0, np.float32)
+    out[:, :o.shape[1]] = o
+    max_new = int(np.max(np.diff(cu), initial=0)) if max_new is None else max_new
+    max_len = int(np.max(kv, initial=0)) if max_len is None else max_len
+    dq, do, d = up(wide), up(out), upload(c)
+    dt, dl, dc, bad = ints(table), ints(kv), ints(cu), ints(np.zeros(1))
+    size = (rows, B, max_new, max_len, H, c["heads"], hd)
+    w, n = ws("cdml_paged_attn_q8_workspace_size", *size)
+    if filth:
+        w.upload(np.full(max(n // 4, 1), np.nan, np.float32), stream())
+    N.check(N.lib().cdml_paged_attn_q8(dq.ptr, ldq, *(b.ptr for b in d), N.CACHE[c["kind"]], n_pages or len(c["k"]),
+                                       c["P"], dt.ptr, table.shape[1], dl.ptr, dc.ptr, do.ptr, ldo, *size, scale, bad.ptr,
+                                       w.ptr, n, stream().handle))
+    out = down(do, out.shape)
+    assert (out[:, o.shape[1]:] == 7.0).all()
+    return out[:, :o.shape[1]], int(down(bad, (1,), np.int32)[0])
+
+
+def unseen_filth(c, table, lens):
+    """NaN scales, and codes that are NaN as e4m3, in every slot that no request has."""
+    if c["kind"] not in ("i8", "f8"):
+        for s in "kv":
+            used = np.zeros((len(c["k"]), c["P"]), bool)
+            mark(used, table, lens, c["P"])
+            c[s][~used] = to_bits(np.full(1, np.nan), c["kind"])[0]
+        return
+    used = np.zeros((len(c["k"]), c["P"]), bool)
+    mark(used, table, lens, c["P"])
+    for s in "kv":
+        c[s] = np.where(used[:, None, :, None], c[s], np.uint8(0x7f if c["kind"] == "f8" else 0x80))
+        c[s + "s"] = np.where(used[:, None], c[s + "s"], np.float32(np.nan))
+
+
+def mark(used, table, lens, P):
+    for b, m in enumerate(lens):
+        at = np.arange(m)
+        used[table[b, at // P], at % P] = True
