@@ -109,6 +109,10 @@ SIGNATURES = {
     "cdml_paged_append_q8": [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp],
     "cdml_paged_attn_q8_workspace_size": [_i] * 7 + [C.POINTER(_sz)],
     "cdml_paged_attn_q8": [_vp, _i] + [_vp] * 4 + [_i, _i, _i, _vp, _i, _vp, _vp, _vp] + [_i] * 8 + [_f, _vp, _vp, _sz, _vp],
+    "cdml_paged_shared": [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp],
+    "cdml_paged_attn_shared_workspace_size": [_i] * 10 + [C.POINTER(_sz)],
+    "cdml_paged_attn_shared": [_vp, _i] + [_vp] * 4 + [_i, _i, _i, _vp, _i] + [_vp] * 5 + [_i] * 11 + [
+        _f, _vp, _vp, _sz, _vp],
     "cdml_paged_copy_q8": [_vp, _vp, _vp, _vp, _i, _sz, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp],
     "cdml_paged_read": [_vp] * 4 + [_i, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp],
     "cdml_beam_select_workspace_size": [_i, _i, _i, C.POINTER(_sz)],

@@ -84,19 +84,59 @@ struct PagedArgs {
   float *few_part;   // [batch][kv_heads][few_rows][few_splits][hd + 2]
   float *tile_part;  // [rows][heads][tile_splits][hd + 2]
   UDiv by_group;
+  // Requests that share their first tokens (SHARED): a launch for what the groups share, in
+  // which a group is one request whose rows are those of all its members, and one for the
+  // tokens behind.  Their chunks leave sums in part [rows][heads][part_splits][hd + 2], the
+  // shared tokens' first.
+  const int *group_start, *shared;
+  int groups;
+  bool prefix;  // which of the two
+  float *part;
+  int part_splits, first_split;
 };
 
 struct PagedSeq {
-  int first, n, len;  // first row, new tokens, tokens in the cache
+  int first, n, len;  // first row, new tokens, tokens in the cache (past the last that counts)
+  int start, table;   // first token that counts, row of the block table
+  bool causal;        // new token i sees those up to len - n + i, else all
 };
 
+// Tokens that request b shares with its group, whole pages.
+__device__ __forceinline__ int shared_tokens(const PagedArgs &a, int b) {
+  return min(max(a.shared[b], 0), a.max_len) & ~((1 << a.page_shift) - 1);
+}
+
+// Request b; of a launch over what groups share, group b.
+template <bool SHARED = false>
 __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &a, int b) {
-  PagedSeq s;
+  PagedSeq s{};
+  if (SHARED && a.prefix) {
+    s.table = min(max(a.group_start[b], 0), a.batch);
+    const int behind = min(max(a.group_start[b + 1], s.table), a.batch);
+    if (behind - s.table < 2) return s;
+    s.first = min(max(a.cu_new[s.table], 0), a.rows);
+    s.len = shared_tokens(a, s.table);
+    s.n = s.len ? min(max(a.cu_new[behind], s.first), a.rows) - s.first : 0;
+    return s;
+  }
   s.first = min(max(a.cu_new[b], 0), a.rows);
   const int end = min(max(a.cu_new[b + 1], s.first), a.rows);
   s.n = min(end - s.first, a.max_new);
   s.len = min(max(a.kv_len[b], 0), a.max_len);
+  s.table = b;
+  s.causal = true;
+  if constexpr (SHARED) s.start = shared_tokens(a, b);
   return s;
+}
+
+// Keys [from, to) of split `split` of `splits`: a chunk from the first on, and the last takes the rest.
+template <bool SHARED>
+__device__ __forceinline__ int split_from(const PagedSeq &s, int split, int chunk) {
+  return (SHARED ? s.start : 0) + split * chunk;
+}
+template <bool SHARED>
+__device__ __forceinline__ int split_to(int from, int split, int splits, int chunk, int kend) {
+  return SHARED && split == splits - 1 ? kend : min(from + chunk, kend);
 }
 
 // A cached value of 8 bits, without its scale.
@@ -121,6 +161,13 @@ int paged_attn_f16(const PagedArgs &a, const PagedKernels &k, bool wide, hipStre
 int paged_attn_bf16(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
 int paged_attn_i8(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
 int paged_attn_f8(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
+
+// The same over what groups share, or over the tokens behind it.
+int paged_shared_f32(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
+int paged_shared_f16(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
+int paged_shared_bf16(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
+int paged_shared_i8(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
+int paged_shared_f8(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st);
 
 // The maximum (log2) of no key at all: no finite score lies below it, and beside any other its
 // weight, with the sum 0 that it comes with, changes nothing.

@@ -939,7 +939,7 @@ constexpr int tile_waves(int hd) {
   if (hd <= 32 || (hd <= 64 && sizeof(T) <= 2)) return 3;
   return hd <= 64 || sizeof(T) <= 2 ? 2 : 1;
 }
-template <typename T, int HD, int BN, bool VEC, bool UNI>
+template <typename T, int HD, int BN, bool VEC, bool UNI, bool SHARED>
 __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kernel(const PagedArgs a) {
   constexpr int NKB = BN / 32;  // 32-key sub-blocks per tile
   typedef PagedStage<T, HD, BN, VEC, UNI> Stage;
@@ -951,9 +951,10 @@ __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kern
   const int hk = blockIdx.x % a.kv_heads, flat = blockIdx.x / a.kv_heads, split = blockIdx.y;
   // the flat-th tile in that order
   int b = -1, tile = 0;
-  for (int b0 = 0, before = 0; b0 < a.batch && b < 0; b0 += 64) {
-    const PagedSeq s = paged_seq(a, min(b0 + lane, a.batch - 1));
-    const int nr = b0 + lane < a.batch ? s.n * a.group : 0;
+  const int seqs = SHARED && a.prefix ? a.groups : a.batch;
+  for (int b0 = 0, before = 0; b0 < seqs && b < 0; b0 += 64) {
+    const PagedSeq s = paged_seq<SHARED>(a, min(b0 + lane, seqs - 1));
+    const int nr = b0 + lane < seqs ? s.n * a.group : 0;
     const int tiles = nr > a.few_rows ? (nr + kPagedTileRows - 1) / kPagedTileRows : 0;
     int mine = tiles, later = 0, at = flat - before;
     int upto = (int)wave_scan(mine);
@@ -986,23 +987,25 @@ __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kern
   }
   if (b < 0) return;
   b = __builtin_amdgcn_readfirstlane(b);
-  const PagedSeq s = paged_seq(a, b);
+  const PagedSeq s = paged_seq<SHARED>(a, b);
   const int nr = s.n * a.group, base = s.len - s.n;
   const int r0 = tile * kPagedTileRows, rw0 = r0 + wave * 32;
-  const int kend = base + a.by_group.div(min(r0 + kPagedTileRows, nr) - 1) + 1;
-  const bool single = s.len <= a.tile_chunk;
-  const int c0 = split * a.tile_chunk, c1 = min(c0 + a.tile_chunk, kend);
+  auto last_seen = [&](int row) { return s.causal ? base + a.by_group.div(row) : s.len - 1; };
+  const int kend = last_seen(min(r0 + kPagedTileRows, nr) - 1) + 1;
+  const bool single = !SHARED && s.len <= a.tile_chunk;
+  const int c0 = split_from<SHARED>(s, split, a.tile_chunk);
+  const int c1 = split_to<SHARED>(c0, split, a.tile_splits, a.tile_chunk, kend);
   if (c0 >= c1 && !(single && split == 0)) return;
 
   const int rr = min(rw0 + li, nr - 1), tok = a.by_group.div(rr), head = hk * a.group + rr - tok * a.group;
-  const int lim = base + tok;  // the last key this lane's row sees
-  const int lim_lo = base + a.by_group.div(min(rw0, nr - 1)), lim_hi = base + a.by_group.div(min(rw0 + 31, nr - 1));
+  const int lim = s.causal ? base + tok : s.len - 1;  // the last key this lane's row sees
+  const int lim_lo = last_seen(min(rw0, nr - 1)), lim_hi = last_seen(min(rw0 + 31, nr - 1));
   const float *qrow = a.q + (size_t)(s.first + tok) * a.ldq + (size_t)head * a.hd;
   PagedRows<T, HD, BN, VEC, UNI> rows;
   rows.init();
   if (c0 < c1) {
     Stage st;
-    st.init(a, b, hk, s.len - 1);
+    st.init(a, s.table, hk, s.len - 1);
     st.lookup_first(a, c0);
     st.load(a, c0);
     st.lookup(a, c0 + BN);
@@ -1043,7 +1046,7 @@ __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kern
       __syncthreads();
     }
     if ((rows.finish() || wide) && rw0 < nr)
-      rows.recompute(a, qrow, a.table + (size_t)b * a.max_blocks, hk, li, hf, c0, min(c1, lim_hi + 1), lim, lim_lo,
+      rows.recompute(a, qrow, a.table + (size_t)s.table * a.max_blocks, hk, li, hf, c0, min(c1, lim_hi + 1), lim, lim_lo,
                      s.len - 1);
   }
   if (rw0 + li >= nr) return;
@@ -1053,7 +1056,9 @@ __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kern
     out = a.o + (size_t)(s.first + tok) * a.ldo + (size_t)head * a.hd;
     f = l == 0.f ? 0.f : 1.0f / l;
   } else {
-    out = a.tile_part + (((size_t)(s.first + tok) * a.heads + head) * a.tile_splits + split) * (a.hd + 2);
+    const size_t at = (size_t)(s.first + tok) * a.heads + head;
+    if constexpr (SHARED) out = a.part + (at * a.part_splits + a.first_split + split) * (a.hd + 2);
+    else out = a.tile_part + (at * a.tile_splits + split) * (a.hd + 2);
     if (hf == 0) {
       out[a.hd] = fmaxf(rows.m_run, kNoKey);
       out[a.hd + 1] = l;
@@ -1353,31 +1358,33 @@ struct SpanRows {
 // the waves' sums are joined.  The next block is loaded into registers while one is
 // multiplied; two workgroups a CU keep 128 KB on the way at head dim 128.  64 x 8192 keys of
 // bf16, 64 heads over 8 of 128: 373 us, 5.8 TB/s.
+// SHARED: rows r0 .. r0 + 15 of nr.
 template <typename T, int HD, bool VEC>
-__global__ void __launch_bounds__(PT_THREADS, sizeof(T) == 2 || HD <= 64 ? 2 : 1) paged_span_kernel(const PagedArgs a) {
+struct SpanShape {
+  static constexpr int ROW = HD + 4;  // floats between rows of the join
+  static constexpr int WAVE_O = 16 * ROW * 4, BLOCK = SpanBlock<T, HD, VEC>::BYTES;
+  static constexpr int WAVE = BLOCK > WAVE_O ? BLOCK : WAVE_O;
+};
+template <typename T, int HD, bool VEC, bool SHARED, int WAVE>
+__device__ __forceinline__ void span_rows(const PagedArgs &a, const PagedSeq &s, int b, int r0, int nr,
+                                          char (&lds)[4][WAVE], float (&red_m)[4][16], float (&red_l)[4][16]) {
   typedef SpanRows<T, HD, VEC> Rows;
   typedef SpanBlock<T, HD, VEC> Block;
-  constexpr int NS = HD / 32, NDB = HD / 16, ROW = HD + 4;  // floats between rows of the join
-  constexpr int WAVE_O = 16 * ROW * 4, WAVE = Block::BYTES > WAVE_O ? Block::BYTES : WAVE_O;
-  __shared__ __attribute__((aligned(16))) char lds[4][WAVE];
-  __shared__ float red_m[4][16], red_l[4][16];
-
-  const int b = blockIdx.z, hk = blockIdx.y, split = blockIdx.x;
-  const PagedSeq s = paged_seq(a, b);
-  const int nr = s.n * a.group;
-  if (nr == 0 || nr > a.few_rows) return;
+  constexpr int NS = HD / 32, NDB = HD / 16, ROW = SpanShape<T, HD, VEC>::ROW;
+  const int hk = SHARED ? blockIdx.y % a.kv_heads : blockIdx.y, split = blockIdx.x;
   const int base = s.len - s.n;
-  const bool single = s.len <= a.few_chunk;
-  const int c0 = split * a.few_chunk, c1 = min(c0 + a.few_chunk, s.len);  // the last row sees all keys
+  const bool single = !SHARED && s.len <= a.few_chunk;
+  const int c0 = split_from<SHARED>(s, split, a.few_chunk);
+  const int c1 = split_to<SHARED>(c0, split, a.few_splits, a.few_chunk, s.len);  // (some row sees all keys)
   if (c0 >= c1 && !(single && split == 0)) return;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = lane & 15, quarter = lane >> 4;
-  const int rr = min(row, nr - 1), tok = a.by_group.div(rr), head = hk * a.group + rr - tok * a.group;
-  const int lim = base + tok, last = s.len - 1;
+  const int rr = min(r0 + row, nr - 1), tok = a.by_group.div(rr), head = hk * a.group + rr - tok * a.group;
+  const int last = s.len - 1, lim = s.causal ? base + tok : last;
   const float *qrow = a.q + (size_t)(s.first + tok) * a.ldq + (size_t)head * a.hd;
-  const int *table = a.table + (size_t)b * a.max_blocks;
+  const int *table = a.table + (size_t)s.table * a.max_blocks;
   const int kv_dim = a.kv_heads * a.hd;
   const T *kc = static_cast<const T *>(a.kc) + (size_t)hk * a.hd, *vc = static_cast<const T *>(a.vc) + (size_t)hk * a.hd;
 
@@ -1419,7 +1426,7 @@ __global__ void __launch_bounds__(PT_THREADS, sizeof(T) == 2 || HD <= 64 ? 2 : 1
 #pragma unroll
   for (int db = 0; db < NDB; ++db) *reinterpret_cast<floatx4 *>(part_o + db * 16 + 4 * quarter) = rows.o[db] * w;
   __syncthreads();
-  for (int t = threadIdx.x; t < nr * HD; t += PT_THREADS) {
+  for (int t = threadIdx.x; t < (SHARED ? min(nr - r0, 16) : nr) * HD; t += PT_THREADS) {
     const int r = t / HD, d = t % HD;
     if (d >= a.hd) continue;
     float x = 0.f, L = 0.f;
@@ -1429,17 +1436,40 @@ __global__ void __launch_bounds__(PT_THREADS, sizeof(T) == 2 || HD <= 64 ? 2 : 1
       x += reinterpret_cast<const float *>(lds[v])[r * ROW + d];
       L += red_l[v][r] * fast_exp2(red_m[v][r] - M);
     }
+    const int i = a.by_group.div(r0 + r), h = hk * a.group + r0 + r - i * a.group;
     if (single) {
-      const int i = a.by_group.div(r), h = hk * a.group + r - i * a.group;
       a.o[(size_t)(s.first + i) * a.ldo + (size_t)h * a.hd + d] = L == 0.f ? 0.f : x / L;
     } else {
-      float *part = a.few_part + ((((size_t)b * a.kv_heads + hk) * a.few_rows + r) * a.few_splits + split) * (a.hd + 2);
+      float *part;
+      if constexpr (SHARED)
+        part = a.part + (((size_t)(s.first + i) * a.heads + h) * a.part_splits + a.first_split + split) * (a.hd + 2);
+      else
+        part = a.few_part + ((((size_t)b * a.kv_heads + hk) * a.few_rows + r) * a.few_splits + split) * (a.hd + 2);
       part[d] = x;
       if (d == 0) {
         part[a.hd] = M;
         part[a.hd + 1] = L;
       }
     }
+  }
+}
+
+template <typename T, int HD, bool VEC, bool SHARED>
+__global__ void __launch_bounds__(PT_THREADS, sizeof(T) == 2 || HD <= 64 ? 2 : 1) paged_span_kernel(const PagedArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[4][SpanShape<T, HD, VEC>::WAVE];
+  __shared__ float red_m[4][16], red_l[4][16];
+  const int b = blockIdx.z;
+  const PagedSeq s = paged_seq<SHARED>(a, b);
+  const int nr = s.n * a.group;
+  if (nr == 0 || nr > a.few_rows) return;
+  if constexpr (SHARED) {
+    // (a group of more rows than the launch was told of takes its time)
+    for (int r0 = blockIdx.y / a.kv_heads * 16; r0 < nr; r0 += gridDim.y / a.kv_heads * 16) {
+      span_rows<T, HD, VEC, true>(a, s, b, r0, nr, lds, red_m, red_l);
+      __syncthreads();
+    }
+  } else {
+    span_rows<T, HD, VEC, false>(a, s, b, 0, nr, lds, red_m, red_l);
   }
 }
 
@@ -1459,22 +1489,37 @@ void launch_rows(const PagedArgs &a, bool wide, hipStream_t st) {
   else launch_rows<T, HD, kVectorCut>(a, st);
 }
 
-template <typename T, int HD, int BN>
+template <typename T, int HD, int BN, bool SHARED = false>
 void launch_tile(const PagedArgs &a, bool wide, hipStream_t st) {
-  const long long tiles = (long long)a.rows * a.group / kPagedTileRows + a.batch;
+  const long long tiles = (long long)a.rows * a.group / kPagedTileRows + (SHARED && a.prefix ? a.groups : a.batch);
   const dim3 grid((unsigned)(tiles * a.kv_heads), a.tile_splits);
   // offsets inside 16 rows of a page fit 32 bits
   const bool uni = a.page_shift >= 4 && (long long)a.kv_heads * a.hd < (1 << 24);
-  if (wide && uni) paged_tile_kernel<T, HD, BN, true, true><<<grid, PT_THREADS, 0, st>>>(a);
-  else if (wide) paged_tile_kernel<T, HD, BN, true, false><<<grid, PT_THREADS, 0, st>>>(a);
-  else paged_tile_kernel<T, HD, BN, false, false><<<grid, PT_THREADS, 0, st>>>(a);
+  if (wide && uni) paged_tile_kernel<T, HD, BN, true, true, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  else if (wide) paged_tile_kernel<T, HD, BN, true, false, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  else paged_tile_kernel<T, HD, BN, false, false, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool SHARED = false>
 void launch_span(const PagedArgs &a, bool wide, hipStream_t st) {
-  const dim3 grid(a.few_splits, a.kv_heads, a.batch);
-  if (wide) paged_span_kernel<T, HD, true><<<grid, PT_THREADS, 0, st>>>(a);
-  else paged_span_kernel<T, HD, false><<<grid, PT_THREADS, 0, st>>>(a);
+  const dim3 grid(a.few_splits, a.kv_heads, SHARED && a.prefix ? a.groups : a.batch);
+  if (wide) paged_span_kernel<T, HD, true, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  else paged_span_kernel<T, HD, false, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+}
+
+template <typename T, bool SHARED>
+int launch_tiles(const PagedArgs &a, bool wide, hipStream_t st) {
+  if (a.hd <= 32) launch_tile<T, 32, 32, SHARED>(a, wide, st);
+  else if (a.hd <= 64) launch_tile<T, 64, 32, SHARED>(a, wide, st);
+  else launch_tile<T, 128, 32, SHARED>(a, wide, st);
+  return check_launch("paged_tile_kernel");
+}
+template <typename T, bool SHARED>
+int launch_spans(const PagedArgs &a, bool wide, hipStream_t st) {
+  if (a.hd <= 32) launch_span<T, 32, SHARED>(a, wide, st);
+  else if (a.hd <= 64) launch_span<T, 64, SHARED>(a, wide, st);
+  else launch_span<T, 128, SHARED>(a, wide, st);
+  return check_launch("paged_span_kernel");
 }
 
 // wide: head dims that are multiples of 8, and 16-byte aligned rows.
@@ -1489,19 +1534,20 @@ int paged_attn(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t
     if (rc) return rc;
   }
   if (k.span) {
-    if (a.hd <= 32) launch_span<T, 32>(a, wide, st);
-    else if (a.hd <= 64) launch_span<T, 64>(a, wide, st);
-    else launch_span<T, 128>(a, wide, st);
-    const int rc = check_launch("paged_span_kernel");
+    const int rc = launch_spans<T, false>(a, wide, st);
     if (rc) return rc;
   }
-  if (k.tile) {
-    if (a.hd <= 32) launch_tile<T, 32, 32>(a, wide, st);
-    else if (a.hd <= 64) launch_tile<T, 64, 32>(a, wide, st);
-    else launch_tile<T, 128, 32>(a, wide, st);
-    return check_launch("paged_tile_kernel");
+  return k.tile ? launch_tiles<T, false>(a, wide, st) : CDML_OK;
+}
+
+// The same over what groups share, or over the tokens behind it (head dims up to 128).
+template <typename T>
+int paged_shared(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st) {
+  if (k.span) {
+    const int rc = launch_spans<T, true>(a, wide, st);
+    if (rc) return rc;
   }
-  return CDML_OK;
+  return k.tile ? launch_tiles<T, true>(a, wide, st) : CDML_OK;
 }
 
 }  // namespace

@@ -4,7 +4,7 @@
 namespace cdml {
 
 int paged_attn_f8(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st) {
-  return paged_attn_q8<F8>(a, k, wide, st);
+  return paged_attn_q8<F8, false>(a, k, wide, st);
 }
 
 }  // namespace cdml

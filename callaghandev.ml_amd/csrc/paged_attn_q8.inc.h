@@ -362,30 +362,24 @@ struct CodeRows {
 // One workgroup: up to 16 rows of a (request, K/V head) against one chunk of its keys.  The
 // four waves take blocks of 32 keys in turn and join their sums at the end; a wave's next
 // block is on the way while one is multiplied.
-template <typename T, int HD, int RUN, bool VEC>
-__global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kernel(const PagedArgs a) {
+template <typename T, int HD, int RUN, bool VEC, bool SHARED>
+__device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s, int b, int r0, int nr,
+                                          float (&lds)[4][16 * (HD + 4)], float (&red_m)[4][16], float (&red_l)[4][16]) {
   typedef CodeRows<T, HD> Rows;
   typedef CodeBlock<T, HD> Block;
   constexpr int NS = HD / 32, NDB = HD / 16, ROW = HD + 4;  // floats between rows of the join
-  __shared__ __attribute__((aligned(16))) float lds[4][16 * ROW];
-  __shared__ float red_m[4][16], red_l[4][16];
-
-  const int b = blockIdx.z, split = blockIdx.x;
-  const int hk = blockIdx.y % a.kv_heads, r0 = blockIdx.y / a.kv_heads * 16;
-  const PagedSeq s = paged_seq(a, b);
-  const int nr = s.n * a.group;
-  if (nr > a.few_rows || r0 >= nr) return;
-  const int base = s.len - s.n;
-  const int kend = base + a.by_group.div(min(r0 + 16, nr) - 1) + 1;  // past the last visible key
-  const bool single = s.len <= a.few_chunk;
-  const int c0 = split * a.few_chunk, c1 = min(c0 + a.few_chunk, kend);
+  const int hk = blockIdx.y % a.kv_heads, split = blockIdx.x, base = s.len - s.n;
+  const int kend = s.causal ? base + a.by_group.div(min(r0 + 16, nr) - 1) + 1 : s.len;  // past the last visible key
+  const bool single = !SHARED && s.len <= a.few_chunk;
+  const int c0 = split_from<SHARED>(s, split, a.few_chunk);
+  const int c1 = split_to<SHARED>(c0, split, a.few_splits, a.few_chunk, kend);
   if (c0 >= c1 && !(single && split == 0)) return;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = lane & 15, quarter = lane >> 4;
   const int rr = min(r0 + row, nr - 1), tok = a.by_group.div(rr), head = hk * a.group + rr - tok * a.group;
-  const int lim = base + tok, last = s.len - 1;
+  const int last = s.len - 1, lim = s.causal ? base + tok : last;
   const float *qrow = a.q + (size_t)(s.first + tok) * a.ldq + (size_t)head * a.hd;
 
   Rows rows;
@@ -393,7 +387,7 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kern
   const int first = c0 + wave * 32;
   if (first < c1) {
     CodeLoader<T, HD, RUN> from;
-    from.init(a, b, hk, first, last);
+    from.init(a, s.table, hk, first, last);
     from.lookup_first(a);
     Block x, y;
     from.load(a, x, first);
@@ -411,7 +405,7 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kern
       rows.add(y, q, lim - k0 - 128 - 4 * quarter);
     }
     if (rows.finish() || wide)
-      rows.recompute(a, qrow, a.table + (size_t)b * a.max_blocks, hk, quarter, first, c1, lim, last);
+      rows.recompute(a, qrow, a.table + (size_t)s.table * a.max_blocks, hk, quarter, first, c1, lim, last);
   }
   // the waves' sums: rows' statistics, then each wave's O scaled to the common maximum
   const float m = fmaxf(rows.m, kNoKey), l = quarters(rows.l, [](float x, float y) { return x + y; });
@@ -436,12 +430,15 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kern
       x += lds[v][r * ROW + d];
       L += red_l[v][r] * fast_exp2(red_m[v][r] - M);
     }
+    const int i = a.by_group.div(r0 + r), h = hk * a.group + r0 + r - i * a.group;
     if (single) {
-      const int i = a.by_group.div(r0 + r), h = hk * a.group + r0 + r - i * a.group;
       a.o[(size_t)(s.first + i) * a.ldo + (size_t)h * a.hd + d] = L == 0.f ? 0.f : x / L;
     } else {
-      float *part =
-          a.few_part + ((((size_t)b * a.kv_heads + hk) * a.few_rows + r0 + r) * a.few_splits + split) * (a.hd + 2);
+      float *part;
+      if constexpr (SHARED)
+        part = a.part + (((size_t)(s.first + i) * a.heads + h) * a.part_splits + a.first_split + split) * (a.hd + 2);
+      else
+        part = a.few_part + ((((size_t)b * a.kv_heads + hk) * a.few_rows + r0 + r) * a.few_splits + split) * (a.hd + 2);
       part[d] = x;
       if (d == 0) {
         part[a.hd] = M;
@@ -451,38 +448,53 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kern
   }
 }
 
-template <typename T, int HD, bool VEC>
-void launch_code(const PagedArgs &a, hipStream_t st) {
-  const dim3 grid(a.few_splits, a.kv_heads * ((a.few_rows + 15) / 16), a.batch);
-  if (a.page_shift >= 4) paged_code_kernel<T, HD, 16, VEC><<<grid, PT_THREADS, 0, st>>>(a);
-  else if (a.page_shift >= 2) paged_code_kernel<T, HD, 4, VEC><<<grid, PT_THREADS, 0, st>>>(a);
-  else paged_code_kernel<T, HD, 1, VEC><<<grid, PT_THREADS, 0, st>>>(a);
+template <typename T, int HD, int RUN, bool VEC, bool SHARED>
+__global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kernel(const PagedArgs a) {
+  __shared__ __attribute__((aligned(16))) float lds[4][16 * (HD + 4)];
+  __shared__ float red_m[4][16], red_l[4][16];
+  const int b = blockIdx.z;
+  const PagedSeq s = paged_seq<SHARED>(a, b);
+  const int nr = s.n * a.group;
+  int r0 = blockIdx.y / a.kv_heads * 16;
+  if (nr > a.few_rows || r0 >= nr) return;
+  if constexpr (SHARED) {
+    // (a group of more rows than the launch was told of takes its time)
+    for (; r0 < nr; r0 += gridDim.y / a.kv_heads * 16) {
+      code_rows<T, HD, RUN, VEC, true>(a, s, b, r0, nr, lds, red_m, red_l);
+      __syncthreads();
+    }
+  } else {
+    code_rows<T, HD, RUN, VEC, false>(a, s, b, r0, nr, lds, red_m, red_l);
+  }
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool VEC, bool SHARED>
+void launch_code(const PagedArgs &a, hipStream_t st) {
+  const int row_groups = SHARED && a.prefix ? 1 : (a.few_rows + 15) / 16;
+  const dim3 grid(a.few_splits, a.kv_heads * row_groups, SHARED && a.prefix ? a.groups : a.batch);
+  if (a.page_shift >= 4) paged_code_kernel<T, HD, 16, VEC, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  else if (a.page_shift >= 2) paged_code_kernel<T, HD, 4, VEC, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  else paged_code_kernel<T, HD, 1, VEC, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+}
+
+template <typename T, int HD, bool SHARED>
 void launch_code(const PagedArgs &a, bool wide, hipStream_t st) {
-  if (wide) launch_code<T, HD, true>(a, st);
-  else launch_code<T, HD, false>(a, st);
+  if (wide) launch_code<T, HD, true, SHARED>(a, st);
+  else launch_code<T, HD, false, SHARED>(a, st);
 }
 
 // wide: head dims that are multiples of 8, and 16-byte aligned rows of Q and O.
-template <typename T>
+template <typename T, bool SHARED>
 int paged_attn_q8(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st) {
   if (k.span) {
-    if (a.hd <= 32) launch_code<T, 32>(a, wide, st);
-    else if (a.hd <= 64) launch_code<T, 64>(a, wide, st);
-    else if (a.hd <= 128) launch_code<T, 128>(a, wide, st);
-    else launch_code<T, 256>(a, wide, st);
+    if (a.hd <= 32) launch_code<T, 32, SHARED>(a, wide, st);
+    else if (a.hd <= 64) launch_code<T, 64, SHARED>(a, wide, st);
+    else if (SHARED || a.hd <= 128) launch_code<T, 128, SHARED>(a, wide, st);
+    else if constexpr (!SHARED) launch_code<T, 256, SHARED>(a, wide, st);
     const int rc = check_launch("paged_code_kernel");
     if (rc) return rc;
   }
-  if (k.tile) {
-    if (a.hd <= 32) launch_tile<T, 32, 32>(a, wide, st);
-    else if (a.hd <= 64) launch_tile<T, 64, 32>(a, wide, st);
-    else launch_tile<T, 128, 32>(a, wide, st);
-    return check_launch("paged_tile_kernel");
-  }
-  return CDML_OK;
+  return k.tile ? launch_tiles<T, SHARED>(a, wide, st) : CDML_OK;
 }
 
 }  // namespace

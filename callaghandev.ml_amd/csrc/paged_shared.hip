@@ -1,0 +1,314 @@
+// Attention for requests that share their first pages (include/cdml.h): what a group shares is
+// found in its tables, read once for all its rows, and joined with each request's own tokens.
+#include <algorithm>
+
+#include "paged_plan.h"
+
+namespace cdml {
+namespace {
+
+constexpr int kFindThreads = 1024;
+
+struct FindArgs {
+  const int *table;
+  int max_blocks;
+  const int *kv_len, *cu, *group_start;
+  int groups, batch, n_pages, page_shift;
+  int *shared;
+};
+
+__device__ __forceinline__ int clamped(int x, int most) { return min(max(x, 0), most); }
+
+// One workgroup a group: the least number of full old pages of a member, then the first
+// column, of every member's row at once, in which a page differs from the first member's.  The
+// last workgroup clears the requests of no group.
+__global__ void __launch_bounds__(kFindThreads) paged_shared_kernel(const FindArgs a) {
+  __shared__ int least;
+  const int g = blockIdx.x, t = threadIdx.x;
+  if (g == a.groups) {
+    const int from = a.groups ? clamped(a.group_start[0], a.batch) : a.batch;
+    const int behind = a.groups ? clamped(a.group_start[a.groups], a.batch) : a.batch;
+    for (int b = t; b < a.batch; b += kFindThreads)
+      if (b < from || b >= behind) a.shared[b] = 0;
+    return;
+  }
+  const int first = clamped(a.group_start[g], a.batch);
+  const int members = min(max(a.group_start[g + 1], first), a.batch) - first;
+  if (members < 2) {
+    if (members == 1 && t == 0) a.shared[first] = 0;
+    return;
+  }
+  if (t == 0) least = a.max_blocks;
+  __syncthreads();
+  int pages = a.max_blocks;
+  for (int b = first + t; b < first + members; b += kFindThreads) {
+    const long long old = (long long)a.kv_len[b] - max(a.cu[b + 1] - a.cu[b], 0);
+    pages = min(pages, (int)(max(old, 0LL) >> a.page_shift));
+  }
+  pages = wave_min(pages);
+  if ((t & 63) == 0) atomicMin(&least, pages);
+  __syncthreads();
+  pages = least;
+  const int *lead = a.table + (size_t)first * a.max_blocks;
+  int differs = pages;
+  constexpr int U = 8;  // loads of a thread in flight
+  const long long total = (long long)members * pages;
+  // (entry i: column i % pages of member i / pages; the first member's own pages are checked, too)
+  int m = pages ? t / pages : 0, c = pages ? t - m * pages : 0;
+  const int dm = pages ? kFindThreads / pages : 0, dc = pages ? kFindThreads - dm * pages : 0;
+  for (long long i = t; i < total;) {
+    int x[U], y[U], col[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = i + (long long)u * kFindThreads < total;
+      col[u] = in ? c : 0;
+      x[u] = lead[col[u]];
+      y[u] = in ? lead[(size_t)m * a.max_blocks + c] : x[u];
+      m += dm;
+      c += dc;
+      if (c >= pages) {
+        c -= pages;
+        ++m;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (x[u] != y[u] || (unsigned)x[u] >= (unsigned)a.n_pages) differs = min(differs, col[u]);
+    i += (long long)U * kFindThreads;
+  }
+  differs = wave_min(differs);
+  if ((t & 63) == 0) atomicMin(&least, differs);
+  __syncthreads();
+  const int tokens = least << a.page_shift;  // (at most a table's tokens)
+  for (int b = first + t; b < first + members; b += kFindThreads) a.shared[b] = tokens;
+}
+
+// How a row's chunks lie in its parts, and where its request's own tokens are cut.
+struct JoinArgs {
+  int prefix_chunk, prefix_splits;  // (of `part_splits`, the first)
+  int few_rows, few_chunk, few_splits, tile_chunk, tile_splits;
+};
+
+// A wave per (row, head).
+__global__ void __launch_bounds__(256) paged_shared_join_kernel(const PagedArgs a, const JoinArgs j) {
+  const int row = blockIdx.x, h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (h >= a.heads) return;
+  const int b = request_of_row(a, row);
+  if (b >= a.batch) return;
+  const PagedSeq s = paged_seq<true>(a, b);
+  const int i = row - s.first;
+  if (i < 0 || i >= s.n) return;
+  const bool few = s.n * a.group <= j.few_rows;
+  const int before = min(chunks_seen(s.start, j.prefix_chunk), j.prefix_splits);
+  const int behind = min(chunks_seen(s.len - s.n + i + 1 - s.start, few ? j.few_chunk : j.tile_chunk),
+                         few ? j.few_splits : j.tile_splits);
+  const float *part = a.part + ((size_t)row * a.heads + h) * a.part_splits * (a.hd + 2);
+  join_two(a, part, before, part + (size_t)j.prefix_splits * (a.hd + 2), behind,
+           a.o + (size_t)row * a.ldo + (size_t)h * a.hd);
+}
+
+struct SharedPlan {
+  bool plain;          // every request reads its own pages
+  bool prefix_tile;
+  int prefix_chunk, prefix_splits;
+  Plan own;
+  int own_splits;
+  size_t floats;
+};
+
+SharedPlan plan_shared(int size, int rows, int batch, int groups, int max_members, int max_new, int max_prefix,
+                       int max_tail, int heads, int kv_heads, int hd) {
+  SharedPlan p{};
+  p.plain = hd > 128 || groups == 0 || max_members < 2 || max_prefix == 0;
+  if (p.plain) {
+    p.own = make_plan(size, rows, batch, max_new, max_prefix + max_tail, heads, kv_heads, hd);
+    p.floats = p.own.few_floats + p.own.tile_floats;
+    return p;
+  }
+  const int group = heads / kv_heads;
+  const long long most = std::min((long long)max_members * max_new, (long long)rows) * group;
+  p.prefix_tile = most > kSpanRows;
+  const long long work = (p.prefix_tile ? (long long)rows * group / kPagedTileRows + groups : groups) * kv_heads;
+  long long splits = (2 * kComputeUnits + work - 1) / work;
+  if (!p.prefix_tile && work >= kComputeUnits) splits = 1;
+  splits = std::min<long long>(splits, (max_prefix + 255) / 256);
+  p.prefix_chunk = round_up((int)((max_prefix + splits - 1) / splits), 128);
+  p.prefix_splits = (max_prefix - 1) / p.prefix_chunk + 1;
+  p.own = make_plan(size, rows, batch, max_new, max_tail, heads, kv_heads, hd, true);
+  p.own_splits = std::max(p.own.kernels.span ? p.own.few_splits : 1, p.own.kernels.tile ? p.own.tile_splits : 1);
+  p.floats = (size_t)rows * heads * (p.prefix_splits + p.own_splits) * (hd + 2);
+  return p;
+}
+
+int check_shared(const char *what, int rows, int batch, int groups, int max_members, int max_new, int max_prefix,
+                 int max_tail, int heads, int kv_heads, int hd) {
+  if (groups < 0 || groups > batch || max_members < 0 || max_prefix < 0 || max_tail < 0 ||
+      (long long)max_prefix + max_tail > INT_MAX / 2)
+    return fail(CDML_E_INVALID, "%s: bad size (batch %d, groups %d, max_members %d, max_prefix %d, max_tail %d)", what,
+                batch, groups, max_members, max_prefix, max_tail);
+  const int rc = check_sizes(what, rows, batch, max_new, max_prefix + max_tail, heads, kv_heads, hd);
+  if (rc) return rc;
+  // (a group's rows run in tiles where a request's do not)
+  if (((long long)rows * (heads / kv_heads) / kPagedTileRows + batch) * kv_heads >= 1 << 24 ||
+      (long long)rows * (heads / kv_heads) > INT_MAX / 2)
+    return fail(CDML_E_INVALID, "%s: problem too large", what);
+  return CDML_OK;
+}
+
+}  // namespace
+}  // namespace cdml
+
+using namespace cdml;
+
+extern "C" int cdml_paged_shared(const int *block_table, int max_blocks, const int *kv_len, const int *cu_new,
+                                 const int *group_start, int groups, int batch, int n_pages, int page_size, int *shared,
+                                 cdml_stream stream) {
+  FindArgs a{};
+  int rc = check_pool("cdml_paged_shared", n_pages, page_size, max_blocks, batch, &a.page_shift);
+  if (rc) return rc;
+  if (groups < 0 || groups > batch)
+    return fail(CDML_E_INVALID, "cdml_paged_shared: %d groups of %d requests", groups, batch);
+  if (batch == 0) return CDML_OK;
+  if (!block_table || !kv_len || !cu_new || !group_start || !shared)
+    return fail(CDML_E_INVALID, "cdml_paged_shared: NULL pointer");
+  rc = ensure_device();
+  if (rc) return rc;
+  a.table = block_table;
+  a.max_blocks = max_blocks;
+  a.kv_len = kv_len;
+  a.cu = cu_new;
+  a.group_start = group_start;
+  a.groups = groups;
+  a.batch = batch;
+  a.n_pages = n_pages;
+  a.shared = shared;
+  paged_shared_kernel<<<groups + 1, kFindThreads, 0, as_hip(stream)>>>(a);
+  return check_launch("paged_shared_kernel");
+}
+
+extern "C" int cdml_paged_attn_shared_workspace_size(int rows, int batch, int groups, int max_members, int max_new,
+                                                     int max_prefix, int max_tail, int num_heads, int num_kv_heads,
+                                                     int head_dim, size_t *bytes) {
+  const char *what = "cdml_paged_attn_shared_workspace_size";
+  if (!bytes) return fail(CDML_E_INVALID, "%s: bytes is NULL", what);
+  const int rc = check_shared(what, rows, batch, groups, max_members, max_new, max_prefix, max_tail, num_heads,
+                              num_kv_heads, head_dim);
+  if (rc) return rc;
+  size_t most = 0;
+  for (int size = 1; size <= 4; size *= 2)  // of any size of cached values
+    most = std::max(most, plan_shared(size, rows, batch, groups, max_members, max_new, max_prefix, max_tail, num_heads,
+                                      num_kv_heads, head_dim)
+                              .floats);
+  *bytes = sizeof(float) * most;
+  return CDML_OK;
+}
+
+extern "C" int cdml_paged_attn_shared(const float *q, int ldq, const void *kcache, const void *vcache,
+                                      const float *kscale, const float *vscale, int cache_type, int n_pages,
+                                      int page_size, const int *block_table, int max_blocks, const int *kv_len,
+                                      const int *cu_new, const int *group_start, const int *shared, float *o, int ldo,
+                                      int rows, int batch, int groups, int max_members, int max_new, int max_prefix,
+                                      int max_tail, int num_heads, int num_kv_heads, int head_dim, float scale, int *bad,
+                                      void *workspace, size_t workspace_bytes, cdml_stream stream) {
+  const char *what = "cdml_paged_attn_shared";
+  PagedArgs a{};
+  int rc = check_pool(what, n_pages, page_size, max_blocks, batch, &a.page_shift);
+  if (rc) return rc;
+  rc = check_shared(what, rows, batch, groups, max_members, max_new, max_prefix, max_tail, num_heads, num_kv_heads,
+                    head_dim);
+  if (rc) return rc;
+  const bool q8 = q8_cache_type(cache_type);
+  const int size = q8 ? 1 : cache_type_bytes(cache_type), max_len = max_prefix + max_tail;
+  if (!size) return fail(CDML_E_INVALID, "%s: unknown cache type %d", what, cache_type);
+  const long long table = (long long)max_blocks * page_size;
+  if (max_prefix > table || max_tail > table)
+    return fail(CDML_E_INVALID, "%s: max_prefix %d or max_tail %d above the table's %lld tokens", what, max_prefix,
+                max_tail, table);
+  const long long dim = (long long)num_heads * head_dim;
+  if (ldq < dim || ldo < dim) return fail(CDML_E_INVALID, "%s: row stride smaller than the heads", what);
+  if (rows == 0 || batch == 0 || max_new == 0) return CDML_OK;
+  if (!q || !kcache || !vcache || !block_table || !kv_len || !cu_new || !group_start || !shared || !o)
+    return fail(CDML_E_INVALID, "%s: NULL pointer", what);
+  if (q8) {
+    rc = check_q8(what, kcache, vcache, kscale, vscale);
+    if (rc) return rc;
+  }
+  size_t need = 0;
+  rc = cdml_paged_attn_shared_workspace_size(rows, batch, groups, max_members, max_new, max_prefix, max_tail, num_heads,
+                                             num_kv_heads, head_dim, &need);
+  if (rc) return rc;
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(CDML_E_INVALID, "%s: %zu bytes of 16-byte aligned workspace needed, %zu given", what, need,
+                workspace_bytes);
+  const SharedPlan p = plan_shared(size, rows, batch, groups, max_members, max_new, max_prefix, max_tail, num_heads,
+                                   num_kv_heads, head_dim);
+  if (p.plain)
+    return paged_attention(what, q8, true, q, ldq, kcache, vcache, kscale, vscale, cache_type, n_pages, page_size,
+                           block_table, max_blocks, kv_len, cu_new, o, ldo, rows, batch, max_new, max_len, num_heads,
+                           num_kv_heads, head_dim, scale, bad, workspace, workspace_bytes, stream);
+  rc = ensure_device();
+  if (rc) return rc;
+  a.q = q;
+  a.kc = kcache;
+  a.vc = vcache;
+  a.ks = kscale;
+  a.vs = vscale;
+  a.width = q8_width(head_dim);
+  a.table = block_table;
+  a.kv_len = kv_len;
+  a.cu_new = cu_new;
+  a.o = o;
+  a.bad = bad;
+  a.ldq = ldq;
+  a.ldo = ldo;
+  a.n_pages = n_pages;
+  a.max_blocks = max_blocks;
+  a.rows = rows;
+  a.batch = batch;
+  a.max_new = max_new;
+  a.max_len = (int)std::min<long long>(max_len, table);
+  a.heads = num_heads;
+  a.kv_heads = num_kv_heads;
+  a.group = num_heads / num_kv_heads;
+  a.hd = head_dim;
+  a.scale_log2 = scale * kLog2e;
+  a.by_group = UDiv::make((uint32_t)a.group);
+  a.group_start = group_start;
+  a.shared = shared;
+  a.groups = groups;
+  a.part = static_cast<float *>(workspace);
+  a.part_splits = p.prefix_splits + p.own_splits;
+  const bool wide = head_dim % 8 == 0 && ldq % 4 == 0 && ldo % 4 == 0 && aligned16(q) && aligned16(o) &&
+                    aligned16(kcache) && aligned16(vcache);
+  const hipStream_t st = as_hip(stream);
+  auto run = [&](const PagedKernels &k) {
+    switch (cache_type) {
+      case CDML_CACHE_F32: return paged_shared_f32(a, k, wide, st);
+      case CDML_CACHE_F16: return paged_shared_f16(a, k, wide, st);
+      case CDML_CACHE_BF16: return paged_shared_bf16(a, k, wide, st);
+      case CDML_CACHE_I8: return paged_shared_i8(a, k, wide, st);
+      default: return paged_shared_f8(a, k, wide, st);
+    }
+  };
+  // what the groups share, all of a group's rows in the same kernel
+  a.prefix = true;
+  a.few_rows = p.prefix_tile ? 0 : INT_MAX;
+  a.few_chunk = a.tile_chunk = p.prefix_chunk;
+  a.few_splits = a.tile_splits = p.prefix_splits;
+  rc = run({false, !p.prefix_tile, p.prefix_tile});
+  if (rc) return rc;
+  // the tokens behind
+  a.prefix = false;
+  a.few_rows = p.own.few_rows;
+  a.few_chunk = p.own.few_chunk;
+  a.few_splits = p.own.few_splits;
+  a.tile_chunk = p.own.tile_chunk;
+  a.tile_splits = p.own.tile_splits;
+  a.first_split = p.prefix_splits;
+  rc = run(p.own.kernels);
+  if (rc) return rc;
+  const JoinArgs j{p.prefix_chunk,  p.prefix_splits, p.own.few_rows,   p.own.few_chunk,
+                   p.own.few_splits, p.own.tile_chunk, p.own.tile_splits};
+  paged_shared_join_kernel<<<dim3((unsigned)rows, (unsigned)(num_heads + 3) / 4), 256, 0, st>>>(a, j);
+  return check_launch("paged_shared_join_kernel");
+}

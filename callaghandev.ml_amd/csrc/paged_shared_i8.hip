@@ -1,0 +1,10 @@
+// Attention over shared prefixes in a paged cache of i8 codes (paged_attn_q8.inc.h).
+#include "paged_attn_q8.inc.h"
+
+namespace cdml {
+
+int paged_shared_i8(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st) {
+  return paged_attn_q8<I8, true>(a, k, wide, st);
+}
+
+}  // namespace cdml

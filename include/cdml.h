@@ -731,6 +731,48 @@ int cdml_paged_attn_q8(const float *q, int ldq, const void *kcache,
                        float scale, int *bad, void *workspace,
                        size_t workspace_bytes, cdml_stream stream);
 
+/* What requests share, found in their tables: group g is the requests
+ * group_start[g] .. group_start[g + 1] - 1 (device int32[groups + 1], which must
+ * not decrease, groups <= batch).  shared[b] (device int32[batch]) receives the
+ * number of first tokens that all members of b's group have in the same pages: whole
+ * pages, no page outside [0, n_pages), and none of the step's new tokens (rows
+ * cu_new[b] .. cu_new[b + 1]) among them.  0 for a group of one, and for requests of
+ * no group. */
+int cdml_paged_shared(const int *block_table, int max_blocks,
+                      const int *kv_len, const int *cu_new,
+                      const int *group_start, int groups, int batch,
+                      int n_pages, int page_size, int *shared,
+                      cdml_stream stream);
+
+/* cdml_paged_attn (of cdml_paged_attn_q8 for 8-bit caches; kscale and vscale are
+ * NULL for others) for groups of requests that share their first tokens, such as
+ * beams and requests behind one prompt: the shared tokens' K and V are read once for
+ * all rows of a group, in which they are one matrix operand, and joined with each
+ * request's own.  shared is what cdml_paged_shared wrote for the same tables, lengths
+ * and groups.  max_members, max_prefix and max_tail bound the members of a group,
+ * shared, and kv_len - shared (either <= max_blocks * page_size); the launches are
+ * sized by them.  Tokens past max_prefix + max_tail are cut off, other excess only
+ * costs time.  Head dims above 128 run as in cdml_paged_attn, each request over its
+ * own table.  Otherwise everything is as there, the workspace
+ * cdml_paged_attn_shared_workspace_size bytes. */
+int cdml_paged_attn_shared_workspace_size(int rows, int batch, int groups,
+                                          int max_members, int max_new,
+                                          int max_prefix, int max_tail,
+                                          int num_heads, int num_kv_heads,
+                                          int head_dim, size_t *bytes);
+int cdml_paged_attn_shared(const float *q, int ldq, const void *kcache,
+                           const void *vcache, const float *kscale,
+                           const float *vscale, int cache_type, int n_pages,
+                           int page_size, const int *block_table,
+                           int max_blocks, const int *kv_len,
+                           const int *cu_new, const int *group_start,
+                           const int *shared, float *o, int ldo, int rows,
+                           int batch, int groups, int max_members, int max_new,
+                           int max_prefix, int max_tail, int num_heads,
+                           int num_kv_heads, int head_dim, float scale,
+                           int *bad, void *workspace, size_t workspace_bytes,
+                           cdml_stream stream);
+
 /* Gives every row b of the tables the state of row parents[b] (device
  * int32[batch]; -1, and any value outside [0, batch), leaves it empty, which
  * also releases a request): full pages become shared, a page that is not full

@@ -155,3 +155,56 @@ def mark(used, table, lens, P):
     for b, m in enumerate(lens):
         at = np.arange(m)
         used[table[b, at // P], at % P] = True
+
+
+# ---- shared prefixes ---------------------------------------------------------------
+
+def shared(table, kv, cu, groups, P, n_pages):
+    """Tokens that every request shares with its group (groups: group_start)."""
+    B, blocks = table.shape
+    out = np.zeros(B, np.int32)
+    for first, behind in zip(groups[:-1], groups[1:]):
+        if behind - first < 2:
+            continue
+        pages = min([blocks] + [max(0, int(kv[b]) - int(cu[b + 1] - cu[b])) // P for b in range(first, behind)])
+        n = 0
+        while n < pages and 0 <= table[first, n] < n_pages and (table[first:behind, n] == table[first, n]).all():
+            n += 1
+        out[first:behind] = n * P
+    return out
+
+
+def call_shared(table, kv, cu, groups, P, n_pages, fill=-9):
+    d = [ints(a) for a in (table, kv, cu, groups, np.full(max(len(kv), 1), fill))]
+    N.check(N.lib().cdml_paged_shared(d[0].ptr, table.shape[1], d[1].ptr, d[2].ptr, d[3].ptr, len(groups) - 1, len(kv),
+                                      n_pages, P, d[4].ptr, stream().handle))
+    return down(d[4], (len(kv),), np.int32)
+
+
+def call_attention_shared(q, c, table, kv, cu, groups, H, scale, o, bounds=None, ldq=None, ldo=None, n_pages=None):
+    """cdml_paged_shared and cdml_paged_attn_shared; bounds: max_members, max_new, max_prefix, max_tail.
+    Returns (o, shared, bad)."""
+    rows, B, hd, P = len(q), len(kv), c["hd"], c["P"]
+    n_pages = n_pages or len(c["k"])
+    ldq, ldo = ldq or q.shape[1], ldo or o.shape[1]
+    wide = np.full((rows, ldq), np.nan, np.float32)
+    wide[:, :q.shape[1]] = q
+    out = np.full((rows, ldo), 7.0, np.float32)
+    out[:, :o.shape[1]] = o
+    if bounds is None:
+        s = shared(table, kv, cu, groups, P, n_pages)
+        bounds = (int(np.max(np.diff(groups), initial=0)), int(np.max(np.diff(cu), initial=0)), int(np.max(s, initial=0)),
+                  int(np.max(kv - s, initial=0)))
+    dq, do, d = up(wide), up(out), upload(c)
+    dt, dl, dc, dg, ds, bad = (ints(a) for a in (table, kv, cu, groups, np.full(max(B, 1), -9), np.zeros(1)))
+    size = (rows, B, len(groups) - 1, *bounds, H, c["heads"], hd)
+    w, n = ws("cdml_paged_attn_shared_workspace_size", *size)
+    w.upload(np.full(max(n // 4, 1), np.nan, np.float32), stream())
+    N.check(N.lib().cdml_paged_shared(dt.ptr, table.shape[1], dl.ptr, dc.ptr, dg.ptr, len(groups) - 1, B, n_pages, P,
+                                      ds.ptr, stream().handle))
+    N.check(N.lib().cdml_paged_attn_shared(dq.ptr, ldq, *(ptr(b) for b in d), N.CACHE[c["kind"]], n_pages, P, dt.ptr,
+                                           table.shape[1], dl.ptr, dc.ptr, dg.ptr, ds.ptr, do.ptr, ldo, *size, scale,
+                                           bad.ptr, w.ptr, n, stream().handle))
+    out = down(do, out.shape)
+    assert (out[:, o.shape[1]:] == 7.0).all()
+    return out[:, :o.shape[1]], down(ds, (B,), np.int32), int(down(bad, (1,), np.int32)[0])
