@@ -81,6 +81,7 @@ struct PagedArgs {
   int heads, kv_heads, group, hd;
   float scale_log2;
   int few_rows, few_chunk, few_splits, tile_chunk, tile_splits;
+  int most_rows;     // of a request of few rows, at most (a hint)
   float *few_part;   // [batch][kv_heads][few_rows][few_splits][hd + 2]
   float *tile_part;  // [rows][heads][tile_splits][hd + 2]
   UDiv by_group;

@@ -114,7 +114,7 @@ int paged_attention(const char *what, bool q8, bool cut, const float *q, int ldq
   a.hd = head_dim;
   a.scale_log2 = scale * kLog2e;
   a.by_group = UDiv::make((uint32_t)a.group);
-  a.few_rows = p.few_rows;
+  a.few_rows = a.most_rows = p.few_rows;
   a.few_chunk = p.few_chunk;
   a.few_splits = p.few_splits;
   a.tile_chunk = p.tile_chunk;

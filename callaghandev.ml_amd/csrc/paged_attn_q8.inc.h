@@ -14,18 +14,22 @@ namespace {
 //   V: lane (row, quarter) has dims VD * row .. + VD - 1 of the keys 4 quarter + 0..3 and
 //      16 + 4 quarter + 0..3, those whose probabilities it holds; product d takes its d-th
 //      dim, so V is transposed as the codes of two keys become a pair of bf16.
-// No byte passes LDS, and a load's address is a base plus an offset that the lane keeps.
+// No code passes LDS, and a load's address is a base plus an offset that the lane keeps.
 template <typename T, int HD>
 struct CodeBlock {
   static constexpr int KD = HD / 4, VD = HD / 16;              // dims a lane, of K and of V
   static constexpr int KW = KD / 4, VW = VD >= 4 ? VD / 4 : 1;  // words of a row
   uint32_t k[2][KW], v[8][VW];
-  vf4 ks[2], vs[2];
+  float scale;  // of key lane % 32: K's in the lower lanes, V's in the upper
 
   static constexpr int KL = KW >= 4 ? KW / 4 : 1;  // loads of K's row, 16 bytes each where it has as many
 
+  // off stays a 32-bit register beside the base, for a load's own addition (the compiler would
+  // widen it ahead of the loop, and add in vector instructions)
   template <int N>
-  static __device__ __forceinline__ void words(uint32_t *w, const T *p) {
+  static __device__ __forceinline__ void words(uint32_t *w, const T *p, uint32_t off) {
+    asm volatile("" : "+v"(off));
+    p += off;
     if constexpr (N == 1) {
       w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p));
     } else {
@@ -37,11 +41,11 @@ struct CodeBlock {
   }
   static __device__ __forceinline__ void k_words(uint32_t (&w)[KW], const T *p, const uint32_t (&off)[KL]) {
 #pragma unroll
-    for (int i = 0; i < KL; ++i) words<KW / KL>(w + KW / KL * i, p + off[i]);
+    for (int i = 0; i < KL; ++i) words<KW / KL>(w + KW / KL * i, p, off[i]);
   }
-  static __device__ __forceinline__ void v_words(uint32_t (&w)[VW], const T *p) {
-    if constexpr (VD >= 4) words<VW>(w, p);
-    else w[0] = *reinterpret_cast<const uint16_t *>(p);
+  static __device__ __forceinline__ void v_words(uint32_t (&w)[VW], const T *p, uint32_t off) {
+    if constexpr (VD >= 4) words<VW>(w, p, off);
+    else w[0] = *reinterpret_cast<const uint16_t *>(p + off);
   }
 
   // The operand of product s over keys 16 h + row
@@ -69,164 +73,127 @@ struct CodeBlock {
   }
 };
 
-// Four scales in a row (aligned to their size alone).
-__device__ __forceinline__ vf4 four_scales(const float *p) {
-  struct __attribute__((packed, aligned(4))) Four {
-    vf4 x;
-  };
-  return reinterpret_cast<const Four *>(p)->x;
-}
-
-// Where a wave's rows of 32 keys lie.  RUN keys, beginning at a multiple of RUN, lie in one page.
-//   RUN 16: a half's page is the same for all lanes.  Lane l holds where half l % 2 of the
-//      wave's block l / 2 lies, of 32 blocks; a block's two are read from there.
-//   RUN 4, 1: every lane looks its rows' pages up, a block ahead.
+// Where a wave's blocks of 32 keys, 128 keys apart, lie.  RUN keys, beginning at a multiple of
+// RUN, lie in one page:
+//   RUN 16, 8: a block's pages are looked up by scalar loads, a block ahead of its rows.
+//   RUN 1: every lane looks its rows' pages up (pages of fewer tokens than 8).
 template <typename T, int HD, int RUN>
 struct CodeLoader {
   typedef CodeBlock<T, HD> Block;
-  static constexpr int NV = RUN == 1 ? 8 : 2;  // pages that a lane's keys of V lie in
-  static constexpr int STRIDE = 128;           // keys from one of a wave's blocks to its next
-  const int *table;
-  const T *kc, *vc;        // the head's
+  typedef const __attribute__((address_space(4))) int *Table;  // nothing writes it in the meantime
+  static constexpr int NP = RUN == 1 ? 1 : 32 / RUN, PER = 16 / RUN;  // pages of a block, and of half of one
+  Table table;
+  const T *kc, *vc;          // the head's
   const float *ks, *vs;
-  uint32_t k_off[Block::KL], v_off;  // of the lane's dims, in bytes; RUN 16: and of its row in a half
-  int row, quarter, width, last, first;
-  int page[RUN == 16 ? 1 : 2 + NV];
-  uint32_t at_lo, at_hi;   // RUN 16: rows before the lane's half
-  uint64_t none;           // RUN 16: halves whose page is none; else lane's rows, as bits
+  const float *side;         // of this lane: K's or V's
+  uint32_t k_off[Block::KL], v_off;  // of the lane's dims, in bytes; RUN > 1: and of its row in a run
+  int row, quarter, width, last;
+  int page[NP];              // of the next block to be loaded
+  int lane_page[RUN == 1 ? 11 : 1];  // RUN 1: of K's rows, V's, and the scale's
 
-  __device__ __forceinline__ void init(const PagedArgs &a, int trow, int hk, int first_key, int last_key) {
+  __device__ __forceinline__ void init(const PagedArgs &a, int trow, int hk, int last_key) {
     const int lane = threadIdx.x & 63;
     row = lane & 15;
     quarter = lane >> 4;
     width = a.width;
     last = last_key;
-    first = first_key;
-    table = a.table + (size_t)trow * a.max_blocks;
+    table = (Table)(uint64_t)(a.table + (size_t)trow * a.max_blocks);
     kc = head_of<T>(a, a.kc, hk);
     vc = head_of<T>(a, a.vc, hk);
     ks = a.ks + ((size_t)hk << a.page_shift);
     vs = a.vs + ((size_t)hk << a.page_shift);
+    side = (lane < 32 ? ks : vs) + (RUN == 1 ? 0 : lane % RUN);
     // Dims past a row's end read its beginning instead: Q is 0 there, and what they give O is
     // not stored.  (Rows are multiples of 16 bytes, so a load lies in a row or past it.)
 #pragma unroll
     for (int i = 0; i < Block::KL; ++i) {
       const int d = Block::KD * quarter + 16 * i;
-      k_off[i] = (RUN == 16 ? row * width : 0) + (d < width ? d : 0);
+      k_off[i] = (RUN == 1 ? 0 : row % RUN * width) + (d < width ? d : 0);
     }
-    v_off = (RUN == 16 ? 4 * quarter * width : 0) + (Block::VD * row < width ? Block::VD * row : 0);
+    v_off = (RUN == 1 ? 0 : 4 * quarter % RUN * width) + (Block::VD * row < width ? Block::VD * row : 0);
   }
-  __device__ __forceinline__ int page_of(const PagedArgs &a, int key) const { return table[min(key, last) >> a.page_shift]; }
-  // RUN 16: the key at which lane's half of the blocks from k0 on begins
-  static __device__ __forceinline__ int half_key(int k0) {
-    const int lane = threadIdx.x & 63;
-    return k0 + STRIDE * (lane >> 1) + 16 * (lane & 1);
-  }
-  // Keys of the lane: of K, half h; of V, place e
+  // Keys of the lane: of K, half h; of V, place e; of the scale
   __device__ __forceinline__ int k_key(int k0, int h) const { return k0 + 16 * h + row; }
   __device__ __forceinline__ int v_key(int k0, int e) const { return k0 + 16 * (e / 4) + 4 * quarter + e % 4; }
+  __device__ __forceinline__ int scale_key(int k0) const { return k0 + (int)(threadIdx.x & 31); }
+  __device__ __forceinline__ int page_of(const PagedArgs &a, int key) const { return table[min(key, last) >> a.page_shift]; }
   // The pages that load() of the block at k0 needs
   __device__ __forceinline__ void lookup(const PagedArgs &a, int k0) {
-    if constexpr (RUN == 16) {
-      page[0] = page_of(a, half_key(k0));
+    if constexpr (RUN > 1) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) page[i] = page_of(a, k0 + RUN * i);
     } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) page[h] = page_of(a, k_key(k0, h));
+      for (int h = 0; h < 2; ++h) lane_page[h] = page_of(a, k_key(k0, h));
 #pragma unroll
-      for (int i = 0; i < NV; ++i) page[2 + i] = page_of(a, v_key(k0, 8 / NV * i));
+      for (int e = 0; e < 8; ++e) lane_page[2 + e] = page_of(a, v_key(k0, e));
+      lane_page[10] = page_of(a, scale_key(k0));
     }
-  }
-  __device__ __forceinline__ void start_group(const PagedArgs &a, int k0) {
-    // (a half past the last key reads the page of that, its rows from the same place)
-    const Slot s = slot_in(a, page[0], half_key(k0));
-    const size_t at = row_at<T>(a, s.at);
-    at_lo = (uint32_t)at;
-    at_hi = (uint32_t)(at >> 32);
-    none = __builtin_amdgcn_ballot_w64(!s.ok);
-    first = k0;
-    lookup(a, k0 + 32 * STRIDE);
-  }
-  __device__ __forceinline__ void lookup_first(const PagedArgs &a) {
-    lookup(a, first);
-    if constexpr (RUN == 16) start_group(a, first);
   }
 
-  // Loads the block at k0 and looks the next one's pages up.  Rows of no page come as zeros.
-  __device__ __forceinline__ void load(const PagedArgs &a, Block &b, int k0) {
-    if constexpr (RUN == 16) {
-      if (k0 - first >= 32 * STRIDE) start_group(a, k0);
-      const int i = (k0 - first) / STRIDE * 2;
+  // Loads the block at k0 and looks the next one's pages up.  What comes from no page: bits of
+  // runs, or of the lane's rows (0, 1: K's, 2 ..: V's, 10: the scale's).
+  __device__ __forceinline__ uint32_t load(const PagedArgs &a, Block &b, int k0) {
+    uint32_t none = 0;
+    if constexpr (RUN > 1) {
+      size_t at[NP];  // rows before the run
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        // (a run past the last key lies in that one's page, its rows at the same places)
+        const Slot s = slot_in(a, page[i], k0 + RUN * i);
+        none |= (uint32_t)!s.ok << i;
+        at[i] = row_at<T>(a, s.at);
+      }
+      lookup(a, k0 + 128);
+      const int lane = threadIdx.x & 31;
+      size_t mine = lane & 16 ? at[PER] : at[0];
+      if constexpr (PER == 2) mine = lane & 8 ? lane & 16 ? at[3] : at[1] : mine;
+      b.scale = side[mine];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const size_t at = (size_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, i + h) << 32 |
-                          (uint32_t)__builtin_amdgcn_readlane(at_lo, i + h);
-        const T *kp = kc + at * width, *vp = vc + at * width;
-        Block::k_words(b.k[h], kp, k_off);
+        const size_t run = PER == 1 ? at[h] : row & 8 ? at[PER * h + PER - 1] : at[PER * h];
+        Block::k_words(b.k[h], kc + run * width, k_off);
+      }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) Block::v_words(b.v[4 * h + e], vp + e * width + v_off);
-        b.ks[h] = four_scales(ks + at + 4 * quarter);
-        b.vs[h] = four_scales(vs + at + 4 * quarter);
+      for (int h = 0; h < 2; ++h) {
+        const size_t run = PER == 1 ? at[h] : quarter & 2 ? at[PER * h + PER - 1] : at[PER * h];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) Block::v_words(b.v[4 * h + e], vc + (run + e) * width, v_off);
       }
     } else {
-      none = 0;
+      auto place = [&](int i, int key) {
+        const Slot s = slot_in(a, lane_page[i], key);
+        none |= (uint32_t)!s.ok << i;
+        return row_at<T>(a, s.at);
+      };
+      b.scale = side[place(10, scale_key(k0))];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const Slot s = slot_in(a, page[h], k_key(k0, h));
-        none |= (uint64_t)!s.ok << h;
-        Block::k_words(b.k[h], kc + row_at<T>(a, s.at) * width, k_off);
-      }
+      for (int h = 0; h < 2; ++h) Block::k_words(b.k[h], kc + place(h, k_key(k0, h)) * width, k_off);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const Slot s = slot_in(a, page[2 + e * NV / 8], v_key(k0, e));
-        none |= (uint64_t)!s.ok << (2 + e);
-        const size_t at = row_at<T>(a, s.at);
-        Block::v_words(b.v[e], vc + at * width + v_off);
-        if constexpr (RUN == 1) {
-          b.ks[e / 4][e % 4] = ks[at];
-          b.vs[e / 4][e % 4] = vs[at];
-        } else if (e % 4 == 0) {
-          b.ks[e / 4] = four_scales(ks + at);
-          b.vs[e / 4] = four_scales(vs + at);
-        }
-      }
-      lookup(a, k0 + STRIDE);
+      for (int e = 0; e < 8; ++e) Block::v_words(b.v[e], vc + place(2 + e, v_key(k0, e)) * width, v_off);
+      lookup(a, k0 + 128);
     }
+    return none;
   }
-  // Rows of no page, and V's past the request's last key, become zeros (the block at k0, the
-  // last that was loaded).
-  __device__ __forceinline__ void clean(Block &b, int k0, int *bad) const {
-    if constexpr (RUN == 16) {
-      const uint32_t wrong = (uint32_t)(none >> (k0 - first) / STRIDE * 2) & 3u;
-      if (wrong == 0 && k0 + 31 <= last) return;
-      if (wrong && bad) *bad = 1;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (wrong >> h & 1) {
-          zero(b.k[h]);
-          b.ks[h] = vf4{};
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((wrong >> h & 1) || v_key(k0, 4 * h + e) > last) {
-            zero(b.v[4 * h + e]);
-            b.vs[h][e] = 0.f;
-          }
-      }
-    } else {
-      if (__builtin_amdgcn_ballot_w64(none != 0) == 0 && k0 + 31 <= last) return;
-      if (none && bad) *bad = 1;
+  // The scale of no page, and V's past the request's last key, become 0; so do the codes where
+  // they may be NaN (F8).  none: what load() of the block returned.
+  __device__ __forceinline__ void clean(Block &b, int k0, uint32_t none, int &bad) const {
+    const bool past = k0 + 31 > last;
+    if (RUN > 1 ? none == 0 : __builtin_amdgcn_ballot_w64(none != 0) == 0) {
+      if (!past) return;
+    } else if (none) {
+      bad = 1;
+    }
+    const int i = RUN == 1 ? 10 : (int)(threadIdx.x & 31) / RUN;
+    if ((none >> i & 1) || ((threadIdx.x & 32) && scale_key(k0) > last)) b.scale = 0.f;
+    if constexpr (std::is_same<T, F8>::value) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if (none >> h & 1) zero(b.k[h]);
+        if (none >> (RUN == 1 ? h : PER * h + (PER == 2 ? row >> 3 : 0)) & 1) zero(b.k[h]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool wrong = none >> (2 + e) & 1;
-        if (wrong) b.ks[e / 4][e % 4] = 0.f;
-        if (wrong || v_key(k0, e) > last) {
+      for (int e = 0; e < 8; ++e)
+        if ((none >> (RUN == 1 ? 2 + e : PER * (e / 4) + (PER == 2 ? quarter >> 1 : 0)) & 1) || v_key(k0, e) > last)
           zero(b.v[e]);
-          b.vs[e / 4][e % 4] = 0.f;
-        }
-      }
     }
   }
   template <int W>
@@ -236,19 +203,61 @@ struct CodeLoader {
   }
 };
 
+// x of the lane N places before (cyclically, of 16).
+template <int N>
+__device__ __forceinline__ float turned(float x) {
+  return dpp<0x120 + N>(x);
+}
+
 // The online softmax of up to 16 rows, one per lane % 16, over blocks of 32 keys, as in SpanRows.
-template <typename T, int HD>
+//   PACK: of up to four rows, one per lane % 4.  The operand's other columns hold the pieces: Q's
+// and the probabilities' first, second and third in columns 0..3, 4..7 and 8..11, zeros in the
+// last.  One product does for three, the parts of a score are added across the columns, those of
+// O once at the end; and the pieces of Q take a third of the registers.
+template <typename T, int HD, bool PACK>
 struct CodeRows {
   typedef CodeBlock<T, HD> Block;
-  static constexpr int NS = HD / 32, NDB = HD / 16;
+  static constexpr int NS = HD / 32, NDB = HD / 16, NP = PACK ? 1 : 3;
+  static constexpr int ROWS = PACK ? 4 : 16;
+  bf16x8 q[NS][NP];
   floatx4 o[NDB];  // register c of o[d]: dim VD * (4 quarter + c) + d
   float m, l;      // the reference (log2 units) and this quarter's sum
+  bool warm;       // every lane has its reference (wave-uniform)
+  uint32_t cut[2];  // PACK: what the lane's piece leaves out of a value, and of the rest
 
   __device__ __forceinline__ void init() {
 #pragma unroll
     for (int d = 0; d < NDB; ++d) o[d] = floatx4{};
     m = -INFINITY;
     l = 0.f;
+    warm = false;
+    const int piece = threadIdx.x >> 2 & 3;
+    cut[0] = piece == 0 ? 0u : piece == 3 ? ~0u : 0xffff0000u;
+    cut[1] = piece < 2 ? 0u : piece == 3 ? ~0u : 0xffff0000u;
+  }
+  // Whether Q is out of the pieces' range (wave-uniform)
+  template <bool VEC>
+  __device__ __forceinline__ bool load_q(const float *qrow, int hd, float scale, int quarter) {
+    bf16x8 all[NS][3];
+    const bool wide = load_q_pieces<NS, VEC>(all, qrow, hd, scale, 8, HD / 4 * quarter);
+    const int piece = threadIdx.x >> 2 & 3;
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+      if constexpr (PACK) {
+        vu4 w;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[3];
+#pragma unroll
+          for (int j = 0; j < 3; ++j) x[j] = __builtin_bit_cast(vu4, all[i][j])[c];
+          w[c] = piece == 0 ? x[0] : piece == 1 ? x[1] : piece == 2 ? x[2] : 0u;
+        }
+        q[i][0] = __builtin_bit_cast(bf16x8, w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j) q[i][j] = all[i][2 - j];  // the corrections first
+      }
+    return wide;
   }
   // Probabilities of the keys up to last_vis (counted from the quarter's first) in place of
   // the scores; o and l follow a reference that rises.
@@ -273,9 +282,35 @@ struct CodeRows {
       p[e] = fast_exp2(p[e] - ref);
       l += p[e];
     }
+    warm = !__builtin_amdgcn_ballot_w64(m == -INFINITY);
   }
-  __device__ __forceinline__ void add(const Block &b, const bf16x8 (&q)[NS][3], int last_vis) {
-    float p[8];
+  // The same without a look at the maximum, once every row has a reference: false, and nothing
+  // changed, where a lane's probabilities sum up to more than 2^32, or to NaN.
+  __device__ __forceinline__ bool try_fast(const float (&s)[8], const vf4 (&ks)[2], float (&p)[8]) {
+    float sum[4];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = fast_exp2(fmaf(s[e], ks[e / 4][e % 4], -m));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] = p[e] + p[e + 4];
+    const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    if (__builtin_amdgcn_ballot_w64(!(all <= kFastSumLimit))) return false;
+    l += all;
+    return true;
+  }
+  // scales: 64 floats of LDS for this wave.  masked: some row does not see all of the block
+  // (wave-uniform).
+  __device__ __forceinline__ void add(const Block &b, float *scales, int quarter, bool masked, int last_vis) {
+    scales[threadIdx.x & 63] = b.scale * (threadIdx.x & 32 ? kCodeScale : 1.f);
+    // (LDS writes and reads of one wave are in order, but not for the compiler)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    vf4 ks[2], vs[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      ks[h] = *reinterpret_cast<const vf4 *>(scales + 16 * h + 4 * quarter);
+      vs[h] = *reinterpret_cast<const vf4 *>(scales + 32 + 16 * h + 4 * quarter);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float raw[8], p[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       floatx4 s = {};
@@ -283,21 +318,44 @@ struct CodeRows {
       for (int i = 0; i < NS; ++i) {
         const bf16x8 k = b.k_operand(h, i);
 #pragma unroll
-        for (int c = 2; c >= 0; --c) s = mfma16x16x32(k, q[i][c], s);
+        for (int c = 0; c < NP; ++c) s = mfma16x16x32(k, q[i][c], s);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[4 * h + e] = s[e] * b.ks[h][e];
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (PACK) {
+          s[e] += turned<8>(s[e]);
+          s[e] += turned<4>(s[e]);
+        }
+        raw[4 * h + e] = s[e];
+      }
     }
-    softmax(p, last_vis);
+    if (!warm || masked || !try_fast(raw, ks, p)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] *= b.vs[e / 4][e % 4];
+      for (int e = 0; e < 8; ++e) p[e] = raw[e] * ks[e / 4][e % 4];
+      softmax(p, last_vis);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] *= vs[e / 4][e % 4];
     bf16x8 pp[3];
-    split_operand(p, kCodeScale, pp);
+    if constexpr (PACK) {
+      // a value's top sixteen bits are its piece, what is left of it the next one's value
+      vu4 w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) p[e] -= __uint_as_float(__float_as_uint(p[e]) & cut[c]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = __builtin_amdgcn_perm(__float_as_uint(p[2 * i + 1]), __float_as_uint(p[2 * i]), 0x07060302u);
+      pp[0] = __builtin_bit_cast(bf16x8, w);
+    } else {
+      split_operand(p, 1.f, pp);
+    }
 #pragma unroll
     for (int d = 0; d < NDB; ++d) {
       const bf16x8 v = b.v_operand(d);
 #pragma unroll
-      for (int c = 2; c >= 0; --c) o[d] = mfma16x16x32(v, pp[c], o[d]);
+      for (int c = NP - 1; c >= 0; --c) o[d] = mfma16x16x32(v, pp[c], o[d]);
     }
   }
   // Undoes the scale of V's scales; whether some row came out non-finite (wave-uniform)
@@ -310,6 +368,20 @@ struct CodeRows {
       for (int c = 0; c < 4; ++c) wrong = fmaf(o[d][c], 0.f, wrong);
     }
     return any_nonfinite(wrong);
+  }
+  // PACK: the pieces' sums of O (after recompute: those of the first lanes)
+  __device__ __forceinline__ void join_pieces(bool recomputed) {
+    if constexpr (PACK) {
+      const bool mine = !recomputed || (threadIdx.x & 12) == 0;
+#pragma unroll
+      for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float x = mine ? o[d][c] : 0.f;
+          x += turned<8>(x);
+          o[d][c] = x + turned<4>(x);
+        }
+    }
   }
   // The rows over the wave's blocks in fp32, value by value and without the keys that a row
   // does not see: for rows that came out non-finite or whose Q is out of the pieces' range.
@@ -360,16 +432,21 @@ struct CodeRows {
 };
 
 // One workgroup: up to 16 rows of a (request, K/V head) against one chunk of its keys.  The
-// four waves take blocks of 32 keys in turn and join their sums at the end; a wave's next
-// block is on the way while one is multiplied.
-template <typename T, int HD, int RUN, bool VEC, bool SHARED>
+// four waves take blocks of 32 keys in turn and join their sums at the end.  A wave's sets of
+// registers go round: all blocks but the one that is multiplied are on the way.
+template <int HD, int RUN>
+constexpr int code_blocks() {
+  return 2;
+}
+template <typename T, int HD, int RUN, bool VEC, bool PACK, bool SHARED>
 __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s, int b, int r0, int nr,
-                                          float (&lds)[4][16 * (HD + 4)], float (&red_m)[4][16], float (&red_l)[4][16]) {
-  typedef CodeRows<T, HD> Rows;
+                                          float (&lds)[4][CodeRows<T, HD, PACK>::ROWS * (HD + 4)], float (&red_m)[4][16], float (&red_l)[4][16],
+                                          float (&scales)[4][64]) {
+  typedef CodeRows<T, HD, PACK> Rows;
   typedef CodeBlock<T, HD> Block;
-  constexpr int NS = HD / 32, NDB = HD / 16, ROW = HD + 4;  // floats between rows of the join
+  constexpr int NDB = HD / 16, ROW = HD + 4, ROWS = Rows::ROWS;  // floats between rows of the join
   const int hk = blockIdx.y % a.kv_heads, split = blockIdx.x, base = s.len - s.n;
-  const int kend = s.causal ? base + a.by_group.div(min(r0 + 16, nr) - 1) + 1 : s.len;  // past the last visible key
+  const int kend = s.causal ? base + a.by_group.div(min(r0 + ROWS, nr) - 1) + 1 : s.len;  // past the last visible key
   const bool single = !SHARED && s.len <= a.few_chunk;
   const int c0 = split_from<SHARED>(s, split, a.few_chunk);
   const int c1 = split_to<SHARED>(c0, split, a.few_splits, a.few_chunk, kend);
@@ -377,9 +454,10 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = lane & 15, quarter = lane >> 4;
+  const int row = lane & (ROWS - 1), quarter = lane >> 4;
   const int rr = min(r0 + row, nr - 1), tok = a.by_group.div(rr), head = hk * a.group + rr - tok * a.group;
   const int last = s.len - 1, lim = s.causal ? base + tok : last;
+  const int lim_lo = s.causal ? base + a.by_group.div(r0) : last;
   const float *qrow = a.q + (size_t)(s.first + tok) * a.ldq + (size_t)head * a.hd;
 
   Rows rows;
@@ -387,40 +465,49 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
   const int first = c0 + wave * 32;
   if (first < c1) {
     CodeLoader<T, HD, RUN> from;
-    from.init(a, s.table, hk, first, last);
-    from.lookup_first(a);
-    Block x, y;
-    from.load(a, x, first);
-    bf16x8 q[NS][3];
-    const bool wide = load_q_pieces<NS, VEC>(q, qrow, a.hd, a.scale_log2, 8, HD / 4 * quarter);
+    from.init(a, s.table, hk, last);
+    from.lookup(a, first);
+    constexpr int U = code_blocks<HD, RUN>();
+    Block block[U];
+    uint32_t none[U];
+    int bad = 0;
     // (past the wave's last block the request's last rows are loaded once more, and left there)
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u) none[u] = from.load(a, block[u], first + 128 * u);
+    const bool wide = rows.template load_q<VEC>(qrow, a.hd, a.scale_log2, quarter);
+    // (left from its middle: a way back to its top with loads unused would make every turn wait for them)
 #pragma unroll 1
-    for (int k0 = first; k0 < c1; k0 += 256) {
-      from.clean(x, k0, a.bad);
-      from.load(a, y, k0 + 128);
-      rows.add(x, q, lim - k0 - 4 * quarter);
-      if (k0 + 128 >= c1) break;
-      from.clean(y, k0 + 128, a.bad);
-      from.load(a, x, k0 + 256);
-      rows.add(y, q, lim - k0 - 128 - 4 * quarter);
+    for (int k0 = first;; k0 += 128 * U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + 128 * u, ahead = (u + U - 1) % U;
+        if (k >= c1) goto summed;
+        none[ahead] = from.load(a, block[ahead], k + 128 * (U - 1));
+        from.clean(block[u], k, none[u], bad);
+        rows.add(block[u], scales[wave], quarter, k + 31 > lim_lo, lim - k - 4 * quarter);
+      }
     }
-    if (rows.finish() || wide)
-      rows.recompute(a, qrow, a.table + (size_t)s.table * a.max_blocks, hk, quarter, first, c1, lim, last);
+  summed:
+    if (bad && a.bad) *a.bad = 1;
+    const bool again = rows.finish() || wide;
+    if (again) rows.recompute(a, qrow, a.table + (size_t)s.table * a.max_blocks, hk, quarter, first, c1, lim, last);
+    rows.join_pieces(again);
   }
   // the waves' sums: rows' statistics, then each wave's O scaled to the common maximum
   const float m = fmaxf(rows.m, kNoKey), l = quarters(rows.l, [](float x, float y) { return x + y; });
-  if (quarter == 0) {
+  if (lane < ROWS) {
     red_m[wave][row] = m;
     red_l[wave][row] = l;
   }
   __syncthreads();
   const float w = fast_exp2(m - fmaxf(fmaxf(red_m[0][row], red_m[1][row]), fmaxf(red_m[2][row], red_m[3][row])));
+  if (!PACK || (lane & 12) == 0)
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int d = 0; d < NDB; ++d) lds[wave][row * ROW + NDB * (4 * quarter + c) + d] = rows.o[d][c] * w;
   __syncthreads();
-  for (int t = threadIdx.x; t < min(nr - r0, 16) * HD; t += PT_THREADS) {
+  for (int t = threadIdx.x; t < min(nr - r0, ROWS) * HD; t += PT_THREADS) {
     const int r = t / HD, d = t % HD;
     if (d >= a.hd) continue;
     float x = 0.f, L = 0.f;
@@ -448,39 +535,45 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
   }
 }
 
-template <typename T, int HD, int RUN, bool VEC, bool SHARED>
+template <typename T, int HD, int RUN, bool VEC, bool PACK, bool SHARED>
 __global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kernel(const PagedArgs a) {
-  __shared__ __attribute__((aligned(16))) float lds[4][16 * (HD + 4)];
+  constexpr int ROWS = CodeRows<T, HD, PACK>::ROWS;
+  __shared__ __attribute__((aligned(16))) float lds[4][ROWS * (HD + 4)];
   __shared__ float red_m[4][16], red_l[4][16];
+  __shared__ __attribute__((aligned(16))) float scales[4][64];
   const int b = blockIdx.z;
   const PagedSeq s = paged_seq<SHARED>(a, b);
   const int nr = s.n * a.group;
-  int r0 = blockIdx.y / a.kv_heads * 16;
+  int r0 = blockIdx.y / a.kv_heads * ROWS;
   if (nr > a.few_rows || r0 >= nr) return;
   if constexpr (SHARED) {
     // (a group of more rows than the launch was told of takes its time)
-    for (; r0 < nr; r0 += gridDim.y / a.kv_heads * 16) {
-      code_rows<T, HD, RUN, VEC, true>(a, s, b, r0, nr, lds, red_m, red_l);
+    for (; r0 < nr; r0 += gridDim.y / a.kv_heads * ROWS) {
+      code_rows<T, HD, RUN, VEC, PACK, true>(a, s, b, r0, nr, lds, red_m, red_l, scales);
       __syncthreads();
     }
   } else {
-    code_rows<T, HD, RUN, VEC, false>(a, s, b, r0, nr, lds, red_m, red_l);
+    code_rows<T, HD, RUN, VEC, PACK, false>(a, s, b, r0, nr, lds, red_m, red_l, scales);
   }
 }
 
-template <typename T, int HD, bool VEC, bool SHARED>
+template <typename T, int HD, bool VEC, bool PACK, bool SHARED>
 void launch_code(const PagedArgs &a, hipStream_t st) {
-  const int row_groups = SHARED && a.prefix ? 1 : (a.few_rows + 15) / 16;
+  constexpr int ROWS = CodeRows<T, HD, PACK>::ROWS;
+  const int row_groups = SHARED && a.prefix ? 1 : (a.few_rows + ROWS - 1) / ROWS;
   const dim3 grid(a.few_splits, a.kv_heads * row_groups, SHARED && a.prefix ? a.groups : a.batch);
-  if (a.page_shift >= 4) paged_code_kernel<T, HD, 16, VEC, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
-  else if (a.page_shift >= 2) paged_code_kernel<T, HD, 4, VEC, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
-  else paged_code_kernel<T, HD, 1, VEC, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  if (a.page_shift >= 4) paged_code_kernel<T, HD, 16, VEC, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  else if (a.page_shift == 3) paged_code_kernel<T, HD, 8, VEC, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  else paged_code_kernel<T, HD, 1, VEC, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
 }
 
 template <typename T, int HD, bool SHARED>
 void launch_code(const PagedArgs &a, bool wide, hipStream_t st) {
-  if (wide) launch_code<T, HD, true, SHARED>(a, st);
-  else launch_code<T, HD, false, SHARED>(a, st);
+  const bool pack = a.most_rows <= 4;
+  if (wide && pack) launch_code<T, HD, true, true, SHARED>(a, st);
+  else if (wide) launch_code<T, HD, true, false, SHARED>(a, st);
+  else if (pack) launch_code<T, HD, false, true, SHARED>(a, st);
+  else launch_code<T, HD, false, false, SHARED>(a, st);
 }
 
 // wide: head dims that are multiples of 8, and 16-byte aligned rows of Q and O.

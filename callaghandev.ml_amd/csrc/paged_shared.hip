@@ -110,6 +110,7 @@ __global__ void __launch_bounds__(256) paged_shared_join_kernel(const PagedArgs 
 struct SharedPlan {
   bool plain;          // every request reads its own pages
   bool prefix_tile;
+  int prefix_rows;     // of a group, at most
   int prefix_chunk, prefix_splits;
   Plan own;
   int own_splits;
@@ -128,6 +129,7 @@ SharedPlan plan_shared(int size, int rows, int batch, int groups, int max_member
   const int group = heads / kv_heads;
   const long long most = std::min((long long)max_members * max_new, (long long)rows) * group;
   p.prefix_tile = most > kSpanRows;
+  p.prefix_rows = (int)std::min<long long>(most, INT_MAX);
   const long long work = (p.prefix_tile ? (long long)rows * group / kPagedTileRows + groups : groups) * kv_heads;
   long long splits = (2 * kComputeUnits + work - 1) / work;
   if (!p.prefix_tile && work >= kComputeUnits) splits = 1;
@@ -293,13 +295,14 @@ extern "C" int cdml_paged_attn_shared(const float *q, int ldq, const void *kcach
   // what the groups share, all of a group's rows in the same kernel
   a.prefix = true;
   a.few_rows = p.prefix_tile ? 0 : INT_MAX;
+  a.most_rows = p.prefix_rows;
   a.few_chunk = a.tile_chunk = p.prefix_chunk;
   a.few_splits = a.tile_splits = p.prefix_splits;
   rc = run({false, !p.prefix_tile, p.prefix_tile});
   if (rc) return rc;
   // the tokens behind
   a.prefix = false;
-  a.few_rows = p.own.few_rows;
+  a.few_rows = a.most_rows = p.own.few_rows;
   a.few_chunk = p.own.few_chunk;
   a.few_splits = p.own.few_splits;
   a.tile_chunk = p.own.tile_chunk;
