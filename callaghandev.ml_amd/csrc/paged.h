@@ -82,19 +82,25 @@ struct PagedArgs {
   float scale_log2;
   int few_rows, few_chunk, few_splits, tile_chunk, tile_splits;
   int most_rows;     // of a request of few rows, at most (a hint)
+  bool wide;         // 16-byte aligned rows of Q, of whole vectors
   float *few_part;   // [batch][kv_heads][few_rows][few_splits][hd + 2]
   float *tile_part;  // [rows][heads][tile_splits][hd + 2]
   UDiv by_group;
   // Requests that share their first tokens (SHARED): a launch for what the groups share, in
   // which a group is one request whose rows are those of all its members, and one for the
-  // tokens behind.  Their chunks leave sums in part [rows][heads][part_splits][hd + 2], the
-  // shared tokens' first.
+  // tokens behind.  Their chunks leave sums in part [rows][heads][part_splits][part_width] and
+  // their maxima (log2) and sums in part_stats [rows][heads][part_splits][2], the shared
+  // tokens' first.  fused: requests of few rows have one chunk of their own, which adds the
+  // shared tokens' and writes o.
   const int *group_start, *shared;
   int groups;
-  bool prefix;  // which of the two
-  float *part;
-  int part_splits, first_split;
+  bool prefix, fused;  // prefix: which of the two launches
+  float *part, *part_stats;
+  int part_splits, part_width, first_split, prefix_chunk, prefix_splits;
 };
+
+// Chunks in which `seen` tokens lie.
+__device__ __forceinline__ int chunks_seen(int seen, int chunk) { return seen <= 0 ? 0 : (seen - 1) / chunk + 1; }
 
 struct PagedSeq {
   int first, n, len;  // first row, new tokens, tokens in the cache (past the last that counts)

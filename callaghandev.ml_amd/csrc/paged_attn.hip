@@ -13,9 +13,9 @@ __device__ __forceinline__ void join_few(const PagedArgs &a, int b, int i, int h
   const PagedSeq s = paged_seq(a, b);
   if (i >= s.n || s.n * a.group > a.few_rows || s.len <= a.few_chunk) return;
   const int hk = a.by_group.div(h), rr = i * a.group + h - hk * a.group;
-  join_chunks(a, a.few_part + (((size_t)b * a.kv_heads + hk) * a.few_rows + rr) * a.few_splits * (a.hd + 2),
-              chunks_seen(s.len - s.n + i + 1, a.few_chunk),
-              a.o + (size_t)(s.first + i) * a.ldo + (size_t)h * a.hd);
+  const float *part = a.few_part + (((size_t)b * a.kv_heads + hk) * a.few_rows + rr) * a.few_splits * (a.hd + 2);
+  const Chunks chunks[1] = {{part, part + a.hd, chunks_seen(s.len - s.n + i + 1, a.few_chunk), a.hd + 2, a.hd + 2}};
+  join_chunks(a.hd, chunks, a.o + (size_t)(s.first + i) * a.ldo + (size_t)h * a.hd);
 }
 
 // Row `row`, head h, of a request that ran in tiles.
@@ -25,8 +25,9 @@ __device__ __forceinline__ void join_tile(const PagedArgs &a, int row, int h) {
   const PagedSeq s = paged_seq(a, b);
   const int i = row - s.first;
   if (i < 0 || i >= s.n || s.n * a.group <= a.few_rows || s.len <= a.tile_chunk) return;
-  join_chunks(a, a.tile_part + ((size_t)row * a.heads + h) * a.tile_splits * (a.hd + 2),
-              chunks_seen(s.len - s.n + i + 1, a.tile_chunk), a.o + (size_t)row * a.ldo + (size_t)h * a.hd);
+  const float *part = a.tile_part + ((size_t)row * a.heads + h) * a.tile_splits * (a.hd + 2);
+  const Chunks chunks[1] = {{part, part + a.hd, chunks_seen(s.len - s.n + i + 1, a.tile_chunk), a.hd + 2, a.hd + 2}};
+  join_chunks(a.hd, chunks, a.o + (size_t)row * a.ldo + (size_t)h * a.hd);
 }
 
 // A wave per (new token, head): the first few_tokens * batch workgroups for the requests of few

@@ -1049,19 +1049,58 @@ __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kern
       rows.recompute(a, qrow, a.table + (size_t)s.table * a.max_blocks, hk, li, hf, c0, min(c1, lim_hi + 1), lim, lim_lo,
                      s.len - 1);
   }
-  if (rw0 + li >= nr) return;
   const float l = halves_sum(rows.l_sum);
+  if constexpr (SHARED && HD >= 64) {
+    // a chunk's sums through LDS, 32 dims at a time, so that a row's are written together
+    constexpr int ROW = 36;  // floats
+    static_assert(sizeof(lds) >= 4 * 32 * ROW * 4, "a wave's rows of 32 dims");
+    float *mine = reinterpret_cast<float *>(lds) + wave * 32 * ROW;
+    if (rw0 + li < nr && hf == 0) {
+      float *stats = a.part_stats + 2 * (((size_t)(s.first + tok) * a.heads + head) * a.part_splits + a.first_split + split);
+      stats[0] = fmaxf(rows.m_run, kNoKey);
+      stats[1] = l;
+    }
+    float *to[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = min(rw0 + 8 * i + (lane >> 3), nr - 1), t = a.by_group.div(row);
+      const size_t at = (size_t)(s.first + t) * a.heads + hk * a.group + row - t * a.group;
+      to[i] = a.part + (at * a.part_splits + a.first_split + split) * a.part_width;
+    }
+#pragma unroll
+    for (int db = 0; db < HD / 32; ++db) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<vf4 *>(mine + li * ROW + 8 * g + 4 * hf) =
+            vf4{rows.oacc[db][4 * g], rows.oacc[db][4 * g + 1], rows.oacc[db][4 * g + 2], rows.oacc[db][4 * g + 3]};
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const int d = db * 32 + 4 * (lane & 7);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (rw0 + 8 * i + (lane >> 3) < nr && d < a.part_width)
+          *reinterpret_cast<vf4 *>(to[i] + d) = *reinterpret_cast<const vf4 *>(mine + (8 * i + (lane >> 3)) * ROW + 4 * (lane & 7));
+    }
+    return;
+  }
+  if (rw0 + li >= nr) return;
   float *out, f = 1.f;
   if (single) {
     out = a.o + (size_t)(s.first + tok) * a.ldo + (size_t)head * a.hd;
     f = l == 0.f ? 0.f : 1.0f / l;
   } else {
     const size_t at = (size_t)(s.first + tok) * a.heads + head;
-    if constexpr (SHARED) out = a.part + (at * a.part_splits + a.first_split + split) * (a.hd + 2);
-    else out = a.tile_part + (at * a.tile_splits + split) * (a.hd + 2);
+    float *stats;
+    if constexpr (SHARED) {
+      out = a.part + (at * a.part_splits + a.first_split + split) * a.part_width;
+      stats = a.part_stats + 2 * (at * a.part_splits + a.first_split + split);
+    } else {
+      out = a.tile_part + (at * a.tile_splits + split) * (a.hd + 2);
+      stats = out + a.hd;
+    }
     if (hf == 0) {
-      out[a.hd] = fmaxf(rows.m_run, kNoKey);
-      out[a.hd + 1] = l;
+      stats[0] = fmaxf(rows.m_run, kNoKey);
+      stats[1] = l;
     }
   }
 #pragma unroll
@@ -1071,8 +1110,8 @@ __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kern
       const int d = db * 32 + 8 * g + 4 * hf;
       const vf4 x = {rows.oacc[db][4 * g] * f, rows.oacc[db][4 * g + 1] * f, rows.oacc[db][4 * g + 2] * f,
                      rows.oacc[db][4 * g + 3] * f};
-      if (VEC && single) {
-        if (d < a.hd) *reinterpret_cast<vf4 *>(out + d) = x;
+      if (SHARED ? true : VEC && single) {
+        if (d < (SHARED ? a.part_width : a.hd)) *reinterpret_cast<vf4 *>(out + d) = x;
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -1352,6 +1391,63 @@ struct SpanRows {
   }
 };
 
+// The end of a workgroup of few rows: the four waves' sums, o (a wave's `wave_floats` apart,
+// rows ROW apart) scaled to the waves' common maximum, become o, or a chunk's part, of rows r0 ..
+template <int HD, int ROWS, int ROW, bool SHARED>
+__device__ __forceinline__ void write_rows(const PagedArgs &a, const PagedSeq &s, int b, int hk, int r0, int nr,
+                                           int split, bool single, const float *o, int wave_floats,
+                                           const float (&red_m)[4][16], const float (&red_l)[4][16]) {
+  const int before = SHARED && single ? min(chunks_seen(s.start, a.prefix_chunk), a.prefix_splits) : 0;
+  for (int t = threadIdx.x; t < min(nr - r0, ROWS) * HD; t += PT_THREADS) {
+    const int r = t / HD, d = t % HD;
+    if (d >= a.hd) continue;
+    float x = 0.f, L = 0.f, M = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r]));
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      x += o[v * wave_floats + r * ROW + d];
+      L += red_l[v][r] * fast_exp2(red_m[v][r] - M);
+    }
+    const int i = a.by_group.div(r0 + r), h = hk * a.group + r0 + r - i * a.group;
+    const size_t head = (size_t)(s.first + i) * a.heads + h;
+    if constexpr (SHARED) {
+      const size_t at = head * a.part_splits;
+      if (!single) {
+        a.part[(at + a.first_split + split) * a.part_width + d] = x;
+        if (d == 0) {
+          float *stats = a.part_stats + (at + a.first_split + split) * 2;
+          stats[0] = M;
+          stats[1] = L;
+        }
+        continue;
+      }
+      // what the group shares
+      const float *stats = a.part_stats + at * 2, *part = a.part + at * a.part_width + d;
+      float top = M;
+#pragma unroll 4
+      for (int c = 0; c < before; ++c) top = fmaxf(top, stats[2 * c]);
+      const float w = fast_exp2(M - top);
+      x *= w;
+      L *= w;
+#pragma unroll 4
+      for (int c = 0; c < before; ++c) {
+        const float wc = fast_exp2(stats[2 * c] - top);
+        x = fmaf(part[(size_t)c * a.part_width], wc, x);
+        L = fmaf(stats[2 * c + 1], wc, L);
+      }
+    }
+    if (single) {
+      a.o[(size_t)(s.first + i) * a.ldo + (size_t)h * a.hd + d] = L == 0.f ? 0.f : x / L;
+    } else {
+      float *part = a.few_part + ((((size_t)b * a.kv_heads + hk) * a.few_rows + r0 + r) * a.few_splits + split) * (a.hd + 2);
+      part[d] = x;
+      if (d == 0) {
+        part[a.hd] = M;
+        part[a.hd + 1] = L;
+      }
+    }
+  }
+}
+
 // One workgroup: the up to 16 rows of a (request, K/V head) against one chunk of its keys.
 // Reading the cache bounds this, and rows fill one small MFMA operand at most, so the four
 // waves split the keys: each walks blocks of 32 through LDS of its own, with no barrier until
@@ -1373,7 +1469,7 @@ __device__ __forceinline__ void span_rows(const PagedArgs &a, const PagedSeq &s,
   constexpr int NS = HD / 32, NDB = HD / 16, ROW = SpanShape<T, HD, VEC>::ROW;
   const int hk = SHARED ? blockIdx.y % a.kv_heads : blockIdx.y, split = blockIdx.x;
   const int base = s.len - s.n;
-  const bool single = !SHARED && s.len <= a.few_chunk;
+  const bool single = SHARED ? a.fused && !a.prefix : s.len <= a.few_chunk;
   const int c0 = split_from<SHARED>(s, split, a.few_chunk);
   const int c1 = split_to<SHARED>(c0, split, a.few_splits, a.few_chunk, s.len);  // (some row sees all keys)
   if (c0 >= c1 && !(single && split == 0)) return;
@@ -1426,32 +1522,8 @@ __device__ __forceinline__ void span_rows(const PagedArgs &a, const PagedSeq &s,
 #pragma unroll
   for (int db = 0; db < NDB; ++db) *reinterpret_cast<floatx4 *>(part_o + db * 16 + 4 * quarter) = rows.o[db] * w;
   __syncthreads();
-  for (int t = threadIdx.x; t < (SHARED ? min(nr - r0, 16) : nr) * HD; t += PT_THREADS) {
-    const int r = t / HD, d = t % HD;
-    if (d >= a.hd) continue;
-    float x = 0.f, L = 0.f;
-    const float M = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r]));
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      x += reinterpret_cast<const float *>(lds[v])[r * ROW + d];
-      L += red_l[v][r] * fast_exp2(red_m[v][r] - M);
-    }
-    const int i = a.by_group.div(r0 + r), h = hk * a.group + r0 + r - i * a.group;
-    if (single) {
-      a.o[(size_t)(s.first + i) * a.ldo + (size_t)h * a.hd + d] = L == 0.f ? 0.f : x / L;
-    } else {
-      float *part;
-      if constexpr (SHARED)
-        part = a.part + (((size_t)(s.first + i) * a.heads + h) * a.part_splits + a.first_split + split) * (a.hd + 2);
-      else
-        part = a.few_part + ((((size_t)b * a.kv_heads + hk) * a.few_rows + r) * a.few_splits + split) * (a.hd + 2);
-      part[d] = x;
-      if (d == 0) {
-        part[a.hd] = M;
-        part[a.hd + 1] = L;
-      }
-    }
-  }
+  write_rows<HD, 16, ROW, SHARED>(a, s, b, hk, r0, nr, split, single, reinterpret_cast<const float *>(lds[0]),
+                                  WAVE / 4, red_m, red_l);
 }
 
 template <typename T, int HD, bool VEC, bool SHARED>

@@ -1,5 +1,6 @@
-// Attention of few rows a K/V head over an 8-bit paged cache, for one of its types T (I8 or
-// F8; included by a file each), and the choice between it and the tiles of paged_attn.inc.h.
+// Attention of few rows a K/V head over a paged cache of one piece (I8, F8 and, for up to four
+// rows, __bf16; included by a file each), and the choice between it and the tiles of
+// paged_attn.inc.h.
 #pragma once
 
 #include "paged_attn.inc.h"
@@ -17,8 +18,8 @@ namespace {
 // No code passes LDS, and a load's address is a base plus an offset that the lane keeps.
 template <typename T, int HD>
 struct CodeBlock {
-  static constexpr int KD = HD / 4, VD = HD / 16;              // dims a lane, of K and of V
-  static constexpr int KW = KD / 4, VW = VD >= 4 ? VD / 4 : 1;  // words of a row
+  static constexpr int KD = HD / 4, VD = HD / 16;  // dims a lane, of K and of V
+  static constexpr int B = sizeof(T), KW = KD * B / 4, VW = VD * B >= 4 ? VD * B / 4 : 1;  // words of a row
   uint32_t k[2][KW], v[8][VW];
   float scale;  // of key lane % 32: K's in the lower lanes, V's in the upper
 
@@ -44,7 +45,7 @@ struct CodeBlock {
     for (int i = 0; i < KL; ++i) words<KW / KL>(w + KW / KL * i, p, off[i]);
   }
   static __device__ __forceinline__ void v_words(uint32_t (&w)[VW], const T *p, uint32_t off) {
-    if constexpr (VD >= 4) words<VW>(w, p, off);
+    if constexpr (VD * B >= 4) words<VW>(w, p, off);
     else w[0] = *reinterpret_cast<const uint16_t *>(p + off);
   }
 
@@ -52,7 +53,10 @@ struct CodeBlock {
   __device__ __forceinline__ bf16x8 k_operand(int h, int s) const {
     vu4 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = code_pair(k[h][2 * s + i / 2], i & 1, T{});
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (kQ8<T>) w[i] = code_pair(k[h][2 * s + i / 2], i & 1, T{});
+      else w[i] = k[h][4 * s + i];
+    }
     return __builtin_bit_cast(bf16x8, w);
   }
   // The operand of dim d of the lane's VD
@@ -60,8 +64,10 @@ struct CodeBlock {
     vu4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t a = v[2 * i][d / 4], b = v[2 * i + 1][d / 4];
-      if constexpr (std::is_same<T, I8>::value) {
+      const uint32_t a = v[2 * i][d * B / 4], b = v[2 * i + 1][d * B / 4];
+      if constexpr (!kQ8<T>) {
+        w[i] = __builtin_amdgcn_perm(b, a, d & 1 ? 0x07060302u : 0x05040100u);
+      } else if constexpr (std::is_same<T, I8>::value) {
         const float x = code_value(I8{(uint8_t)(a >> 8 * (d % 4))}), y = code_value(I8{(uint8_t)(b >> 8 * (d % 4))});
         w[i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
       } else {
@@ -84,9 +90,8 @@ struct CodeLoader {
   static constexpr int NP = RUN == 1 ? 1 : 32 / RUN, PER = 16 / RUN;  // pages of a block, and of half of one
   Table table;
   const T *kc, *vc;          // the head's
-  const float *ks, *vs;
-  const float *side;         // of this lane: K's or V's
-  uint32_t k_off[Block::KL], v_off;  // of the lane's dims, in bytes; RUN > 1: and of its row in a run
+  const float *side;         // 8 bits: the scales of this lane, K's or V's
+  uint32_t k_off[Block::KL], v_off;  // of the lane's dims, in elements; RUN > 1: and of its row in a run
   int row, quarter, width, last;
   int page[NP];              // of the next block to be loaded
   int lane_page[RUN == 1 ? 11 : 1];  // RUN 1: of K's rows, V's, and the scale's
@@ -95,22 +100,21 @@ struct CodeLoader {
     const int lane = threadIdx.x & 63;
     row = lane & 15;
     quarter = lane >> 4;
-    width = a.width;
+    width = row_step<T>(a);
+    const int dims = kQ8<T> ? a.width : a.hd;
     last = last_key;
     table = (Table)(uint64_t)(a.table + (size_t)trow * a.max_blocks);
     kc = head_of<T>(a, a.kc, hk);
     vc = head_of<T>(a, a.vc, hk);
-    ks = a.ks + ((size_t)hk << a.page_shift);
-    vs = a.vs + ((size_t)hk << a.page_shift);
-    side = (lane < 32 ? ks : vs) + (RUN == 1 ? 0 : lane % RUN);
+    if constexpr (kQ8<T>) side = (lane < 32 ? a.ks : a.vs) + ((size_t)hk << a.page_shift) + (RUN == 1 ? 0 : lane % RUN);
     // Dims past a row's end read its beginning instead: Q is 0 there, and what they give O is
-    // not stored.  (Rows are multiples of 16 bytes, so a load lies in a row or past it.)
+    // not stored.  (A head's rows are multiples of 16 bytes, so a load lies in one or past it.)
 #pragma unroll
     for (int i = 0; i < Block::KL; ++i) {
-      const int d = Block::KD * quarter + 16 * i;
-      k_off[i] = (RUN == 1 ? 0 : row % RUN * width) + (d < width ? d : 0);
+      const int d = Block::KD * quarter + 16 / Block::B * i;
+      k_off[i] = (RUN == 1 ? 0 : row % RUN * width) + (d < dims ? d : 0);
     }
-    v_off = (RUN == 1 ? 0 : 4 * quarter % RUN * width) + (Block::VD * row < width ? Block::VD * row : 0);
+    v_off = (RUN == 1 ? 0 : 4 * quarter % RUN * width) + (Block::VD * row < dims ? Block::VD * row : 0);
   }
   // Keys of the lane: of K, half h; of V, place e; of the scale
   __device__ __forceinline__ int k_key(int k0, int h) const { return k0 + 16 * h + row; }
@@ -131,6 +135,9 @@ struct CodeLoader {
     }
   }
 
+  // Elements before a row or run
+  __device__ __forceinline__ size_t element(size_t at) const { return kQ8<T> ? at * width : at; }
+
   // Loads the block at k0 and looks the next one's pages up.  What comes from no page: bits of
   // runs, or of the lane's rows (0, 1: K's, 2 ..: V's, 10: the scale's).
   __device__ __forceinline__ uint32_t load(const PagedArgs &a, Block &b, int k0) {
@@ -145,20 +152,22 @@ struct CodeLoader {
         at[i] = row_at<T>(a, s.at);
       }
       lookup(a, k0 + 128);
-      const int lane = threadIdx.x & 31;
-      size_t mine = lane & 16 ? at[PER] : at[0];
-      if constexpr (PER == 2) mine = lane & 8 ? lane & 16 ? at[3] : at[1] : mine;
-      b.scale = side[mine];
+      if constexpr (kQ8<T>) {
+        const int lane = threadIdx.x & 31;
+        size_t mine = lane & 16 ? at[PER] : at[0];
+        if constexpr (PER == 2) mine = lane & 8 ? lane & 16 ? at[3] : at[1] : mine;
+        b.scale = side[mine];
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const size_t run = PER == 1 ? at[h] : row & 8 ? at[PER * h + PER - 1] : at[PER * h];
-        Block::k_words(b.k[h], kc + run * width, k_off);
+        Block::k_words(b.k[h], kc + element(run), k_off);
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const size_t run = PER == 1 ? at[h] : quarter & 2 ? at[PER * h + PER - 1] : at[PER * h];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) Block::v_words(b.v[4 * h + e], vc + (run + e) * width, v_off);
+        for (int e = 0; e < 4; ++e) Block::v_words(b.v[4 * h + e], vc + element(run) + e * width, v_off);
       }
     } else {
       auto place = [&](int i, int key) {
@@ -166,17 +175,17 @@ struct CodeLoader {
         none |= (uint32_t)!s.ok << i;
         return row_at<T>(a, s.at);
       };
-      b.scale = side[place(10, scale_key(k0))];
+      if constexpr (kQ8<T>) b.scale = side[place(10, scale_key(k0))];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) Block::k_words(b.k[h], kc + place(h, k_key(k0, h)) * width, k_off);
+      for (int h = 0; h < 2; ++h) Block::k_words(b.k[h], kc + element(place(h, k_key(k0, h))), k_off);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) Block::v_words(b.v[e], vc + place(2 + e, v_key(k0, e)) * width, v_off);
+      for (int e = 0; e < 8; ++e) Block::v_words(b.v[e], vc + element(place(2 + e, v_key(k0, e))), v_off);
       lookup(a, k0 + 128);
     }
     return none;
   }
-  // The scale of no page, and V's past the request's last key, become 0; so do the codes where
-  // they may be NaN (F8).  none: what load() of the block returned.
+  // The scale of no page, and V's past the request's last key, become 0; so do the values where
+  // they may be NaN (not I8).  none: what load() of the block returned.
   __device__ __forceinline__ void clean(Block &b, int k0, uint32_t none, int &bad) const {
     const bool past = k0 + 31 > last;
     if (RUN > 1 ? none == 0 : __builtin_amdgcn_ballot_w64(none != 0) == 0) {
@@ -185,8 +194,8 @@ struct CodeLoader {
       bad = 1;
     }
     const int i = RUN == 1 ? 10 : (int)(threadIdx.x & 31) / RUN;
-    if ((none >> i & 1) || ((threadIdx.x & 32) && scale_key(k0) > last)) b.scale = 0.f;
-    if constexpr (std::is_same<T, F8>::value) {
+    if (!kQ8<T> || (none >> i & 1) || ((threadIdx.x & 32) && scale_key(k0) > last)) b.scale = 0.f;
+    if constexpr (!std::is_same<T, I8>::value) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         if (none >> (RUN == 1 ? h : PER * h + (PER == 2 ? row >> 3 : 0)) & 1) zero(b.k[h]);
@@ -300,16 +309,20 @@ struct CodeRows {
   // scales: 64 floats of LDS for this wave.  masked: some row does not see all of the block
   // (wave-uniform).
   __device__ __forceinline__ void add(const Block &b, float *scales, int quarter, bool masked, int last_vis) {
-    scales[threadIdx.x & 63] = b.scale * (threadIdx.x & 32 ? kCodeScale : 1.f);
-    // (LDS writes and reads of one wave are in order, but not for the compiler)
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     vf4 ks[2], vs[2];
+    if constexpr (kQ8<T>) {
+      scales[threadIdx.x & 63] = b.scale * (threadIdx.x & 32 ? kCodeScale : 1.f);
+      // (LDS writes and reads of one wave are in order, but not for the compiler)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      ks[h] = *reinterpret_cast<const vf4 *>(scales + 16 * h + 4 * quarter);
-      vs[h] = *reinterpret_cast<const vf4 *>(scales + 32 + 16 * h + 4 * quarter);
+      for (int h = 0; h < 2; ++h) {
+        ks[h] = *reinterpret_cast<const vf4 *>(scales + 16 * h + 4 * quarter);
+        vs[h] = *reinterpret_cast<const vf4 *>(scales + 32 + 16 * h + 4 * quarter);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    } else {
+      ks[0] = ks[1] = vf4{1.f, 1.f, 1.f, 1.f};
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     float raw[8], p[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -334,8 +347,10 @@ struct CodeRows {
       for (int e = 0; e < 8; ++e) p[e] = raw[e] * ks[e / 4][e % 4];
       softmax(p, last_vis);
     }
+    if constexpr (kQ8<T>) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] *= vs[e / 4][e % 4];
+      for (int e = 0; e < 8; ++e) p[e] *= vs[e / 4][e % 4];
+    }
     bf16x8 pp[3];
     if constexpr (PACK) {
       // a value's top sixteen bits are its piece, what is left of it the next one's value
@@ -363,7 +378,7 @@ struct CodeRows {
     float wrong = l * 0.f;
 #pragma unroll
     for (int d = 0; d < NDB; ++d) {
-      o[d] *= kCodeUnscale;
+      if constexpr (kQ8<T>) o[d] *= kCodeUnscale;
 #pragma unroll
       for (int c = 0; c < 4; ++c) wrong = fmaf(o[d][c], 0.f, wrong);
     }
@@ -389,10 +404,13 @@ struct CodeRows {
                                             int first, int c1, int lim, int last) {
     init();
     const T *kc = head_of<T>(a, a.kc, hk), *vc = head_of<T>(a, a.vc, hk);
-    const size_t head = (size_t)hk << a.page_shift;
-    auto row_of = [&](int key, size_t &at) {
+    auto row_of = [&](int key, size_t &at, const float *scales, float &scale) {
       const Slot s = slot_in(a, table[key >> a.page_shift], key);
       at = row_at<T>(a, s.at);
+      if constexpr (kQ8<T>) {
+        scale = scales[((size_t)hk << a.page_shift) + at];
+        at *= a.width;
+      }
       return s.ok;
     };
 #pragma unroll 1
@@ -401,12 +419,12 @@ struct CodeRows {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         size_t at;
-        const bool ok = row_of(min(k0 + 16 * (e / 4) + 4 * quarter + e % 4, last), at);
+        float s = 1.f;
+        const bool ok = row_of(min(k0 + 16 * (e / 4) + 4 * quarter + e % 4, last), at, a.ks, s);
         p[e] = 0.f;
         if (!ok) continue;
-        const float s = a.ks[head + at];
 #pragma unroll 1
-        for (int d = 0; d < a.hd; ++d) p[e] = fmaf(cached(kc[at * a.width + d], s), qrow[d] * a.scale_log2, p[e]);
+        for (int d = 0; d < a.hd; ++d) p[e] = fmaf(cached(kc[at + d], s), qrow[d] * a.scale_log2, p[e]);
       }
       softmax(p, lim - k0 - 4 * quarter);
 #pragma unroll
@@ -417,14 +435,14 @@ struct CodeRows {
           const int key = k0 + 16 * (e / 4) + 4 * q + e % 4;
           if (key > lim) continue;
           size_t at;
-          if (!row_of(key, at)) continue;
-          const float s = a.vs[head + at];
+          float s = 1.f;
+          if (!row_of(key, at, a.vs, s)) continue;
 #pragma unroll
           for (int i = 0; i < NDB; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const int d = NDB * (4 * quarter + c) + i;
-              if (d < a.hd) o[i][c] = fmaf(w, cached(vc[at * a.width + d], s), o[i][c]);
+              if (d < a.hd) o[i][c] = fmaf(w, cached(vc[at + d], s), o[i][c]);
             }
         }
     }
@@ -438,7 +456,7 @@ template <int HD, int RUN>
 constexpr int code_blocks() {
   return 2;
 }
-template <typename T, int HD, int RUN, bool VEC, bool PACK, bool SHARED>
+template <typename T, int HD, int RUN, bool PACK, bool SHARED>
 __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s, int b, int r0, int nr,
                                           float (&lds)[4][CodeRows<T, HD, PACK>::ROWS * (HD + 4)], float (&red_m)[4][16], float (&red_l)[4][16],
                                           float (&scales)[4][64]) {
@@ -447,7 +465,7 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
   constexpr int NDB = HD / 16, ROW = HD + 4, ROWS = Rows::ROWS;  // floats between rows of the join
   const int hk = blockIdx.y % a.kv_heads, split = blockIdx.x, base = s.len - s.n;
   const int kend = s.causal ? base + a.by_group.div(min(r0 + ROWS, nr) - 1) + 1 : s.len;  // past the last visible key
-  const bool single = !SHARED && s.len <= a.few_chunk;
+  const bool single = SHARED ? a.fused && !a.prefix : s.len <= a.few_chunk;
   const int c0 = split_from<SHARED>(s, split, a.few_chunk);
   const int c1 = split_to<SHARED>(c0, split, a.few_splits, a.few_chunk, kend);
   if (c0 >= c1 && !(single && split == 0)) return;
@@ -474,7 +492,8 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
     // (past the wave's last block the request's last rows are loaded once more, and left there)
 #pragma unroll
     for (int u = 0; u < U - 1; ++u) none[u] = from.load(a, block[u], first + 128 * u);
-    const bool wide = rows.template load_q<VEC>(qrow, a.hd, a.scale_log2, quarter);
+    const bool wide = a.wide ? rows.template load_q<true>(qrow, a.hd, a.scale_log2, quarter)
+                             : rows.template load_q<false>(qrow, a.hd, a.scale_log2, quarter);
     // (left from its middle: a way back to its top with loads unused would make every turn wait for them)
 #pragma unroll 1
     for (int k0 = first;; k0 += 128 * U) {
@@ -507,35 +526,10 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
 #pragma unroll
     for (int d = 0; d < NDB; ++d) lds[wave][row * ROW + NDB * (4 * quarter + c) + d] = rows.o[d][c] * w;
   __syncthreads();
-  for (int t = threadIdx.x; t < min(nr - r0, ROWS) * HD; t += PT_THREADS) {
-    const int r = t / HD, d = t % HD;
-    if (d >= a.hd) continue;
-    float x = 0.f, L = 0.f;
-    const float M = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r]));
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      x += lds[v][r * ROW + d];
-      L += red_l[v][r] * fast_exp2(red_m[v][r] - M);
-    }
-    const int i = a.by_group.div(r0 + r), h = hk * a.group + r0 + r - i * a.group;
-    if (single) {
-      a.o[(size_t)(s.first + i) * a.ldo + (size_t)h * a.hd + d] = L == 0.f ? 0.f : x / L;
-    } else {
-      float *part;
-      if constexpr (SHARED)
-        part = a.part + (((size_t)(s.first + i) * a.heads + h) * a.part_splits + a.first_split + split) * (a.hd + 2);
-      else
-        part = a.few_part + ((((size_t)b * a.kv_heads + hk) * a.few_rows + r0 + r) * a.few_splits + split) * (a.hd + 2);
-      part[d] = x;
-      if (d == 0) {
-        part[a.hd] = M;
-        part[a.hd + 1] = L;
-      }
-    }
-  }
+  write_rows<HD, ROWS, ROW, SHARED>(a, s, b, hk, r0, nr, split, single, lds[0], ROWS * ROW, red_m, red_l);
 }
 
-template <typename T, int HD, int RUN, bool VEC, bool PACK, bool SHARED>
+template <typename T, int HD, int RUN, bool PACK, bool SHARED>
 __global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kernel(const PagedArgs a) {
   constexpr int ROWS = CodeRows<T, HD, PACK>::ROWS;
   __shared__ __attribute__((aligned(16))) float lds[4][ROWS * (HD + 4)];
@@ -549,42 +543,47 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kern
   if constexpr (SHARED) {
     // (a group of more rows than the launch was told of takes its time)
     for (; r0 < nr; r0 += gridDim.y / a.kv_heads * ROWS) {
-      code_rows<T, HD, RUN, VEC, PACK, true>(a, s, b, r0, nr, lds, red_m, red_l, scales);
+      code_rows<T, HD, RUN, PACK, true>(a, s, b, r0, nr, lds, red_m, red_l, scales);
       __syncthreads();
     }
   } else {
-    code_rows<T, HD, RUN, VEC, PACK, false>(a, s, b, r0, nr, lds, red_m, red_l, scales);
+    code_rows<T, HD, RUN, PACK, false>(a, s, b, r0, nr, lds, red_m, red_l, scales);
   }
 }
 
-template <typename T, int HD, bool VEC, bool PACK, bool SHARED>
+template <typename T, int HD, bool PACK, bool SHARED>
 void launch_code(const PagedArgs &a, hipStream_t st) {
   constexpr int ROWS = CodeRows<T, HD, PACK>::ROWS;
   const int row_groups = SHARED && a.prefix ? 1 : (a.few_rows + ROWS - 1) / ROWS;
   const dim3 grid(a.few_splits, a.kv_heads * row_groups, SHARED && a.prefix ? a.groups : a.batch);
-  if (a.page_shift >= 4) paged_code_kernel<T, HD, 16, VEC, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
-  else if (a.page_shift == 3) paged_code_kernel<T, HD, 8, VEC, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
-  else paged_code_kernel<T, HD, 1, VEC, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  if (a.page_shift >= 4) paged_code_kernel<T, HD, 16, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  else if (a.page_shift == 3) paged_code_kernel<T, HD, 8, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  else paged_code_kernel<T, HD, 1, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
 }
 
 template <typename T, int HD, bool SHARED>
-void launch_code(const PagedArgs &a, bool wide, hipStream_t st) {
-  const bool pack = a.most_rows <= 4;
-  if (wide && pack) launch_code<T, HD, true, true, SHARED>(a, st);
-  else if (wide) launch_code<T, HD, true, false, SHARED>(a, st);
-  else if (pack) launch_code<T, HD, false, true, SHARED>(a, st);
-  else launch_code<T, HD, false, false, SHARED>(a, st);
+void launch_code(const PagedArgs &a, hipStream_t st) {
+  if (a.most_rows <= 4) launch_code<T, HD, true, SHARED>(a, st);
+  else if constexpr (kQ8<T>) launch_code<T, HD, false, SHARED>(a, st);
+}
+
+// Requests of few rows
+template <typename T, bool SHARED>
+int launch_codes(const PagedArgs &a, hipStream_t st) {
+  if (a.hd <= 32) launch_code<T, 32, SHARED>(a, st);
+  else if (a.hd <= 64) launch_code<T, 64, SHARED>(a, st);
+  else if (SHARED || a.hd <= 128) launch_code<T, 128, SHARED>(a, st);
+  else if constexpr (!SHARED) launch_code<T, 256, SHARED>(a, st);
+  return check_launch("paged_code_kernel");
 }
 
 // wide: head dims that are multiples of 8, and 16-byte aligned rows of Q and O.
 template <typename T, bool SHARED>
-int paged_attn_q8(const PagedArgs &a, const PagedKernels &k, bool wide, hipStream_t st) {
+int paged_attn_q8(const PagedArgs &args, const PagedKernels &k, bool wide, hipStream_t st) {
+  PagedArgs a = args;
+  a.wide = wide;
   if (k.span) {
-    if (a.hd <= 32) launch_code<T, 32, SHARED>(a, wide, st);
-    else if (a.hd <= 64) launch_code<T, 64, SHARED>(a, wide, st);
-    else if (SHARED || a.hd <= 128) launch_code<T, 128, SHARED>(a, wide, st);
-    else if constexpr (!SHARED) launch_code<T, 256, SHARED>(a, wide, st);
-    const int rc = check_launch("paged_code_kernel");
+    const int rc = launch_codes<T, SHARED>(a, st);
     if (rc) return rc;
   }
   return k.tile ? launch_tiles<T, SHARED>(a, wide, st) : CDML_OK;

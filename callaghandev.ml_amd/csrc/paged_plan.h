@@ -15,30 +15,34 @@ int paged_attention(const char *what, bool q8, bool cut, const float *q, int ldq
 
 namespace {
 
-// o = sum_s w_s o_s / sum_s w_s l_s with w_s = 2^(m_s - M) over n chunks, one wave; the
-// chunks' statistics lie one to a lane, 64 chunks at a time.
+// Chunks' sums: n of them, `stride` floats apart, each of a maximum (log2) and a sum in stats,
+// `stats_stride` apart.
+struct Chunks {
+  const float *o, *stats;
+  int n, stride, stats_stride;
+};
 struct Join {
   float M, L, acc[4];
 };
-__device__ __forceinline__ float join_most(const PagedArgs &a, const float *part, int n, float M) {
-  for (int c = threadIdx.x & 63; c < n; c += 64) M = fmaxf(M, part[(size_t)c * (a.hd + 2) + a.hd]);
+__device__ __forceinline__ float join_most(const Chunks &p, float M) {
+  for (int c = threadIdx.x & 63; c < p.n; c += 64) M = fmaxf(M, p.stats[(size_t)c * p.stats_stride]);
   return M;
 }
-__device__ __forceinline__ void join_add(const PagedArgs &a, const float *part, int n, Join &t) {
-  const int lane = threadIdx.x & 63, stride = a.hd + 2;
-  for (int c0 = 0; c0 < n; c0 += 64) {
-    const float *p = part + (size_t)c0 * stride;
-    const int m = min(n - c0, 64);
-    const float w = lane < m ? fast_exp2(p[(size_t)lane * stride + a.hd] - t.M) : 0.f;
-    t.L += lane < m ? p[(size_t)lane * stride + a.hd + 1] * w : 0.f;
+__device__ __forceinline__ void join_add(int hd, const Chunks &part, Join &t) {
+  const int lane = threadIdx.x & 63;
+  for (int c0 = 0; c0 < part.n; c0 += 64) {
+    const float *p = part.o + (size_t)c0 * part.stride, *st = part.stats + (size_t)c0 * part.stats_stride;
+    const int m = min(part.n - c0, 64);
+    const float w = lane < m ? fast_exp2(st[(size_t)lane * part.stats_stride] - t.M) : 0.f;
+    t.L += lane < m ? st[(size_t)lane * part.stats_stride + 1] * w : 0.f;
     constexpr int U = 8;  // chunks in flight; past the last one it is read again and left out
     for (int c = 0; c < m; c += U) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (lane + 64 * j >= a.hd) continue;
+        if (lane + 64 * j >= hd) continue;
         float x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = p[(size_t)min(c + u, m - 1) * stride + lane + 64 * j];
+        for (int u = 0; u < U; ++u) x[u] = p[(size_t)min(c + u, m - 1) * part.stride + lane + 64 * j];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const float wc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), min(c + u, m - 1)));
@@ -48,27 +52,22 @@ __device__ __forceinline__ void join_add(const PagedArgs &a, const float *part, 
     }
   }
 }
-__device__ __forceinline__ void join_end(const PagedArgs &a, Join &t, float *o) {
+// o = sum_s w_s o_s / sum_s w_s l_s with w_s = 2^(m_s - M) over the chunks of N places, one wave;
+// the chunks' statistics lie one to a lane, 64 chunks at a time.
+template <int N>
+__device__ __forceinline__ void join_chunks(int hd, const Chunks (&part)[N], float *o) {
   const int lane = threadIdx.x & 63;
+  Join t{};
+  t.M = kNoKey;
+#pragma unroll
+  for (int i = 0; i < N; ++i) t.M = join_most(part[i], t.M);
+  t.M = wave_max(t.M);
+#pragma unroll
+  for (int i = 0; i < N; ++i) join_add(hd, part[i], t);
   t.L = wave_sum(t.L);
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    if (lane + 64 * j < a.hd) o[lane + 64 * j] = t.L == 0.f ? 0.f : t.acc[j] / t.L;
-}
-__device__ __forceinline__ void join_chunks(const PagedArgs &a, const float *part, int n, float *o) {
-  Join t{};
-  t.M = wave_max(join_most(a, part, n, kNoKey));
-  join_add(a, part, n, t);
-  join_end(a, t, o);
-}
-// The same over the chunks of two places
-__device__ __forceinline__ void join_two(const PagedArgs &a, const float *part, int n, const float *part2, int n2,
-                                         float *o) {
-  Join t{};
-  t.M = wave_max(join_most(a, part2, n2, join_most(a, part, n, kNoKey)));
-  join_add(a, part, n, t);
-  join_add(a, part2, n2, t);
-  join_end(a, t, o);
+    if (lane + 64 * j < hd) o[lane + 64 * j] = t.L == 0.f ? 0.f : t.acc[j] / t.L;
 }
 
 // The request that row `row` is of (a wave's question), batch if of none: requests that end at
@@ -84,8 +83,6 @@ __device__ __forceinline__ int request_of_row(const PagedArgs &a, int row) {
   }
   return b;
 }
-
-__device__ __forceinline__ int chunks_seen(int seen, int chunk) { return seen <= 0 ? 0 : (seen - 1) / chunk + 1; }
 
 // Which kernels run and how keys are split, from the sizes alone.
 struct Plan {
@@ -135,7 +132,9 @@ inline Plan make_plan(int size, int rows, int batch, int max_new, int max_len, i
   p.few_rows = most < 1 ? 1 : k.tile ? kSpanRows : most;
   const long long pairs = (long long)(batch < 1 ? 1 : batch) * kv_heads;
   const long long groups = k.rows ? (p.few_rows + kVecRows - 1) / kVecRows : (p.few_rows + kSpanRows - 1) / kSpanRows;
-  if (k.span) {
+  if (k.span && shared && len <= 1024) {
+    p.few_chunk = round_up(len, 128);  // one chunk, which adds what the group shares
+  } else if (k.span) {
     // a whole request to a workgroup where these fill the CUs (16 x 16 pairs of 4096 bf16 keys:
     // 48.5 us, 55.3 in two chunks, 96 in chunks of 512), else two workgroups for every CU
     const long long many = pairs * groups;

@@ -19,15 +19,17 @@ struct FindArgs {
 
 __device__ __forceinline__ int clamped(int x, int most) { return min(max(x, 0), most); }
 
-// One workgroup a group: the least number of full old pages of a member, then the first
-// column, of every member's row at once, in which a page differs from the first member's.  The
-// last workgroup clears the requests of no group.
+// One workgroup a group: the least number of full old pages of a member, and the first column
+// of the tables in which a member's page differs from the first member's.  A wave takes every
+// sixteenth member, a lane every 64th column; the first 512 columns are read before it is known
+// how many count, so that both answers come in one wait.  The last workgroup clears the
+// requests of no group.
 __global__ void __launch_bounds__(kFindThreads) paged_shared_kernel(const FindArgs a) {
   __shared__ int least;
-  const int g = blockIdx.x, t = threadIdx.x;
+  const int g = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   if (g == a.groups) {
     const int from = a.groups ? clamped(a.group_start[0], a.batch) : a.batch;
-    const int behind = a.groups ? clamped(a.group_start[a.groups], a.batch) : a.batch;
+    const int behind = a.groups ? clamped(a.group_start[a.groups], a.batch) : 0;
     for (int b = t; b < a.batch; b += kFindThreads)
       if (b < from || b >= behind) a.shared[b] = 0;
     return;
@@ -38,73 +40,77 @@ __global__ void __launch_bounds__(kFindThreads) paged_shared_kernel(const FindAr
     if (members == 1 && t == 0) a.shared[first] = 0;
     return;
   }
+  const int *lead = a.table + (size_t)first * a.max_blocks;
+  constexpr int WAVES = kFindThreads / 64, K = 8, U = 4;  // columns of a lane, members of a wave at a time
+  // the first of columns [c0, c0 + 512) below `columns` that differs, of this lane's
+  auto compare = [&](int c0, int columns) {
+    int x[K], differs = INT_MAX;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = c0 + 64 * k + lane;
+      x[k] = c < columns ? lead[c] : 0;
+    }
+    for (int m = wave; m < members; m += WAVES * U) {
+      int y[U][K];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int *row = lead + (size_t)min(m + WAVES * u, members - 1) * a.max_blocks;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const int c = c0 + 64 * k + lane;
+          y[u][k] = c < columns ? row[c] : 0;
+        }
+      }
+#pragma unroll
+      for (int k = K - 1; k >= 0; --k) {
+        bool same = (unsigned)x[k] < (unsigned)a.n_pages;
+#pragma unroll
+        for (int u = 0; u < U; ++u) same &= x[k] == y[u][k];
+        const int c = c0 + 64 * k + lane;
+        if (!same && c < columns) differs = min(differs, c);
+      }
+    }
+    return differs;
+  };
   if (t == 0) least = a.max_blocks;
-  __syncthreads();
   int pages = a.max_blocks;
   for (int b = first + t; b < first + members; b += kFindThreads) {
     const long long old = (long long)a.kv_len[b] - max(a.cu[b + 1] - a.cu[b], 0);
-    pages = min(pages, (int)(max(old, 0LL) >> a.page_shift));
+    pages = min(pages, (int)min(max(old, 0LL) >> a.page_shift, (long long)a.max_blocks));
   }
-  pages = wave_min(pages);
-  if ((t & 63) == 0) atomicMin(&least, pages);
+  pages = wave_min(min(pages, compare(0, a.max_blocks)));
   __syncthreads();
-  pages = least;
-  const int *lead = a.table + (size_t)first * a.max_blocks;
-  int differs = pages;
-  constexpr int U = 8;  // loads of a thread in flight
-  const long long total = (long long)members * pages;
-  // (entry i: column i % pages of member i / pages; the first member's own pages are checked, too)
-  int m = pages ? t / pages : 0, c = pages ? t - m * pages : 0;
-  const int dm = pages ? kFindThreads / pages : 0, dc = pages ? kFindThreads - dm * pages : 0;
-  for (long long i = t; i < total;) {
-    int x[U], y[U], col[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = i + (long long)u * kFindThreads < total;
-      col[u] = in ? c : 0;
-      x[u] = lead[col[u]];
-      y[u] = in ? lead[(size_t)m * a.max_blocks + c] : x[u];
-      m += dm;
-      c += dc;
-      if (c >= pages) {
-        c -= pages;
-        ++m;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (x[u] != y[u] || (unsigned)x[u] >= (unsigned)a.n_pages) differs = min(differs, col[u]);
-    i += (long long)U * kFindThreads;
+  if (lane == 0) atomicMin(&least, pages);
+  __syncthreads();
+  for (int c0 = 64 * K; c0 < least; c0 += 64 * K) {
+    const int differs = wave_min(compare(c0, least));
+    __syncthreads();
+    if (lane == 0) atomicMin(&least, differs);
+    __syncthreads();
   }
-  differs = wave_min(differs);
-  if ((t & 63) == 0) atomicMin(&least, differs);
-  __syncthreads();
   const int tokens = least << a.page_shift;  // (at most a table's tokens)
   for (int b = first + t; b < first + members; b += kFindThreads) a.shared[b] = tokens;
 }
 
-// How a row's chunks lie in its parts, and where its request's own tokens are cut.
-struct JoinArgs {
-  int prefix_chunk, prefix_splits;  // (of `part_splits`, the first)
-  int few_rows, few_chunk, few_splits, tile_chunk, tile_splits;
-};
-
-// A wave per (row, head).
-__global__ void __launch_bounds__(256) paged_shared_join_kernel(const PagedArgs a, const JoinArgs j) {
+// A wave per (row, head); not for rows that the fused kernel wrote.
+__global__ void __launch_bounds__(256) paged_shared_join_kernel(const PagedArgs a) {
   const int row = blockIdx.x, h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (h >= a.heads) return;
   const int b = request_of_row(a, row);
   if (b >= a.batch) return;
   const PagedSeq s = paged_seq<true>(a, b);
   const int i = row - s.first;
-  if (i < 0 || i >= s.n) return;
-  const bool few = s.n * a.group <= j.few_rows;
-  const int before = min(chunks_seen(s.start, j.prefix_chunk), j.prefix_splits);
-  const int behind = min(chunks_seen(s.len - s.n + i + 1 - s.start, few ? j.few_chunk : j.tile_chunk),
-                         few ? j.few_splits : j.tile_splits);
-  const float *part = a.part + ((size_t)row * a.heads + h) * a.part_splits * (a.hd + 2);
-  join_two(a, part, before, part + (size_t)j.prefix_splits * (a.hd + 2), behind,
-           a.o + (size_t)row * a.ldo + (size_t)h * a.hd);
+  const bool few = s.n * a.group <= a.few_rows;
+  if (i < 0 || i >= s.n || (few && a.fused)) return;
+  const size_t at = ((size_t)row * a.heads + h) * a.part_splits, own = at + a.prefix_splits;
+  const Chunks chunks[2] = {
+      {a.part + at * a.part_width, a.part_stats + at * 2,
+       min(chunks_seen(s.start, a.prefix_chunk), a.prefix_splits), a.part_width, 2},
+      {a.part + own * a.part_width, a.part_stats + own * 2,
+       min(chunks_seen(s.len - s.n + i + 1 - s.start, few ? a.few_chunk : a.tile_chunk),
+           few ? a.few_splits : a.tile_splits),
+       a.part_width, 2}};
+  join_chunks(a.hd, chunks, a.o + (size_t)row * a.ldo + (size_t)h * a.hd);
 }
 
 struct SharedPlan {
@@ -114,7 +120,8 @@ struct SharedPlan {
   int prefix_chunk, prefix_splits;
   Plan own;
   int own_splits;
-  size_t floats;
+  bool fused;          // of the requests of few rows
+  size_t parts, floats;
 };
 
 SharedPlan plan_shared(int size, int rows, int batch, int groups, int max_members, int max_new, int max_prefix,
@@ -138,7 +145,9 @@ SharedPlan plan_shared(int size, int rows, int batch, int groups, int max_member
   p.prefix_splits = (max_prefix - 1) / p.prefix_chunk + 1;
   p.own = make_plan(size, rows, batch, max_new, max_tail, heads, kv_heads, hd, true);
   p.own_splits = std::max(p.own.kernels.span ? p.own.few_splits : 1, p.own.kernels.tile ? p.own.tile_splits : 1);
-  p.floats = (size_t)rows * heads * (p.prefix_splits + p.own_splits) * (hd + 2);
+  p.fused = p.own.kernels.span && p.own.few_splits == 1;
+  p.parts = (size_t)rows * heads * (p.prefix_splits + p.own_splits);
+  p.floats = p.parts * (round_up(hd, 4) + 2);
   return p;
 }
 
@@ -279,7 +288,12 @@ extern "C" int cdml_paged_attn_shared(const float *q, int ldq, const void *kcach
   a.shared = shared;
   a.groups = groups;
   a.part = static_cast<float *>(workspace);
+  a.part_width = round_up(head_dim, 4);
+  a.part_stats = a.part + p.parts * a.part_width;
   a.part_splits = p.prefix_splits + p.own_splits;
+  a.prefix_chunk = p.prefix_chunk;
+  a.prefix_splits = p.prefix_splits;
+  a.fused = p.fused;
   const bool wide = head_dim % 8 == 0 && ldq % 4 == 0 && ldo % 4 == 0 && aligned16(q) && aligned16(o) &&
                     aligned16(kcache) && aligned16(vcache);
   const hipStream_t st = as_hip(stream);
@@ -310,8 +324,7 @@ extern "C" int cdml_paged_attn_shared(const float *q, int ldq, const void *kcach
   a.first_split = p.prefix_splits;
   rc = run(p.own.kernels);
   if (rc) return rc;
-  const JoinArgs j{p.prefix_chunk,  p.prefix_splits, p.own.few_rows,   p.own.few_chunk,
-                   p.own.few_splits, p.own.tile_chunk, p.own.tile_splits};
-  paged_shared_join_kernel<<<dim3((unsigned)rows, (unsigned)(num_heads + 3) / 4), 256, 0, st>>>(a, j);
+  if (p.fused && !p.own.kernels.tile) return CDML_OK;
+  paged_shared_join_kernel<<<dim3((unsigned)rows, (unsigned)(num_heads + 3) / 4), 256, 0, st>>>(a);
   return check_launch("paged_shared_join_kernel");
 }
