@@ -99,6 +99,14 @@ struct PagedArgs {
   int part_splits, part_width, first_split, prefix_chunk, prefix_splits;
 };
 
+// The kernel's arguments, read again: what a kernel's end needs is not held in scalar registers
+// throughout (a kernel whose one argument is a PagedArgs).
+__device__ __forceinline__ const PagedArgs &args_again() {
+  auto p = (const __attribute__((address_space(4))) PagedArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const PagedArgs *)p;
+}
+
 // Chunks in which `seen` tokens lie.
 __device__ __forceinline__ int chunks_seen(int seen, int chunk) { return seen <= 0 ? 0 : (seen - 1) / chunk + 1; }
 

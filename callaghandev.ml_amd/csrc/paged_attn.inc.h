@@ -1420,19 +1420,31 @@ __device__ __forceinline__ void write_rows(const PagedArgs &a, const PagedSeq &s
         }
         continue;
       }
-      // what the group shares
+      // what the group shares, several chunks on the way; past the last one it is read again and left out
       const float *stats = a.part_stats + at * 2, *part = a.part + at * a.part_width + d;
-      float top = M;
-#pragma unroll 4
-      for (int c = 0; c < before; ++c) top = fmaxf(top, stats[2 * c]);
-      const float w = fast_exp2(M - top);
-      x *= w;
-      L *= w;
-#pragma unroll 4
-      for (int c = 0; c < before; ++c) {
-        const float wc = fast_exp2(stats[2 * c] - top);
-        x = fmaf(part[(size_t)c * a.part_width], wc, x);
-        L = fmaf(stats[2 * c + 1], wc, L);
+      constexpr int U = 8;
+      for (int c0 = 0; c0 < before; c0 += U) {
+        typedef float vf2 __attribute__((ext_vector_type(2)));
+        vf2 st[U];
+        float y[U], top = M;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int c = min(c0 + u, before - 1);
+          st[u] = *reinterpret_cast<const vf2 *>(stats + 2 * c);
+          y[u] = part[(size_t)c * a.part_width];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) top = fmaxf(top, st[u][0]);
+        const float w = fast_exp2(M - top);
+        x *= w;
+        L *= w;
+        M = top;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float wc = c0 + u < before ? fast_exp2(st[u][0] - M) : 0.f;
+          x = fmaf(y[u], wc, x);
+          L = fmaf(st[u][1], wc, L);
+        }
       }
     }
     if (single) {
@@ -1537,7 +1549,9 @@ __global__ void __launch_bounds__(PT_THREADS, sizeof(T) == 2 || HD <= 64 ? 2 : 1
   if constexpr (SHARED) {
     // (a group of more rows than the launch was told of takes its time)
     for (int r0 = blockIdx.y / a.kv_heads * 16; r0 < nr; r0 += gridDim.y / a.kv_heads * 16) {
-      span_rows<T, HD, VEC, true>(a, s, b, r0, nr, lds, red_m, red_l);
+      // (arguments read in every turn: held across turns, they would fill the registers)
+      const PagedArgs &z = args_again();
+      span_rows<T, HD, VEC, true>(z, paged_seq<true>(z, b), b, r0, nr, lds, red_m, red_l);
       __syncthreads();
     }
   } else {

@@ -10,8 +10,10 @@ namespace {
 
 // How a head's rows go through the lanes of a wave (row = lane % 16, quarter = lane / 16), 32
 // keys at a time, straight from the cache into the operands of the 16x16x32 MFMA:
-//   K: lane (row, quarter) has dims KD * quarter .. + KD - 1 of keys row and 16 + row.  A dot
-//      product's order is free, so product s takes the lane's s-th eight dims, of Q too.
+//   K: lane (row, quarter) has 16 bytes of every 64 of keys row and 16 + row, the quarters side by
+//      side.  A dot product's order is free, so product s takes the lane's s-th eight dims, of
+//      Q too.  (A quarter of a row to a lane, whose loads touch four times the segments:
+//      64 requests behind 8192 bf16 tokens OLDUS -> NEWUS us.)
 //   V: lane (row, quarter) has dims VD * row .. + VD - 1 of the keys 4 quarter + 0..3 and
 //      16 + 4 quarter + 0..3, those whose probabilities it holds; product d takes its d-th
 //      dim, so V is transposed as the codes of two keys become a pair of bf16.
@@ -24,6 +26,12 @@ struct CodeBlock {
   float scale;  // of key lane % 32: K's in the lower lanes, V's in the upper
 
   static constexpr int KL = KW >= 4 ? KW / 4 : 1;  // loads of K's row, 16 bytes each where it has as many
+  // The dims of load i, and of product s, of a quarter
+  static __device__ __forceinline__ constexpr int k_dim(int i, int quarter) { return KD / KL * (4 * i + quarter); }
+  static __device__ __forceinline__ constexpr int q_dim(int s, int quarter) {
+    constexpr int PER = KD / KL / 8;  // products of a load
+    return k_dim(s / PER, quarter) + s % PER * 8;
+  }
 
   // off stays a 32-bit register beside the base, for a load's own addition (the compiler would
   // widen it ahead of the loop, and add in vector instructions)
@@ -91,7 +99,7 @@ struct CodeLoader {
   Table table;
   const T *kc, *vc;          // the head's
   const float *side;         // 8 bits: the scales of this lane, K's or V's
-  uint32_t k_off[Block::KL], v_off;  // of the lane's dims, in elements; RUN > 1: and of its row in a run
+  uint32_t k_off[Block::KL], v_off[RUN == 1 ? 1 : 4];  // of the lane's dims, in elements; RUN > 1: and of its rows in a run
   int row, quarter, width, last;
   int page[NP];              // of the next block to be loaded
   int lane_page[RUN == 1 ? 11 : 1];  // RUN 1: of K's rows, V's, and the scale's
@@ -111,10 +119,12 @@ struct CodeLoader {
     // not stored.  (A head's rows are multiples of 16 bytes, so a load lies in one or past it.)
 #pragma unroll
     for (int i = 0; i < Block::KL; ++i) {
-      const int d = Block::KD * quarter + 16 / Block::B * i;
+      const int d = Block::k_dim(i, quarter);
       k_off[i] = (RUN == 1 ? 0 : row % RUN * width) + (d < dims ? d : 0);
     }
-    v_off = (RUN == 1 ? 0 : 4 * quarter % RUN * width) + (Block::VD * row < dims ? Block::VD * row : 0);
+#pragma unroll
+    for (int e = 0; e < (RUN == 1 ? 1 : 4); ++e)
+      v_off[e] = (RUN == 1 ? 0 : (4 * quarter % RUN + e) * width) + (Block::VD * row < dims ? Block::VD * row : 0);
   }
   // Keys of the lane: of K, half h; of V, place e; of the scale
   __device__ __forceinline__ int k_key(int k0, int h) const { return k0 + 16 * h + row; }
@@ -167,7 +177,7 @@ struct CodeLoader {
       for (int h = 0; h < 2; ++h) {
         const size_t run = PER == 1 ? at[h] : quarter & 2 ? at[PER * h + PER - 1] : at[PER * h];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) Block::v_words(b.v[4 * h + e], vc + element(run) + e * width, v_off);
+        for (int e = 0; e < 4; ++e) Block::v_words(b.v[4 * h + e], vc + element(run), v_off[e]);
       }
     } else {
       auto place = [&](int i, int key) {
@@ -179,7 +189,7 @@ struct CodeLoader {
 #pragma unroll
       for (int h = 0; h < 2; ++h) Block::k_words(b.k[h], kc + element(place(h, k_key(k0, h))), k_off);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) Block::v_words(b.v[e], vc + element(place(2 + e, v_key(k0, e))), v_off);
+      for (int e = 0; e < 8; ++e) Block::v_words(b.v[e], vc + element(place(2 + e, v_key(k0, e))), v_off[0]);
       lookup(a, k0 + 128);
     }
     return none;
@@ -244,29 +254,64 @@ struct CodeRows {
     cut[0] = piece == 0 ? 0u : piece == 3 ? ~0u : 0xffff0000u;
     cut[1] = piece < 2 ? 0u : piece == 3 ? ~0u : 0xffff0000u;
   }
-  // Whether Q is out of the pieces' range (wave-uniform)
+  // Four values of a row from dim d on, zeros past the head dim
+  template <bool VEC>
+  static __device__ __forceinline__ vf4 q_values(const float *qrow, int d, int hd) {
+    vf4 x;
+    if constexpr (VEC) {
+      x = *reinterpret_cast<const vf4 *>(qrow + min(d, hd - 4));
+      if (d >= hd) x = vf4{};
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float t = qrow[min(d + c, hd - 1)];
+        x[c] = d + c < hd ? t : 0.f;
+      }
+    }
+    return x;
+  }
+  // Q's pieces; whether Q is out of their range (wave-uniform, as in load_q_pieces).  PACK: a
+  // value's top sixteen bits are its piece, what is left of it the next one's value.
   template <bool VEC>
   __device__ __forceinline__ bool load_q(const float *qrow, int hd, float scale, int quarter) {
-    bf16x8 all[NS][3];
-    const bool wide = load_q_pieces<NS, VEC>(all, qrow, hd, scale, 8, HD / 4 * quarter);
-    const int piece = threadIdx.x >> 2 & 3;
+    vf4 x[NS][2];
 #pragma unroll
     for (int i = 0; i < NS; ++i)
-      if constexpr (PACK) {
-        vu4 w;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[3];
+      for (int h = 0; h < 2; ++h) x[i][h] = q_values<VEC>(qrow, Block::q_dim(i, quarter) + 4 * h, hd);
+    uint32_t most = 0, least = ~0u;  // of 2 |x|, and of 2 |x| - 1 as integers, which leaves zeros out
 #pragma unroll
-          for (int j = 0; j < 3; ++j) x[j] = __builtin_bit_cast(vu4, all[i][j])[c];
-          w[c] = piece == 0 ? x[0] : piece == 1 ? x[1] : piece == 2 ? x[2] : 0u;
-        }
-        q[i][0] = __builtin_bit_cast(bf16x8, w);
-      } else {
+    for (int i = 0; i < NS; ++i) {
+      float y[8];
 #pragma unroll
-        for (int j = 0; j < 3; ++j) q[i][j] = all[i][2 - j];  // the corrections first
+      for (int e = 0; e < 8; ++e) {
+        y[e] = x[i][e / 4][e % 4] * scale;
+        const uint32_t twice = __float_as_uint(y[e]) << 1;
+        most = max(most, twice);
+        least = min(least, twice - 1u);
       }
-    return wide;
+      if constexpr (PACK) {
+        q[i][0] = piece_of(y);
+      } else {
+        bf16x8 all[3];
+        split_operand(y, 1.f, all);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) q[i][j] = all[2 - j];  // the corrections first
+      }
+    }
+    return __builtin_amdgcn_ballot_w64(most >= (100u + 127u) << 24 || least < (17u << 24) - 1u) != 0;
+  }
+  // PACK: this lane's piece of eight values
+  __device__ __forceinline__ bf16x8 piece_of(float (&x)[8]) const {
+    vu4 w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) x[e] -= __uint_as_float(__float_as_uint(x[e]) & cut[c]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1]), __float_as_uint(x[2 * i]), 0x07060302u);
+    return __builtin_bit_cast(bf16x8, w);
   }
   // Probabilities of the keys up to last_vis (counted from the quarter's first) in place of
   // the scores; o and l follow a reference that rises.
@@ -353,16 +398,7 @@ struct CodeRows {
     }
     bf16x8 pp[3];
     if constexpr (PACK) {
-      // a value's top sixteen bits are its piece, what is left of it the next one's value
-      vu4 w;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) p[e] -= __uint_as_float(__float_as_uint(p[e]) & cut[c]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = __builtin_amdgcn_perm(__float_as_uint(p[2 * i + 1]), __float_as_uint(p[2 * i]), 0x07060302u);
-      pp[0] = __builtin_bit_cast(bf16x8, w);
+      pp[0] = piece_of(p);
     } else {
       split_operand(p, 1.f, pp);
     }
@@ -384,17 +420,15 @@ struct CodeRows {
     }
     return any_nonfinite(wrong);
   }
-  // PACK: the pieces' sums of O (after recompute: those of the first lanes)
+  // PACK: the pieces' sums of O (recompute's are whole in every lane)
   __device__ __forceinline__ void join_pieces(bool recomputed) {
-    if constexpr (PACK) {
-      const bool mine = !recomputed || (threadIdx.x & 12) == 0;
+    if (PACK && !recomputed) {
 #pragma unroll
       for (int d = 0; d < NDB; ++d)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float x = mine ? o[d][c] : 0.f;
-          x += turned<8>(x);
-          o[d][c] = x + turned<4>(x);
+          o[d][c] += turned<8>(o[d][c]);
+          o[d][c] += turned<4>(o[d][c]);
         }
     }
   }
@@ -507,9 +541,13 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
       }
     }
   summed:
-    if (bad && a.bad) *a.bad = 1;
+    const PagedArgs &z = args_again();
+    if (bad && z.bad) *z.bad = 1;
     const bool again = rows.finish() || wide;
-    if (again) rows.recompute(a, qrow, a.table + (size_t)s.table * a.max_blocks, hk, quarter, first, c1, lim, last);
+    if (again) {
+      const float *row = z.q + (size_t)(s.first + tok) * z.ldq + (size_t)head * z.hd;
+      rows.recompute(z, row, z.table + (size_t)s.table * z.max_blocks, hk, quarter, first, c1, lim, last);
+    }
     rows.join_pieces(again);
   }
   // the waves' sums: rows' statistics, then each wave's O scaled to the common maximum
@@ -526,7 +564,7 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
 #pragma unroll
     for (int d = 0; d < NDB; ++d) lds[wave][row * ROW + NDB * (4 * quarter + c) + d] = rows.o[d][c] * w;
   __syncthreads();
-  write_rows<HD, ROWS, ROW, SHARED>(a, s, b, hk, r0, nr, split, single, lds[0], ROWS * ROW, red_m, red_l);
+  write_rows<HD, ROWS, ROW, SHARED>(args_again(), s, b, hk, r0, nr, split, single, lds[0], ROWS * ROW, red_m, red_l);
 }
 
 template <typename T, int HD, int RUN, bool PACK, bool SHARED>
@@ -543,7 +581,9 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kern
   if constexpr (SHARED) {
     // (a group of more rows than the launch was told of takes its time)
     for (; r0 < nr; r0 += gridDim.y / a.kv_heads * ROWS) {
-      code_rows<T, HD, RUN, PACK, true>(a, s, b, r0, nr, lds, red_m, red_l, scales);
+      // (arguments read in every turn: held across turns, they would fill the registers)
+      const PagedArgs &z = args_again();
+      code_rows<T, HD, RUN, PACK, true>(z, paged_seq<true>(z, b), b, r0, nr, lds, red_m, red_l, scales);
       __syncthreads();
     }
   } else {
