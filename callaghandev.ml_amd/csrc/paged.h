@@ -83,6 +83,7 @@ struct PagedArgs {
   int few_rows, few_chunk, few_splits, tile_chunk, tile_splits;
   int most_rows;     // of a request of few rows, at most (a hint)
   bool wide;         // 16-byte aligned rows of Q, of whole vectors
+  bool lone_waves;   // SHARED: requests have so few keys that a wave takes all of a K/V head
   float *few_part;   // [batch][kv_heads][few_rows][few_splits][hd + 2]
   float *tile_part;  // [rows][heads][tile_splits][hd + 2]
   UDiv by_group;

@@ -1391,19 +1391,22 @@ struct SpanRows {
   }
 };
 
-// The end of a workgroup of few rows: the four waves' sums, o (a wave's `wave_floats` apart,
-// rows ROW apart) scaled to the waves' common maximum, become o, or a chunk's part, of rows r0 ..
-template <int HD, int ROWS, int ROW, bool SHARED>
+// The end of few rows, of a workgroup or (WAVES 1) a wave: its WAVES waves' sums, o (a wave's
+// `wave_floats` apart, rows ROW apart) scaled to their common maximum, become o, or a chunk's
+// part, of rows r0 ..
+template <int HD, int ROWS, int ROW, bool SHARED, int WAVES = 4>
 __device__ __forceinline__ void write_rows(const PagedArgs &a, const PagedSeq &s, int b, int hk, int r0, int nr,
                                            int split, bool single, const float *o, int wave_floats,
-                                           const float (&red_m)[4][16], const float (&red_l)[4][16]) {
+                                           const float (*red_m)[16], const float (*red_l)[16]) {
   const int before = SHARED && single ? min(chunks_seen(s.start, a.prefix_chunk), a.prefix_splits) : 0;
-  for (int t = threadIdx.x; t < min(nr - r0, ROWS) * HD; t += PT_THREADS) {
+  for (int t = threadIdx.x % (64 * WAVES); t < min(nr - r0, ROWS) * HD; t += 64 * WAVES) {
     const int r = t / HD, d = t % HD;
     if (d >= a.hd) continue;
-    float x = 0.f, L = 0.f, M = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r]));
+    float x = 0.f, L = 0.f, M = red_m[0][r];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
+    for (int v = 1; v < WAVES; ++v) M = fmaxf(M, red_m[v][r]);
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) {
       x += o[v * wave_floats + r * ROW + d];
       L += red_l[v][r] * fast_exp2(red_m[v][r] - M);
     }

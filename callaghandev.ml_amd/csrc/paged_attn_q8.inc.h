@@ -87,11 +87,11 @@ struct CodeBlock {
   }
 };
 
-// Where a wave's blocks of 32 keys, 128 keys apart, lie.  RUN keys, beginning at a multiple of
+// Where a wave's blocks of 32 keys, STRIDE keys apart, lie.  RUN keys, beginning at a multiple of
 // RUN, lie in one page:
 //   RUN 16, 8: a block's pages are looked up by scalar loads, a block ahead of its rows.
 //   RUN 1: every lane looks its rows' pages up (pages of fewer tokens than 8).
-template <typename T, int HD, int RUN>
+template <typename T, int HD, int RUN, int STRIDE>
 struct CodeLoader {
   typedef CodeBlock<T, HD> Block;
   typedef const __attribute__((address_space(4))) int *Table;  // nothing writes it in the meantime
@@ -161,7 +161,7 @@ struct CodeLoader {
         none |= (uint32_t)!s.ok << i;
         at[i] = row_at<T>(a, s.at);
       }
-      lookup(a, k0 + 128);
+      lookup(a, k0 + STRIDE);
       if constexpr (kQ8<T>) {
         const int lane = threadIdx.x & 31;
         size_t mine = lane & 16 ? at[PER] : at[0];
@@ -190,7 +190,7 @@ struct CodeLoader {
       for (int h = 0; h < 2; ++h) Block::k_words(b.k[h], kc + element(place(h, k_key(k0, h))), k_off);
 #pragma unroll
       for (int e = 0; e < 8; ++e) Block::v_words(b.v[e], vc + element(place(2 + e, v_key(k0, e))), v_off[0]);
-      lookup(a, k0 + 128);
+      lookup(a, k0 + STRIDE);
     }
     return none;
   }
@@ -435,7 +435,7 @@ struct CodeRows {
   // The rows over the wave's blocks in fp32, value by value and without the keys that a row
   // does not see: for rows that came out non-finite or whose Q is out of the pieces' range.
   __device__ __forceinline__ void recompute(const PagedArgs &a, const float *qrow, const int *table, int hk, int quarter,
-                                            int first, int c1, int lim, int last) {
+                                            int first, int stride, int c1, int lim, int last) {
     init();
     const T *kc = head_of<T>(a, a.kc, hk), *vc = head_of<T>(a, a.vc, hk);
     auto row_of = [&](int key, size_t &at, const float *scales, float &scale) {
@@ -448,7 +448,7 @@ struct CodeRows {
       return s.ok;
     };
 #pragma unroll 1
-    for (int k0 = first; k0 < c1; k0 += 128) {
+    for (int k0 = first; k0 < c1; k0 += stride) {
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -490,14 +490,15 @@ template <int HD, int RUN>
 constexpr int code_blocks() {
   return 2;
 }
-template <typename T, int HD, int RUN, bool PACK, bool SHARED>
-__device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s, int b, int r0, int nr,
+template <typename T, int HD, int RUN, bool PACK, bool SHARED, int WAVES>
+__device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s, int b, int hk, int r0, int nr,
                                           float (&lds)[4][CodeRows<T, HD, PACK>::ROWS * (HD + 4)], float (&red_m)[4][16], float (&red_l)[4][16],
                                           float (&scales)[4][64]) {
   typedef CodeRows<T, HD, PACK> Rows;
   typedef CodeBlock<T, HD> Block;
   constexpr int NDB = HD / 16, ROW = HD + 4, ROWS = Rows::ROWS;  // floats between rows of the join
-  const int hk = blockIdx.y % a.kv_heads, split = blockIdx.x, base = s.len - s.n;
+  constexpr int STRIDE = 32 * WAVES;
+  const int split = blockIdx.x, base = s.len - s.n;
   const int kend = s.causal ? base + a.by_group.div(min(r0 + ROWS, nr) - 1) + 1 : s.len;  // past the last visible key
   const bool single = SHARED ? a.fused && !a.prefix : s.len <= a.few_chunk;
   const int c0 = split_from<SHARED>(s, split, a.few_chunk);
@@ -514,9 +515,9 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
 
   Rows rows;
   rows.init();
-  const int first = c0 + wave * 32;
+  const int first = c0 + wave % WAVES * 32;
   if (first < c1) {
-    CodeLoader<T, HD, RUN> from;
+    CodeLoader<T, HD, RUN, STRIDE> from;
     from.init(a, s.table, hk, last);
     from.lookup(a, first);
     constexpr int U = code_blocks<HD, RUN>();
@@ -525,17 +526,17 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
     int bad = 0;
     // (past the wave's last block the request's last rows are loaded once more, and left there)
 #pragma unroll
-    for (int u = 0; u < U - 1; ++u) none[u] = from.load(a, block[u], first + 128 * u);
+    for (int u = 0; u < U - 1; ++u) none[u] = from.load(a, block[u], first + STRIDE * u);
     const bool wide = a.wide ? rows.template load_q<true>(qrow, a.hd, a.scale_log2, quarter)
                              : rows.template load_q<false>(qrow, a.hd, a.scale_log2, quarter);
     // (left from its middle: a way back to its top with loads unused would make every turn wait for them)
 #pragma unroll 1
-    for (int k0 = first;; k0 += 128 * U) {
+    for (int k0 = first;; k0 += STRIDE * U) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int k = k0 + 128 * u, ahead = (u + U - 1) % U;
+        const int k = k0 + STRIDE * u, ahead = (u + U - 1) % U;
         if (k >= c1) goto summed;
-        none[ahead] = from.load(a, block[ahead], k + 128 * (U - 1));
+        none[ahead] = from.load(a, block[ahead], k + STRIDE * (U - 1));
         from.clean(block[u], k, none[u], bad);
         rows.add(block[u], scales[wave], quarter, k + 31 > lim_lo, lim - k - 4 * quarter);
       }
@@ -546,28 +547,37 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
     const bool again = rows.finish() || wide;
     if (again) {
       const float *row = z.q + (size_t)(s.first + tok) * z.ldq + (size_t)head * z.hd;
-      rows.recompute(z, row, z.table + (size_t)s.table * z.max_blocks, hk, quarter, first, c1, lim, last);
+      rows.recompute(z, row, z.table + (size_t)s.table * z.max_blocks, hk, quarter, first, STRIDE, c1, lim, last);
     }
     rows.join_pieces(again);
   }
   // the waves' sums: rows' statistics, then each wave's O scaled to the common maximum
   const float m = fmaxf(rows.m, kNoKey), l = quarters(rows.l, [](float x, float y) { return x + y; });
+  auto barrier = [] {
+    if constexpr (WAVES == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    else __syncthreads();
+  };
   if (lane < ROWS) {
     red_m[wave][row] = m;
     red_l[wave][row] = l;
   }
-  __syncthreads();
-  const float w = fast_exp2(m - fmaxf(fmaxf(red_m[0][row], red_m[1][row]), fmaxf(red_m[2][row], red_m[3][row])));
+  barrier();
+  float w = 1.f;
+  if constexpr (WAVES > 1)
+    w = fast_exp2(m - fmaxf(fmaxf(red_m[0][row], red_m[1][row]), fmaxf(red_m[2][row], red_m[3][row])));
   if (!PACK || (lane & 12) == 0)
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int d = 0; d < NDB; ++d) lds[wave][row * ROW + NDB * (4 * quarter + c) + d] = rows.o[d][c] * w;
-  __syncthreads();
-  write_rows<HD, ROWS, ROW, SHARED>(args_again(), s, b, hk, r0, nr, split, single, lds[0], ROWS * ROW, red_m, red_l);
+  barrier();
+  const int v = WAVES == 1 ? wave : 0;
+  write_rows<HD, ROWS, ROW, SHARED, WAVES>(args_again(), s, b, hk, r0, nr, split, single, lds[v], ROWS * ROW, red_m + v,
+                                           red_l + v);
 }
 
-template <typename T, int HD, int RUN, bool PACK, bool SHARED>
+// WAVES 1: a wave to a (request, K/V head), which has few keys.
+template <typename T, int HD, int RUN, bool PACK, bool SHARED, int WAVES>
 __global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kernel(const PagedArgs a) {
   constexpr int ROWS = CodeRows<T, HD, PACK>::ROWS;
   __shared__ __attribute__((aligned(16))) float lds[4][ROWS * (HD + 4)];
@@ -576,35 +586,50 @@ __global__ void __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) paged_code_kern
   const int b = blockIdx.z;
   const PagedSeq s = paged_seq<SHARED>(a, b);
   const int nr = s.n * a.group;
-  int r0 = blockIdx.y / a.kv_heads * ROWS;
+  // K/V head and group of rows
+  int y = blockIdx.y, groups = gridDim.y / a.kv_heads;
+  if constexpr (WAVES == 1) {
+    y = y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    groups = 1;
+    if (y >= a.kv_heads) return;
+  }
+  const int hk = y % a.kv_heads;
+  int r0 = y / a.kv_heads * ROWS;
   if (nr > a.few_rows || r0 >= nr) return;
   if constexpr (SHARED) {
     // (a group of more rows than the launch was told of takes its time)
-    for (; r0 < nr; r0 += gridDim.y / a.kv_heads * ROWS) {
+    for (; r0 < nr; r0 += groups * ROWS) {
       // (arguments read in every turn: held across turns, they would fill the registers)
       const PagedArgs &z = args_again();
-      code_rows<T, HD, RUN, PACK, true>(z, paged_seq<true>(z, b), b, r0, nr, lds, red_m, red_l, scales);
-      __syncthreads();
+      code_rows<T, HD, RUN, PACK, true, WAVES>(z, paged_seq<true>(z, b), b, hk, r0, nr, lds, red_m, red_l, scales);
+      if constexpr (WAVES == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      else __syncthreads();
     }
   } else {
-    code_rows<T, HD, RUN, PACK, false>(a, s, b, r0, nr, lds, red_m, red_l, scales);
+    code_rows<T, HD, RUN, PACK, false, WAVES>(a, s, b, hk, r0, nr, lds, red_m, red_l, scales);
   }
 }
 
-template <typename T, int HD, bool PACK, bool SHARED>
+template <typename T, int HD, bool PACK, bool SHARED, int WAVES>
 void launch_code(const PagedArgs &a, hipStream_t st) {
   constexpr int ROWS = CodeRows<T, HD, PACK>::ROWS;
   const int row_groups = SHARED && a.prefix ? 1 : (a.few_rows + ROWS - 1) / ROWS;
-  const dim3 grid(a.few_splits, a.kv_heads * row_groups, SHARED && a.prefix ? a.groups : a.batch);
-  if (a.page_shift >= 4) paged_code_kernel<T, HD, 16, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
-  else if (a.page_shift == 3) paged_code_kernel<T, HD, 8, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
-  else paged_code_kernel<T, HD, 1, PACK, SHARED><<<grid, PT_THREADS, 0, st>>>(a);
+  const int y = WAVES == 1 ? (a.kv_heads + 3) / 4 : a.kv_heads * row_groups;
+  const dim3 grid(a.few_splits, y, SHARED && a.prefix ? a.groups : a.batch);
+  if (a.page_shift >= 4) paged_code_kernel<T, HD, 16, PACK, SHARED, WAVES><<<grid, PT_THREADS, 0, st>>>(a);
+  else if (a.page_shift == 3) paged_code_kernel<T, HD, 8, PACK, SHARED, WAVES><<<grid, PT_THREADS, 0, st>>>(a);
+  else paged_code_kernel<T, HD, 1, PACK, SHARED, WAVES><<<grid, PT_THREADS, 0, st>>>(a);
 }
 
 template <typename T, int HD, bool SHARED>
 void launch_code(const PagedArgs &a, hipStream_t st) {
-  if (a.most_rows <= 4) launch_code<T, HD, true, SHARED>(a, st);
-  else if constexpr (kQ8<T>) launch_code<T, HD, false, SHARED>(a, st);
+  if (a.most_rows <= 4) {
+    if constexpr (SHARED)
+      if (a.lone_waves) return launch_code<T, HD, true, SHARED, 1>(a, st);
+    launch_code<T, HD, true, SHARED, 4>(a, st);
+  } else if constexpr (kQ8<T>) {
+    launch_code<T, HD, false, SHARED, 4>(a, st);
+  }
 }
 
 // Requests of few rows
