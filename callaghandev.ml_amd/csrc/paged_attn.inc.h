@@ -464,13 +464,13 @@ struct PagedStage {
     last = last_key;
     if constexpr (Q8) scales = (kside ? a.ks : a.vs) + ((size_t)hk << a.page_shift);
   }
-  // 8 bits: the first wave of either half has the tile's scales, a key's to two lanes
+  // 8 bits: the first wave of either half has the tile's scales
   static __device__ __forceinline__ bool has_scales() {
     return (__builtin_amdgcn_readfirstlane(threadIdx.x) & 64) == 0;
   }
-  __device__ __forceinline__ int scale_key(int k0) const { return min(k0 + (int)(threadIdx.x & 31), last); }
+  __device__ __forceinline__ int scale_key(int k0) const { return min(k0 + (int)(threadIdx.x % BN), last); }
   __device__ __forceinline__ void lookup_scale(const PagedArgs &a, int k0) {
-    static_assert(!Q8 || BN == 32, "a key to a lane");
+    static_assert(!Q8 || 64 % BN == 0, "a key to a lane");
     if constexpr (Q8)
       if (has_scales()) scale_page = table[scale_key(k0) >> a.page_shift];
   }
@@ -483,7 +483,7 @@ struct PagedStage {
   }
   __device__ __forceinline__ void store_scale(char *lds) const {
     if constexpr (Q8)
-      if (has_scales()) reinterpret_cast<float *>(lds + SCALES)[(kside ? 0 : BN) + (threadIdx.x & 31)] = scale;
+      if (has_scales()) reinterpret_cast<float *>(lds + SCALES)[(kside ? 0 : BN) + threadIdx.x % BN] = scale;
   }
   // Load i's row in the tile, without the lane's part
   __device__ __forceinline__ int row_of(int i) const {
@@ -693,6 +693,9 @@ struct PagedRows {
 
   // -inf for the keys past this lane's last one (as an offset in its half's sub-block)
   __device__ __forceinline__ void apply_mask(floatx16 &sacc, int last_vis) const {
+    // (keeps the branch around the mask: the compiler would make every sub-block's scores pass
+    // 32 selections of it.  4 x 4096 tokens, 16 heads of 64, f8: 437 -> 432 us)
+    asm volatile("" : "+v"(last_vis));
 #pragma unroll
     for (int r = 0; r < 16; ++r) sacc[r] = acc_key(r) <= last_vis ? sacc[r] : -INFINITY;
   }
@@ -948,7 +951,10 @@ __global__ void __launch_bounds__(PT_THREADS, tile_waves<T>(HD)) paged_tile_kern
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 31, hf = lane >> 5;
-  const int hk = blockIdx.x % a.kv_heads, flat = blockIdx.x / a.kv_heads, split = blockIdx.y;
+  // (SHARED: tiles run slowest, so that those beyond the last, which have no work, come after all
+  // others and leave no CU to two workgroups while another has none)
+  const int hk = blockIdx.x % a.kv_heads, nth = blockIdx.x / a.kv_heads;
+  const int flat = SHARED ? nth / a.tile_splits : nth, split = SHARED ? nth - flat * a.tile_splits : blockIdx.y;
   // the flat-th tile in that order
   int b = -1, tile = 0;
   const int seqs = SHARED && a.prefix ? a.groups : a.batch;
@@ -1398,16 +1404,19 @@ template <int HD, int ROWS, int ROW, bool SHARED, int WAVES = 4>
 __device__ __forceinline__ void write_rows(const PagedArgs &a, const PagedSeq &s, int b, int hk, int r0, int nr,
                                            int split, bool single, const float *o, int wave_floats,
                                            const float (*red_m)[16], const float (*red_l)[16]) {
+  constexpr int W = SHARED ? 4 : 1;  // dims of a thread
   const int before = SHARED && single ? min(chunks_seen(s.start, a.prefix_chunk), a.prefix_splits) : 0;
-  for (int t = threadIdx.x % (64 * WAVES); t < min(nr - r0, ROWS) * HD; t += 64 * WAVES) {
-    const int r = t / HD, d = t % HD;
+  for (int t = threadIdx.x % (64 * WAVES); t < min(nr - r0, ROWS) * (HD / W); t += 64 * WAVES) {
+    const int r = t / (HD / W), d = t % (HD / W) * W;
     if (d >= a.hd) continue;
-    float x = 0.f, L = 0.f, M = red_m[0][r];
+    typedef float V __attribute__((ext_vector_type(W)));
+    V x = {};
+    float L = 0.f, M = red_m[0][r];
 #pragma unroll
     for (int v = 1; v < WAVES; ++v) M = fmaxf(M, red_m[v][r]);
 #pragma unroll
     for (int v = 0; v < WAVES; ++v) {
-      x += o[v * wave_floats + r * ROW + d];
+      x += *reinterpret_cast<const V *>(o + v * wave_floats + r * ROW + d);
       L += red_l[v][r] * fast_exp2(red_m[v][r] - M);
     }
     const int i = a.by_group.div(r0 + r), h = hk * a.group + r0 + r - i * a.group;
@@ -1415,7 +1424,7 @@ __device__ __forceinline__ void write_rows(const PagedArgs &a, const PagedSeq &s
     if constexpr (SHARED) {
       const size_t at = head * a.part_splits;
       if (!single) {
-        a.part[(at + a.first_split + split) * a.part_width + d] = x;
+        *reinterpret_cast<V *>(a.part + (at + a.first_split + split) * a.part_width + d) = x;
         if (d == 0) {
           float *stats = a.part_stats + (at + a.first_split + split) * 2;
           stats[0] = M;
@@ -1429,12 +1438,13 @@ __device__ __forceinline__ void write_rows(const PagedArgs &a, const PagedSeq &s
       for (int c0 = 0; c0 < before; c0 += U) {
         typedef float vf2 __attribute__((ext_vector_type(2)));
         vf2 st[U];
-        float y[U], top = M;
+        V y[U];
+        float top = M;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int c = min(c0 + u, before - 1);
           st[u] = *reinterpret_cast<const vf2 *>(stats + 2 * c);
-          y[u] = part[(size_t)c * a.part_width];
+          y[u] = *reinterpret_cast<const V *>(part + (size_t)c * a.part_width);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) top = fmaxf(top, st[u][0]);
@@ -1445,16 +1455,20 @@ __device__ __forceinline__ void write_rows(const PagedArgs &a, const PagedSeq &s
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const float wc = c0 + u < before ? fast_exp2(st[u][0] - M) : 0.f;
-          x = fmaf(y[u], wc, x);
+#pragma unroll
+          for (int c = 0; c < W; ++c) x[c] = fmaf(y[u][c], wc, x[c]);
           L = fmaf(st[u][1], wc, L);
         }
       }
     }
     if (single) {
-      a.o[(size_t)(s.first + i) * a.ldo + (size_t)h * a.hd + d] = L == 0.f ? 0.f : x / L;
+      float *out = a.o + (size_t)(s.first + i) * a.ldo + (size_t)h * a.hd + d;
+#pragma unroll
+      for (int c = 0; c < W; ++c)
+        if (W == 1 || d + c < a.hd) out[c] = L == 0.f ? 0.f : x[c] / L;
     } else {
       float *part = a.few_part + ((((size_t)b * a.kv_heads + hk) * a.few_rows + r0 + r) * a.few_splits + split) * (a.hd + 2);
-      part[d] = x;
+      part[d] = x[0];
       if (d == 0) {
         part[a.hd] = M;
         part[a.hd + 1] = L;
@@ -1581,7 +1595,7 @@ void launch_rows(const PagedArgs &a, bool wide, hipStream_t st) {
 template <typename T, int HD, int BN, bool SHARED = false>
 void launch_tile(const PagedArgs &a, bool wide, hipStream_t st) {
   const long long tiles = (long long)a.rows * a.group / kPagedTileRows + (SHARED && a.prefix ? a.groups : a.batch);
-  const dim3 grid((unsigned)(tiles * a.kv_heads), a.tile_splits);
+  const dim3 grid((unsigned)(tiles * a.kv_heads * (SHARED ? a.tile_splits : 1)), SHARED ? 1 : a.tile_splits);
   // offsets inside 16 rows of a page fit 32 bits
   const bool uni = a.page_shift >= 4 && (long long)a.kv_heads * a.hd < (1 << 24);
   if (wide && uni) paged_tile_kernel<T, HD, BN, true, true, SHARED><<<grid, PT_THREADS, 0, st>>>(a);

@@ -48,9 +48,9 @@ struct CodeBlock {
       for (int c = 0; c < N; ++c) w[c] = t[c];
     }
   }
-  static __device__ __forceinline__ void k_words(uint32_t (&w)[KW], const T *p, const uint32_t (&off)[KL]) {
+  static __device__ __forceinline__ void k_words(uint32_t (&w)[KW], const T *p, const uint32_t (&off)[KL], uint32_t used) {
 #pragma unroll
-    for (int i = 0; i < KL; ++i) words<KW / KL>(w + KW / KL * i, p, off[i]);
+    for (int i = 0; i < KL; ++i) words<KW / KL>(w + KW / KL * i, p, off[i] & used);
   }
   static __device__ __forceinline__ void v_words(uint32_t (&w)[VW], const T *p, uint32_t off) {
     if constexpr (VD * B >= 4) words<VW>(w, p, off);
@@ -150,8 +150,10 @@ struct CodeLoader {
 
   // Loads the block at k0 and looks the next one's pages up.  What comes from no page: bits of
   // runs, or of the lane's rows (0, 1: K's, 2 ..: V's, 10: the scale's).
-  __device__ __forceinline__ uint32_t load(const PagedArgs &a, Block &b, int k0) {
+  // A block from key `end` on is not used: its lanes read the same few bytes.
+  __device__ __forceinline__ uint32_t load(const PagedArgs &a, Block &b, int k0, int end) {
     uint32_t none = 0;
+    const uint32_t used = k0 < end ? ~0u : 0u;
     if constexpr (RUN > 1) {
       size_t at[NP];  // rows before the run
 #pragma unroll
@@ -171,13 +173,13 @@ struct CodeLoader {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const size_t run = PER == 1 ? at[h] : row & 8 ? at[PER * h + PER - 1] : at[PER * h];
-        Block::k_words(b.k[h], kc + element(run), k_off);
+        Block::k_words(b.k[h], kc + element(run), k_off, used);
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const size_t run = PER == 1 ? at[h] : quarter & 2 ? at[PER * h + PER - 1] : at[PER * h];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) Block::v_words(b.v[4 * h + e], vc + element(run), v_off[e]);
+        for (int e = 0; e < 4; ++e) Block::v_words(b.v[4 * h + e], vc + element(run), v_off[e] & used);
       }
     } else {
       auto place = [&](int i, int key) {
@@ -187,9 +189,9 @@ struct CodeLoader {
       };
       if constexpr (kQ8<T>) b.scale = side[place(10, scale_key(k0))];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) Block::k_words(b.k[h], kc + element(place(h, k_key(k0, h))), k_off);
+      for (int h = 0; h < 2; ++h) Block::k_words(b.k[h], kc + element(place(h, k_key(k0, h))), k_off, used);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) Block::v_words(b.v[e], vc + element(place(2 + e, v_key(k0, e))), v_off[0]);
+      for (int e = 0; e < 8; ++e) Block::v_words(b.v[e], vc + element(place(2 + e, v_key(k0, e))), v_off[0] & used);
       lookup(a, k0 + STRIDE);
     }
     return none;
@@ -524,9 +526,8 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
     Block block[U];
     uint32_t none[U];
     int bad = 0;
-    // (past the wave's last block the request's last rows are loaded once more, and left there)
 #pragma unroll
-    for (int u = 0; u < U - 1; ++u) none[u] = from.load(a, block[u], first + STRIDE * u);
+    for (int u = 0; u < U - 1; ++u) none[u] = from.load(a, block[u], first + STRIDE * u, c1);
     const bool wide = a.wide ? rows.template load_q<true>(qrow, a.hd, a.scale_log2, quarter)
                              : rows.template load_q<false>(qrow, a.hd, a.scale_log2, quarter);
     // (left from its middle: a way back to its top with loads unused would make every turn wait for them)
@@ -536,7 +537,7 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
       for (int u = 0; u < U; ++u) {
         const int k = k0 + STRIDE * u, ahead = (u + U - 1) % U;
         if (k >= c1) goto summed;
-        none[ahead] = from.load(a, block[ahead], k + STRIDE * (U - 1));
+        none[ahead] = from.load(a, block[ahead], k + STRIDE * (U - 1), c1);
         from.clean(block[u], k, none[u], bad);
         rows.add(block[u], scales[wave], quarter, k + 31 > lim_lo, lim - k - 4 * quarter);
       }
