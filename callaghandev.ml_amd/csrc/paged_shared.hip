@@ -125,10 +125,33 @@ struct SharedPlan {
   size_t parts, floats;
 };
 
+// Whether reading what the groups share once, in a launch of its own whose sums have to be joined,
+// takes less time than every request's reading of its own pages, from the sizes alone (us):
+//   requests of few rows read at 6 TB/s, in tiles a CU takes `tile` us for 32 keys of 128 rows,
+//   0.6 of that where a wave or two have rows;
+//   the launch and the joins take 12 us.
+// 64 requests behind 8192 tokens, 32 heads over 8 of 128, bf16: 70 us, 199 by cdml_paged_attn;
+// 105 requests in 5 groups behind 4102, 27 new tokens, 8 heads of 64, bf16: 115, 193; but 264 in 6
+// behind 109, 27 new, one head of 96: 50 and 25; 26 in 2 behind 881, 7 heads over 1 of 128, fp32:
+// 49 and 25.
+bool worth_sharing(int size, int batch, int groups, int max_members, int max_new, int max_prefix, int group,
+                   int kv_heads, int hd) {
+  const double tile = (hd <= 32 ? 0.5 : hd <= 64 ? 0.85 : 1.5) * (size == 4 ? 1.8 : 1);
+  auto us = [&](double readers, double rows) {
+    const double keys = readers * kv_heads * max_prefix;
+    if (rows <= kSpanRows) return keys * 2 * hd * size / 6e6;
+    const double tiles = (double)(long long)((rows + kPagedTileRows - 1) / kPagedTileRows);
+    return keys / 32 * tiles * tile * (rows <= kPagedTileRows / 2 ? 0.6 : 1) / kComputeUnits;
+  };
+  const double rows = (double)max_new * group;
+  return us(batch, rows) - us(groups, rows * max_members) > 12;
+}
+
 SharedPlan plan_shared(int size, int rows, int batch, int groups, int max_members, int max_new, int max_prefix,
                        int max_tail, int heads, int kv_heads, int hd) {
   SharedPlan p{};
-  p.plain = hd > 128 || groups == 0 || max_members < 2 || max_prefix == 0;
+  p.plain = hd > 128 || groups == 0 || max_members < 2 || max_prefix == 0 ||
+            !worth_sharing(size, batch, groups, max_members, max_new, max_prefix, heads / kv_heads, kv_heads, hd);
   if (p.plain) {
     p.own = make_plan(size, rows, batch, max_new, max_prefix + max_tail, heads, kv_heads, hd);
     p.floats = p.own.few_floats + p.own.tile_floats;
@@ -138,10 +161,26 @@ SharedPlan plan_shared(int size, int rows, int batch, int groups, int max_member
   const long long most = std::min((long long)max_members * max_new, (long long)rows) * group;
   p.prefix_tile = most > kSpanRows;
   p.prefix_rows = (int)std::min<long long>(most, INT_MAX);
-  const long long work = (p.prefix_tile ? (long long)rows * group / kPagedTileRows + groups : groups) * kv_heads;
-  long long splits = (2 * kComputeUnits + work - 1) / work;
-  if (!p.prefix_tile && work >= kComputeUnits) splits = 1;
-  splits = std::min<long long>(splits, (max_prefix + 255) / 256);
+  // The split of the shared tokens that takes the least time: `unit` keys take as long as any
+  // others, `start` of them a workgroup's beginning and end; a turn of `slots` workgroups more
+  // takes 0.7 of the first.  64 requests behind 8192 tokens, 32 heads over 8 of 128, bf16 (16 tiles): 16
+  // splits 40 us, 22 (two workgroups on some CUs, one on the others) 45, 32 37, but with
+  // twice the parts to join; 16 x 8 beams behind 2048, i8 (256 spans): one split 37.9 us with
+  // the joins, two 36.3, four 41.5.
+  const long long all = (long long)rows * group;
+  const long long tiles = groups * std::max<long long>(1, (all / groups + kPagedTileRows / 2) / kPagedTileRows);
+  const long long work = (p.prefix_tile ? tiles : groups) * kv_heads;
+  const int unit = p.prefix_tile ? 32 : 128, start = p.prefix_tile ? 6 : 4;
+  const int slots = p.prefix_tile ? kComputeUnits : 2 * kComputeUnits;
+  long long splits = 1, least = LLONG_MAX;
+  for (long long n = 1; n <= (max_prefix + 255) / 256 && n * work <= 4 * slots + work; ++n) {
+    const long long turns = (n * work + slots - 1) / slots;
+    const long long cost = (3 + 7 * turns) * ((max_prefix + n * unit - 1) / (n * unit) + start);
+    if (cost < least) {
+      least = cost;
+      splits = n;
+    }
+  }
   p.prefix_chunk = round_up((int)((max_prefix + splits - 1) / splits), 128);
   p.prefix_splits = (max_prefix - 1) / p.prefix_chunk + 1;
   p.own = make_plan(size, rows, batch, max_new, max_tail, heads, kv_heads, hd, true);
