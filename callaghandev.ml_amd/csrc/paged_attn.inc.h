@@ -292,10 +292,48 @@ struct Pieces<F8> : Pieces<__bf16> {};
 // (common.h); those of 2^87 and more over V's codes come out infinite, and are recomputed.
 constexpr float kCodeScale = 1099511627776.f, kCodeUnscale = 1.f / kCodeScale;  // 2^40
 
+// The three pieces of eight values as in split_operand, with what a piece leaves of a value from a
+// dot product of the pair (seven instructions a pair for eleven), which takes subnormal numbers as
+// zeros: for probabilities times a scale of V and kCodeScale, whose pieces those are far below.
+__device__ __forceinline__ void split_codes(const float (&x)[8], bf16x8 (&p)[3]) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  // (-1, 0) and (0, -1) from registers: an inline constant of this instruction is another pair
+  uint32_t one = 0x0000bf80u, other = 0xbf800000u;
+  asm volatile("" : "+s"(one), "+s"(other));
+  const bf16x2 first = __builtin_bit_cast(bf16x2, one), second = __builtin_bit_cast(bf16x2, other);
+  uint32_t w[3][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[0][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+    const bf16x2 h = __builtin_bit_cast(bf16x2, w[0][i]);
+    const float ra = __builtin_amdgcn_fdot2_f32_bf16(h, first, x[2 * i], false);
+    const float rb = __builtin_amdgcn_fdot2_f32_bf16(h, second, x[2 * i + 1], false);
+    w[1][i] = pack_bf16(ra, rb);
+    const bf16x2 m = __builtin_bit_cast(bf16x2, w[1][i]);
+    w[2][i] = pack_bf16(__builtin_amdgcn_fdot2_f32_bf16(m, first, ra, false),
+                        __builtin_amdgcn_fdot2_f32_bf16(m, second, rb, false));
+  }
+#pragma unroll
+  for (int j = 0; j < 3; ++j) p[j] = __builtin_bit_cast(bf16x8, (vu4{w[j][0], w[j][1], w[j][2], w[j][3]}));
+}
+
 // Codes (dims 2 i, 2 i + 1 of four in w) as a pair of bf16 values, which hold them exactly.
+// Byte i of w as a signed number.  (One instruction, where the compiler takes two.)
+__device__ __forceinline__ float signed_byte(uint32_t w, int i) {
+  float x;
+  if (i == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(x) : "v"(w));
+  if (i == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(x) : "v"(w));
+  if (i == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(x) : "v"(w));
+  if (i == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(x) : "v"(w));
+  return x;
+}
+// Byte i of each of two words as a pair of bf16 values.
+__device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int i) {
+  return __builtin_amdgcn_perm(__float_as_uint(signed_byte(b, i)), __float_as_uint(signed_byte(a, i)), 0x07060302u);
+}
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, I8) {
-  const float a = (float)(int8_t)(w >> 16 * i), b = (float)(int8_t)(w >> (16 * i + 8));
-  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  return __builtin_amdgcn_perm(__float_as_uint(signed_byte(w, 2 * i + 1)), __float_as_uint(signed_byte(w, 2 * i)),
+                               0x07060302u);
 }
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, F8) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -347,8 +385,7 @@ __device__ __forceinline__ void put_v(char *d, int plane, const typename Raw4<T>
   constexpr int NP = Pieces<T>::N;
   if constexpr (kQ8<T>) {
     if constexpr (std::is_same<T, I8>::value) {
-      const float x = code_value(I8{(uint8_t)(a >> 8 * c)}), y = code_value(I8{(uint8_t)(b >> 8 * c)});
-      *reinterpret_cast<uint32_t *>(d) = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+      *reinterpret_cast<uint32_t *>(d) = byte_pair(a, b, c);
     } else {
       *reinterpret_cast<uint32_t *>(d) = __builtin_amdgcn_perm(code_pair(b, c / 2, T{}), code_pair(a, c / 2, T{}),
                                                                c & 1 ? 0x07060302u : 0x05040100u);
@@ -742,8 +779,10 @@ struct PagedRows {
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[4 * g + e] *= w[e];
           }
+          split_codes(x, pp);
+        } else {
+          split_operand(x, 1.f, pp);
         }
-        split_operand(x, 1.f, pp);
       }
 #pragma unroll
       for (int i = 0; i < PC::PRODUCTS; ++i) oacc[db] = mfma32x32x16(v[j % AHEAD][PC::A[i]], pp[PC::B[i]], oacc[db]);

@@ -76,8 +76,7 @@ struct CodeBlock {
       if constexpr (!kQ8<T>) {
         w[i] = __builtin_amdgcn_perm(b, a, d & 1 ? 0x07060302u : 0x05040100u);
       } else if constexpr (std::is_same<T, I8>::value) {
-        const float x = code_value(I8{(uint8_t)(a >> 8 * (d % 4))}), y = code_value(I8{(uint8_t)(b >> 8 * (d % 4))});
-        w[i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+        w[i] = byte_pair(a, b, d % 4);
       } else {
         w[i] = __builtin_amdgcn_perm(code_pair(b, d / 2 % 2, T{}), code_pair(a, d / 2 % 2, T{}),
                                      d & 1 ? 0x07060302u : 0x05040100u);
@@ -402,7 +401,7 @@ struct CodeRows {
     if constexpr (PACK) {
       pp[0] = piece_of(p);
     } else {
-      split_operand(p, 1.f, pp);
+      split_codes(p, pp);
     }
 #pragma unroll
     for (int d = 0; d < NDB; ++d) {
