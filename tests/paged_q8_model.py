@@ -181,9 +181,36 @@ def call_shared(table, kv, cu, groups, P, n_pages, fill=-9):
     return down(d[4], (len(kv),), np.int32)
 
 
-def call_attention_shared(q, c, table, kv, cu, groups, H, scale, o, bounds=None, ldq=None, ldo=None, n_pages=None):
-    """cdml_paged_shared and cdml_paged_attn_shared; bounds: max_members, max_new, max_prefix, max_tail.
+def forced(c, table, kv, cu, groups, H):
+    """Bounds (max_members, max_new, max_prefix, max_tail) for which the entry shares, whatever there is to be shared,
+    and a table of as many columns; None where no length of a prefix is worth it.  (The entry's own estimate: requests
+    of few rows read at 6 TB/s, tiles of 128 rows and 32 keys take a time of their own, a launch and a join 12 us.)"""
+    (B, blocks), P, hd, kv_heads = table.shape, c["P"], c["hd"], c["heads"]
+    size = {"f32": 4, "f16": 2, "bf16": 2, "i8": 1, "f8": 1}[c["kind"]]
+    members, new = int(np.max(np.diff(groups), initial=0)), int(np.max(np.diff(cu), initial=0))
+    tile = (0.5 if hd <= 32 else 0.85 if hd <= 64 else 1.5) * (1.8 if size == 4 else 1)
+
+    def us(readers, rows):  # a key
+        if rows <= 16:
+            return readers * kv_heads * 2 * hd * size / 6e6
+        return readers * kv_heads / 32 * -(-rows // 128) * tile * (0.6 if rows <= 64 else 1) / 256
+    rows = new * (H // kv_heads)
+    gain = us(B, rows) - us(len(groups) - 1, rows * members)
+    if hd > 128 or members < 2 or gain <= 0 or 13 / gain > 2 ** 22:
+        return None
+    most = max(int(13 / gain) + 1, blocks * P)
+    more = -(-most // P) - blocks
+    return np.concatenate([table, np.full((B, more), -1, np.int32)], 1), (members, new, most, blocks * P)
+
+
+def call_attention_shared(q, c, table, kv, cu, groups, H, scale, o, bounds=None, ldq=None, ldo=None, n_pages=None,
+                          force=False):
+    """cdml_paged_shared and cdml_paged_attn_shared; bounds: max_members, max_new, max_prefix, max_tail.  force:
+    bounds for which it shares, shown by tables in which only the first member of a group holds what is shared.
     Returns (o, shared, bad)."""
+    lead = forced(c, table, kv, cu, groups, H) if force else None
+    if lead:
+        table, bounds = lead
     rows, B, hd, P = len(q), len(kv), c["hd"], c["P"]
     n_pages = n_pages or len(c["k"])
     ldq, ldo = ldq or q.shape[1], ldo or o.shape[1]
@@ -202,6 +229,12 @@ def call_attention_shared(q, c, table, kv, cu, groups, H, scale, o, bounds=None,
     w.upload(np.full(max(n // 4, 1), np.nan, np.float32), stream())
     N.check(N.lib().cdml_paged_shared(dt.ptr, table.shape[1], dl.ptr, dc.ptr, dg.ptr, len(groups) - 1, B, n_pages, P,
                                       ds.ptr, stream().handle))
+    if lead:
+        alone, s = table.copy(), down(ds, (B,), np.int32)
+        for first, behind in zip(groups[:-1], groups[1:]):
+            for b in range(first + 1, behind):
+                alone[b, :s[b] // P] = -1
+        dt = ints(alone)
     N.check(N.lib().cdml_paged_attn_shared(dq.ptr, ldq, *(ptr(b) for b in d), N.CACHE[c["kind"]], n_pages, P, dt.ptr,
                                            table.shape[1], dl.ptr, dc.ptr, dg.ptr, ds.ptr, do.ptr, ldo, *size, scale,
                                            bad.ptr, w.ptr, n, stream().handle))

@@ -55,11 +55,11 @@ def case_of(r, kind, groups, prefix, tails, news, P, H, HK, hd, pad=2, batch=Non
     return q, c, table, np.array(lens, np.int32), cu, np.array(groups, np.int32), o
 
 
-def check(q, c, table, kv, cu, groups, o, H, scale=None, **more):
+def check(q, c, table, kv, cu, groups, o, H, scale=None, force=True, **more):
     if scale is None:
         scale = float(np.float32(1) / np.sqrt(np.float32(c["hd"])))
     want, tol = M.attention(q, c["kx"], c["vx"], table, kv, cu, c["P"], H, c["heads"], scale, o)
-    got, found, bad = Q.call_attention_shared(q, c, table, kv, cu, groups, H, scale, o, **more)
+    got, found, bad = Q.call_attention_shared(q, c, table, kv, cu, groups, H, scale, o, force=force, **more)
     np.testing.assert_array_equal(found, Q.shared(table, kv, cu, groups, c["P"], len(c["k"])))
     assert bad == 0
     compare(got, want, tol + underflow(c, kv))
@@ -127,7 +127,9 @@ def test_single_tokens_behind_a_prefix(kind, H, HK, hd, P):
     tails[[0, 6, 20]] = 1
     news = [1] * 31
     news[2] = news[12] = 0
-    check(*case_of(r, kind, groups, prefix, tails, news, P, H, HK, hd), H)
+    case = case_of(r, kind, groups, prefix, tails, news, P, H, HK, hd)
+    check(*case, H)
+    check(*case, H, force=False)
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -137,8 +139,11 @@ def test_chunks_behind_a_prefix(kind, H, HK, hd, P):
     groups = [0, 3, 8, 10]
     prefix = [max(1, n // P) for n in (70, 200, 33)]
     tails = [40, 1, 130, 9, 60, 33, 2, 300, 64, 65]
-    news = [40, 1, 100, 9, 0, 2, 1, 290, 64, 1]
-    check(*case_of(r, kind, groups, prefix, tails, news, P, H, HK, hd), H)
+    for most in (290, 70, 20, 5):
+        news = [min(n, most) for n in (40, 1, 100, 9, 0, 2, 1, 290, 64, 1)]
+        case = case_of(r, kind, groups, prefix, tails, news, P, H, HK, hd)
+        check(*case, H)
+        check(*case, H, force=False)
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -166,16 +171,19 @@ def test_requests_of_no_group_and_groups_that_part_early(kind, hd):
 
 @pytest.mark.parametrize("kind", ["bf16", "f32", "i8"])
 @pytest.mark.parametrize("bounds", [(6, 4, 300, 300), (2, 4, 112, 60), (6, 4, 16, 156), (6, 4, 160, 12), (1, 4, 112, 60),
-                                    (6, 4, 0, 172), (6, 4, 172, 0), (4096, 4, 112, 60)])
+                                    (6, 4, 0, 172), (6, 4, 172, 0), (4096, 4, 112, 60), (2, 1, 70000, 60),
+                                    (2, 4, 70000, 0), (6, 4, 70000, 12), (3, 1, 70000, 600), (6, 2, 70000, 70000)])
 def test_bounds_only_cost_time(kind, bounds):
     # of members, prefixes and tails, larger and smaller ones than there are (their sum holds every length)
     r = rng(76)
     groups = [0, 6, 12]
-    case = case_of(r, kind, groups, [7, 5], [60, 1, 40, 4, 9, 20] * 2, [1, 1, 4, 4, 1, 2] * 2, 16, 4, 2, 64)
-    blocks = max(case[2].shape[1], 38)
+    most = bounds[1]
+    news = [min(n, most) for n in [1, 1, 4, 4, 1, 2] * 2]
+    case = case_of(r, kind, groups, [7, 5], [60, 1, 40, 4, 9, 20] * 2, news, 16, 4, 2, 64)
+    blocks = max(case[2].shape[1], -(-max(bounds[2:]) // 16), 38)
     case = list(case)
     case[2] = np.concatenate([case[2], np.full((12, blocks - case[2].shape[1]), -1, np.int32)], 1)
-    check(*case, 4, bounds=bounds)
+    check(*case, 4, bounds=bounds, force=False)
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -215,7 +223,7 @@ def test_pages_that_are_none(kind, members):
     zeros = np.where((table >= 0) & (table < n), table, n)
     k, v = (np.concatenate([c[s], np.zeros((1, 16, 64))]) for s in ("kx", "vx"))
     want, tol = M.attention(q, k, v, zeros, kv, cu, 16, 2, 1, 0.125, o)
-    got, found, bad = Q.call_attention_shared(q, c, table, kv, cu, g, 2, 0.125, o)
+    got, found, bad = Q.call_attention_shared(q, c, table, kv, cu, g, 2, 0.125, o, force=True)
     assert bad == 1 and (found == 64).all()
     compare(got, want, tol + underflow(c, kv))
 
@@ -248,8 +256,9 @@ def test_a_step_in_a_graph(kind):
     r = rng(82)
     groups, P, H, HK, hd, B = [0, 4, 7], 16, 4, 2, 64, 7
     q, c, table, kv, cu, g, o = case_of(r, kind, groups, [9, 5], [70, 60, 50, 40, 30, 20, 70], [1] * B, P, H, HK, hd, pad=0)
+    table, (members, new, prefix, _) = Q.forced(c, table, kv, cu, g, H)
     L, st, n_pages = N.lib(), stream(), len(c["k"])
-    size = (B, B, 2, 4, 1, 144, 80, H, HK, hd)
+    size = (B, B, 2, members, new, prefix, 80, H, HK, hd)
     d = Q.upload(c)
     dt, dl, dc, dg, ds = M.ints(table), M.ints(kv), M.ints(cu), M.ints(g), M.ints(np.zeros(B))
     dq, do = up(q), up(o)
