@@ -204,8 +204,9 @@ int check_shared(const char *what, int rows, int batch, int groups, int max_memb
                 batch, groups, max_members, max_prefix, max_tail);
   const int rc = check_sizes(what, rows, batch, max_new, max_prefix + max_tail, heads, kv_heads, hd);
   if (rc) return rc;
-  // (a group's rows run in tiles where a request's do not)
+  // (a group's rows run in tiles where a request's do not; a workgroup of the join to a row)
   if (((long long)rows * (heads / kv_heads) / kPagedTileRows + batch) * kv_heads >= 1 << 24 ||
+      rows >= 1 << 24 ||
       (long long)rows * (heads / kv_heads) > INT_MAX / 2)
     return fail(CDML_E_INVALID, "%s: problem too large", what);
   return CDML_OK;

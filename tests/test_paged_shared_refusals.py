@@ -27,11 +27,15 @@ def test_attention_refusals():
         {"groups": -1}, {"groups": 7}, {"max_members": -1}, {"max_prefix": -1}, {"max_tail": -1}, {"max_tail": 65},
         {"max_prefix": 65},
         {"max_prefix": BIG, "max_tail": BIG}, {"heads": 0}, {"kv_heads": 0}, {"kv_heads": 3}, {"hd": 0}, {"hd": 257},
-        {"ldq": 255}, {"ldo": 255}, {"max_new": BIG}, {"kc": ODD}, {"vc": ODD}, {"rows": 2 ** 30},
-        {"ws": None}, {"ws": ODD}, {"bytes": 4}] + [
+        {"ldq": 255}, {"ldo": 255}, {"max_new": BIG}, {"kc": ODD}, {"vc": ODD}, {"rows": 2 ** 30}, {"rows": 2 ** 24}] + [
         {k: None} for k in ("q", "kc", "vc", "ks", "vs", "table", "kv_len", "cu", "group_start", "shared", "o")])
     for empty in ({"rows": 0}, {"batch": 0, "groups": 0}, {"max_new": 0}):
         assert N.lib().cdml_paged_attn_shared(*{**ATTN, **empty, "q": None}.values()) == N.OK
+
+
+# Sizes that are worth sharing; those above run as every request's own, which needs no workspace.
+SHARING = {**ATTN, "max_blocks": 1024, "ldq": 4096, "ldo": 4096, "rows": 64, "batch": 64, "groups": 1, "max_members": 64,
+           "max_prefix": 8192, "max_tail": 512, "heads": 32, "kv_heads": 8, "hd": 128}
 
 
 def test_attention_workspace():
@@ -40,5 +44,7 @@ def test_attention_workspace():
     assert n(6, 6, 2, 3, 1, 32, 32, 4, 2, 64, None) == N.E_INVALID
     assert n(6, 6, 7, 3, 1, 32, 32, 4, 2, 64, C.byref(size)) == N.E_INVALID
     assert n(6, 6, 2, 3, 1, 32, 32, 4, 3, 64, C.byref(size)) == N.E_INVALID
-    assert n(6, 6, 2, 3, 1, 32, 32, 4, 2, 64, C.byref(size)) == N.OK and size.value > 0
-    refused("cdml_paged_attn_shared", {**ATTN, "bytes": size.value}, [{"bytes": size.value - 1}])
+    assert n(6, 6, 2, 3, 1, 32, 32, 4, 2, 64, C.byref(size)) == N.OK and size.value == 0
+    assert n(64, 64, 1, 64, 1, 8192, 512, 32, 8, 128, C.byref(size)) == N.OK and size.value > 0
+    refused("cdml_paged_attn_shared", {**SHARING, "bytes": size.value}, [
+        {"ws": None}, {"ws": ODD}, {"bytes": 4}, {"bytes": size.value - 1}])
