@@ -317,7 +317,6 @@ __device__ __forceinline__ void split_codes(const float (&x)[8], bf16x8 (&p)[3])
   for (int j = 0; j < 3; ++j) p[j] = __builtin_bit_cast(bf16x8, (vu4{w[j][0], w[j][1], w[j][2], w[j][3]}));
 }
 
-// Codes (dims 2 i, 2 i + 1 of four in w) as a pair of bf16 values, which hold them exactly.
 // Byte i of w as a signed number.  (One instruction, where the compiler takes two.)
 __device__ __forceinline__ float signed_byte(uint32_t w, int i) {
   float x;
@@ -331,6 +330,7 @@ __device__ __forceinline__ float signed_byte(uint32_t w, int i) {
 __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int i) {
   return __builtin_amdgcn_perm(__float_as_uint(signed_byte(b, i)), __float_as_uint(signed_byte(a, i)), 0x07060302u);
 }
+// Codes (dims 2 i, 2 i + 1 of four in w) as a pair of bf16 values, which hold them exactly.
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, I8) {
   return __builtin_amdgcn_perm(__float_as_uint(signed_byte(w, 2 * i + 1)), __float_as_uint(signed_byte(w, 2 * i)),
                                0x07060302u);
@@ -973,6 +973,12 @@ struct PagedRows {
 // (bf16, 32 heads over 8 of 128) 765 to 840 us, as much.  The matrix cores are busy 51% of the
 // cycles (46% at head dim 128) beside six (four) vector instructions for each of theirs; and
 // cycles are long: the clock falls to 1.9 GHz (2.0) under their power.
+//   8-bit caches (4 x 4096 tokens, 16 heads of 64, f8: 418 to 435 us by card, 316 to 329 TFLOP/s;
+// ragged chunks, 32 heads over 8 of 128, i8: 792 to 821) are no faster than bf16 ones: codes
+// are one piece, too, and the products are as many.  A key's scale meets its score in the
+// subtraction of the reference and its probability ahead of the split.  Two tiles in hand, the
+// products of one between the exponentials of the other, took 455 us.  Counters: the matrix
+// cores are busy 43% of the cycles (44% at head dim 128), the vector units 51% (34%).
 constexpr int kTileClasses = 8;
 // Waves a SIMD that registers are kept for; LDS holds as many.  16-bit caches, 16 heads of 64,
 // 4 x 2048 of 4096 tokens: three 331 us (bf16) and 506 (fp16), two 348 and 530.

@@ -13,7 +13,7 @@ namespace {
 //   K: lane (row, quarter) has 16 bytes of every 64 of keys row and 16 + row, the quarters side by
 //      side.  A dot product's order is free, so product s takes the lane's s-th eight dims, of
 //      Q too.  (A quarter of a row to a lane, whose loads touch four times the segments:
-//      64 requests behind 8192 bf16 tokens OLDUS -> NEWUS us.)
+//      64 requests behind 8192 bf16 tokens 87 -> 78 us.)
 //   V: lane (row, quarter) has dims VD * row .. + VD - 1 of the keys 4 quarter + 0..3 and
 //      16 + 4 quarter + 0..3, those whose probabilities it holds; product d takes its d-th
 //      dim, so V is transposed as the codes of two keys become a pair of bf16.
@@ -485,12 +485,13 @@ struct CodeRows {
 };
 
 // One workgroup: up to 16 rows of a (request, K/V head) against one chunk of its keys.  The
-// four waves take blocks of 32 keys in turn and join their sums at the end.  A wave's sets of
-// registers go round: all blocks but the one that is multiplied are on the way.
-template <int HD, int RUN>
-constexpr int code_blocks() {
-  return 2;
-}
+// four waves take blocks of 32 keys in turn and join their sums at the end; a wave's next block
+// is on the way while one is multiplied.  (Two on the way: 64 ragged requests, 32 heads over 8,
+// f8, 131 us for 129; 8 x 2048 keys 15.7 for 14.6.)
+//   What bounds it: HBM where requests are equal and long, 64 x 8192 keys, 16 heads of 128, i8: 329
+// us, 6.7 TB/s of codes and scales.  Ragged requests (2048 to 8192 keys, 32 heads over 8, f8)
+// take 126 us, 4.9 TB/s: workgroups end at different times (in chunks of 4096 keys 154).
+constexpr int kCodeBlocks = 2;
 template <typename T, int HD, int RUN, bool PACK, bool SHARED, int WAVES>
 __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s, int b, int hk, int r0, int nr,
                                           float (&lds)[4][CodeRows<T, HD, PACK>::ROWS * (HD + 4)], float (&red_m)[4][16], float (&red_l)[4][16],
@@ -521,7 +522,7 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
     CodeLoader<T, HD, RUN, STRIDE> from;
     from.init(a, s.table, hk, last);
     from.lookup(a, first);
-    constexpr int U = code_blocks<HD, RUN>();
+    constexpr int U = kCodeBlocks;
     Block block[U];
     uint32_t none[U];
     int bad = 0;

@@ -133,7 +133,7 @@ inline Plan make_plan(int size, int rows, int batch, int max_new, int max_len, i
   const long long pairs = (long long)(batch < 1 ? 1 : batch) * kv_heads;
   const long long groups = k.rows ? (p.few_rows + kVecRows - 1) / kVecRows : (p.few_rows + kSpanRows - 1) / kSpanRows;
   if (k.span && shared && len <= 1024) {
-    p.few_chunk = round_up(len, 128);  // one chunk, which adds what the group shares
+    p.few_chunk = round_up(len, 128);  // one chunk, in whose kernel the join is
   } else if (k.span) {
     // a whole request to a workgroup where these fill the CUs (16 x 16 pairs of 4096 bf16 keys:
     // 48.5 us, 55.3 in two chunks, 96 in chunks of 512), else two workgroups for every CU
