@@ -752,8 +752,9 @@ int cdml_paged_shared(const int *block_table, int max_blocks,
  * and groups.  max_members, max_prefix and max_tail bound the members of a group,
  * shared, and kv_len - shared (either <= max_blocks * page_size); the launches are
  * sized by them.  Tokens past max_prefix + max_tail are cut off, other excess only
- * costs time.  Head dims above 128 run as in cdml_paged_attn, each request over its
- * own table.  Otherwise everything is as there, the workspace
+ * costs time.  Head dims above 128, and sizes at which one launch over all would not
+ * save what its join costs, run as in cdml_paged_attn, each request over its own
+ * table.  Otherwise everything is as there, the workspace
  * cdml_paged_attn_shared_workspace_size bytes. */
 int cdml_paged_attn_shared_workspace_size(int rows, int batch, int groups,
                                           int max_members, int max_new,

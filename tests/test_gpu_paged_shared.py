@@ -295,6 +295,51 @@ def test_a_step_in_a_graph(kind):
     N.check(L.cdml_graph_destroy(graph))
 
 
+@pytest.mark.parametrize("kind", ["bf16", "i8"])
+def test_two_streams_at_once(kind):
+    """Calls over one cache that overlap, each with its own workspace: the bits of calls alone."""
+    r = rng(83)
+    P, H, HK, hd, B = 16, 8, 4, 64, 12
+    q, c, table, kv, cu, g, o = case_of(r, kind, [0, 7, 12], [40, 21], [70] * B, [1] * B, P, H, HK, hd, pad=3)
+    table, (members, new, prefix, _) = Q.forced(c, table, kv, cu, g, H)
+    L, n_pages, rows = N.lib(), len(c["k"]), len(q)
+    size = (rows, B, 2, members, new, prefix, 80, H, HK, hd)
+    d = Q.upload(c)
+    dt, dl, dc, dg = M.ints(table), M.ints(kv), M.ints(cu), M.ints(g)
+    streams = [stream(), N.Stream()]
+    queries = [q, r.standard_normal(q.shape).astype(np.float32)]
+    dq, do, ds = [up(x) for x in queries], [up(o), up(o)], [M.ints(np.zeros(B)), M.ints(np.zeros(B))]
+    w = [M.ws("cdml_paged_attn_shared_workspace_size", *size) for _ in streams]
+
+    def call(i):
+        st = streams[i].handle
+        N.check(L.cdml_paged_shared(dt.ptr, table.shape[1], dl.ptr, dc.ptr, dg.ptr, 2, B, n_pages, P, ds[i].ptr, st))
+        N.check(L.cdml_paged_attn_shared(dq[i].ptr, H * hd, *(Q.ptr(b) for b in d), N.CACHE[kind], n_pages, P, dt.ptr,
+                                         table.shape[1], dl.ptr, dc.ptr, dg.ptr, ds[i].ptr, do[i].ptr, H * hd, *size,
+                                         0.125, None, w[i][0].ptr, w[i][1], st))
+
+    def results():
+        for s in streams:
+            s.synchronize()
+        return [down(x, o.shape) for x in do]
+
+    for i in range(2):
+        call(i)
+        streams[i].synchronize()
+    alone = results()
+    for i in range(2):
+        want, tol = M.attention(queries[i], c["kx"], c["vx"], table, kv, cu, P, H, HK, 0.125, o)
+        compare(alone[i], want, tol + underflow(c, kv))
+    for x in do:
+        x.upload(o, streams[0])
+    streams[0].synchronize()
+    for _ in range(8):
+        call(0)
+        call(1)
+    for got, want in zip(results(), alone):
+        np.testing.assert_array_equal(got, want)
+
+
 @pytest.mark.parametrize("kind", ["f32", "i8", "f8"])
 def test_prompts_beams_and_reordering_together(kind):
     """A run as a server makes it: ragged prompts planned and appended for the first beam of each, the tables
