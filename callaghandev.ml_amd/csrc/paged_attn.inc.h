@@ -297,7 +297,7 @@ constexpr float kCodeScale = 1099511627776.f, kCodeUnscale = 1.f / kCodeScale;  
 // zeros: for probabilities times a scale of V and kCodeScale, whose pieces those are far below.
 __device__ __forceinline__ void split_codes(const float (&x)[8], bf16x8 (&p)[3]) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  // (-1, 0) and (0, -1) from registers: an inline constant of this instruction is another pair
+  // (-1, 0) and (0, -1), kept in registers
   uint32_t one = 0x0000bf80u, other = 0xbf800000u;
   asm volatile("" : "+s"(one), "+s"(other));
   const bf16x2 first = __builtin_bit_cast(bf16x2, one), second = __builtin_bit_cast(bf16x2, other);

@@ -566,11 +566,12 @@ __device__ __forceinline__ void code_rows(const PagedArgs &a, const PagedSeq &s,
   float w = 1.f;
   if constexpr (WAVES > 1)
     w = fast_exp2(m - fmaxf(fmaxf(red_m[0][row], red_m[1][row]), fmaxf(red_m[2][row], red_m[3][row])));
-  if (!PACK || (lane & 12) == 0)
+  if (!PACK || (lane & 12) == 0) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < 4; ++c)
 #pragma unroll
-    for (int d = 0; d < NDB; ++d) lds[wave][row * ROW + NDB * (4 * quarter + c) + d] = rows.o[d][c] * w;
+      for (int d = 0; d < NDB; ++d) lds[wave][row * ROW + NDB * (4 * quarter + c) + d] = rows.o[d][c] * w;
+  }
   barrier();
   const int v = WAVES == 1 ? wave : 0;
   write_rows<HD, ROWS, ROW, SHARED, WAVES>(args_again(), s, b, hk, r0, nr, split, single, lds[v], ROWS * ROW, red_m + v,
