@@ -57,7 +57,7 @@ int workspace_size(const char *what, bool q8, int rows, int batch, int max_new, 
 
 }  // namespace
 
-int paged_attention(const char *what, bool q8, bool cut, const float *q, int ldq, const void *kcache, const void *vcache,
+int paged_attention(const char *what, bool q8, bool shared, const float *q, int ldq, const void *kcache, const void *vcache,
               const float *kscale, const float *vscale, int cache_type, int n_pages, int page_size,
               const int *block_table, int max_blocks, const int *kv_len, const int *cu_new, float *o, int ldo, int rows,
               int batch, int max_new, int max_len, int num_heads, int num_kv_heads, int head_dim, float scale, int *bad,
@@ -70,7 +70,7 @@ int paged_attention(const char *what, bool q8, bool cut, const float *q, int ldq
   const int size = q8 ? (int)q8_cache_type(cache_type) : cache_type_bytes(cache_type);
   if (!size) return fail(CDML_E_INVALID, "%s: unknown cache type %d", what, cache_type);
   const long long table = (long long)max_blocks * page_size;
-  if (!cut && max_len > table)
+  if (!shared && max_len > table)
     return fail(CDML_E_INVALID, "%s: max_len %d above the table's %lld tokens", what, max_len, table);
   const long long dim = (long long)num_heads * head_dim;
   if (ldq < dim || ldo < dim) return fail(CDML_E_INVALID, "%s: row stride smaller than the heads", what);
@@ -82,8 +82,9 @@ int paged_attention(const char *what, bool q8, bool cut, const float *q, int ldq
     if (rc) return rc;
   }
   const Plan p = make_plan(size, rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim);
-  size_t need = 0;
-  rc = workspace_size(what, q8, rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim, &need);
+  // (shared: that entry's size covers the plans of the types that run plain, and has been checked)
+  size_t need = sizeof(float) * (p.few_floats + p.tile_floats);
+  if (!shared) rc = workspace_size(what, q8, rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim, &need);
   if (rc) return rc;
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(CDML_E_INVALID, "%s: %zu bytes of 16-byte aligned workspace needed, %zu given", what, need,

@@ -5,9 +5,10 @@
 
 namespace cdml {
 
-// cdml_paged_attn and cdml_paged_attn_q8 for an entry of its own name.  cut: a max_len above the
-// table's tokens is allowed, and cut to them.
-int paged_attention(const char *what, bool q8, bool cut, const float *q, int ldq, const void *kcache,
+// cdml_paged_attn and cdml_paged_attn_q8 for an entry of its own name.  shared: for
+// cdml_paged_attn_shared, whose max_len may be above the table's tokens and is cut to them, and
+// whose workspace holds what this cache type needs, not what any type would.
+int paged_attention(const char *what, bool q8, bool shared, const float *q, int ldq, const void *kcache,
                     const void *vcache, const float *kscale, const float *vscale, int cache_type, int n_pages,
                     int page_size, const int *block_table, int max_blocks, const int *kv_len, const int *cu_new,
                     float *o, int ldo, int rows, int batch, int max_new, int max_len, int num_heads, int num_kv_heads,
