@@ -1,5 +1,7 @@
 // Data movement of 8-bit paged caches (include/cdml.h): rows quantised as they are written,
 // the copies of a reordering, and cached rows of any type read back as fp32.
+#include <algorithm>
+
 #include "paged.h"
 
 namespace cdml {
@@ -244,7 +246,9 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const ReadArgs a) {
   constexpr int W = VEC ? 4 : 1, U = 4;
   typedef Cached<TYPE, W> Item;
   __shared__ int slots[kReadRows];
-  const int row0 = blockIdx.x * a.block_rows, n_rows = min(a.block_rows, a.rows - row0);
+  const long long block = (long long)blockIdx.z * gridDim.x + blockIdx.x;
+  if (block * a.block_rows >= a.rows) return;
+  const int row0 = (int)block * a.block_rows, n_rows = min(a.block_rows, a.rows - row0);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (int i = wave; i < n_rows; i += 4) {
     const int s = slot_of_row(a, row0 + i);
@@ -436,7 +440,10 @@ extern "C" int cdml_paged_read(const void *kcache, const void *vcache, const flo
   const bool past = (size_t)rows * dim * 8 > (32u << 20);
   a.by_head = UDiv::make((uint32_t)a.per_head);
   a.by_row = UDiv::make((uint32_t)a.per_row);
-  const dim3 grid((unsigned)((rows - 1) / a.block_rows + 1), 2);
+  // an axis of a launch holds less than 2^32 threads, and one of more runs short without an error:
+  // from 2^23 workgroups on, the third axis counts the turns of the first
+  const unsigned blocks = (unsigned)((rows - 1) / a.block_rows) + 1, along = std::min(blocks, 1u << 23);
+  const dim3 grid(along, 2, (blocks - 1) / along + 1);
   const hipStream_t st = as_hip(stream);
   switch (cache_type) {
     case CDML_CACHE_F32: launch_read<CDML_CACHE_F32>(a, vec, past, grid, st); break;
