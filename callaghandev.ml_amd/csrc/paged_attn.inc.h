@@ -1528,96 +1528,84 @@ __device__ __forceinline__ void write_rows(const PagedArgs &a, const PagedSeq &s
 // the waves' sums are joined.  The next block is loaded into registers while one is
 // multiplied; two workgroups a CU keep 128 KB on the way at head dim 128.  64 x 8192 keys of
 // bf16, 64 heads over 8 of 128: 373 us, 5.8 TB/s.
-// SHARED: rows r0 .. r0 + 15 of nr.
-template <typename T, int HD, bool VEC>
-struct SpanShape {
-  static constexpr int ROW = HD + 4;  // floats between rows of the join
-  static constexpr int WAVE_O = 16 * ROW * 4, BLOCK = SpanBlock<T, HD, VEC>::BYTES;
-  static constexpr int WAVE = BLOCK > WAVE_O ? BLOCK : WAVE_O;
-};
-template <typename T, int HD, bool VEC, bool SHARED, int WAVE>
-__device__ __forceinline__ void span_rows(const PagedArgs &a, const PagedSeq &s, int b, int r0, int nr,
-                                          char (&lds)[4][WAVE], float (&red_m)[4][16], float (&red_l)[4][16]) {
+// SHARED: a group's rows sixteen at a time (one of more than the launch was told of takes its time).
+//   The body stays in the kernel: in a function that the kernel calls, always inlined, it takes 6 to
+// 16 registers more, which spill at head dim 128 (28 x 1225 keys, 12 heads over 4 of 96, bf16: 16.4
+// us for 15.2).
+template <typename T, int HD, bool VEC, bool SHARED>
+__global__ void __launch_bounds__(PT_THREADS, sizeof(T) == 2 || HD <= 64 ? 2 : 1) paged_span_kernel(const PagedArgs args) {
   typedef SpanRows<T, HD, VEC> Rows;
   typedef SpanBlock<T, HD, VEC> Block;
-  constexpr int NS = HD / 32, NDB = HD / 16, ROW = SpanShape<T, HD, VEC>::ROW;
-  const int hk = SHARED ? blockIdx.y % a.kv_heads : blockIdx.y, split = blockIdx.x;
-  const int base = s.len - s.n;
-  const bool single = SHARED ? a.fused && !a.prefix : s.len <= a.few_chunk;
-  const int c0 = split_from<SHARED>(s, split, a.few_chunk);
-  const int c1 = split_to<SHARED>(c0, split, a.few_splits, a.few_chunk, s.len);  // (some row sees all keys)
-  if (c0 >= c1 && !(single && split == 0)) return;
-
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = lane & 15, quarter = lane >> 4;
-  const int rr = min(r0 + row, nr - 1), tok = a.by_group.div(rr), head = hk * a.group + rr - tok * a.group;
-  const int last = s.len - 1, lim = s.causal ? base + tok : last;
-  const float *qrow = a.q + (size_t)(s.first + tok) * a.ldq + (size_t)head * a.hd;
-  const int *table = a.table + (size_t)s.table * a.max_blocks;
-  const int kv_dim = a.kv_heads * a.hd;
-  const T *kc = static_cast<const T *>(a.kc) + (size_t)hk * a.hd, *vc = static_cast<const T *>(a.vc) + (size_t)hk * a.hd;
-
-  Rows rows;
-  rows.init();
-  const int first = c0 + wave * 32;
-  if (first < c1) {
-    char *mine = lds[wave];
-    // this lane's key (lane % 32 of the block) and its page, a block ahead of its rows
-    auto key_at = [&](int k0) { return min(k0 + (lane & 31), last); };
-    auto page_at = [&](int k0) { return table[key_at(k0) >> a.page_shift]; };
-    Block blk;
-    blk.load(a, kc, vc, kv_dim, page_at(first), key_at(first));
-    int page = page_at(first + 128);
-    bf16x8 q[NS][3];
-    const bool wide = load_q_pieces<NS, VEC>(q, qrow, a.hd, a.scale_log2, 32, 8 * quarter);
-#pragma unroll 1
-    for (int k0 = first; k0 < c1; k0 += 128) {
-      blk.clean(k0, last, a.bad);
-      blk.store(mine);
-      blk.load(a, kc, vc, kv_dim, page, key_at(k0 + 128));
-      page = page_at(k0 + 256);
-      // the LDS writes above are this wave's own: in order, but not for the compiler
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      rows.add(mine, q, row, quarter, lim - k0 - 4 * quarter);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
-    if (rows.finish() || wide) rows.recompute(a, qrow, table, kc, vc, quarter, first, c1, lim, last);
-  }
-  // the waves' sums: rows' statistics, then each wave's O scaled to the common maximum
-  const float m = fmaxf(rows.m, kNoKey), l = quarters(rows.l, [](float x, float y) { return x + y; });
-  if (quarter == 0) {
-    red_m[wave][row] = m;
-    red_l[wave][row] = l;
-  }
-  __syncthreads();
-  const float w = fast_exp2(m - fmaxf(fmaxf(red_m[0][row], red_m[1][row]), fmaxf(red_m[2][row], red_m[3][row])));
-  float *part_o = reinterpret_cast<float *>(lds[wave]) + row * ROW;
-#pragma unroll
-  for (int db = 0; db < NDB; ++db) *reinterpret_cast<floatx4 *>(part_o + db * 16 + 4 * quarter) = rows.o[db] * w;
-  __syncthreads();
-  write_rows<HD, 16, ROW, SHARED>(a, s, b, hk, r0, nr, split, single, reinterpret_cast<const float *>(lds[0]),
-                                  WAVE / 4, red_m, red_l);
-}
-
-template <typename T, int HD, bool VEC, bool SHARED>
-__global__ void __launch_bounds__(PT_THREADS, sizeof(T) == 2 || HD <= 64 ? 2 : 1) paged_span_kernel(const PagedArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[4][SpanShape<T, HD, VEC>::WAVE];
+  constexpr int NS = HD / 32, NDB = HD / 16, ROW = HD + 4;  // floats between rows of the join
+  constexpr int WAVE_O = 16 * ROW * 4, WAVE = Block::BYTES > WAVE_O ? Block::BYTES : WAVE_O;
+  __shared__ __attribute__((aligned(16))) char lds[4][WAVE];
   __shared__ float red_m[4][16], red_l[4][16];
-  const int b = blockIdx.z;
-  const PagedSeq s = paged_seq<SHARED>(a, b);
-  const int nr = s.n * a.group;
-  if (nr == 0 || nr > a.few_rows) return;
-  if constexpr (SHARED) {
-    // (a group of more rows than the launch was told of takes its time)
-    for (int r0 = blockIdx.y / a.kv_heads * 16; r0 < nr; r0 += gridDim.y / a.kv_heads * 16) {
-      // (arguments read in every turn: held across turns, they would fill the registers)
-      const PagedArgs &z = args_again();
-      span_rows<T, HD, VEC, true>(z, paged_seq<true>(z, b), b, r0, nr, lds, red_m, red_l);
-      __syncthreads();
+
+  const int b = blockIdx.z, hk = blockIdx.y, split = blockIdx.x;
+  for (int r0 = 0;; r0 += 16) {
+    // (SHARED: arguments read in every turn: held across turns, they would fill the registers)
+    const PagedArgs &a = SHARED ? args_again() : args;
+    const PagedSeq s = paged_seq<SHARED>(a, b);
+    const int nr = s.n * a.group;
+    if (r0 >= nr || nr > a.few_rows) return;
+    const int base = s.len - s.n;
+    const bool single = SHARED ? a.fused && !a.prefix : s.len <= a.few_chunk;
+    const int c0 = split_from<SHARED>(s, split, a.few_chunk);
+    const int c1 = split_to<SHARED>(c0, split, a.few_splits, a.few_chunk, s.len);  // (some row sees all keys)
+    if (c0 >= c1 && !(single && split == 0)) return;
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = lane & 15, quarter = lane >> 4;
+    const int rr = min(r0 + row, nr - 1), tok = a.by_group.div(rr), head = hk * a.group + rr - tok * a.group;
+    const int last = s.len - 1, lim = s.causal ? base + tok : last;
+    const float *qrow = a.q + (size_t)(s.first + tok) * a.ldq + (size_t)head * a.hd;
+    const int *table = a.table + (size_t)s.table * a.max_blocks;
+    const int kv_dim = a.kv_heads * a.hd;
+    const T *kc = static_cast<const T *>(a.kc) + (size_t)hk * a.hd, *vc = static_cast<const T *>(a.vc) + (size_t)hk * a.hd;
+
+    Rows rows;
+    rows.init();
+    const int first = c0 + wave * 32;
+    if (first < c1) {
+      char *mine = lds[wave];
+      // this lane's key (lane % 32 of the block) and its page, a block ahead of its rows
+      auto key_at = [&](int k0) { return min(k0 + (lane & 31), last); };
+      auto page_at = [&](int k0) { return table[key_at(k0) >> a.page_shift]; };
+      Block blk;
+      blk.load(a, kc, vc, kv_dim, page_at(first), key_at(first));
+      int page = page_at(first + 128);
+      bf16x8 q[NS][3];
+      const bool wide = load_q_pieces<NS, VEC>(q, qrow, a.hd, a.scale_log2, 32, 8 * quarter);
+#pragma unroll 1
+      for (int k0 = first; k0 < c1; k0 += 128) {
+        blk.clean(k0, last, a.bad);
+        blk.store(mine);
+        blk.load(a, kc, vc, kv_dim, page, key_at(k0 + 128));
+        page = page_at(k0 + 256);
+        // the LDS writes above are this wave's own: in order, but not for the compiler
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        rows.add(mine, q, row, quarter, lim - k0 - 4 * quarter);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+      if (rows.finish() || wide) rows.recompute(a, qrow, table, kc, vc, quarter, first, c1, lim, last);
     }
-  } else {
-    span_rows<T, HD, VEC, false>(a, s, b, 0, nr, lds, red_m, red_l);
+    // the waves' sums: rows' statistics, then each wave's O scaled to the common maximum
+    const float m = fmaxf(rows.m, kNoKey), l = quarters(rows.l, [](float x, float y) { return x + y; });
+    if (quarter == 0) {
+      red_m[wave][row] = m;
+      red_l[wave][row] = l;
+    }
+    __syncthreads();
+    const float w = fast_exp2(m - fmaxf(fmaxf(red_m[0][row], red_m[1][row]), fmaxf(red_m[2][row], red_m[3][row])));
+    float *part_o = reinterpret_cast<float *>(lds[wave]) + row * ROW;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) *reinterpret_cast<floatx4 *>(part_o + db * 16 + 4 * quarter) = rows.o[db] * w;
+    __syncthreads();
+    write_rows<HD, 16, ROW, SHARED>(a, s, b, hk, r0, nr, split, single, reinterpret_cast<const float *>(lds[0]),
+                                    WAVE / 4, red_m, red_l);
+    if (!SHARED || r0 + 16 >= nr) return;
+    __syncthreads();
   }
 }
 
