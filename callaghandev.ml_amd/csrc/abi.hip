@@ -449,9 +449,11 @@ int cdml_argmax_rows(const float *x, int rows, int cols, int ld, int *out, int o
                 rows, cols, ld, out_stride);
   if (rows == 0) return CDML_OK;
   if (!x || !out) return fail(CDML_E_INVALID, "cdml_argmax_rows: NULL pointer");
-  int rc = ensure_device();
+  const long long blocks = ((long long)rows + 3) / 4;
+  int rc = check_axis("cdml_argmax_rows", blocks, 256);
+  if (!rc) rc = ensure_device();
   if (rc) return rc;
-  argmax_rows_kernel<<<dim3((rows + 3) / 4), dim3(256), 0, as_hip(stream)>>>(x, rows, cols, ld, out,
+  argmax_rows_kernel<<<dim3((unsigned)blocks), dim3(256), 0, as_hip(stream)>>>(x, rows, cols, ld, out,
                                                                             out_stride);
   return check_launch("argmax_rows_kernel");
 }
@@ -462,7 +464,8 @@ int cdml_embed_tokens(const int *ids, int count, const float *table, int vocab, 
     return fail(CDML_E_INVALID, "cdml_embed_tokens: negative size");
   if (count == 0 || dim == 0) return CDML_OK;
   if (!ids || !table || !out) return fail(CDML_E_INVALID, "cdml_embed_tokens: NULL pointer");
-  int rc = ensure_device();
+  int rc = check_axis("cdml_embed_tokens", count, 64);
+  if (!rc) rc = ensure_device();
   if (rc) return rc;
   int vec4 = (dim % 4 == 0) && aligned16(table) && aligned16(out);
   embed_kernel<<<dim3(count), dim3(64), 0, as_hip(stream)>>>(ids, count, table, vocab, dim, out,
@@ -477,7 +480,8 @@ int cdml_kv_cache_append(const float *k_new, const float *v_new, float *kcache, 
   if (batch == 0) return CDML_OK;
   if (!k_new || !v_new || !kcache || !vcache || !positions)
     return fail(CDML_E_INVALID, "cdml_kv_cache_append: NULL pointer");
-  int rc = ensure_device();
+  int rc = check_axis("cdml_kv_cache_append", batch, 256);
+  if (!rc) rc = ensure_device();
   if (rc) return rc;
   kv_append_kernel<<<dim3(batch), dim3(256), 0, as_hip(stream)>>>(k_new, v_new, kcache, vcache,
                                                                  positions, t_max, dim);

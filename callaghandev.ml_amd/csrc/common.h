@@ -30,6 +30,12 @@ int num_cus();
 
 // Checks the launch that was just enqueued.
 int check_launch(const char *what);
+// An axis of a launch holds less than 2^32 threads, and a launch of more runs short without an
+// error: refuses `workgroups` of `threads`.
+inline int check_axis(const char *what, long long workgroups, int threads) {
+  if (workgroups * threads < 1LL << 32) return CDML_OK;
+  return fail(CDML_E_INVALID, "%s: problem too large (%lld workgroups of %d threads)", what, workgroups, threads);
+}
 
 inline hipStream_t as_hip(cdml_stream s) { return reinterpret_cast<hipStream_t>(s); }
 

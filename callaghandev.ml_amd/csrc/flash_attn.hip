@@ -627,6 +627,12 @@ using namespace cdml;
 
 namespace cdml {
 
+static int check_items(int batch, int lq, int num_heads, int hd) {
+  return check_axis("cdml_sdpa_fwd",
+                    hd > 128 ? (long long)batch * lq : (long long)batch * num_heads * ((lq + FA_BM - 1LL) / FA_BM),
+                    FA_THREADS);
+}
+
 // Launches the forward kernels; the arguments are validated by the caller.
 // causal here admits lq != lk (key j visible to query i iff j <= i).
 int flash_forward(const float *q, int ldq, const float *k, int ldk, const float *v, int ldv,
@@ -650,6 +656,8 @@ int flash_forward(const float *q, int ldq, const float *k, int ldk, const float 
   a.scale_log2 = scale * kLog2e;
 
   const int hd = a.hd;
+  const int rc = check_items(batch, lq, num_heads, hd);
+  if (rc) return rc;
   if (hd > 128) {
     if (lse) return fail(CDML_E_INVALID, "flash_forward: no row statistics above head dim 128");
     a.n_qt = lq;
@@ -665,9 +673,7 @@ int flash_forward(const float *q, int ldq, const float *k, int ldk, const float 
   a.n_qt = (lq + FA_BM - 1) / FA_BM;
   a.by_bh = UDiv::make((uint32_t)a.n_bh);
   a.by_heads = UDiv::make((uint32_t)num_heads);
-  long long total = (long long)batch * num_heads * a.n_qt;
-  if (total > (1LL << 30)) return fail(CDML_E_INVALID, "cdml_sdpa_fwd: problem too large");
-  a.n_items = (int)total;
+  a.n_items = a.n_bh * a.n_qt;
   if (hd_pad == 32) launch_hd<32, 32>(a, causal, vec, st);
   else if (hd_pad == 64) launch_hd<64, 32>(a, causal, vec, st);
   else launch_hd<128, 32>(a, causal, vec, st);
@@ -695,7 +701,8 @@ int sdpa_fwd_impl(const float *q, int ldq, const float *k, int ldk, const float 
   if (batch == 0 || lq == 0) return CDML_OK;
   if (lk == 0) return fail(CDML_E_INVALID, "cdml_sdpa_fwd: lk must be >= 1");
   if (!q || !k || !v || !o) return fail(CDML_E_INVALID, "cdml_sdpa_fwd: NULL pointer");
-  int rc = ensure_device();
+  int rc = check_items(batch, lq, num_heads, dim / num_heads);
+  if (!rc) rc = ensure_device();
   if (rc) return rc;
   return flash_forward(q, ldq, k, ldk, v, ldv, o, ldo, lse, batch, lq, lk, dim, num_heads, scale,
                        causal != 0, mask, as_hip(stream));

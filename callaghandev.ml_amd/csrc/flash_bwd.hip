@@ -1569,7 +1569,11 @@ int sdpa_bwd_impl(const float *q, int ldq, const float *k, int ldk, const float 
   if (batch == 0 || (lq == 0 && lk == 0)) return CDML_OK;
   if ((lq && (!dq || !q || !dout)) || (lk && (!dk || !dv || !k || !v)))
     return fail(CDML_E_INVALID, "%s: NULL pointer", what);
-  rc = ensure_device();
+  const int head = dim / num_heads;
+  if (lq && lk)
+    rc = check_axis(what, (long long)batch * num_heads * ((std::max(lq, lk) + BW_TILE - 1LL) / BW_TILE),
+                    head <= 64 && paired_keys(head) ? 2 * BW_THREADS : BW_THREADS);
+  if (!rc) rc = ensure_device();
   if (rc) return rc;
   hipStream_t st = as_hip(stream);
   if (lq == 0 || lk == 0) {  // nothing attends: every gradient is 0
@@ -1581,8 +1585,6 @@ int sdpa_bwd_impl(const float *q, int ldq, const float *k, int ldk, const float 
   if (!workspace || workspace_bytes < need)
     return fail(CDML_E_INVALID, "%s: workspace of %zu bytes needed, %zu given", what, need,
                 workspace_bytes);
-  if ((long long)batch * num_heads * ((std::max(lq, lk) + BW_TILE - 1) / BW_TILE) > (1LL << 30))
-    return fail(CDML_E_INVALID, "%s: problem too large", what);
 
   BwdArgs a{};
   a.q = q;

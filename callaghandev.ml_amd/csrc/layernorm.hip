@@ -138,9 +138,11 @@ extern "C" int cdml_residual_layernorm(const float *a, const float *b, const flo
   if (rows == 0 || features == 0) return CDML_OK;
   if (!a || !b || !gamma || !beta || !y)
     return fail(CDML_E_INVALID, "cdml_residual_layernorm: NULL pointer");
-  int rc = ensure_device();
+  const long long blocks = ((long long)rows + 3) / 4;
+  int rc = check_axis("cdml_residual_layernorm", blocks, 256);
+  if (!rc) rc = ensure_device();
   if (rc) return rc;
-  const dim3 grid((rows + 3) / 4), block(256);
+  const dim3 grid((unsigned)blocks), block(256);
   hipStream_t st = as_hip(stream);
   const int rcache = row_cache(features);
   if (rcache >= 4 && features <= 64 * rcache && features % 4 == 0 && aligned16(a) && aligned16(b) &&

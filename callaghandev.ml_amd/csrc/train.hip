@@ -137,7 +137,7 @@ constexpr int ln_waves(int rc) { return rc >= 32 ? 4 : 16; }
 constexpr int ln_block_rows(int rc) { return rc == 4 ? 32 : kLnRowsPerBlock; }
 inline int ln_blocks(int rows, int features) {
   const int r = ln_block_rows(row_cache(features));
-  return (rows + r - 1) / r;
+  return (int)(((long long)rows + r - 1) / r);
 }
 
 template <int RC, int WAVES = ln_waves(RC), int ROWS = ln_block_rows(RC)>
@@ -771,9 +771,11 @@ extern "C" int cdml_residual_layernorm_fwd(const float *a, const float *b, const
     return fail(CDML_E_INVALID, "cdml_residual_layernorm_fwd: NULL pointer");
   if (features > 64 * kRowCache)
     return fail(CDML_E_INVALID, "cdml_residual_layernorm_fwd: more than %d features", 64 * kRowCache);
-  int rc = ensure_device();
+  const long long blocks = ((long long)rows + 3) / 4;
+  int rc = check_axis("cdml_residual_layernorm_fwd", blocks, 256);
+  if (!rc) rc = ensure_device();
   if (rc) return rc;
-  const dim3 grid((rows + 3) / 4), block(256);
+  const dim3 grid((unsigned)blocks), block(256);
   hipStream_t st = as_hip(stream);
   const int rcache = row_cache(features);
   const bool v4 = rcache >= 4 && features % 4 == 0 && aligned16(a) && aligned16(b) && aligned16(gamma) &&
@@ -829,7 +831,8 @@ extern "C" int cdml_layernorm_backward(const float *dout, const float *dout2,
   if (need && (!workspace || workspace_bytes < need))
     return fail(CDML_E_INVALID, "cdml_layernorm_backward: workspace of %zu bytes needed, %zu given", need,
                 workspace_bytes);
-  int rc = ensure_device();
+  int rc = check_axis("cdml_layernorm_backward", ln_blocks(rows, features), 64 * ln_waves(row_cache(features)));
+  if (!rc) rc = ensure_device();
   if (rc) return rc;
   hipStream_t st = as_hip(stream);
   const int nblk = ln_blocks(rows, features);
@@ -901,7 +904,8 @@ extern "C" int cdml_cross_entropy(const float *logits, int ldl, const int *targe
     return fail(CDML_E_INVALID, "cdml_cross_entropy: NULL pointer");
   if (!workspace || workspace_bytes < (size_t)(rows > 0 ? rows : 1) * sizeof(float))
     return fail(CDML_E_INVALID, "cdml_cross_entropy: workspace too small");
-  int rc = ensure_device();
+  int rc = check_axis("cdml_cross_entropy", rows, 256);
+  if (!rc) rc = ensure_device();
   if (rc) return rc;
   hipStream_t st = as_hip(stream);
   float *row_loss = static_cast<float *>(workspace);

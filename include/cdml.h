@@ -19,6 +19,9 @@
  *     stream) and return; only *_synchronize and cdml_event_elapsed_ms block.
  *   - Every function returns a status; CDML_OK is 0.  On failure
  *     cdml_last_error() returns a message for the calling thread.
+ *   - A size that takes more workgroups than an axis of a launch holds (2^24 of
+ *     256 threads, so 2^24 rows of cdml_cross_entropy or 2^26 of a layer norm)
+ *     is CDML_E_INVALID.
  *   - Calls on distinct streams from distinct threads are safe.  One stream
  *     is not re-entrant.
  *
