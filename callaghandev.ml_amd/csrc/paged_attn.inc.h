@@ -731,7 +731,9 @@ struct PagedRows {
   // -inf for the keys past this lane's last one (as an offset in its half's sub-block)
   __device__ __forceinline__ void apply_mask(floatx16 &sacc, int last_vis) const {
     // (keeps the branch around the mask: the compiler would make every sub-block's scores pass
-    // 32 selections of it.  4 x 4096 tokens, 16 heads of 64, f8: 437 -> 432 us)
+    // 32 selections of it.  4 x 4096 tokens, 16 heads of 64, f8: 437 -> 432 us; 24 ragged chunks,
+    // 32 heads over 8 of 128, fp32 1758 -> 1713, fp16 1195 -> 1181, bf16 780 -> 772; but 16 chunks of
+    // 300 tokens over 2500, bf16 of 128, 251 -> 268, the one of 36 such shapes that loses over 2%)
     asm volatile("" : "+v"(last_vis));
 #pragma unroll
     for (int r = 0; r < 16; ++r) sacc[r] = acc_key(r) <= last_vis ? sacc[r] : -INFINITY;
@@ -968,9 +970,9 @@ struct PagedRows {
 // they need a scale: a probability then loses what lies below 2^-35 of its row's largest, and
 // a value what lies below 2^-40 of the largest beside it, while its part in the sum, the
 // product of the two, may be as large as any.
-//   What bounds it: 4 x 4096 tokens (fp32, 16 heads of 64) take 745 to 840 us by card, 1.0
+//   What bounds it: 4 x 4096 tokens (fp32, 16 heads of 64) take 710 to 840 us by card, 1.0
 // PFLOP/s of bf16 products where the library's largest plain ones reach 1.13; ragged chunks
-// (bf16, 32 heads over 8 of 128) 765 to 840 us, as much.  The matrix cores are busy 51% of the
+// (bf16, 32 heads over 8 of 128) 745 to 840 us, as much.  The matrix cores are busy 51% of the
 // cycles (46% at head dim 128) beside six (four) vector instructions for each of theirs; and
 // cycles are long: the clock falls to 1.9 GHz (2.0) under their power.
 //   8-bit caches (4 x 4096 tokens, 16 heads of 64, f8: 418 to 435 us by card, 316 to 329 TFLOP/s;

@@ -12,8 +12,8 @@ namespace {
 // keys at a time, straight from the cache into the operands of the 16x16x32 MFMA:
 //   K: lane (row, quarter) has 16 bytes of every 64 of keys row and 16 + row, the quarters side by
 //      side.  A dot product's order is free, so product s takes the lane's s-th eight dims, of
-//      Q too.  (A quarter of a row to a lane, whose loads touch four times the segments:
-//      64 requests behind 8192 bf16 tokens 87 -> 78 us.)
+//      Q too.  (A quarter of a row to a lane, whose loads touch four times the segments: 64
+//      requests behind 8192 bf16 tokens 74.4 us, 68.1 so.)
 //   V: lane (row, quarter) has dims VD * row .. + VD - 1 of the keys 4 quarter + 0..3 and
 //      16 + 4 quarter + 0..3, those whose probabilities it holds; product d takes its d-th
 //      dim, so V is transposed as the codes of two keys become a pair of bf16.

@@ -188,7 +188,10 @@ SharedPlan plan_shared(int size, int rows, int batch, int groups, int max_member
   p.fused = p.own.kernels.span && p.own.few_splits == 1;
   // Where requests and heads fill the SIMDs without a split, four waves on a few keys wait for each
   // other longer than they read: 16 x 8 beams of 16 heads, up to 100 tokens of their own, i8, 51.3
-  // us with four, 38.1 with one; but 64 requests of 8 heads, up to 500, bf16, 78.3 and 96.5.
+  // us with four, 38.1 with one; but 64 requests of 8 heads, up to 500, bf16, 78.3 and 96.5.  Over 144
+  // calls (i8 and bf16, head dims 64 and 128, 256 to 8192 pairs, tails of up to 8 to 500 tokens
+  // behind 2048) the 88 that have one wave take 3 to 49% less so; of the others, tails of up to
+  // 500 of 1024 pairs would take 2 to 9% less with one, all else longer.
   const long long pairs = (long long)batch * kv_heads;
   p.lone_waves = p.fused && pairs >= 4 * kComputeUnits && 4LL * max_tail <= pairs;
   p.parts = (size_t)rows * heads * (p.prefix_splits + p.own_splits);

@@ -740,7 +740,8 @@ int cdml_paged_attn_q8(const float *q, int ldq, const void *kcache,
  * number of first tokens that all members of b's group have in the same pages: whole
  * pages, no page outside [0, n_pages), and none of the step's new tokens (rows
  * cu_new[b] .. cu_new[b + 1]) among them.  0 for a group of one, and for requests of
- * no group. */
+ * no group.  A member without tokens, such as a released request, shares none, and
+ * neither does then its group: keep such requests out of the groups. */
 int cdml_paged_shared(const int *block_table, int max_blocks,
                       const int *kv_len, const int *cu_new,
                       const int *group_start, int groups, int batch,
