@@ -33,7 +33,7 @@ int check_launch(const char *what);
 // An axis of a launch holds less than 2^32 threads, and a launch of more runs short without an
 // error: refuses `workgroups` of `threads`.
 inline int check_axis(const char *what, long long workgroups, int threads) {
-  if (workgroups * threads < 1LL << 32) return CDML_OK;
+  if (workgroups < (1LL << 32) / threads) return CDML_OK;
   return fail(CDML_E_INVALID, "%s: problem too large (%lld workgroups of %d threads)", what, workgroups, threads);
 }
 

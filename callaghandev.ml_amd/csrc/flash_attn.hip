@@ -628,9 +628,9 @@ using namespace cdml;
 namespace cdml {
 
 static int check_items(int batch, int lq, int num_heads, int hd) {
-  return check_axis("cdml_sdpa_fwd",
-                    hd > 128 ? (long long)batch * lq : (long long)batch * num_heads * ((lq + FA_BM - 1LL) / FA_BM),
-                    FA_THREADS);
+  if (hd > 128) return check_axis("cdml_sdpa_fwd", (long long)batch * lq, FA_THREADS);
+  const int rc = check_axis("cdml_sdpa_fwd", (long long)batch * num_heads, FA_THREADS);
+  return rc ? rc : check_axis("cdml_sdpa_fwd", (long long)batch * num_heads * ((lq + FA_BM - 1LL) / FA_BM), FA_THREADS);
 }
 
 // Launches the forward kernels; the arguments are validated by the caller.

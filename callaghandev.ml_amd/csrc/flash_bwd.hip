@@ -1569,10 +1569,10 @@ int sdpa_bwd_impl(const float *q, int ldq, const float *k, int ldk, const float 
   if (batch == 0 || (lq == 0 && lk == 0)) return CDML_OK;
   if ((lq && (!dq || !q || !dout)) || (lk && (!dk || !dv || !k || !v)))
     return fail(CDML_E_INVALID, "%s: NULL pointer", what);
-  const int head = dim / num_heads;
-  if (lq && lk)
-    rc = check_axis(what, (long long)batch * num_heads * ((std::max(lq, lk) + BW_TILE - 1LL) / BW_TILE),
-                    head <= 64 && paired_keys(head) ? 2 * BW_THREADS : BW_THREADS);
+  const int head = dim / num_heads, threads = head <= 64 && paired_keys(head) ? 2 * BW_THREADS : BW_THREADS;
+  const long long pairs = (long long)batch * num_heads;
+  if (lq && lk) rc = check_axis(what, pairs, threads);
+  if (!rc && lq && lk) rc = check_axis(what, pairs * ((std::max(lq, lk) + BW_TILE - 1LL) / BW_TILE), threads);
   if (!rc) rc = ensure_device();
   if (rc) return rc;
   hipStream_t st = as_hip(stream);

@@ -41,9 +41,11 @@ CASES = [
     ("cdml_layernorm_backward", ln_bwd(2 ** 28 - 64, 8), [{"rows": 2 ** 28 - 63}, {"rows": 2 ** 31 - 1}]),
     ("cdml_cross_entropy", dict(x=P, ldl=2, targets=P, rows=2 ** 24 - 1, dim=2, eff=5, gs=1.0, ls=1.0, loss=P, dx=P, lddl=2,
                                 ws=P, bytes=WS, stream=None), [{"rows": 2 ** 24}]),
-    ("cdml_sdpa_fwd", fwd(2 ** 22 - 1, 5, 32, 4), [{"batch": 2 ** 22}, {"batch": 2 ** 21, "lq": 129, "lk": 129}]),
+    ("cdml_sdpa_fwd", fwd(2 ** 22 - 1, 5, 32, 4), [{"batch": 2 ** 22}, {"batch": 2 ** 21, "lq": 129, "lk": 129},
+                                                 {"batch": 2 ** 31 - 1, "lq": 2 ** 31 - 1, "heads": 32}]),
     ("cdml_sdpa_fwd", fwd(2 ** 23 - 1, 2, 200, 1), [{"batch": 2 ** 23}, {"batch": 2 ** 20, "lq": 16}]),
-    ("cdml_sdpa_bwd", bwd(2 ** 22 - 1, 5, 32, 4), [{"batch": 2 ** 22}, {"batch": 2 ** 21, "lq": 129}]),
+    ("cdml_sdpa_bwd", bwd(2 ** 22 - 1, 5, 32, 4), [{"batch": 2 ** 22}, {"batch": 2 ** 21, "lq": 129},
+                                                 {"batch": 2 ** 31 - 1, "lq": 2 ** 31 - 1, "heads": 32}]),
     ("cdml_sdpa_bwd", bwd(2 ** 21 - 1, 5, 160, 4), [{"batch": 2 ** 21}]),
 ]
 
